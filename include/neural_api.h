@@ -339,6 +339,87 @@ int   neural_dropout_backward(const float *grad_output, float *grad_input, const
 int      neural_dropout_seed(uint32_t seed);
 uint64_t neural_dropout_draws(void);
 
+/* NEW, no counterpart in the reference (its neural_dropout_forward, above,
+ * draws from one serial stream, stores a byte per element and takes f32 only):
+ * inverted dropout whose mask is a function of the element's index and a key,
+ * so that none is stored, nothing is kept between calls, and the backward call
+ * makes the same mask again.  f32 and f64 tensors.
+ *
+ * Element i of the flat tensor is place e = i % 8 of group g = i / 8.
+ * Philox4x32-10 (Salmon, Moraes, Dror, Shaw 2011) with the 64-bit key `seed`
+ * gives four words for each counter (64-bit block number, 64-bit `offset`);
+ * half e (16 bits, low half of a word first) of block 2 g is the upper and of
+ * block 2 g + 1 the lower half of the element's draw r.  Dropped, +0, where
+ * r < round(p 2^32) (whatever `in` holds there); else in * scale with scale = 1 /
+ * (1 - p) rounded to the dtype.  p = 0 keeps and p = 1 drops every element.
+ * Calls with different (seed, offset) have independent masks, of any size.
+ *
+ * key: host memory, read during the call, or device memory, read by the kernel:
+ * a captured graph then takes a new mask in each replay when the caller changes
+ * the words between replays.  8-byte aligned.
+ * Returns NEURAL_ERR_NULL_POINTER, DTYPE_MISMATCH, SHAPE_MISMATCH (element counts
+ * differ) or INVALID_ARGUMENT (p outside [0, 1] or NaN, non-contiguous tensors, a
+ * misaligned key, `out` overlapping `in` without being it: in place is fine). */
+typedef struct {
+    uint64_t seed;
+    uint64_t offset;
+} NeuralDropoutKey;
+int neural_counter_dropout_forward(NeuralTensor *out, const NeuralTensor *in, double p,
+                                   const NeuralDropoutKey *key);
+int neural_counter_dropout_backward(NeuralTensor *grad_in, const NeuralTensor *grad_out, double p,
+                                    const NeuralDropoutKey *key);
+
+/* ---- Layer norm (NEW) ---------------------------------------------------------
+ * The reference's layernorm_create / _forward / _backward objects are outside
+ * this library (listed below); these work on tensors, with no object.  Rows over the last dimension of contiguous
+ * f32 / f64 tensors of any rank >= 1; all tensors of a call have one dtype.
+ *
+ * Forward: mean = sum x / C, rstd = 1 / sqrt(sum (x - mean)^2 / C + eps), out =
+ * (x - mean) rstd gamma + beta, in double, rounded once per value.  gamma, beta
+ * (C values; NULL: 1 and 0); mean, rstd (one value per row, for the backward
+ * call; may be NULL).  `out` may be `in`.  A row that holds NaN or an infinity
+ * is NaN; no other row is touched by it.
+ *
+ * Backward, from the saved mean and rstd: xh = (in - mean) rstd, w = grad_out
+ * gamma, grad_in = rstd (w - mean_C(w) - xh mean_C(w xh)), grad_gamma = sum over
+ * rows of grad_out xh, grad_beta = sum over rows of grad_out.  Any output may be NULL, not all.
+ * grad_in may be grad_out or in.  The sums' order depends on the shape and the device
+ * alone: equal calls give equal bits.
+ *
+ * Joined with what precedes it in a transformer's sublayer: hidden = residual +
+ * dropout(in) and the norm of hidden, in one pass.  hidden has the bits of neural_add(residual,
+ * neural_counter_dropout_forward(in, p, key)), and out, mean and rstd those of
+ * neural_layer_norm_forward on it.  p = 0: no dropout (key may be NULL), for
+ * inference.  hidden may be NULL where no backward call follows.  out or hidden
+ * may be `in` or `residual`.
+ * Its backward: d = neural_layer_norm_backward's grad_in at `hidden` + grad_hidden
+ * (the gradient that reaches hidden along the residual stream; may be NULL);
+ * grad_residual = d, grad_in = the dropout's gradient of d, bit for bit.  Any output may
+ * be NULL, not all; grad_in or grad_residual may be grad_out, hidden or grad_hidden.
+ *
+ * Where a gradient of gamma or beta is asked for, the call takes device memory for
+ * partial sums from the library's cache; while the stream is being captured, memory of
+ * the graph's own, held until the process ends, so graphs may replay side by side.
+ *
+ * Errors: NULL_POINTER, DTYPE_MISMATCH, DIM_MISMATCH (a 0-d tensor), SHAPE_MISMATCH,
+ * INVALID_ARGUMENT (non-contiguous tensors, eps negative or not finite, p or key as
+ * above, outputs that overlap an input, other than as allowed, or each other). */
+int neural_layer_norm_forward(NeuralTensor *out, const NeuralTensor *in, const NeuralTensor *gamma,
+                              const NeuralTensor *beta, double eps, NeuralTensor *mean, NeuralTensor *rstd);
+int neural_layer_norm_backward(NeuralTensor *grad_in, NeuralTensor *grad_gamma, NeuralTensor *grad_beta,
+                               const NeuralTensor *grad_out, const NeuralTensor *in, const NeuralTensor *gamma,
+                               const NeuralTensor *mean, const NeuralTensor *rstd);
+int neural_dropout_add_layer_norm_forward(NeuralTensor *out, NeuralTensor *hidden, const NeuralTensor *in,
+                                          const NeuralTensor *residual, const NeuralTensor *gamma,
+                                          const NeuralTensor *beta, double p, const NeuralDropoutKey *key,
+                                          double eps, NeuralTensor *mean, NeuralTensor *rstd);
+int neural_dropout_add_layer_norm_backward(NeuralTensor *grad_in, NeuralTensor *grad_residual,
+                                           NeuralTensor *grad_gamma, NeuralTensor *grad_beta,
+                                           const NeuralTensor *grad_out, const NeuralTensor *grad_hidden,
+                                           const NeuralTensor *hidden, const NeuralTensor *gamma,
+                                           const NeuralTensor *mean, const NeuralTensor *rstd, double p,
+                                           const NeuralDropoutKey *key);
+
 /* ---- 2-D f64 tensor ops: neural_api.h:1273-1305, tensor_ops.c:15-148 ---------- */
 int tensor_concat_2d(const double *a, const double *b, int64_t rows_a, int64_t cols_a,
                      int64_t rows_b, int64_t cols_b, int64_t axis, double *out,

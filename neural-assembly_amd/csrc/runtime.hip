@@ -204,6 +204,21 @@ void dev_free(void *p)
     r.live.erase(it);
 }
 
+void *dev_alloc_own(size_t bytes)
+{
+    g_dev_allocs.fetch_add(1, std::memory_order_relaxed);
+    g_hip_mallocs.fetch_add(1, std::memory_order_relaxed);
+    hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
+    const bool relaxed = hipThreadExchangeStreamCaptureMode(&mode) == hipSuccess;
+    void *p = nullptr;
+    if (hipMalloc(&p, bytes ? bytes : 1) != hipSuccess) {
+        (void)hipGetLastError();
+        p = nullptr;
+    }
+    if (relaxed) (void)hipThreadExchangeStreamCaptureMode(&mode);
+    return p;
+}
+
 bool is_device_ptr(const void *p)
 {
     if (!p) return false;

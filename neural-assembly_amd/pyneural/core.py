@@ -130,6 +130,11 @@ class NeuralBufferInfo(ctypes.Structure):
     ]
 
 
+class DropoutKeyC(ctypes.Structure):
+    """NeuralDropoutKey: what a counter-based dropout mask is made from."""
+    _fields_ = [("seed", ctypes.c_uint64), ("offset", ctypes.c_uint64)]
+
+
 _vp, _i, _i64, _u64, _d, _f = (ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_uint64,
                                 ctypes.c_double, ctypes.c_float)
 _u64p = ctypes.POINTER(ctypes.c_uint64)
@@ -270,6 +275,13 @@ _SIGS = {
     "neural_dropout_backward": (_i, [_vp, _vp, _vp, _u64, _f]),
     "neural_dropout_seed": (_i, [ctypes.c_uint32]),
     "neural_dropout_draws": (_u64, []),
+    "neural_counter_dropout_forward": (_i, [_vp, _vp, _d, _vp]),
+    "neural_counter_dropout_backward": (_i, [_vp, _vp, _d, _vp]),
+    # layer norm
+    "neural_layer_norm_forward": (_i, [_vp, _vp, _vp, _vp, _d, _vp, _vp]),
+    "neural_layer_norm_backward": (_i, [_vp] * 8),
+    "neural_dropout_add_layer_norm_forward": (_i, [_vp] * 6 + [_d, _vp, _d, _vp, _vp]),
+    "neural_dropout_add_layer_norm_backward": (_i, [_vp] * 10 + [_d, _vp]),
     # tensor ops
     "tensor_concat_2d": (_i, [_vp, _vp, _i64, _i64, _i64, _i64, _i64, _vp, _i64p, _i64p]),
     "tensor_split_2d": (_i, [_vp, _i64, _i64, _i64, _i64, _vp, _vp, _i64p, _i64p, _i64p, _i64p]),

@@ -9,14 +9,17 @@ output and makes one library call.  Loss modules: CrossEntropyLoss
 (nn.py:193-301 -> neural_dropout_forward / _backward) keeps its mask in device
 memory.  Fused epilogues: add_relu (vec_add_relu_fusion, fusion.asm:200-226)
 and bias_add_act (bias add of nn_layers.asm:472-539 followed by an
-activation, one pass).
+activation, one pass).  Without a reference counterpart: CounterDropout (a mask
+made from a seed and a call number, never stored), LayerNorm and
+DropoutAddLayerNorm (the residual add, dropout and norm that end a transformer's
+sublayer, in one pass), each with its backward pass.
 """
 
 import ctypes
 
 import numpy as np
 
-from .core import _lib, _check_error, NeuralDtype
+from .core import _lib, _check_error, DropoutKeyC, NeuralDtype
 from .tensor import Tensor
 
 
@@ -261,6 +264,155 @@ def dropout_seed(seed: int) -> None:
     """Position the dropout stream as srand(seed) positions the C library's
     rand() (the stream starts as srand(1))."""
     _check_error(_lib.neural_dropout_seed(ctypes.c_uint32(seed & 0xFFFFFFFF)), "dropout seed")
+
+
+class CounterDropout(Module):
+    """Inverted dropout whose mask is a function of the element's index, ``seed``
+    and the number of the call (neural_counter_dropout_forward; the offset of
+    call k is ``offset + k``): none is stored, and ``backward`` makes the last
+    forward's again.  float32 and float64; identity in eval mode."""
+
+    def __init__(self, p: float = 0.5, seed: int = 0, offset: int = 0):
+        super().__init__()
+        if not 0.0 <= p <= 1.0:
+            raise ValueError(f"Dropout probability must be in [0, 1], got {p}")
+        self.p = p
+        self.seed = seed
+        self.offset = offset  # of the next call
+        self._last = None     # (p, key) of the last forward
+
+    def _next(self):
+        p, key = (self.p, DropoutKeyC(self.seed, self.offset)) if self.training else (0.0, DropoutKeyC(0, 0))
+        self._last = (p, key)
+        return p, key
+
+    def _took(self):
+        if self.training:
+            self.offset = (self.offset + 1) & 0xFFFFFFFFFFFFFFFF
+
+    def forward(self, x: Tensor) -> Tensor:
+        src = x.contiguous()
+        out = Tensor.create(x.shape, x.dtype)
+        p, key = self._next()
+        _check_error(_lib.neural_counter_dropout_forward(out._ptr, src._ptr, p, ctypes.byref(key)),
+                     "counter dropout forward")
+        self._took()
+        return out
+
+    def backward(self, grad_output: Tensor) -> Tensor:
+        if self._last is None:
+            raise RuntimeError("CounterDropout.backward called before forward")
+        p, key = self._last
+        go = grad_output.contiguous()
+        gi = Tensor.create(grad_output.shape, grad_output.dtype)
+        _check_error(_lib.neural_counter_dropout_backward(gi._ptr, go._ptr, p, ctypes.byref(key)),
+                     "counter dropout backward")
+        return gi
+
+    def __repr__(self) -> str:
+        return f"CounterDropout(p={self.p}, seed={self.seed})"
+
+
+class LayerNorm(Module):
+    """(x - mean) / sqrt(var + eps) * gamma + beta over the last dimension
+    (neural_layer_norm_forward).  ``backward`` returns the input's gradient and
+    leaves those of gamma and beta in their ``grad``."""
+
+    def __init__(self, num_features: int, eps: float = 1e-5, dtype: int = NeuralDtype.FLOAT32):
+        super().__init__()
+        if num_features < 1:
+            raise ValueError(f"num_features must be >= 1, got {num_features}")
+        self.num_features = num_features
+        self.eps = eps
+        self.gamma = Tensor.ones([num_features], dtype)
+        self.beta = Tensor.zeros([num_features], dtype)
+        self._saved = None
+
+    def parameters(self):
+        return [self.gamma, self.beta]
+
+    def _stats(self, x: Tensor):
+        if not x.shape or x.shape[-1] != self.num_features:
+            raise ValueError(f"expected a last dimension of {self.num_features}, got shape {x.shape}")
+        rows = x.numel // self.num_features
+        return Tensor.create([rows], x.dtype), Tensor.create([rows], x.dtype)
+
+    def _grads(self):
+        self.gamma.grad = Tensor.create([self.num_features], self.gamma.dtype)
+        self.beta.grad = Tensor.create([self.num_features], self.beta.dtype)
+        return self.gamma.grad, self.beta.grad
+
+    def forward(self, x: Tensor) -> Tensor:
+        src = x.contiguous()
+        out = Tensor.create(x.shape, x.dtype)
+        mean, rstd = self._stats(src)
+        _check_error(_lib.neural_layer_norm_forward(out._ptr, src._ptr, self.gamma._ptr, self.beta._ptr, self.eps,
+                                                    mean._ptr, rstd._ptr), "layer norm forward")
+        self._saved = (src, mean, rstd)
+        return out
+
+    def backward(self, grad_output: Tensor) -> Tensor:
+        if self._saved is None:
+            raise RuntimeError("LayerNorm.backward called before forward")
+        x, mean, rstd = self._saved
+        go = grad_output.contiguous()
+        gi = Tensor.create(x.shape, x.dtype)
+        dgamma, dbeta = self._grads()
+        _check_error(_lib.neural_layer_norm_backward(gi._ptr, dgamma._ptr, dbeta._ptr, go._ptr, x._ptr,
+                                                     self.gamma._ptr, mean._ptr, rstd._ptr), "layer norm backward")
+        return gi
+
+    def __repr__(self) -> str:
+        return f"LayerNorm({self.num_features}, eps={self.eps})"
+
+
+class DropoutAddLayerNorm(LayerNorm):
+    """The end of a transformer's sublayer in one pass: hidden = residual +
+    dropout(x), out = norm(hidden) (neural_dropout_add_layer_norm_forward);
+    dropout as CounterDropout's, none in eval mode.  ``forward`` returns (out,
+    hidden): a block that normalises first hands ``hidden`` on as its residual
+    stream.  ``backward`` takes the gradients of both (that of hidden may be None) and
+    returns those of x and residual."""
+
+    def __init__(self, num_features: int, p: float = 0.1, eps: float = 1e-5, dtype: int = NeuralDtype.FLOAT32,
+                 seed: int = 0, offset: int = 0):
+        super().__init__(num_features, eps, dtype)
+        self.dropout = CounterDropout(p, seed, offset)
+
+    def train(self, mode: bool = True):
+        self.dropout.train(mode)
+        return super().train(mode)
+
+    def forward(self, x: Tensor, residual: Tensor):
+        src, res = x.contiguous(), residual.contiguous()
+        mean, rstd = self._stats(src)
+        out, hidden = Tensor.create(x.shape, x.dtype), Tensor.create(x.shape, x.dtype)
+        p, key = self.dropout._next()
+        rc = _lib.neural_dropout_add_layer_norm_forward(out._ptr, hidden._ptr, src._ptr, res._ptr, self.gamma._ptr,
+                                                        self.beta._ptr, p, ctypes.byref(key), self.eps, mean._ptr,
+                                                        rstd._ptr)
+        _check_error(rc, "dropout + add + layer norm forward")
+        self.dropout._took()
+        self._saved = (hidden, mean, rstd)
+        return out, hidden
+
+    def backward(self, grad_output: Tensor, grad_hidden: Tensor = None):
+        if self._saved is None:
+            raise RuntimeError("DropoutAddLayerNorm.backward called before forward")
+        hidden, mean, rstd = self._saved
+        go = grad_output.contiguous()
+        gh = grad_hidden.contiguous() if grad_hidden is not None else None
+        gi, gr = Tensor.create(hidden.shape, hidden.dtype), Tensor.create(hidden.shape, hidden.dtype)
+        dgamma, dbeta = self._grads()
+        p, key = self.dropout._last
+        rc = _lib.neural_dropout_add_layer_norm_backward(gi._ptr, gr._ptr, dgamma._ptr, dbeta._ptr, go._ptr,
+                                                         gh._ptr if gh is not None else None, hidden._ptr,
+                                                         self.gamma._ptr, mean._ptr, rstd._ptr, p, ctypes.byref(key))
+        _check_error(rc, "dropout + add + layer norm backward")
+        return gi, gr
+
+    def __repr__(self) -> str:
+        return f"DropoutAddLayerNorm({self.num_features}, p={self.dropout.p}, eps={self.eps})"
 
 
 def add_relu(a: Tensor, b: Tensor) -> Tensor:

@@ -1,0 +1,633 @@
+"""Layer norm and its join with dropout and the residual add, forward and
+backward, against long double forms of the definitions (tests/sublayer_ref.py)
+with bounds that count roundings: widths around every group size and past the
+registers, few and many rows, both dtypes, extreme rows, optional tensors, in
+place, any alignment, streams, graphs, and the refusals."""
+
+import ctypes
+
+import numpy as np
+import pytest
+
+import sublayer_ref as ref
+from conftest import GPU, same_bits
+
+pytestmark = GPU
+
+DT = [np.float32, np.float64]
+EPS = 1e-5
+# group sizes end at these widths (f32, f64 half): 16 / 64 / 128 / 256 / 512 / 1024 / 2048 / ... values
+COLS = [1, 2, 3, 4, 5, 7, 8, 9, 15, 16, 17, 19, 20, 31, 33, 64, 65, 67, 96, 127, 128, 130, 197, 255, 256, 257, 260, 511,
+        512, 514, 520, 577, 768, 1001, 1023, 1024, 1025, 1028, 1032, 2047, 2048, 2049, 2056, 4095, 4096, 4097, 4104,
+        8191, 8192, 8193, 8200, 16384, 16385, 16392]
+WIDE = [32767, 32768, 32769, 32776, 65536, 65539, 65544, 70001]
+
+
+def _key(pn, seed, offset):
+    return ctypes.byref(pn.core.DropoutKeyC(seed, offset))
+
+
+def _p(t):
+    return t._ptr if t is not None else None
+
+
+def _rows(rng, rows, cols, dt):
+    x = rng.normal(0.5, 1.5, (rows, cols))
+    x[:, rng.integers(0, cols, 1 + cols // 200)] *= 20
+    return x.astype(dt)
+
+
+def _case(rng, rows, cols, dt):
+    return {"x": _rows(rng, rows, cols, dt), "res": rng.normal(0, 2, (rows, cols)).astype(dt),
+            "g": rng.normal(1, 0.3, cols).astype(dt), "b": rng.normal(0, 0.5, cols).astype(dt),
+            "dy": rng.normal(0, 1, (rows, cols)).astype(dt), "dh": rng.normal(0, 1, (rows, cols)).astype(dt)}
+
+
+def _forward(pn, x, g, b, eps=EPS):
+    T = pn.Tensor
+    tx, tg, tb = T.from_numpy(x), None if g is None else T.from_numpy(g), None if b is None else T.from_numpy(b)
+    R = int(np.prod(x.shape[:-1]))
+    y, mean, rstd = T.create(x.shape, tx.dtype), T.create([R], tx.dtype), T.create([R], tx.dtype)
+    assert pn.core._lib.neural_layer_norm_forward(y._ptr, tx._ptr, _p(tg), _p(tb), eps, mean._ptr, rstd._ptr) == 0
+    return y.numpy(), mean.numpy(), rstd.numpy()
+
+
+def _backward(pn, dy, x, g, mean, rstd, want=("dx", "dg", "db")):
+    T = pn.Tensor
+    t = [T.from_numpy(v) if v is not None else None for v in (dy, x, g, mean, rstd)]
+    C = x.shape[-1]
+    outs = {"dx": T.create(x.shape, t[1].dtype), "dg": T.create([C], t[1].dtype), "db": T.create([C], t[1].dtype)}
+    o = [outs[k]._ptr if k in want else None for k in ("dx", "dg", "db")]
+    assert pn.core._lib.neural_layer_norm_backward(*o, *[_p(v) for v in t]) == 0
+    return [outs[k].numpy() if k in want else None for k in ("dx", "dg", "db")]
+
+
+def _joined(pn, c, p, key, eps=EPS, hidden=True):
+    T = pn.Tensor
+    x, res, g, b = (T.from_numpy(c[k]) for k in ("x", "res", "g", "b"))
+    R = c["x"].size // c["x"].shape[-1]
+    y, h = T.create(c["x"].shape, x.dtype), T.create(c["x"].shape, x.dtype) if hidden else None
+    mean, rstd = T.create([R], x.dtype), T.create([R], x.dtype)
+    assert pn.core._lib.neural_dropout_add_layer_norm_forward(y._ptr, _p(h), x._ptr, res._ptr, g._ptr, b._ptr, p,
+                                                              key, eps, mean._ptr, rstd._ptr) == 0
+    return y.numpy(), h.numpy() if hidden else None, mean.numpy(), rstd.numpy()
+
+
+def _joined_grad(pn, c, h, mean, rstd, p, key, with_dh=True):
+    T = pn.Tensor
+    dy, dh, th, g, m, r = (T.from_numpy(v) for v in (c["dy"], c["dh"], h, c["g"], mean, rstd))
+    C = h.shape[-1]
+    dx, dres = T.create(h.shape, th.dtype), T.create(h.shape, th.dtype)
+    dg, db = T.create([C], th.dtype), T.create([C], th.dtype)
+    assert pn.core._lib.neural_dropout_add_layer_norm_backward(
+        dx._ptr, dres._ptr, dg._ptr, db._ptr, dy._ptr, dh._ptr if with_dh else None, th._ptr, g._ptr, m._ptr, r._ptr,
+        p, key) == 0
+    return dx.numpy(), dres.numpy(), dg.numpy(), db.numpy()
+
+
+def _check_forward(pn, x, g, b, eps=EPS):
+    got = _forward(pn, x, g, b, eps)
+    want, bound = ref.norm(x.reshape(-1, x.shape[-1]), g, b, eps)
+    for name, o, w, lim in zip(("y", "mean", "rstd"), got, want, bound):
+        ref.within(o.reshape(w.shape), w, lim, name)
+    return got
+
+
+def _check_all(pn, rng, rows, cols, dt, p=0.2):
+    """Every form at one size: the stand-alone calls against the definitions, the
+    joined ones against the stand-alone calls, bit for bit."""
+    c = _case(rng, rows, cols, dt)
+    _, mean, rstd = _check_forward(pn, c["x"], c["g"], c["b"])
+    got = _backward(pn, c["dy"], c["x"], c["g"], mean, rstd)
+    want, bound = ref.norm_grad(c["dy"], c["x"], c["g"], mean, rstd, parts=rows)
+    for name, o, w, lim in zip(("dx", "dgamma", "dbeta"), got, want, bound):
+        ref.within(o, w, lim, name)
+    # only the input's gradient, and only the sums: the same bits
+    same_bits(_backward(pn, c["dy"], c["x"], c["g"], mean, rstd, ("dx",))[0], got[0])
+    only = _backward(pn, c["dy"], c["x"], c["g"], mean, rstd, ("dg", "db"))
+    same_bits(only[1], got[1])
+    same_bits(only[2], got[2])
+    for q in (p, 0.0):
+        key = _key(pn, 5, cols)
+        h = c["res"] + (ref.dropout(c["x"], q, 5, cols) if q else c["x"])
+        y, hg, m, r = _joined(pn, c, q, key if q else None)
+        same_bits(hg, h)
+        for o, w in zip((y, m, r), _forward(pn, h, c["g"], c["b"])):
+            same_bits(o, w)
+        same_bits(_joined(pn, c, q, key, hidden=False)[0], y)
+        dx, dres, dg, db = _joined_grad(pn, c, h, m, r, q, key)
+        sx, sg, sb = _backward(pn, c["dy"], h, c["g"], m, r)
+        same_bits(dres, sx + c["dh"])
+        same_bits(dx, ref.dropout(dres, q, 5, cols) if q else dres)
+        same_bits(dg, sg)
+        same_bits(db, sb)
+        dx, dres, dg, db = _joined_grad(pn, c, h, m, r, q, key, with_dh=False)
+        same_bits(dres, sx)
+        same_bits(dx, ref.dropout(sx, q, 5, cols) if q else sx)
+
+
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("cols", COLS)
+def test_widths(pn, rng, dt, cols):
+    _check_all(pn, rng, 5 if cols > 64 else 131, cols, dt)
+
+
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("cols", WIDE)
+def test_wide_rows(pn, rng, dt, cols):
+    _check_all(pn, rng, 3, cols, dt)
+
+
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("rows,cols", [(1, 1), (1, 768), (2, 4096), (70000, 5), (40000, 16), (20011, 40), (9001, 100),
+                                       (5000, 260), (4500, 520), (2100, 1030), (1300, 2100), (1100, 4099)])
+def test_row_counts(pn, rng, dt, rows, cols):
+    """One row, and more rows than the backward pass has groups of lanes."""
+    _check_all(pn, rng, rows, cols, dt)
+
+
+@pytest.mark.parametrize("dt", DT)
+def test_optional_tensors(pn, rng, dt):
+    """gamma or beta of ones / zeros and none give the same bits; statistics
+    may be left out; leading dimensions do not matter."""
+    lib, T = pn.core._lib, pn.Tensor
+    x = _rows(rng, 24, 130, dt)
+    one, zero = np.ones(130, dt), np.zeros(130, dt)
+    y, mean, rstd = _check_forward(pn, x, None, None)
+    for g, b in ((one, zero), (None, zero), (one, None)):
+        same_bits(_forward(pn, x, g, b)[0], y)
+    tx, ty = T.from_numpy(x.reshape(2, 3, 4, 130)), T.create([2, 3, 4, 130], T.from_numpy(x).dtype)
+    assert lib.neural_layer_norm_forward(ty._ptr, tx._ptr, None, None, EPS, None, None) == 0
+    same_bits(ty.numpy().reshape(24, 130), y)
+    dy = rng.normal(0, 1, x.shape).astype(dt)
+    for a, w in zip(_backward(pn, dy, x, None, mean, rstd), _backward(pn, dy, x, one, mean, rstd)):
+        same_bits(a, w)
+    v = T.from_numpy(x[0].copy())  # a rank-1 tensor is one row
+    o = T.create([130], v.dtype)
+    assert lib.neural_layer_norm_forward(o._ptr, v._ptr, None, None, EPS, None, None) == 0
+    same_bits(o.numpy(), y[0])
+
+
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("cols", [24, 300, 2050, 70001])
+def test_extreme_rows(pn, rng, dt, cols):
+    """Rows of one value, of a value far from their spread, of the largest and
+    of subnormal values; eps of 0 and large."""
+    x = _rows(rng, 12, cols, dt)
+    x[0] = 3.25
+    x[1] = 0.0
+    x[2] = 1e6 + rng.normal(0, 1, cols)
+    x[3] = -3e38 if dt == np.float32 else -1e150
+    x[4] = (3e38 if dt == np.float32 else 1e150) * np.where(np.arange(cols) % 2, 1, -1)
+    x[5] = 1e-42 * rng.normal(0, 1, cols)
+    x[6] = 1e-20
+    x[6, 0] = 1e20
+    for eps in (EPS, 1e-12, 100.0):
+        _check_forward(pn, x, None, None, eps)
+    varied = x[7:]
+    _check_forward(pn, varied, None, None, 0.0)
+    # a constant row and eps = 0: (x - mean) / 0 = 0 / 0 where the mean is exact
+    y = _forward(pn, np.full((2, 16), 3.0, dt), None, None, 0.0)
+    assert np.isnan(y[0]).all() and np.isinf(y[2]).all() and (y[1] == 3.0).all()
+
+
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("cols", [10, 100, 777, 5000, 70001])
+def test_nan_and_infinity_stay_in_their_rows(pn, rng, dt, cols):
+    x = _rows(rng, 9, cols, dt)
+    clean = _forward(pn, x, None, None)
+    x[1, cols // 2] = np.nan
+    x[4, 0] = np.inf
+    x[7, cols - 1] = -np.inf
+    y, mean, rstd = _forward(pn, x, None, None)
+    bad = [1, 4, 7]
+    assert np.isnan(y[bad]).all() and np.isnan(rstd[bad]).all()
+    assert np.isnan(mean[1]) and mean[4] == np.inf and mean[7] == -np.inf
+    good = [0, 2, 3, 5, 6, 8]
+    for a, b in zip((y, mean, rstd), clean):
+        same_bits(a[good], b[good])
+    # dropped in the joined form, they are not there
+    c = _case(rng, 4, cols, dt)
+    keep = ref.keep(4 * cols, 0.5, 1, 2).reshape(4, cols)
+    c["x"][~keep] = np.nan
+    got = _joined(pn, c, 0.5, _key(pn, 1, 2))
+    c["x"][~keep] = 0.0
+    for a, b in zip(got, _joined(pn, c, 0.5, _key(pn, 1, 2))):
+        same_bits(a, b)
+    assert np.isfinite(got[0]).all()
+
+
+def _numeric(f, x, at, step):
+    lo, hi = x.copy(), x.copy()
+    lo.reshape(-1)[at] -= step
+    hi.reshape(-1)[at] += step
+    return (f(hi) - f(lo)) / (hi.reshape(-1)[at] - lo.reshape(-1)[at])
+
+
+def test_gradients_by_differences(pn, rng):
+    """f64: the joined form's gradients against central differences of a
+    weighted sum of both its outputs.  The difference is off by step^2 / 6 times
+    the third derivative (of order 10 here) and by roundings of the sum (of size
+    1e2, D each) over the step: 1e-4 gives 2e-8 and 1e-9, held to 1e-6."""
+    rows, cols, p = 3, 21, 0.3
+    c = _case(rng, rows, cols, np.float64)
+    c["x"] = rng.normal(0, 1, (rows, cols))
+    key = _key(pn, 9, 9)
+
+    def loss(**kw):
+        y, h, _, _ = _joined(pn, {**c, **kw}, p, key)
+        return float((y * c["dy"]).sum() + (h * c["dh"]).sum())
+
+    _, h, mean, rstd = _joined(pn, c, p, key)
+    dx, dres, dg, db = _joined_grad(pn, c, h, mean, rstd, p, key)
+    for name, grad in (("x", dx), ("res", dres), ("g", dg), ("b", db)):
+        for at in rng.choice(c[name].size, min(12, c[name].size), replace=False):
+            d = _numeric(lambda v: loss(**{name: v}), c[name], at, 1e-4)
+            assert abs(d - grad.reshape(-1)[at]) <= 1e-6 * max(1.0, abs(d)), (name, at, d, grad.reshape(-1)[at])
+
+
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("cols", [30, 64, 1001, 2048, 5000, 40000, 70001])
+def test_in_place(pn, rng, dt, cols):
+    """Outputs over the inputs they may replace: the same bits."""
+    lib, T = pn.core._lib, pn.Tensor
+    c = _case(rng, 6, cols, dt)
+    key = _key(pn, 3, 3)
+    want = _forward(pn, c["x"], c["g"], c["b"])
+    g, b = T.from_numpy(c["g"]), T.from_numpy(c["b"])
+    x = T.from_numpy(c["x"])
+    assert lib.neural_layer_norm_forward(x._ptr, x._ptr, g._ptr, b._ptr, EPS, None, None) == 0
+    same_bits(x.numpy(), want[0])
+    grads = _backward(pn, c["dy"], c["x"], c["g"], want[1], want[2])
+    m, r = T.from_numpy(want[1]), T.from_numpy(want[2])
+    for over in ("dy", "x"):
+        t = {k: T.from_numpy(c[k]) for k in ("dy", "x")}
+        dg, db = T.create([cols], g.dtype), T.create([cols], g.dtype)
+        assert lib.neural_layer_norm_backward(t[over]._ptr, dg._ptr, db._ptr, t["dy"]._ptr, t["x"]._ptr, g._ptr,
+                                              m._ptr, r._ptr) == 0
+        for o, w in zip((t[over], dg, db), grads):
+            same_bits(o.numpy(), w)
+    y, h, hm, hr = _joined(pn, c, 0.3, key)
+    for out_over, hid_over in (("x", "res"), ("res", "x"), ("x", None), ("res", None), (None, "res"), (None, "x")):
+        t = {k: T.from_numpy(c[k]) for k in ("x", "res")}
+        out = t[out_over] if out_over else T.create(c["x"].shape, g.dtype)
+        hid = t[hid_over] if hid_over else None
+        assert lib.neural_dropout_add_layer_norm_forward(out._ptr, _p(hid), t["x"]._ptr, t["res"]._ptr, g._ptr,
+                                                         b._ptr, 0.3, key, EPS, None, None) == 0
+        same_bits(out.numpy(), y)
+        if hid is not None:
+            same_bits(hid.numpy(), h)
+    dx, dres, dg, db = _joined_grad(pn, c, h, hm, hr, 0.3, key)
+    m, r = T.from_numpy(hm), T.from_numpy(hr)
+    for dx_over, dres_over in (("dy", "dh"), ("dh", "dy"), ("h", "dh"), ("dh", "h"), ("dy", "h")):
+        t = {"dy": T.from_numpy(c["dy"]), "dh": T.from_numpy(c["dh"]), "h": T.from_numpy(h)}
+        tg, tb = T.create([cols], g.dtype), T.create([cols], g.dtype)
+        assert lib.neural_dropout_add_layer_norm_backward(t[dx_over]._ptr, t[dres_over]._ptr, tg._ptr, tb._ptr,
+                                                          t["dy"]._ptr, t["dh"]._ptr, t["h"]._ptr, g._ptr, m._ptr,
+                                                          r._ptr, 0.3, key) == 0
+        for o, w in zip((t[dx_over], t[dres_over], tg, tb), (dx, dres, dg, db)):
+            same_bits(o.numpy(), w)
+
+
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("cols", [7, 96, 513, 1024, 3001, 9000, 70001])
+@pytest.mark.parametrize("shift", [0, 1, 3])
+def test_alignment_and_guards(pn, rng, dt, cols, shift):
+    """Buffers that start anywhere give the bits of aligned ones, and nothing
+    around the outputs is written."""
+    import torch
+    rows = 7
+    c = _case(rng, rows, cols, dt)
+    key = _key(pn, 2, 8)
+    y, h, mean, rstd = _joined(pn, c, 0.1, key)
+    grads = _joined_grad(pn, c, h, mean, rstd, 0.1, key)
+    tdt = torch.float32 if dt == np.float32 else torch.float64
+    held = []
+
+    def placed(v):
+        big = torch.full((v.size + 64,), 5.0, dtype=tdt, device="cuda")
+        view = big[16 + shift:16 + shift + v.size].view(v.shape)
+        view.copy_(torch.from_numpy(v))
+        held.append((big, view, v.size))
+        return pn.Tensor.from_torch(view), view
+
+    def check(view, want):
+        same_bits(view.cpu().numpy(), want)
+
+    ins = {k: placed(v) for k, v in {**c, "h": h, "mean": mean, "rstd": rstd}.items()}
+    outs = {k: placed(np.zeros_like(v)) for k, v in {"y": y, "oh": h, "om": mean, "or": rstd, "dx": grads[0],
+                                                     "dres": grads[1], "dg": grads[2], "db": grads[3]}.items()}
+    P = lambda k: (outs.get(k) or ins.get(k))[0]._ptr  # noqa: E731
+    torch.cuda.synchronize()
+    lib = pn.core._lib
+    assert lib.neural_dropout_add_layer_norm_forward(P("y"), P("oh"), P("x"), P("res"), P("g"), P("b"), 0.1, key, EPS,
+                                                     P("om"), P("or")) == 0
+    assert lib.neural_dropout_add_layer_norm_backward(P("dx"), P("dres"), P("dg"), P("db"), P("dy"), P("dh"), P("h"),
+                                                      P("g"), P("mean"), P("rstd"), 0.1, key) == 0
+    pn.synchronize()
+    for k, want in zip(("y", "oh", "om", "or", "dx", "dres", "dg", "db"), (y, h, mean, rstd, *grads)):
+        check(outs[k][1], want)
+    for big, view, n in held:
+        assert bool((big[:16 + shift] == 5).all()) and bool((big[16 + shift + n:] == 5).all())
+
+
+def test_equal_calls_equal_bits(pn, rng):
+    for rows, cols in ((5000, 96), (3000, 768), (700, 5001)):
+        c = _case(rng, rows, cols, np.float32)
+        _, mean, rstd = _forward(pn, c["x"], c["g"], c["b"])
+        first = _backward(pn, c["dy"], c["x"], c["g"], mean, rstd)
+        for _ in range(3):
+            for a, w in zip(_backward(pn, c["dy"], c["x"], c["g"], mean, rstd), first):
+                same_bits(a, w)
+
+
+def test_host_buffers(pn, rng):
+    """Tensors over host memory: written back by each call."""
+    c = _case(rng, 11, 100, np.float32)
+    want = _forward(pn, c["x"], c["g"], c["b"])
+    y, mean, rstd = np.zeros_like(c["x"]), np.zeros(11, np.float32), np.zeros(11, np.float32)
+    Z = pn.Tensor.from_numpy_zero_copy
+    t = [Z(v) for v in (y, c["x"], c["g"], c["b"], mean, rstd)]
+    assert pn.core._lib.neural_layer_norm_forward(t[0]._ptr, t[1]._ptr, t[2]._ptr, t[3]._ptr, EPS, t[4]._ptr,
+                                                  t[5]._ptr) == 0
+    for a, w in zip((y, mean, rstd), want):
+        same_bits(a, w)
+
+
+def test_empty(pn):
+    lib, T = pn.core._lib, pn.Tensor
+    x, g, m = T.create([0, 5]), T.ones([5]), T.create([0])
+    assert lib.neural_layer_norm_forward(x._ptr, x._ptr, g._ptr, g._ptr, EPS, m._ptr, None) == 0
+    dg, db = T.ones([5]), T.ones([5])
+    assert lib.neural_layer_norm_backward(x._ptr, dg._ptr, db._ptr, x._ptr, x._ptr, g._ptr, m._ptr, m._ptr) == 0
+    assert not dg.numpy().any() and not db.numpy().any()  # sums over no rows
+    e = T.create([5, 0])
+    z = T.create([0])
+    assert lib.neural_layer_norm_forward(e._ptr, e._ptr, z._ptr, z._ptr, EPS, None, None) == 0
+    assert lib.neural_layer_norm_backward(e._ptr, None, None, e._ptr, e._ptr, None, z._ptr, z._ptr) == 0
+
+
+def test_refusals(pn):
+    import torch
+    E, lib, T = pn.NeuralError, pn.core._lib, pn.Tensor
+    f, k = lib.neural_layer_norm_forward, lib.neural_layer_norm_backward
+    jf, jk = lib.neural_dropout_add_layer_norm_forward, lib.neural_dropout_add_layer_norm_backward
+    x, y, z = T.zeros([4, 6]), T.zeros([4, 6]), T.zeros([4, 6])
+    g, b, m, r = T.ones([6]), T.ones([6]), T.zeros([4]), T.zeros([4])
+    X, Y, Z, G, B, M, R = (t._ptr for t in (x, y, z, g, b, m, r))
+    key = _key(pn, 0, 0)
+    assert f(None, X, G, B, EPS, M, R) == E.NULL_POINTER
+    assert f(Y, None, G, B, EPS, M, R) == E.NULL_POINTER
+    assert jf(Y, Z, X, None, G, B, 0.0, None, EPS, M, R) == E.NULL_POINTER
+    w = T.zeros([4, 6])
+    W = w._ptr
+    assert jf(Y, Z, X, W, G, B, 0.5, None, EPS, M, R) == E.NULL_POINTER  # no key
+    assert k(None, None, None, Y, X, G, M, R) == E.NULL_POINTER
+    assert k(Z, None, None, None, X, G, M, R) == E.NULL_POINTER
+    assert k(Z, None, None, Y, X, G, None, R) == E.NULL_POINTER
+    assert k(Z, None, None, Y, X, G, M, None) == E.NULL_POINTER
+    d6, d46 = T.ones([6], pn.float64), T.zeros([4, 6], pn.float64)
+    assert f(d46._ptr, X, G, B, EPS, M, R) == E.DTYPE_MISMATCH
+    assert f(Y, X, d6._ptr, B, EPS, M, R) == E.DTYPE_MISMATCH
+    assert k(Z, d6._ptr, None, Y, X, G, M, R) == E.DTYPE_MISMATCH
+    s5, s46, s24 = T.ones([5]), T.zeros([6, 4]), T.zeros([24])
+    assert f(Y, X, s5._ptr, B, EPS, M, R) == E.SHAPE_MISMATCH
+    assert f(Y, X, G, s5._ptr, EPS, M, R) == E.SHAPE_MISMATCH
+    assert f(Y, X, G, B, EPS, s5._ptr, R) == E.SHAPE_MISMATCH
+    assert f(s46._ptr, X, G, B, EPS, M, R) == E.SHAPE_MISMATCH
+    assert f(s24._ptr, X, G, B, EPS, M, R) == E.SHAPE_MISMATCH
+    assert k(Z, s5._ptr, None, Y, X, G, M, R) == E.SHAPE_MISMATCH
+    assert k(Z, None, None, s46._ptr, X, G, M, R) == E.SHAPE_MISMATCH
+    s0, s0b = T.create([]), T.create([])
+    assert f(s0b._ptr, s0._ptr, None, None, EPS, None, None) == E.DIM_MISMATCH
+    for eps in (-1e-9, float("nan"), float("inf")):
+        assert f(Y, X, G, B, eps, M, R) == E.INVALID_ARGUMENT
+    for p in (-0.1, 1.1, float("nan")):
+        assert jf(Y, Z, X, W, G, B, p, key, EPS, M, R) == E.INVALID_ARGUMENT
+        assert jk(Z, None, None, None, Y, None, X, G, M, R, p, key) == E.INVALID_ARGUMENT
+    t = torch.zeros(8, 6, device="cuda")
+    strided, lower, upper = (T.from_torch(v) for v in (t[::2], t[:4], t[2:6]))
+    assert f(strided._ptr, X, G, B, EPS, M, R) == E.INVALID_ARGUMENT
+    assert f(Y, strided._ptr, G, B, EPS, M, R) == E.INVALID_ARGUMENT
+    assert f(upper._ptr, lower._ptr, G, B, EPS, M, R) == E.INVALID_ARGUMENT   # overlap, not in place
+    assert f(Y, X, G, B, EPS, M, M) == E.INVALID_ARGUMENT                     # one tensor, two outputs
+    assert jf(Y, Y, X, W, G, B, 0.0, None, EPS, M, R) == E.INVALID_ARGUMENT
+    assert jk(Z, Z, None, None, Y, None, X, G, M, R, 0.5, key) == E.INVALID_ARGUMENT
+    assert k(Z, G, None, Y, X, G, M, R) == E.INVALID_ARGUMENT                 # grad_gamma over gamma
+    row = T.from_torch(t[0])
+    assert k(Z, None, row._ptr, Y, lower._ptr, G, M, R) == E.INVALID_ARGUMENT  # grad_beta inside the input
+    for v in (y, z):
+        assert not v.numpy().any()
+    same_bits(g.numpy(), np.ones(6, np.float32))
+
+
+def _graph_of(torch, stream, calls):
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        calls()
+    return graph
+
+
+def test_graph_replays(pn, rng):
+    """A captured step (joined forward, backward, with a key in device memory that the
+    graph itself advances), replayed with the program's own calls in between;
+    a second graph of the same calls, replayed on another stream at the same
+    time, shares no workspace with it."""
+    import torch
+    lib, T = pn.core._lib, pn.Tensor
+    rows, cols, p = 700, 1030, 0.2
+    s = [torch.cuda.Stream(), torch.cuda.Stream()]
+    sides = []
+    try:
+        for i in range(2):
+            c = _case(rng, rows, cols, np.float32)
+            t = {k: torch.from_numpy(v).cuda() for k, v in c.items()}
+            for k, n in (("y", None), ("h", None), ("dx", None), ("dres", None), ("m", rows), ("r", rows),
+                         ("dg", cols), ("db", cols)):
+                t[k] = torch.zeros(n if n else (rows, cols), device="cuda")
+            t["key"] = torch.tensor([i, 0], dtype=torch.int64, device="cuda")
+            w = {k: T.from_torch(v) for k, v in t.items() if k != "key"}
+            pn.set_stream(s[i].cuda_stream)
+            torch.cuda.synchronize()
+
+            def step(t=t, w=w):
+                P = lambda k: w[k]._ptr  # noqa: E731
+                key = t["key"].data_ptr()
+                assert lib.neural_dropout_add_layer_norm_forward(P("y"), P("h"), P("x"), P("res"), P("g"), P("b"), p,
+                                                                 key, EPS, P("m"), P("r")) == 0
+                assert lib.neural_dropout_add_layer_norm_backward(P("dx"), P("dres"), P("dg"), P("db"), P("dy"),
+                                                                  P("dh"), P("h"), P("g"), P("m"), P("r"), p, key) == 0
+                t["key"][1] += 1
+
+            sides.append((c, t, w, _graph_of(torch, s[i], step)))
+        pn.set_stream(None)
+        torch.cuda.synchronize()
+        for replay in range(4):
+            for i, (c, t, w, graph) in enumerate(sides):  # both at once
+                with torch.cuda.stream(s[i]):
+                    graph.replay()
+            torch.cuda.synchronize()
+            for i, (c, t, w, graph) in enumerate(sides):
+                key = _key(pn, i, replay)
+                y, h, m, r = _joined(pn, c, p, key)  # the program's own calls, which use the cached workspace
+                grads = _joined_grad(pn, c, h, m, r, p, key)
+                for k, v in zip(("y", "h", "m", "r", "dx", "dres", "dg", "db"), (y, h, m, r, *grads)):
+                    same_bits(t[k].cpu().numpy(), v)
+                    t[k].fill_(9.0)
+            lib.neural_hip_empty_cache()
+            torch.cuda.synchronize()
+    finally:
+        pn.set_stream(None)
+
+
+def test_other_stream(pn, rng):
+    """On a stream of the caller's, behind work that is still running there."""
+    import torch
+    c = _case(rng, 300, 1500, np.float32)
+    want = _forward(pn, c["x"], c["g"], c["b"])
+    s = torch.cuda.Stream()
+    try:
+        with torch.cuda.stream(s):
+            x = torch.zeros(300, 1500, device="cuda")
+            big = torch.randn(4096, 4096, device="cuda")
+            y = torch.empty_like(x)
+            g, b, src = (torch.from_numpy(c[k]).cuda() for k in ("g", "b", "x"))
+            T = pn.Tensor.from_torch
+            X, Y, Gm, Bt = T(x), T(y), T(g), T(b)
+            pn.set_stream(s.cuda_stream)
+            for _ in range(10):
+                big = big @ big * 1e-3
+            x.copy_(src)
+            assert pn.core._lib.neural_layer_norm_forward(Y._ptr, X._ptr, Gm._ptr, Bt._ptr, EPS, None, None) == 0
+            z = y + 0
+        s.synchronize()
+        same_bits(z.cpu().numpy(), want[0])
+    finally:
+        pn.set_stream(None)
+
+
+def test_threads(pn, rng):
+    """Backward calls from several host threads at once: each its own workspace."""
+    import threading
+    cases = [_case(rng, 400 + 100 * i, 700 + 300 * i, np.float32) for i in range(4)]
+    want = []
+    for c in cases:
+        _, m, r = _forward(pn, c["x"], c["g"], c["b"])
+        want.append((m, r, _backward(pn, c["dy"], c["x"], c["g"], m, r)))
+    bad = []
+
+    def work(i):
+        m, r, w = want[i]
+        for _ in range(5):
+            got = _backward(pn, cases[i]["dy"], cases[i]["x"], cases[i]["g"], m, r)
+            if not all(np.array_equal(a, b) for a, b in zip(got, w)):
+                bad.append(i)
+
+    ts = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    [t.start() for t in ts]
+    [t.join() for t in ts]
+    assert not bad
+
+
+def test_many_elements(pn):
+    """More than 2^32 elements: the last rows, and the sums over all of them.
+    Every row is the same, so dbeta is rows dy exactly, as are the rows' results."""
+    import torch
+    cols = 4096
+    rows = (1 << 20) + 3
+    need = 2 * 4 * rows * cols
+    torch.cuda.empty_cache()
+    pn.core._lib.neural_hip_empty_cache()
+    if torch.cuda.mem_get_info()[0] < need + (4 << 30):
+        pytest.skip("not enough free device memory")
+    lib, T = pn.core._lib, pn.Tensor
+    one = torch.arange(cols, device="cuda", dtype=torch.float32) % 7 - 3
+    x = one.repeat(rows, 1)
+    dy = torch.full((rows, cols), 0.5, device="cuda")
+    m, r = torch.empty(rows, device="cuda"), torch.empty(rows, device="cuda")
+    dg, db = torch.empty(cols, device="cuda"), torch.empty(cols, device="cuda")
+    X, DY, M, R, DG, DB = (T.from_torch(v) for v in (x, dy, m, r, dg, db))
+    y0 = one.repeat(2, 1)
+    Y0 = T.from_torch(y0)
+    torch.cuda.synchronize()
+    assert lib.neural_layer_norm_forward(Y0._ptr, Y0._ptr, None, None, EPS, None, None) == 0
+    tail = x[-2:].clone()
+    torch.cuda.synchronize()
+    assert lib.neural_layer_norm_forward(X._ptr, X._ptr, None, None, EPS, M._ptr, R._ptr) == 0
+    pn.synchronize()
+    assert torch.equal(x[-2:], y0) and torch.equal(x[:2], y0) and not torch.equal(x[-2:], tail)
+    assert bool((m == m[0]).all()) and bool((r == r[0]).all())
+    M0, R1 = torch.zeros_like(m), torch.ones_like(r)
+    Z, O = T.from_torch(M0), T.from_torch(R1)
+    torch.cuda.synchronize()
+    assert lib.neural_layer_norm_backward(DY._ptr, DG._ptr, DB._ptr, DY._ptr, X._ptr, None, Z._ptr, O._ptr) == 0
+    pn.synchronize()
+    # dy = 1/2 (rows is odd and under 2^24): exact in f32 up to the last rounding
+    assert bool((db == rows * 0.5).all())
+    want = y0[0].double() * (rows * 0.5)
+    assert bool(((dg.double() - want).abs() <= 2.0 ** -22 * want.abs()).all())
+    assert torch.equal(dy[-1], dy[0]) and torch.equal(dy[rows // 2], dy[0]) and not bool((dy[0] == 0.5).all())
+    del X, DY, x, dy
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("dt", DT)
+def test_modules_train_together(pn, rng, dt):
+    """Two sublayers' ends as a program has them (normalise, dropout, join), forward
+    and backward through the modules, against the same chain of long double
+    forms.  Each f32 stage rounds once, and the stages' condition here is
+    below 50: 4 stages of 2^-24, times 50, times the largest value."""
+    code = pn.float32 if dt == np.float32 else pn.float64
+    rows, cols = 60, 190
+    x, r0 = _rows(rng, rows, cols, dt), rng.normal(0, 1, (rows, cols)).astype(dt)
+    pre, drop, end = pn.LayerNorm(cols, dtype=code), pn.CounterDropout(0.1, 3), pn.DropoutAddLayerNorm(
+        cols, 0.2, dtype=code, seed=4)
+    gam = {m: (rng.normal(1, 0.2, cols).astype(dt), rng.normal(0, 0.2, cols).astype(dt)) for m in (pre, end)}
+    for m, (g, b) in gam.items():
+        m.gamma, m.beta = pn.Tensor.from_numpy(g), pn.Tensor.from_numpy(b)
+    a = pre(pn.Tensor.from_numpy(x))
+    d = drop(a)
+    y, h = end(d, pn.Tensor.from_numpy(r0))
+    dy, dh = rng.normal(0, 1, (rows, cols)).astype(dt), rng.normal(0, 1, (rows, cols)).astype(dt)
+    gx, gr = end.backward(pn.Tensor.from_numpy(dy), pn.Tensor.from_numpy(dh))
+    dx = pre.backward(drop.backward(gx))
+    L = np.longdouble
+
+    def ln(v, g, b):
+        c = v - v.mean(-1, keepdims=True)
+        s = 1 / np.sqrt((c * c).mean(-1, keepdims=True) + L(EPS))
+        return c * s * g + b, c * s, s
+
+    def lnb(g_out, xh, s, g):
+        w = g_out * g
+        return s * (w - w.mean(-1, keepdims=True) - xh * (w * xh).mean(-1, keepdims=True))
+
+    (g1, b1), (g2, b2) = (tuple(v.astype(L) for v in gam[m]) for m in (pre, end))
+    la, xh1, s1 = ln(x.astype(L), g1, b1)
+    m1 = ref.keep(rows * cols, 0.1, 3, 0).reshape(rows, cols) / L(0.9)
+    m2 = ref.keep(rows * cols, 0.2, 4, 0).reshape(rows, cols) / L(0.8)
+    lh = r0.astype(L) + la * m1 * m2
+    ly, xh2, s2 = ln(lh, g2, b2)
+    lr = lnb(dy.astype(L), xh2, s2, g2) + dh
+    l1 = lr * m2 * m1
+    ldx = lnb(l1, xh1, s1, g1)
+    want = {"y": ly, "h": lh, "gr": lr, "dx": ldx, "dg2": (dy * xh2).sum(0), "db2": dy.astype(L).sum(0),
+            "dg1": (l1 * xh1).sum(0), "db1": l1.sum(0)}
+    got = {"y": y, "h": h, "gr": gr, "dx": dx, "dg2": end.gamma.grad, "db2": end.beta.grad, "dg1": pre.gamma.grad,
+           "db1": pre.beta.grad}
+    for k in want:
+        lim = 200 * ref.U[np.dtype(dt)] * np.abs(want[k]).max() * (rows if k[0] == "d" and k != "dx" else 1)
+        assert np.abs(got[k].numpy() - want[k]).max() <= lim, k
+    for m in (pre, drop, end):
+        m.eval()
+    y2, h2 = end(drop(a), pn.Tensor.from_numpy(r0))
+    same_bits(h2.numpy(), r0 + a.numpy())
+    same_bits(y2.numpy(), _forward(pn, h2.numpy(), *gam[end])[0])
+    # AdamW takes the parameters and the gradients the modules left
+    opt = pn.AdamW(learning_rate=1e-2)
+    ps = pre.parameters() + end.parameters()
+    before = [p.numpy() for p in ps]
+    opt.step(ps, [p.grad for p in ps])
+    assert all(not np.array_equal(b, p.numpy()) for b, p in zip(before, ps))
+    with pytest.raises(ValueError):
+        pre(pn.Tensor.zeros([3, cols + 1], code))
