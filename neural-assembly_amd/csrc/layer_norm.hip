@@ -38,6 +38,25 @@ NH_DEV double fresh(T v)
     return double(v);
 }
 
+// s / n from inv = 1 / n: the quotient corrected by its remainder, so that a row of one
+// value has exactly that mean (its sum is exact in double).  The remainder of an
+// infinity is NaN: it stays as it is.
+NH_DEV double over(double s, int64_t n, double inv)
+{
+    const double m = s * inv, c = __builtin_fma(__builtin_fma(-m, double(n), s), inv, m);
+    return c == c ? c : m;
+}
+
+// 1 / sqrt(v) from the hardware's estimate y and one third-order step: with e = 1 - v y^2,
+// y (1 + e / 2 + 3 e^2 / 8).  0, infinity and NaN take the estimate.
+NH_DEV double rsqrt_d(double v)
+{
+    const double y = __builtin_amdgcn_rsq(v);
+    const double e = __builtin_fma(-(v * y), y, 1.0);
+    const double r = __builtin_fma(y * e, __builtin_fma(e, 0.375, 0.5), y);
+    return v > 0.0 && v < __builtin_inf() ? r : y;
+}
+
 // ---- keep bits of a row's vectors ----------------------------------------------------------
 
 // Keep bits of the elements of a row that a lane holds.  Where the row's width is
@@ -56,20 +75,14 @@ struct RowKeep {
         tail = 0;
         if ((cols & 7) == 0) {
             const int64_t v0 = r * (cols / VN) + lane;
-            if constexpr (VPT < P) {
 #pragma unroll
-                for (int k = 0; k < VPT; k++)
-                    m[k] = keep_mask(uint64_t(v0 + k * NT) / P, key) >> ((8 / P / 2) * (lane & (P - 1)));
-            } else {
-#pragma unroll
-                for (int k0 = 0; k0 < VPT; k0 += P) {
-                    const uint32_t own = keep_mask(uint64_t(v0 + (k0 + (lane & (P - 1))) * NT) / P, key);
-                    m[k0] = mask_of<T, 0>(own, lane);
-                    if (k0 + 1 < VPT) m[k0 + 1] = mask_of<T, 1>(own, lane);
-                    if constexpr (P == 4) {
-                        if (k0 + 2 < VPT) m[k0 + 2] = mask_of<T, 2>(own, lane);
-                        if (k0 + 3 < VPT) m[k0 + 3] = mask_of<T, 3>(own, lane);
-                    }
+            for (int k0 = 0; k0 < VPT; k0 += P) {
+                const uint32_t own = keep_mask(uint64_t(v0 + (k0 + (lane & (P - 1))) * NT) / P, key);
+                m[k0] = mask_of<T, 0>(own, lane);
+                if (k0 + 1 < VPT) m[k0 + 1] = mask_of<T, 1>(own, lane);
+                if constexpr (P == 4) {
+                    if (k0 + 2 < VPT) m[k0 + 2] = mask_of<T, 2>(own, lane);
+                    if (k0 + 3 < VPT) m[k0 + 3] = mask_of<T, 3>(own, lane);
                 }
             }
             return;
@@ -109,9 +122,9 @@ struct LnArgs {
     DropArgs drop;
 };
 
-// One row per group of NT lanes, VPT vectors per lane and one scalar.  Bound by
-// HBM while enough rows are in flight.
-template <typename T, int NT, int VPT, int MODE>
+// One row per group of NT lanes, VPT vectors per lane, the first F of them whole, and
+// one scalar.  Bound by HBM while enough rows are in flight.
+template <typename T, int NT, int VPT, int F, int MODE>
 __global__ __launch_bounds__(NT < 256 ? 256 : NT) void k_ln_rows(LnArgs<T> a, int64_t r_base)
 {
     using V = typename Vec16<T>::type;
@@ -127,7 +140,7 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void k_ln_rows(LnArgs<T> a, in
     if (RPB > 1 && r >= a.rows) return;  // uniform per group; a block of one row has one
     const int64_t cols = a.cols;
     const RowCut<T> cut(cols);
-    const auto in_row = [&](int k) { return lane + k * NT < cut.ncv; };
+    const auto in_row = [&](int k) { return k < F || lane + k * NT < cut.ncv; };
     const bool has_t = lane < cut.rem;
     const int64_t at = r * cols;
     V v[VPT];
@@ -179,7 +192,8 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void k_ln_rows(LnArgs<T> a, in
             for (int j = 0; j < VN; j++) s += double(v[k][j]);
         }
     if (has_t) s += double(vt);
-    const double mean = G::sum(s, lds_s) / double(cols);
+    const double inv_c = 1.0 / double(cols);
+    const double mean = over(G::sum(s, lds_s), cols, inv_c);
     double q = 0.0;
 #pragma unroll
     for (int k = 0; k < VPT; k++)
@@ -194,7 +208,7 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void k_ln_rows(LnArgs<T> a, in
         const double d = double(vt) - mean;
         q = __builtin_fma(d, d, q);
     }
-    const double rstd = 1.0 / sqrt(G::sum(q, lds_q) / double(cols) + a.eps);
+    const double rstd = rsqrt_d(G::sum(q, lds_q) * inv_c + a.eps);
     if (lane == 0) {
         if (a.mean) a.mean[r] = T(mean);
         if (a.rstd) a.rstd[r] = T(rstd);
@@ -270,31 +284,36 @@ __global__ __launch_bounds__(kLnWide) void k_ln_wide(LnArgs<T> a, int64_t r_base
     }
 }
 
-template <typename T, int MODE, int NT, int VPT>
+template <typename T, int MODE, int NT, int VPT, int F = VPT - 1>
 static void launch_ln_rows(const LnArgs<T> &a)
 {
     for_row_launches(a.rows, NT < 256 ? 256 / NT : 1, [&](unsigned g, int64_t base) {
-        NH_LAUNCH((k_ln_rows<T, NT, VPT, MODE>), dim3(g), dim3(NT < 256 ? 256 : NT), 0, stream(), a, base);
+        NH_LAUNCH((k_ln_rows<T, NT, VPT, F, MODE>), dim3(g), dim3(NT < 256 ? 256 : NT), 0, stream(), a, base);
     });
 }
 
-// The smallest group whose registers hold the row (as launch_softmax).
+// The fewest of LO to 4 vectors per lane of NT that hold the row.
+template <typename T, int MODE, int NT, int LO>
+static void launch_ln_exact(const LnArgs<T> &a, int64_t ncv)
+{
+    if constexpr (LO < 4) {
+        if (ncv > NT * LO) return launch_ln_exact<T, MODE, NT, LO + 1>(a, ncv);
+    }
+    launch_ln_rows<T, MODE, NT, LO>(a);
+}
+
 template <typename T, int MODE>
 static int launch_ln(const LnArgs<T> &a)
 {
     const int64_t ncv = a.cols / Vec16<T>::n;
-    if (ncv <= 4) launch_ln_rows<T, MODE, 4, 1>(a);
-    else if (ncv <= 16) launch_ln_rows<T, MODE, 16, 1>(a);
-    else if (ncv <= 16 * 2) launch_ln_rows<T, MODE, 16, 2>(a);
-    else if (ncv <= 16 * 4) launch_ln_rows<T, MODE, 16, 4>(a);
-    else if (ncv <= 64 * 2) launch_ln_rows<T, MODE, 64, 2>(a);
-    else if (ncv <= 64 * 4) launch_ln_rows<T, MODE, 64, 4>(a);
-    else if (ncv <= 256 * 2) launch_ln_rows<T, MODE, 256, 2>(a);
-    else if (ncv <= 256 * 4) launch_ln_rows<T, MODE, 256, 4>(a);
-    else if (ncv <= 256 * 8) launch_ln_rows<T, MODE, 256, 8>(a);
-    else if (ncv <= 512 * 8) launch_ln_rows<T, MODE, 512, 8>(a);
-    else if (ncv <= 1024 * 8) launch_ln_rows<T, MODE, 1024, 8>(a);
-    else if (ncv <= 1024 * 16) launch_ln_rows<T, MODE, 1024, 16>(a);
+    if (ncv <= 4 * 4) launch_ln_exact<T, MODE, 4, 1>(a, ncv);
+    else if (ncv <= 16 * 4) launch_ln_exact<T, MODE, 16, 2>(a, ncv);
+    else if (ncv <= 64 * 4) launch_ln_exact<T, MODE, 64, 2>(a, ncv);
+    else if (ncv <= 256 * 4) launch_ln_exact<T, MODE, 256, 2>(a, ncv);
+    else if (ncv <= 512 * 4) launch_ln_exact<T, MODE, 512, 3>(a, ncv);
+    else if (ncv <= 1024 * 4) launch_ln_exact<T, MODE, 1024, 3>(a, ncv);
+    else if (ncv <= 1024 * 8) launch_ln_rows<T, MODE, 1024, 8, 4>(a);
+    else if (ncv <= 1024 * 16) launch_ln_rows<T, MODE, 1024, 16, 8>(a);
     else
         for_row_launches(a.rows, 1, [&](unsigned g, int64_t base) {
             NH_LAUNCH((k_ln_wide<T, MODE>), dim3(g), dim3(kLnWide), 0, stream(), a, base);
@@ -314,90 +333,134 @@ struct LnGradArgs {
 };
 
 // Groups of NT lanes walk the rows, r = group, group + groups, ...: each tensor
-// read once, the row's two sums by one exchange (LDS slots alternate between
-// rows, so one barrier a row is enough), and each lane's columns of dgamma and
-// dbeta summed in its registers over the rows.  SUMS: those are wanted.  The
-// block's groups fold theirs through LDS and the block leaves one row of
-// partials.
+// read once, the next row's loads issued before this one is worked on, the row's
+// two sums by one exchange (LDS slots alternate between rows, so one barrier a row
+// is enough), and each lane's columns of dgamma and dbeta summed over the rows in
+// its registers, in double, or, for a block of 1024 (whose lanes have 128
+// registers), in LDS in the rows' type.  SUMS: those are wanted.  The block's groups
+// fold theirs through LDS and the block leaves one row of partials, in the rows' type
+// (a partial's rounding is 2^-24 of one of some hundred terms of a sum that is
+// rounded so itself).
+template <typename T, int NT, int VPT, bool SUMS>
+struct LnGradPlan {
+    static constexpr int NB = NT < 256 ? 256 : NT, RPB = NB / NT;
+    static constexpr bool kLdsSums = SUMS && NT == 1024;
+    static constexpr int kWaves = NT == 1024 ? 4 : (VPT >= 3 ? 2 : (NT == 512 ? 2 : 3));  // per SIMD
+    static constexpr int kPerCu = kWaves * 256 / NB;                                      // resident blocks
+};
+
 template <typename T, int NT, int VPT, int MODE, bool SUMS>
-__global__ __launch_bounds__(NT < 256 ? 256 : NT) void k_ln_grad(LnGradArgs<T> a)
+__global__ __launch_bounds__((LnGradPlan<T, NT, VPT, SUMS>::NB), (LnGradPlan<T, NT, VPT, SUMS>::kWaves)) void k_ln_grad(
+    LnGradArgs<T> a)
 {
     using V = typename Vec16<T>::type;
     using U = typename VecU<T>::type;
     using G = RowGrp<NT>;
     using K = RowKeep<T, NT, VPT>;
-    constexpr int VN = Vec16<T>::n;
-    constexpr int NB = NT < 256 ? 256 : NT, RPB = NB / NT;
+    using Plan = LnGradPlan<T, NT, VPT, SUMS>;
+    constexpr int VN = Vec16<T>::n, RPB = Plan::RPB;
+    constexpr bool LS = Plan::kLdsSums, RS = SUMS && !LS;
     __shared__ double lds_s[2][G::kWaves], lds_q[2][G::kWaves];
     __shared__ uint8_t lds_keep[2][MODE == LN_DROP ? RPB : 1][MODE == LN_DROP ? K::kBytes : 1];
+    __shared__ V lds_g[LS ? VPT : 1][LS ? NT : 1], lds_b[LS ? VPT : 1][LS ? NT : 1];
     const int lane = threadIdx.x % NT, sub = threadIdx.x / NT;
     const int64_t cols = a.cols;
     const RowCut<T> cut(cols);
-    const auto in_row = [&](int k) { return lane + k * NT < cut.ncv; };
+    const auto in_row = [&](int k) { return k < VPT - 1 || lane + k * NT < cut.ncv; };
     const bool has_t = lane < cut.rem;
     const double inv_c = 1.0 / double(cols);
+    const U *gv = reinterpret_cast<const U *>(a.gamma) + lane;
     V g[VPT];
     T gt = T(1);
 #pragma unroll
     for (int k = 0; k < VPT; k++) {
 #pragma unroll
         for (int j = 0; j < VN; j++) g[k][j] = T(1);
-        if (a.gamma && in_row(k)) g[k] = *(reinterpret_cast<const U *>(a.gamma) + lane + k * NT);
+        if (a.gamma && in_row(k)) g[k] = gv[k * NT];
     }
     if (a.gamma && has_t) gt = a.gamma[cut.sc(lane)];
-    double sg[SUMS ? VPT : 1][VN], sb[SUMS ? VPT : 1][VN], sgt = 0.0, sbt = 0.0;
+    double sg[RS ? VPT : 1][VN], sb[RS ? VPT : 1][VN], sgt = 0.0, sbt = 0.0;
 #pragma unroll
-    for (int k = 0; k < (SUMS ? VPT : 1); k++) {
+    for (int k = 0; k < VPT; k++) {
+        if constexpr (RS) {
 #pragma unroll
-        for (int j = 0; j < VN; j++) sg[k][j] = sb[k][j] = 0.0;
+            for (int j = 0; j < VN; j++) sg[k][j] = sb[k][j] = 0.0;
+        } else if constexpr (LS) {
+            V z;
+#pragma unroll
+            for (int j = 0; j < VN; j++) z[j] = T(0);
+            lds_g[k][lane] = lds_b[k][lane] = z;  // a lane's own slots
+        }
     }
     const DropKey key(a.drop);
     const T scale = T(a.drop.scale);
-    int odd = 0;
-    for (int64_t r = int64_t(blockIdx.x) * RPB + sub; r < a.rows; r += int64_t(gridDim.x) * RPB, odd ^= 1) {
-        const int64_t at = r * cols;
+    struct Row {
         V x[VPT], dy[VPT], dh[MODE == LN_PLAIN ? 1 : VPT];
-        T xt = T(0), dyt = T(0), dht = T(0);
+        T xt, dyt, dht, mean, rstd;
+    };
+    const auto load = [&](Row &w, int64_t r) {
+        const int64_t at = r * cols;
+        w.mean = a.mean[r];
+        w.rstd = a.rstd[r];
 #pragma unroll
         for (int k = 0; k < VPT; k++)
-            if (in_row(k)) x[k] = __builtin_nontemporal_load(reinterpret_cast<const U *>(a.h + at) + lane + k * NT);
+            if (in_row(k)) w.x[k] = __builtin_nontemporal_load(reinterpret_cast<const U *>(a.h + at) + lane + k * NT);
 #pragma unroll
         for (int k = 0; k < VPT; k++)
-            if (in_row(k)) dy[k] = __builtin_nontemporal_load(reinterpret_cast<const U *>(a.dy + at) + lane + k * NT);
+            if (in_row(k)) w.dy[k] = __builtin_nontemporal_load(reinterpret_cast<const U *>(a.dy + at) + lane + k * NT);
         if (has_t) {
-            xt = a.h[at + cut.sc(lane)];
-            dyt = a.dy[at + cut.sc(lane)];
+            w.xt = a.h[at + cut.sc(lane)];
+            w.dyt = a.dy[at + cut.sc(lane)];
         }
         if constexpr (MODE != LN_PLAIN) {
+            if (a.dh) {
 #pragma unroll
-            for (int k = 0; k < VPT; k++) {
-#pragma unroll
-                for (int j = 0; j < VN; j++) dh[k][j] = T(0);
-                if (a.dh && in_row(k))
-                    dh[k] = __builtin_nontemporal_load(reinterpret_cast<const U *>(a.dh + at) + lane + k * NT);
+                for (int k = 0; k < VPT; k++)
+                    if (in_row(k))
+                        w.dh[k] = __builtin_nontemporal_load(reinterpret_cast<const U *>(a.dh + at) + lane + k * NT);
+                if (has_t) w.dht = a.dh[at + cut.sc(lane)];
             }
-            if (a.dh && has_t) dht = a.dh[at + cut.sc(lane)];
         }
-        const double mean = double(a.mean[r]), rstd = double(a.rstd[r]);
+    };
+    const int64_t step = int64_t(gridDim.x) * RPB;
+    int64_t r = int64_t(blockIdx.x) * RPB + sub;
+    Row w, next;
+    if (r < a.rows) load(w, r);
+    for (int odd = 0; r < a.rows; r += step, odd ^= 1) {
+        if (r + step < a.rows) load(next, r + step);
+        const int64_t at = r * cols;
+        const double mean = double(w.mean), rstd = double(w.rstd);
         K keep;
         if constexpr (MODE == LN_DROP) keep.make(r, cols, cut, lane, key, lds_keep[odd][sub]);
         double s = 0.0, q = 0.0;
-        const auto sums = [&](T xv, T dyv, T gv, double &ag, double &ab) {
-            const double xh = (double(xv) - mean) * rstd, w = double(dyv) * fresh(gv);
-            s += w;
-            q = __builtin_fma(w, xh, q);
-            if constexpr (SUMS) {
-                ag = __builtin_fma(double(dyv), xh, ag);
-                ab += double(dyv);
-            }
+        const auto sums = [&](T xv, T dyv, T gv1, double &ag, double &ab) {
+            const double d = double(dyv), xh = (double(xv) - mean) * rstd, wv = d * fresh(gv1);
+            s += wv;
+            q = __builtin_fma(wv, xh, q);
+            ag = __builtin_fma(d, xh, ag);
+            ab += d;
         };
 #pragma unroll
         for (int k = 0; k < VPT; k++)
             if (in_row(k)) {
+                if constexpr (LS) {
+                    V vg = lds_g[k][lane], vb = lds_b[k][lane];
 #pragma unroll
-                for (int j = 0; j < VN; j++) sums(x[k][j], dy[k][j], g[k][j], sg[SUMS ? k : 0][j], sb[SUMS ? k : 0][j]);
+                    for (int j = 0; j < VN; j++) {
+                        double ag = double(vg[j]), ab = double(vb[j]);
+                        sums(w.x[k][j], w.dy[k][j], g[k][j], ag, ab);
+                        vg[j] = T(ag);
+                        vb[j] = T(ab);
+                    }
+                    lds_g[k][lane] = vg;
+                    lds_b[k][lane] = vb;
+                } else {
+#pragma unroll
+                    for (int j = 0; j < VN; j++)
+                        sums(w.x[k][j], w.dy[k][j], g[k][j], sg[RS ? k : 0][j], sb[RS ? k : 0][j]);
+                }
             }
-        if (has_t) sums(xt, dyt, gt, sgt, sbt);
+        if (has_t) sums(w.xt, w.dyt, gt, sgt, sbt);
         // both sums over the row by one exchange
         const auto add = [](double p, double t) { return p + t; };
         s = G::part(s, add);
@@ -417,18 +480,21 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void k_ln_grad(LnGradArgs<T> a
             }
         }
         const double c1 = s * inv_c, c2 = q * inv_c;
-        const auto grad = [&](T xv, T dyv, T gv) {
-            const double xh = (fresh(xv) - mean) * rstd, w = fresh(dyv) * fresh(gv);
-            return T(rstd * (__builtin_fma(-xh, c2, w - c1)));
+        const auto grad = [&](T xv, T dyv, T gv1) {
+            const double xh = (fresh(xv) - mean) * rstd, wv = fresh(dyv) * fresh(gv1);
+            return T(rstd * (__builtin_fma(-xh, c2, wv - c1)));
         };
 #pragma unroll
         for (int k = 0; k < VPT; k++)
             if (in_row(k)) {
                 V o;
 #pragma unroll
-                for (int j = 0; j < VN; j++) o[j] = grad(x[k][j], dy[k][j], g[k][j]);
+                for (int j = 0; j < VN; j++) o[j] = grad(w.x[k][j], w.dy[k][j], g[k][j]);
                 if constexpr (MODE != LN_PLAIN) {
-                    if (a.dh) o = o + dh[k];
+                    if (a.dh) {
+#pragma unroll
+                        for (int j = 0; j < VN; j++) o[j] = o[j] + w.dh[k][j];
+                    }
                     if (a.dres) __builtin_nontemporal_store(o, reinterpret_cast<U *>(a.dres + at) + lane + k * NT);
                 }
                 if constexpr (MODE == LN_DROP) {
@@ -439,14 +505,15 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void k_ln_grad(LnGradArgs<T> a
             }
         if (has_t) {
             const int64_t i = at + cut.sc(lane);
-            T o = grad(xt, dyt, gt);
+            T o = grad(w.xt, w.dyt, gt);
             if constexpr (MODE != LN_PLAIN) {
-                if (a.dh) o = o + dht;
+                if (a.dh) o = o + w.dht;
                 if (a.dres) a.dres[i] = o;
             }
             if constexpr (MODE == LN_DROP) o = dropped<T>(o, scale, keep.tail, 0);
             if (a.dx) a.dx[i] = o;
         }
+        w = next;
     }
     if constexpr (SUMS) {
         T *pg = a.part + int64_t(blockIdx.x) * 2 * cols, *pb = pg + cols;
@@ -455,10 +522,15 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void k_ln_grad(LnGradArgs<T> a
             for (int k = 0; k < VPT; k++)
                 if (in_row(k)) {
                     V og, ob;
+                    if constexpr (LS) {
+                        og = lds_g[k][lane];
+                        ob = lds_b[k][lane];
+                    } else {
 #pragma unroll
-                    for (int j = 0; j < VN; j++) {
-                        og[j] = T(sg[k][j]);
-                        ob[j] = T(sb[k][j]);
+                        for (int j = 0; j < VN; j++) {
+                            og[j] = T(sg[k][j]);
+                            ob[j] = T(sb[k][j]);
+                        }
                     }
                     *(reinterpret_cast<U *>(pg) + lane + k * NT) = og;
                     *(reinterpret_cast<U *>(pb) + lane + k * NT) = ob;
@@ -494,24 +566,40 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void k_ln_grad(LnGradArgs<T> a
                 }
             };
 #pragma unroll
-            for (int k = 0; k < VPT; k++) across(std::integral_constant<int, VN>{}, sg[k], sb[k], int64_t(lane + k * NT) * VN, in_row(k));
+            for (int k = 0; k < VPT; k++)
+                across(std::integral_constant<int, VN>{}, sg[k], sb[k], int64_t(lane + k * NT) * VN, in_row(k));
             if (cut.rem) across(std::integral_constant<int, 1>{}, &sgt, &sbt, cut.sc(lane), has_t);
         }
     }
 }
 
 // Column sums of the partials: [n][2 cols] -> dgamma, dbeta.  A block of 16
-// waves takes 64 columns, the waves the partials in turn.
+// waves takes 64 columns, the waves the partials in turn, eight in flight each.
 template <typename T>
 __global__ __launch_bounds__(1024) void k_ln_fold(const T *__restrict__ part, int64_t n, int64_t cols,
                                                   T *__restrict__ dgamma, T *__restrict__ dbeta)
 {
+    constexpr int UN = 8;
     __shared__ double sh[16][64];
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     const int64_t c = int64_t(blockIdx.x) * 64 + lane;
     double s = 0.0;
-    if (c < 2 * cols)
-        for (int64_t i = w; i < n; i += 16) s += double(part[i * 2 * cols + c]);
+    if (c < 2 * cols) {
+        const T *p = part + c;
+        int64_t i = w;
+        for (; i + 16 * (UN - 1) < n; i += 16 * UN) {
+            T v[UN];
+#pragma unroll
+            for (int u = 0; u < UN; u++) v[u] = p[(i + 16 * u) * 2 * cols];
+#pragma unroll
+            for (int u = 0; u < UN; u++) s += double(v[u]);
+        }
+        T v[UN];
+#pragma unroll
+        for (int u = 0; u < UN; u++) v[u] = i + 16 * u < n ? p[(i + 16 * u) * 2 * cols] : T(0);
+#pragma unroll
+        for (int u = 0; u < UN; u++) s += double(v[u]);
+    }
     sh[w][lane] = s;
     __syncthreads();
     if (w == 0 && c < 2 * cols) {
@@ -599,46 +687,47 @@ struct Partials {
     }
 };
 
-// Blocks that walk the rows: what the CUs hold at once, no more than rows.
-static int64_t grad_blocks(int64_t rows, int rpb, int per_cu)
-{
-    const int64_t most = int64_t(num_cus()) * per_cu, need = ceil_div(rows, int64_t(rpb));
-    return need < most ? need : most;
-}
-
 template <typename T, int MODE, int NT, int VPT>
 static int launch_ln_grad_rows(LnGradArgs<T> a, T *dgamma, T *dbeta)
 {
-    constexpr int NB = NT < 256 ? 256 : NT;
-    const bool sums = dgamma || dbeta;
-    const int64_t nb = grad_blocks(a.rows, NB / NT, 1024 / NB);
+    constexpr bool kSums = true;
+    using Plan = LnGradPlan<T, NT, VPT, kSums>;
+    // as many blocks as the CUs hold at once, no more than rows
+    const int64_t most = int64_t(num_cus()) * Plan::kPerCu, need = ceil_div(a.rows, int64_t(Plan::RPB));
+    const int64_t nb = need < most ? need : most;
     Partials part;
-    if (sums) {
+    if (dgamma || dbeta) {
         NH_TRY(part.open(size_t(nb) * 2 * size_t(a.cols) * sizeof(T)));
         a.part = static_cast<T *>(part.p);
-        NH_LAUNCH((k_ln_grad<T, NT, VPT, MODE, true>), dim3(unsigned(nb)), dim3(NB), 0, stream(), a);
+        NH_LAUNCH((k_ln_grad<T, NT, VPT, MODE, true>), dim3(unsigned(nb)), dim3(Plan::NB), 0, stream(), a);
         NH_LAUNCH((k_ln_fold<T>), dim3(unsigned(ceil_div(2 * a.cols, 64))), dim3(1024), 0, stream(), a.part, nb, a.cols,
                   dgamma, dbeta);
     } else {
-        NH_LAUNCH((k_ln_grad<T, NT, VPT, MODE, false>), dim3(unsigned(nb)), dim3(NB), 0, stream(), a);
+        NH_LAUNCH((k_ln_grad<T, NT, VPT, MODE, false>), dim3(unsigned(nb)), dim3(Plan::NB), 0, stream(), a);
     }
     return check_launch();
+}
+
+// The fewest of LO to 4 vectors per lane of NT that hold the row.
+template <typename T, int MODE, int NT, int LO>
+static int launch_ln_grad_exact(const LnGradArgs<T> &a, int64_t ncv, T *dgamma, T *dbeta)
+{
+    if constexpr (LO < 4) {
+        if (ncv > NT * LO) return launch_ln_grad_exact<T, MODE, NT, LO + 1>(a, ncv, dgamma, dbeta);
+    }
+    return launch_ln_grad_rows<T, MODE, NT, LO>(a, dgamma, dbeta);
 }
 
 template <typename T, int MODE>
 static int launch_ln_grad(LnGradArgs<T> a, T *dgamma, T *dbeta)
 {
     const int64_t ncv = a.cols / Vec16<T>::n;
-    if (ncv <= 4) return launch_ln_grad_rows<T, MODE, 4, 1>(a, dgamma, dbeta);
-    if (ncv <= 16) return launch_ln_grad_rows<T, MODE, 16, 1>(a, dgamma, dbeta);
-    if (ncv <= 16 * 2) return launch_ln_grad_rows<T, MODE, 16, 2>(a, dgamma, dbeta);
-    if (ncv <= 64) return launch_ln_grad_rows<T, MODE, 64, 1>(a, dgamma, dbeta);
-    if (ncv <= 64 * 2) return launch_ln_grad_rows<T, MODE, 64, 2>(a, dgamma, dbeta);
-    if (ncv <= 64 * 4) return launch_ln_grad_rows<T, MODE, 64, 4>(a, dgamma, dbeta);
-    if (ncv <= 256 * 2) return launch_ln_grad_rows<T, MODE, 256, 2>(a, dgamma, dbeta);
-    if (ncv <= 256 * 4) return launch_ln_grad_rows<T, MODE, 256, 4>(a, dgamma, dbeta);
-    if (ncv <= 512 * 4) return launch_ln_grad_rows<T, MODE, 512, 4>(a, dgamma, dbeta);
-    if (ncv <= 1024 * 4) return launch_ln_grad_rows<T, MODE, 1024, 4>(a, dgamma, dbeta);
+    if (ncv <= 4 * 4) return launch_ln_grad_exact<T, MODE, 4, 1>(a, ncv, dgamma, dbeta);
+    if (ncv <= 16 * 4) return launch_ln_grad_exact<T, MODE, 16, 2>(a, ncv, dgamma, dbeta);
+    if (ncv <= 64 * 4) return launch_ln_grad_exact<T, MODE, 64, 2>(a, ncv, dgamma, dbeta);
+    if (ncv <= 256 * 4) return launch_ln_grad_exact<T, MODE, 256, 2>(a, ncv, dgamma, dbeta);
+    if (ncv <= 512 * 4) return launch_ln_grad_exact<T, MODE, 512, 3>(a, ncv, dgamma, dbeta);
+    if (ncv <= 1024 * 4) return launch_ln_grad_exact<T, MODE, 1024, 3>(a, ncv, dgamma, dbeta);
     // the columns first: the row pass may write over what they read
     Partials part;
     if (dgamma || dbeta) {
