@@ -28,14 +28,13 @@ namespace nh {
 
 enum { LN_PLAIN = 0, LN_ADD = 1, LN_DROP = 2 };
 
-// v as a double made here: hides where v came from, or the compiler keeps the
-// doubles of an earlier pass over the row (two or more registers per value, and spills)
-// instead of converting again.
-template <typename T>
-NH_DEV double fresh(T v)
+// Hides where v's values came from, in place: or the compiler keeps the doubles that an
+// earlier pass over the row made of them (two or more registers per value, and
+// spills) instead of converting again.
+template <typename V>
+NH_DEV void hide(V &v)
 {
     asm("" : "+v"(v));
-    return double(v);
 }
 
 // s / n from inv = 1 / n: the quotient corrected by its remainder, so that a row of one
@@ -198,9 +197,10 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void k_ln_rows(LnArgs<T> a, in
 #pragma unroll
     for (int k = 0; k < VPT; k++)
         if (in_row(k)) {
+            hide(v[k]);
 #pragma unroll
             for (int j = 0; j < VN; j++) {
-                const double d = fresh<T>(v[k][j]) - mean;
+                const double d = double(v[k][j]) - mean;
                 q = __builtin_fma(d, d, q);
             }
         }
@@ -214,7 +214,7 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void k_ln_rows(LnArgs<T> a, in
         if (a.rstd) a.rstd[r] = T(rstd);
     }
     const auto out = [&](T xv, T g, T b) {
-        return T(__builtin_fma((fresh(xv) - mean) * rstd, double(g), double(b)));
+        return T(__builtin_fma((double(xv) - mean) * rstd, double(g), double(b)));
     };
 #pragma unroll
     for (int k = 0; k < VPT; k++)
@@ -227,6 +227,7 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void k_ln_rows(LnArgs<T> a, in
             }
             if (a.gamma) g = *(reinterpret_cast<const U *>(a.gamma) + lane + k * NT);
             if (a.beta) b = *(reinterpret_cast<const U *>(a.beta) + lane + k * NT);
+            hide(v[k]);
 #pragma unroll
             for (int j = 0; j < VN; j++) o[j] = out(v[k][j], g[j], b[j]);
             __builtin_nontemporal_store(o, reinterpret_cast<U *>(a.y + at) + lane + k * NT);
@@ -332,52 +333,58 @@ struct LnGradArgs {
     DropArgs drop;
 };
 
+// How a group's lanes hold a row of the backward pass, and how many groups a CU
+// holds.  NT lanes, VPT vectors each.  Up to 4 vectors: gamma and the sums of dgamma and dbeta
+// (in double) in registers.  5 to 8: the sums in LDS, in the rows' type (128 KB at
+// most), gamma from the L2 for each row.  More: no sums (k_ln_cols takes them).
+template <typename T, int NT, int VPT>
+struct LnGradPlan {
+    static constexpr int NB = NT < 256 ? 256 : NT, RPB = NB / NT;
+    static constexpr bool kRegs = VPT <= 4;
+    static constexpr int F = VPT <= 8 ? VPT - 1 : VPT / 2;  // vectors that are whole
+    static constexpr int kWaves = VPT >= 3 || NT >= 512 ? 2 : 3;  // per SIMD
+    static constexpr int kPerCu = kWaves * 256 / NB;              // resident blocks
+};
+
 // Groups of NT lanes walk the rows, r = group, group + groups, ...: each tensor
 // read once, the next row's loads issued before this one is worked on, the row's
 // two sums by one exchange (LDS slots alternate between rows, so one barrier a row
-// is enough), and each lane's columns of dgamma and dbeta summed over the rows in
-// its registers, in double, or, for a block of 1024 (whose lanes have 128
-// registers), in LDS in the rows' type.  SUMS: those are wanted.  The block's groups
-// fold theirs through LDS and the block leaves one row of partials, in the rows' type
-// (a partial's rounding is 2^-24 of one of some hundred terms of a sum that is
-// rounded so itself).
-template <typename T, int NT, int VPT, bool SUMS>
-struct LnGradPlan {
-    static constexpr int NB = NT < 256 ? 256 : NT, RPB = NB / NT;
-    static constexpr bool kLdsSums = SUMS && NT == 1024;
-    static constexpr int kWaves = NT == 1024 ? 4 : (VPT >= 3 ? 2 : (NT == 512 ? 2 : 3));  // per SIMD
-    static constexpr int kPerCu = kWaves * 256 / NB;                                      // resident blocks
-};
-
+// is enough), and each lane's columns of dgamma and dbeta summed over the rows (SUMS).
+// The block's groups fold theirs through LDS and the block leaves one row of
+// partials, in the rows' type (the rounding of one of some hundred terms of a sum that is
+// itself rounded so).  `block` of `blocks`.
 template <typename T, int NT, int VPT, int MODE, bool SUMS>
-__global__ __launch_bounds__((LnGradPlan<T, NT, VPT, SUMS>::NB), (LnGradPlan<T, NT, VPT, SUMS>::kWaves)) void k_ln_grad(
-    LnGradArgs<T> a)
+NH_DEV void ln_grad_rows(const LnGradArgs<T> &a, int64_t block, int64_t blocks)
 {
     using V = typename Vec16<T>::type;
     using U = typename VecU<T>::type;
     using G = RowGrp<NT>;
     using K = RowKeep<T, NT, VPT>;
-    using Plan = LnGradPlan<T, NT, VPT, SUMS>;
+    using Plan = LnGradPlan<T, NT, VPT>;
     constexpr int VN = Vec16<T>::n, RPB = Plan::RPB;
-    constexpr bool LS = Plan::kLdsSums, RS = SUMS && !LS;
+    constexpr bool LS = SUMS && !Plan::kRegs, RS = SUMS && Plan::kRegs;
     __shared__ double lds_s[2][G::kWaves], lds_q[2][G::kWaves];
     __shared__ uint8_t lds_keep[2][MODE == LN_DROP ? RPB : 1][MODE == LN_DROP ? K::kBytes : 1];
     __shared__ V lds_g[LS ? VPT : 1][LS ? NT : 1], lds_b[LS ? VPT : 1][LS ? NT : 1];
     const int lane = threadIdx.x % NT, sub = threadIdx.x / NT;
     const int64_t cols = a.cols;
     const RowCut<T> cut(cols);
-    const auto in_row = [&](int k) { return k < VPT - 1 || lane + k * NT < cut.ncv; };
+    const auto in_row = [&](int k) { return k < Plan::F || lane + k * NT < cut.ncv; };
     const bool has_t = lane < cut.rem;
     const double inv_c = 1.0 / double(cols);
-    const U *gv = reinterpret_cast<const U *>(a.gamma) + lane;
-    V g[VPT];
-    T gt = T(1);
+    V g[Plan::kRegs ? VPT : 1];
+    const auto gamma = [&](int k) {
+        V v;
 #pragma unroll
-    for (int k = 0; k < VPT; k++) {
+        for (int j = 0; j < VN; j++) v[j] = T(1);
+        if (a.gamma && in_row(k)) v = *(reinterpret_cast<const U *>(a.gamma) + lane + k * NT);
+        return v;
+    };
+    if constexpr (Plan::kRegs) {
 #pragma unroll
-        for (int j = 0; j < VN; j++) g[k][j] = T(1);
-        if (a.gamma && in_row(k)) g[k] = gv[k * NT];
+        for (int k = 0; k < VPT; k++) g[k] = gamma(k);
     }
+    T gt = T(1);
     if (a.gamma && has_t) gt = a.gamma[cut.sc(lane)];
     double sg[RS ? VPT : 1][VN], sb[RS ? VPT : 1][VN], sgt = 0.0, sbt = 0.0;
 #pragma unroll
@@ -395,8 +402,8 @@ __global__ __launch_bounds__((LnGradPlan<T, NT, VPT, SUMS>::NB), (LnGradPlan<T, 
     const DropKey key(a.drop);
     const T scale = T(a.drop.scale);
     struct Row {
-        V x[VPT], dy[VPT], dh[MODE == LN_PLAIN ? 1 : VPT];
-        T xt, dyt, dht, mean, rstd;
+        V x[VPT], dy[VPT];
+        T xt, dyt, mean, rstd;
     };
     const auto load = [&](Row &w, int64_t r) {
         const int64_t at = r * cols;
@@ -412,29 +419,32 @@ __global__ __launch_bounds__((LnGradPlan<T, NT, VPT, SUMS>::NB), (LnGradPlan<T, 
             w.xt = a.h[at + cut.sc(lane)];
             w.dyt = a.dy[at + cut.sc(lane)];
         }
-        if constexpr (MODE != LN_PLAIN) {
-            if (a.dh) {
-#pragma unroll
-                for (int k = 0; k < VPT; k++)
-                    if (in_row(k))
-                        w.dh[k] = __builtin_nontemporal_load(reinterpret_cast<const U *>(a.dh + at) + lane + k * NT);
-                if (has_t) w.dht = a.dh[at + cut.sc(lane)];
-            }
-        }
     };
-    const int64_t step = int64_t(gridDim.x) * RPB;
-    int64_t r = int64_t(blockIdx.x) * RPB + sub;
+    const int64_t step = blocks * RPB;
+    int64_t r = block * RPB + sub;
     Row w, next;
     if (r < a.rows) load(w, r);
     for (int odd = 0; r < a.rows; r += step, odd ^= 1) {
-        if (r + step < a.rows) load(next, r + step);
         const int64_t at = r * cols;
+        constexpr bool kEarly = MODE != LN_PLAIN && VPT <= 8;  // dh fits beside x and dy
+        V dh[kEarly ? VPT : 1];
+        T dht = T(0);
+        if constexpr (MODE != LN_PLAIN) {
+            if (a.dh) {
+#pragma unroll
+                for (int k = 0; k < (kEarly ? VPT : 0); k++)
+                    if (in_row(k))
+                        dh[k] = __builtin_nontemporal_load(reinterpret_cast<const U *>(a.dh + at) + lane + k * NT);
+                if (has_t) dht = a.dh[at + cut.sc(lane)];
+            }
+        }
+        if (VPT <= 8 && r + step < a.rows) load(next, r + step);
         const double mean = double(w.mean), rstd = double(w.rstd);
         K keep;
         if constexpr (MODE == LN_DROP) keep.make(r, cols, cut, lane, key, lds_keep[odd][sub]);
         double s = 0.0, q = 0.0;
-        const auto sums = [&](T xv, T dyv, T gv1, double &ag, double &ab) {
-            const double d = double(dyv), xh = (double(xv) - mean) * rstd, wv = d * fresh(gv1);
+        const auto sums = [&](T xv, T dyv, T gv, double &ag, double &ab) {
+            const double d = double(dyv), xh = (double(xv) - mean) * rstd, wv = d * double(gv);
             s += wv;
             q = __builtin_fma(wv, xh, q);
             ag = __builtin_fma(d, xh, ag);
@@ -443,21 +453,34 @@ __global__ __launch_bounds__((LnGradPlan<T, NT, VPT, SUMS>::NB), (LnGradPlan<T, 
 #pragma unroll
         for (int k = 0; k < VPT; k++)
             if (in_row(k)) {
+                V gk, vg, vb;
+                if constexpr (Plan::kRegs) gk = g[k];
+                else gk = gamma(k);
                 if constexpr (LS) {
-                    V vg = lds_g[k][lane], vb = lds_b[k][lane];
+                    vg = lds_g[k][lane];
+                    vb = lds_b[k][lane];
+                }
 #pragma unroll
-                    for (int j = 0; j < VN; j++) {
+                for (int j = 0; j < VN; j++) {
+                    if constexpr (LS) {
                         double ag = double(vg[j]), ab = double(vb[j]);
-                        sums(w.x[k][j], w.dy[k][j], g[k][j], ag, ab);
+                        sums(w.x[k][j], w.dy[k][j], gk[j], ag, ab);
                         vg[j] = T(ag);
                         vb[j] = T(ab);
+                    } else {
+                        sums(w.x[k][j], w.dy[k][j], gk[j], sg[RS ? k : 0][j], sb[RS ? k : 0][j]);
                     }
+                }
+                if constexpr (RS) {
+                    // taken here: the compiler would put them off past the stores, with
+                    // their operands' doubles kept until then
+#pragma unroll
+                    for (int j = 0; j < VN; j++) asm volatile("" : "+v"(sg[k][j]), "+v"(sb[k][j]));
+                }
+                if constexpr (LS) {
                     lds_g[k][lane] = vg;
                     lds_b[k][lane] = vb;
-                } else {
-#pragma unroll
-                    for (int j = 0; j < VN; j++)
-                        sums(w.x[k][j], w.dy[k][j], g[k][j], sg[RS ? k : 0][j], sb[RS ? k : 0][j]);
+                    asm volatile("" : "+v"(s), "+v"(q) : : "memory");  // one vector's terms in registers at a time
                 }
             }
         if (has_t) sums(w.xt, w.dyt, gt, sgt, sbt);
@@ -480,20 +503,31 @@ __global__ __launch_bounds__((LnGradPlan<T, NT, VPT, SUMS>::NB), (LnGradPlan<T, 
             }
         }
         const double c1 = s * inv_c, c2 = q * inv_c;
-        const auto grad = [&](T xv, T dyv, T gv1) {
-            const double xh = (fresh(xv) - mean) * rstd, wv = fresh(dyv) * fresh(gv1);
+        const auto grad = [&](T xv, T dyv, T gv) {
+            const double xh = (double(xv) - mean) * rstd, wv = double(dyv) * double(gv);
             return T(rstd * (__builtin_fma(-xh, c2, wv - c1)));
         };
 #pragma unroll
         for (int k = 0; k < VPT; k++)
-            if (in_row(k)) {
-                V o;
+            if ((MODE != LN_PLAIN || a.dx) && in_row(k)) {
+                hide(w.x[k]);
+                hide(w.dy[k]);
+                V o, gk;
+                if constexpr (Plan::kRegs) {
+                    hide(g[k]);
+                    gk = g[k];
+                } else {
+                    gk = gamma(k);
+                }
 #pragma unroll
-                for (int j = 0; j < VN; j++) o[j] = grad(w.x[k][j], w.dy[k][j], g[k][j]);
+                for (int j = 0; j < VN; j++) o[j] = grad(w.x[k][j], w.dy[k][j], gk[j]);
                 if constexpr (MODE != LN_PLAIN) {
                     if (a.dh) {
+                        V d;
+                        if constexpr (kEarly) d = dh[k];
+                        else d = __builtin_nontemporal_load(reinterpret_cast<const U *>(a.dh + at) + lane + k * NT);
 #pragma unroll
-                        for (int j = 0; j < VN; j++) o[j] = o[j] + w.dh[k][j];
+                        for (int j = 0; j < VN; j++) o[j] = o[j] + d[j];
                     }
                     if (a.dres) __builtin_nontemporal_store(o, reinterpret_cast<U *>(a.dres + at) + lane + k * NT);
                 }
@@ -501,22 +535,24 @@ __global__ __launch_bounds__((LnGradPlan<T, NT, VPT, SUMS>::NB), (LnGradPlan<T, 
 #pragma unroll
                     for (int j = 0; j < VN; j++) o[j] = dropped<T>(o[j], scale, keep.m[k], K::bit(j));
                 }
-                if (a.dx) __builtin_nontemporal_store(o, reinterpret_cast<U *>(a.dx + at) + lane + k * NT);
+                if (MODE == LN_PLAIN || a.dx)
+                    __builtin_nontemporal_store(o, reinterpret_cast<U *>(a.dx + at) + lane + k * NT);
             }
         if (has_t) {
             const int64_t i = at + cut.sc(lane);
             T o = grad(w.xt, w.dyt, gt);
             if constexpr (MODE != LN_PLAIN) {
-                if (a.dh) o = o + w.dht;
+                if (a.dh) o = o + dht;
                 if (a.dres) a.dres[i] = o;
             }
             if constexpr (MODE == LN_DROP) o = dropped<T>(o, scale, keep.tail, 0);
             if (a.dx) a.dx[i] = o;
         }
-        w = next;
+        if constexpr (VPT <= 8) w = next;
+        else if (r + step < a.rows) load(w, r + step);  // no registers for two rows
     }
     if constexpr (SUMS) {
-        T *pg = a.part + int64_t(blockIdx.x) * 2 * cols, *pb = pg + cols;
+        T *pg = a.part + block * 2 * cols, *pb = pg + cols;
         if constexpr (RPB == 1) {
 #pragma unroll
             for (int k = 0; k < VPT; k++)
@@ -571,6 +607,65 @@ __global__ __launch_bounds__((LnGradPlan<T, NT, VPT, SUMS>::NB), (LnGradPlan<T, 
             if (cut.rem) across(std::integral_constant<int, 1>{}, &sgt, &sbt, cut.sc(lane), has_t);
         }
     }
+}
+
+template <typename T, int NT, int VPT, int MODE, bool SUMS>
+__global__ __launch_bounds__((LnGradPlan<T, NT, VPT>::NB), (LnGradPlan<T, NT, VPT>::kWaves)) void k_ln_grad(
+    LnGradArgs<T> a)
+{
+    ln_grad_rows<T, NT, VPT, MODE, SUMS>(a, blockIdx.x, gridDim.x);
+}
+
+// Sums of few rows, without partials: 16 columns a block of NB lanes, the rows
+// by NB / 16 streams of 8 rows in flight, folded in LDS.
+template <typename T, int NB>
+NH_DEV void ln_few_cols(const LnGradArgs<T> &a, int64_t block, T *dgamma, T *dbeta)
+{
+    constexpr int S = NB / 16, UN = 8;
+    __shared__ double sh[2][S][16];
+    const int cl = threadIdx.x & 15, st = threadIdx.x >> 4;
+    const int64_t cols = a.cols, c = block * 16 + cl;
+    double g = 0.0, b = 0.0;
+    if (c < cols)
+        for (int64_t r = st; r < a.rows; r += S * UN) {
+            T dy[UN], x[UN], m[UN], rs[UN];
+#pragma unroll
+            for (int u = 0; u < UN; u++)
+                if (r + u * S < a.rows) {
+                    const int64_t q = r + u * S;
+                    dy[u] = a.dy[q * cols + c];
+                    x[u] = a.h[q * cols + c];
+                    m[u] = a.mean[q];
+                    rs[u] = a.rstd[q];
+                }
+#pragma unroll
+            for (int u = 0; u < UN; u++)
+                if (r + u * S < a.rows) {
+                    const double d = double(dy[u]);
+                    g = __builtin_fma(d, (double(x[u]) - double(m[u])) * double(rs[u]), g);
+                    b += d;
+                }
+        }
+    sh[0][st][cl] = g;
+    sh[1][st][cl] = b;
+    __syncthreads();
+    if (st < 2 && c < cols) {
+        double t = sh[st][0][cl];
+        for (int i = 1; i < S; i++) t += sh[st][i][cl];
+        T *out = st ? dbeta : dgamma;
+        if (out) out[c] = T(t);
+    }
+}
+
+// The backward pass of few rows in one launch: blocks 0 .. nrows - 1 take the rows,
+// the others columns (which read x and dy again, from the caches).  Either
+// part may be absent.
+template <typename T, int NT, int VPT, int MODE>
+__global__ __launch_bounds__((LnGradPlan<T, NT, VPT>::NB)) void k_ln_grad_few(LnGradArgs<T> a, int nrows, T *dgamma,
+                                                                             T *dbeta)
+{
+    if (int(blockIdx.x) < nrows) ln_grad_rows<T, NT, VPT, MODE, false>(a, blockIdx.x, nrows);
+    else ln_few_cols<T, LnGradPlan<T, NT, VPT>::NB>(a, int64_t(blockIdx.x) - nrows, dgamma, dbeta);
 }
 
 // Column sums of the partials: [n][2 cols] -> dgamma, dbeta.  A block of 16
@@ -643,28 +738,59 @@ __global__ __launch_bounds__(kLnWide) void k_ln_grad_wide(LnGradArgs<T> a, int64
     }
 }
 
-// Their column sums: 64 columns a block, the rows of its chunk by 16 waves.
+// Column sums beside a row pass that cannot hold them: 64 lanes of VN columns a block, the
+// rows of its chunk by 8 waves, four in flight each.
 template <typename T>
-__global__ __launch_bounds__(1024) void k_ln_cols(LnGradArgs<T> a, int64_t chunk)
+__global__ __launch_bounds__(512) void k_ln_cols(LnGradArgs<T> a, int64_t chunk)
 {
-    __shared__ double sh[2][16][64];
+    using V = typename Vec16<T>::type;
+    using U = typename VecU<T>::type;
+    constexpr int VN = Vec16<T>::n, W = 8, UN = 4;
+    __shared__ double sh[W][2 * VN][64];
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const int64_t cols = a.cols, c = int64_t(blockIdx.x) * 64 + lane;
+    const int64_t cols = a.cols, c = (int64_t(blockIdx.x) * 64 + lane) * VN;
     const int64_t r0 = int64_t(blockIdx.y) * chunk, r1 = r0 + chunk < a.rows ? r0 + chunk : a.rows;
-    double g = 0.0, b = 0.0;
-    if (c < cols)
-        for (int64_t r = r0 + w; r < r1; r += 16) {
-            const double dy = double(a.dy[r * cols + c]);
-            g = __builtin_fma(dy, (double(a.h[r * cols + c]) - double(a.mean[r])) * double(a.rstd[r]), g);
-            b += dy;
-        }
-    sh[0][w][lane] = g;
-    sh[1][w][lane] = b;
+    const bool whole = c + VN <= cols;
+    double s[2 * VN];
+#pragma unroll
+    for (int j = 0; j < 2 * VN; j++) s[j] = 0.0;
+    for (int64_t r = r0 + w; r < r1; r += W * UN) {
+        V x[UN], dy[UN];
+#pragma unroll
+        for (int u = 0; u < UN; u++)
+            if (r + u * W < r1) {
+                const int64_t at = (r + u * W) * cols + c;
+                if (whole) {
+                    x[u] = *reinterpret_cast<const U *>(a.h + at);
+                    dy[u] = *reinterpret_cast<const U *>(a.dy + at);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < VN; j++) {
+                        x[u][j] = c + j < cols ? a.h[at + j] : T(0);
+                        dy[u][j] = c + j < cols ? a.dy[at + j] : T(0);
+                    }
+                }
+            }
+#pragma unroll
+        for (int u = 0; u < UN; u++)
+            if (r + u * W < r1) {
+                const double mean = double(a.mean[r + u * W]), rstd = double(a.rstd[r + u * W]);
+#pragma unroll
+                for (int j = 0; j < VN; j++) {
+                    const double d = double(dy[u][j]);
+                    s[j] = __builtin_fma(d, (double(x[u][j]) - mean) * rstd, s[j]);
+                    s[VN + j] += d;
+                }
+            }
+    }
+#pragma unroll
+    for (int j = 0; j < 2 * VN; j++) sh[w][j][lane] = s[j];
     __syncthreads();
-    if (w < 2 && c < cols) {
-        double t = sh[w][0][lane];
-        for (int i = 1; i < 16; i++) t += sh[w][i][lane];
-        a.part[(int64_t(blockIdx.y) * 2 + w) * cols + c] = T(t);
+    // wave w folds columns' sum w of each lane (2 VN <= W)
+    if (w < 2 * VN && c + w % VN < cols) {
+        double t = sh[0][w][lane];
+        for (int i = 1; i < W; i++) t += sh[i][w][lane];
+        a.part[(int64_t(blockIdx.y) * 2 + w / VN) * cols + c + w % VN] = T(t);
     }
 }
 
@@ -687,62 +813,95 @@ struct Partials {
     }
 };
 
-template <typename T, int MODE, int NT, int VPT>
-static int launch_ln_grad_rows(LnGradArgs<T> a, T *dgamma, T *dbeta)
+// Column sums by k_ln_cols and a fold.
+template <typename T>
+static int launch_ln_cols(LnGradArgs<T> a, T *dgamma, T *dbeta)
 {
-    constexpr bool kSums = true;
-    using Plan = LnGradPlan<T, NT, VPT, kSums>;
-    // as many blocks as the CUs hold at once, no more than rows
-    const int64_t most = int64_t(num_cus()) * Plan::kPerCu, need = ceil_div(a.rows, int64_t(Plan::RPB));
-    const int64_t nb = need < most ? need : most;
+    const int64_t gx = ceil_div(a.cols, 64 * Vec16<T>::n);
+    int64_t chunks = ceil_div(int64_t(num_cus()) * 2, gx);
+    const int64_t most = ceil_div(a.rows, 32);
+    chunks = chunks < most ? chunks : most;
+    const int64_t chunk = ceil_div(a.rows, chunks);
+    chunks = ceil_div(a.rows, chunk);
     Partials part;
-    if (dgamma || dbeta) {
-        NH_TRY(part.open(size_t(nb) * 2 * size_t(a.cols) * sizeof(T)));
-        a.part = static_cast<T *>(part.p);
-        NH_LAUNCH((k_ln_grad<T, NT, VPT, MODE, true>), dim3(unsigned(nb)), dim3(Plan::NB), 0, stream(), a);
-        NH_LAUNCH((k_ln_fold<T>), dim3(unsigned(ceil_div(2 * a.cols, 64))), dim3(1024), 0, stream(), a.part, nb, a.cols,
-                  dgamma, dbeta);
-    } else {
-        NH_LAUNCH((k_ln_grad<T, NT, VPT, MODE, false>), dim3(unsigned(nb)), dim3(Plan::NB), 0, stream(), a);
-    }
+    NH_TRY(part.open(size_t(chunks) * 2 * size_t(a.cols) * sizeof(T)));
+    a.part = static_cast<T *>(part.p);
+    NH_LAUNCH((k_ln_cols<T>), dim3(unsigned(gx), unsigned(chunks)), dim3(512), 0, stream(), a, chunk);
+    NH_LAUNCH((k_ln_fold<T>), dim3(unsigned(ceil_div(2 * a.cols, 64))), dim3(1024), 0, stream(), a.part, chunks, a.cols,
+              dgamma, dbeta);
     return check_launch();
 }
 
-// The fewest of LO to 4 vectors per lane of NT that hold the row.
-template <typename T, int MODE, int NT, int LO>
+// Few rows: what the one launch of k_ln_grad_few is for.  By the shape alone, so that equal
+// rows give equal sums whatever else a call asks for.
+constexpr int64_t kFewRows = 512, kFewValues = int64_t(1) << 20;
+static bool few_rows(int64_t rows, int64_t cols) { return rows <= kFewRows && rows * cols <= kFewValues; }
+
+template <typename T, int MODE, int NT, int VPT>
+static int launch_ln_grad_rows(const LnGradArgs<T> &a0, T *dgamma, T *dbeta)
+{
+    using Plan = LnGradPlan<T, NT, VPT>;
+    LnGradArgs<T> a = a0;
+    const bool sums = dgamma || dbeta, rows = a.dx || a.dres;
+    const int64_t need = ceil_div(a.rows, int64_t(Plan::RPB));
+    if (few_rows(a.rows, a.cols)) {
+        const auto few = [&](int64_t nr, int64_t nc) {
+            NH_LAUNCH((k_ln_grad_few<T, NT, VPT, MODE>), dim3(unsigned(nr + nc)), dim3(Plan::NB), 0, stream(), a, int(nr),
+                      dgamma, dbeta);
+        };
+        const int64_t nr = rows ? need : 0, nc = sums ? ceil_div(a.cols, 16) : 0;
+        // the columns read what an output in place writes over: they go first then
+        const bool over = a.dx == a.h || a.dx == a.dy || a.dres == a.h || a.dres == a.dy;
+        if (rows && sums && over) {
+            few(0, nc);
+            few(nr, 0);
+        } else {
+            few(nr, nc);
+        }
+        return check_launch();
+    }
+    // as many blocks as the CUs hold at once, no more than rows
+    const int64_t most = int64_t(num_cus()) * Plan::kPerCu;
+    const int64_t nb = need < most ? need : most;
+    if constexpr (VPT <= 8) {
+        if (sums) {
+            Partials part;
+            NH_TRY(part.open(size_t(nb) * 2 * size_t(a.cols) * sizeof(T)));
+            a.part = static_cast<T *>(part.p);
+            NH_LAUNCH((k_ln_grad<T, NT, VPT, MODE, true>), dim3(unsigned(nb)), dim3(Plan::NB), 0, stream(), a);
+            NH_LAUNCH((k_ln_fold<T>), dim3(unsigned(ceil_div(2 * a.cols, 64))), dim3(1024), 0, stream(), a.part, nb,
+                      a.cols, dgamma, dbeta);
+            return check_launch();
+        }
+    } else if (sums) {
+        NH_TRY(launch_ln_cols(a, dgamma, dbeta));
+    }
+    if (rows) NH_LAUNCH((k_ln_grad<T, NT, VPT, MODE, false>), dim3(unsigned(nb)), dim3(Plan::NB), 0, stream(), a);
+    return check_launch();
+}
+
+// The fewest of LO to HI vectors per lane of NT that hold the row.
+template <typename T, int MODE, int NT, int LO, int HI>
 static int launch_ln_grad_exact(const LnGradArgs<T> &a, int64_t ncv, T *dgamma, T *dbeta)
 {
-    if constexpr (LO < 4) {
-        if (ncv > NT * LO) return launch_ln_grad_exact<T, MODE, NT, LO + 1>(a, ncv, dgamma, dbeta);
+    if constexpr (LO < HI) {
+        if (ncv > NT * LO) return launch_ln_grad_exact<T, MODE, NT, LO + 1, HI>(a, ncv, dgamma, dbeta);
     }
     return launch_ln_grad_rows<T, MODE, NT, LO>(a, dgamma, dbeta);
 }
 
 template <typename T, int MODE>
-static int launch_ln_grad(LnGradArgs<T> a, T *dgamma, T *dbeta)
+static int launch_ln_grad(const LnGradArgs<T> &a, T *dgamma, T *dbeta)
 {
     const int64_t ncv = a.cols / Vec16<T>::n;
-    if (ncv <= 4 * 4) return launch_ln_grad_exact<T, MODE, 4, 1>(a, ncv, dgamma, dbeta);
-    if (ncv <= 16 * 4) return launch_ln_grad_exact<T, MODE, 16, 2>(a, ncv, dgamma, dbeta);
-    if (ncv <= 64 * 4) return launch_ln_grad_exact<T, MODE, 64, 2>(a, ncv, dgamma, dbeta);
-    if (ncv <= 256 * 4) return launch_ln_grad_exact<T, MODE, 256, 2>(a, ncv, dgamma, dbeta);
-    if (ncv <= 512 * 4) return launch_ln_grad_exact<T, MODE, 512, 3>(a, ncv, dgamma, dbeta);
-    if (ncv <= 1024 * 4) return launch_ln_grad_exact<T, MODE, 1024, 3>(a, ncv, dgamma, dbeta);
+    if (ncv <= 4 * 4) return launch_ln_grad_exact<T, MODE, 4, 1, 4>(a, ncv, dgamma, dbeta);
+    if (ncv <= 16 * 4) return launch_ln_grad_exact<T, MODE, 16, 2, 4>(a, ncv, dgamma, dbeta);
+    if (ncv <= 64 * 4) return launch_ln_grad_exact<T, MODE, 64, 2, 4>(a, ncv, dgamma, dbeta);
+    if (ncv <= 256 * 4) return launch_ln_grad_exact<T, MODE, 256, 2, 4>(a, ncv, dgamma, dbeta);
+    if (ncv <= 512 * 8) return launch_ln_grad_exact<T, MODE, 512, 3, 8>(a, ncv, dgamma, dbeta);
+    if (ncv <= 512 * 16) return launch_ln_grad_rows<T, MODE, 512, 16>(a, dgamma, dbeta);
     // the columns first: the row pass may write over what they read
-    Partials part;
-    if (dgamma || dbeta) {
-        const int64_t gx = ceil_div(a.cols, 64);
-        int64_t chunks = ceil_div(int64_t(num_cus()) * 2, gx);
-        const int64_t most = ceil_div(a.rows, 16);
-        chunks = chunks < most ? chunks : most;
-        const int64_t chunk = ceil_div(a.rows, chunks);
-        chunks = ceil_div(a.rows, chunk);
-        NH_TRY(part.open(size_t(chunks) * 2 * size_t(a.cols) * sizeof(T)));
-        a.part = static_cast<T *>(part.p);
-        NH_LAUNCH((k_ln_cols<T>), dim3(unsigned(gx), unsigned(chunks)), dim3(1024), 0, stream(), a, chunk);
-        NH_LAUNCH((k_ln_fold<T>), dim3(unsigned(ceil_div(2 * a.cols, 64))), dim3(1024), 0, stream(), a.part, chunks,
-                  a.cols, dgamma, dbeta);
-    }
+    if (dgamma || dbeta) NH_TRY(launch_ln_cols(a, dgamma, dbeta));
     if (a.dx || a.dres)
         for_row_launches(a.rows, 1, [&](unsigned g, int64_t base) {
             NH_LAUNCH((k_ln_grad_wide<T, MODE>), dim3(g), dim3(kLnWide), 0, stream(), a, base);
