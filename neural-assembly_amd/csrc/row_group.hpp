@@ -7,7 +7,7 @@
 namespace nh {
 
 // Group-wide max (NaN-ignoring) and sum over the NT lanes that share a row:
-// 4, 16 or 32 lanes of a wave or the whole wave (DPP moves, and swizzles across
+// 4, 8, 16 or 32 lanes of a wave or the whole wave (DPP moves, and swizzles across
 // 16 and 32), or a block of NT lanes through LDS.  (The f64 maximum by six
 // swizzles and NaN tests per row: [65536, 256] forward loss 41.3 us, now 37.7.)
 template <int NT>
@@ -26,7 +26,7 @@ struct RowGrp {
     NH_DEV static T part(T v, C comb)
     {
 #pragma unroll
-        for (int i = 0; i < (NT == 4 ? 2 : 4); i++) v = comb(v, dpp(v, i));
+        for (int i = 0; i < (NT == 4 ? 2 : NT == 8 ? 3 : 4); i++) v = comb(v, dpp(v, i));
         if constexpr (NT >= 32) v = comb(v, __shfl_xor(v, 16, 64));
         if constexpr (NT >= 64) v = comb(v, __shfl_xor(v, 32, 64));
         return v;

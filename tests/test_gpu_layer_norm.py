@@ -217,6 +217,36 @@ def test_nan_and_infinity_stay_in_their_rows(pn, rng, dt, cols):
     assert np.isfinite(got[0]).all()
 
 
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("rows,cols", [(511, 40), (512, 1001), (513, 1001), (512, 8192), (513, 8192), (512, 8200),
+                                       (2049, 2048), (777, 6001), (600, 12003), (700, 16385), (520, 33000), (20000, 12),
+                                       (30001, 33), (6000, 130), (5003, 390), (1200, 4100), (600, 70001)])
+def test_column_sums_exact(pn, dt, rows, cols):
+    """Small whole numbers, mean 0 and rstd 1: every term and sum of dgamma and
+    dbeta is a whole number below 2^24, so any order gives the same bits, in
+    each form that the sizes select; dx to its bound (torch in double)."""
+    import torch
+    tdt = torch.float32 if dt == np.float32 else torch.float64
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(rows * 7 + cols)
+    draw = lambda lo, hi, *s: torch.randint(lo, hi, s, device="cuda", generator=gen).to(tdt)  # noqa: E731
+    x, dy, g = draw(-3, 4, rows, cols), draw(-3, 4, rows, cols), draw(1, 4, cols)
+    m, r = torch.zeros(rows, dtype=tdt, device="cuda"), torch.ones(rows, dtype=tdt, device="cuda")
+    dx, dg, db = torch.empty_like(x), torch.full_like(g, 9), torch.full_like(g, 9)
+    T = pn.Tensor.from_torch
+    t = [T(v) for v in (dx, dg, db, dy, x, g, m, r)]
+    torch.cuda.synchronize()
+    assert pn.core._lib.neural_layer_norm_backward(*[v._ptr for v in t]) == 0
+    pn.synchronize()
+    X, DY, W = x.double(), dy.double(), dy.double() * g.double()
+    assert torch.equal(dg.double(), (DY * X).sum(0)) and torch.equal(db.double(), DY.sum(0))
+    want = W - W.mean(1, keepdim=True) - X * (W * X).mean(1, keepdim=True)
+    # W and X are at most 9 and 3, the means' sums exact: under 16 roundings of values below 100, and
+    # the last to the type
+    lim = 100 * 16 * ref.D + (ref.U[np.dtype(dt)] if dt == np.float32 else 0) * want.abs()
+    assert bool(((dx.double() - want).abs() <= lim).all())
+
+
 def _numeric(f, x, at, step):
     lo, hi = x.copy(), x.copy()
     lo.reshape(-1)[at] -= step
