@@ -19,13 +19,24 @@ struct LnGradPlan {
     static constexpr bool kGammaRegs = VPT <= 4 || VPT == 7 || VPT == 8;
     static constexpr bool kGammaLds = VPT == 5 || VPT == 6;            // 144 KB with the sums
     // Two rows in turn, not copied from one to the other, which waits for the second's
-    // loads before the third's are issued: for the one block that a CU holds.
-    static constexpr bool kTurns = NT == 512 && VPT <= 8;
+    // loads before the third's are issued: for the one block that a CU holds, where
+    // the registers allow it.  f32 [6710, 5000] 86.7 -> 79.8 us, joined 136 -> 130;
+    // where other blocks fill the wait it loses ([43690, 768] 71.8, with it 75.8).
+    static constexpr bool turns(int mode)
+    {
+        return NT == 512 && (mode == LN_PLAIN ? VPT <= 8 : VPT <= 6 && VPT != 4);
+    }
     static constexpr int F = VPT <= 8 ? VPT - 1 : VPT / 2;  // vectors that are whole
     static constexpr int kWaves = VPT >= 3 || NT >= 512 ? 2 : 3;  // per SIMD
     static constexpr int kPerCu = kWaves * 256 / NB;              // resident blocks
 };
 
+// Bound by HBM: three streams (the joined forms five), and for the listed widths within
+// 10% of a copy of the same bytes: f32 [16384, 4096] 135 us where the copy takes 134, and 4.9
+// for the partials' fold (k_ln_fold); joined 224 and 4.9 (225); [200000, 96] 39.8 and 4.6 (38).
+// f64 rows of an odd width, whose accesses straddle one 128-byte line in eight: 39.9 and
+// 5.4 at [4096, 2049] (33).
+//
 // Groups of NT lanes walk the rows, r = group, group + groups, ...: each tensor
 // read once, the next row's loads issued before this one is worked on, the row's
 // two sums by one exchange (LDS slots alternate between rows, so one barrier a row
@@ -233,7 +244,7 @@ NH_DEV void ln_grad_rows(const LnGradArgs<T> &a, int64_t block, int64_t blocks)
     };
     Row w;
     if (r < a.rows) load(w, r);
-    if constexpr (Plan::kTurns && MODE == LN_PLAIN) {
+    if constexpr (Plan::turns(MODE)) {
         Row v;
         while (r < a.rows) {
             work(w, v, r, 0, true);
@@ -393,7 +404,10 @@ NH_DEV void ln_few_cols(const LnGradArgs<T> &a, int64_t block, T *dgamma, T *dbe
 
 // The backward pass of few rows in one launch: blocks 0 .. nrows - 1 take the rows,
 // the others columns (which read x and dy again, from the caches).  Either
-// part may be absent.
+// part may be absent.  Bound by latency; against the row pass and a fold of its
+// partials (two launches and a round trip): f32 [197, 768] 7.9 -> 3.9 us, [256, 4096] 11.5 ->
+// 5.6, [512, 4096] 17.1 -> 10.7, f64 [512, 1024] 13.1 -> 6.9.  From some 1000 rows a column's
+// stream of rows is longer than that ([1000, 1000] 11.1, 20).
 template <typename T, int NT, int VPT, int MODE>
 __global__ __launch_bounds__((LnGradPlan<T, NT, VPT>::NB)) void k_ln_grad_few(LnGradArgs<T> a, int nrows, T *dgamma,
                                                                              T *dbeta)
