@@ -36,7 +36,7 @@ struct LnArgs {
 };
 
 // How a group's lanes hold a row: NT lanes, VPT vectors each, the first F of them whole.
-// kAhead: two rows, one in flight while the other is worked on, and gamma and beta in registers.
+// kAhead: two rows, one in flight while the other is worked on.
 // Then a CU holds about 12 vectors a lane and SIMD of rows in flight (48 KB); more
 // or fewer wait longer: f32 [8192, 4096] (4 vectors) 45.7 us with 3 waves a SIMD, 47.4 with
 // 4, and 50.7 with a row per block; [16384, 2048] (2 vectors) 46.9 with 5, 48.0 with 6,
@@ -46,6 +46,10 @@ template <typename T, int NT, int VPT, int MODE>
 struct LnPlan {
     static constexpr int NB = NT < 256 ? 256 : NT, RPB = NB / NT;
     static constexpr bool kAhead = MODE == LN_PLAIN && NT < 1024;
+    // gamma and beta are loaded before the row's sums, not behind them: joined f32 [64, 4096]
+    // 4.5 -> 4.1 us, [8192, 4096] 93.0 -> 89.5 (with dropout 93.0, 92.4; [4096, 1024], from the
+    // caches, 12.5 -> 13.4: 96 registers instead of 64)
+    static constexpr bool kParams = kAhead || (VPT <= 4 && NT < 1024);
     static constexpr int F = NT < 1024 || VPT <= 4 ? VPT - 1 : VPT / 2;
     static constexpr int kWaves = !kAhead ? (NT == 1024 ? 4 : 1) : VPT >= 5 ? 2 : VPT >= 3 ? 3 : VPT == 2 ? 5 : 8;
     static constexpr int kPerCu = kWaves * 256 / NB;  // resident blocks
@@ -78,8 +82,8 @@ __global__ __launch_bounds__((LnPlan<T, NT, VPT, MODE>::NB), (LnPlan<T, NT, VPT,
         if (p && in_row(k)) v = *(reinterpret_cast<const U *>(p) + lane + k * NT);
         return v;
     };
-    V g[Plan::kAhead ? VPT : 1], b[Plan::kAhead ? VPT : 1];
-    if constexpr (Plan::kAhead) {
+    V g[Plan::kParams ? VPT : 1], b[Plan::kParams ? VPT : 1];
+    if constexpr (Plan::kParams) {
 #pragma unroll
         for (int k = 0; k < VPT; k++) {
             g[k] = param(a.gamma, k, T(1));
@@ -174,7 +178,7 @@ __global__ __launch_bounds__((LnPlan<T, NT, VPT, MODE>::NB), (LnPlan<T, NT, VPT,
             if (in_row(k)) {
                 hide(w.x[k]);
                 V gk, bk, o;
-                if constexpr (Plan::kAhead) {
+                if constexpr (Plan::kParams) {
                     hide(g[k]);
                     hide(b[k]);
                     gk = g[k];

@@ -169,6 +169,55 @@ def test_optional_tensors(pn, rng, dt):
 
 
 @pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("rows,cols", [(6, 50), (900, 50), (700, 5003), (3, 40000), (3, 70001)])
+def test_each_output_alone(pn, rng, dt, rows, cols):
+    """Every output of the backward calls left out in turn, or alone: the others
+    keep their bits.  p of 1 drops the sublayer's output and its gradient."""
+    lib, T = pn.core._lib, pn.Tensor
+    c = _case(rng, rows, cols, dt)
+    key = _key(pn, 6, 6)
+    y, h, mean, rstd = _joined(pn, c, 0.3, key)
+    want = _joined_grad(pn, c, h, mean, rstd, 0.3, key)
+    dy, dh, th, g, m, r = (T.from_numpy(v) for v in (c["dy"], c["dh"], h, c["g"], mean, rstd))
+    shapes = [h.shape, h.shape, [cols], [cols]]
+    for take in ((0,), (1,), (2,), (3,), (0, 2), (1, 3), (0, 1), (1, 2, 3), (0, 2, 3)):
+        o = [T.create(shapes[i], g.dtype) if i in take else None for i in range(4)]
+        assert lib.neural_dropout_add_layer_norm_backward(*[_p(v) for v in o], dy._ptr, dh._ptr, th._ptr, g._ptr,
+                                                          m._ptr, r._ptr, 0.3, key) == 0
+        for i in take:
+            same_bits(o[i].numpy(), want[i])
+    y, h, mean, rstd = _joined(pn, c, 1.0, key)
+    same_bits(h, c["res"] + dt(0))
+    dx, dres, _, _ = _joined_grad(pn, c, h, mean, rstd, 1.0, key)
+    assert not dx.any() and not np.signbit(dx).any() and dres.any()
+
+
+@pytest.mark.parametrize("dt", DT)
+def test_joined_on_host_buffers(pn, rng, dt):
+    """Tensors over host memory in both joined calls, the hidden state in place
+    of the residual, two wrappers of one buffer among them."""
+    c = _case(rng, 9, 77, dt)
+    key = _key(pn, 1, 5)
+    y, h, mean, rstd = _joined(pn, c, 0.4, key)
+    grads = _joined_grad(pn, c, h, mean, rstd, 0.4, key)
+    Z, lib = pn.Tensor.from_numpy_zero_copy, pn.core._lib
+    b = {k: v.copy() for k, v in c.items()}
+    b.update(y=np.zeros_like(y), m=np.zeros_like(mean), r=np.zeros_like(rstd), dg=np.zeros_like(c["g"]),
+             db=np.zeros_like(c["g"]))
+    t = {k: Z(v) for k, v in b.items()}
+    again = Z(b["res"])  # the same buffer: the hidden state goes over the residual
+    assert lib.neural_dropout_add_layer_norm_forward(t["y"]._ptr, again._ptr, t["x"]._ptr, t["res"]._ptr, t["g"]._ptr,
+                                                     t["b"]._ptr, 0.4, key, EPS, t["m"]._ptr, t["r"]._ptr) == 0
+    for a, w in zip((b["y"], b["res"], b["m"], b["r"]), (y, h, mean, rstd)):
+        same_bits(a, w)
+    assert lib.neural_dropout_add_layer_norm_backward(t["dy"]._ptr, t["dh"]._ptr, t["dg"]._ptr, t["db"]._ptr,
+                                                      t["dy"]._ptr, t["dh"]._ptr, t["res"]._ptr, t["g"]._ptr,
+                                                      t["m"]._ptr, t["r"]._ptr, 0.4, key) == 0
+    for a, w in zip((b["dy"], b["dh"], b["dg"], b["db"]), grads):
+        same_bits(a, w)
+
+
+@pytest.mark.parametrize("dt", DT)
 @pytest.mark.parametrize("cols", [24, 300, 2050, 70001])
 def test_extreme_rows(pn, rng, dt, cols):
     """Rows of one value, of a value far from their spread, of the largest and
