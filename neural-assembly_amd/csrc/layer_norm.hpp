@@ -1,5 +1,5 @@
 // layer_norm.hpp -- what the forward (layer_norm.hip) and the backward pass
-// (layer_norm_grad.hip) of layer norm share: the modes, rounding helpers and the keep bits
+// (layer_norm_grad_impl.hpp) of layer norm share: the modes, rounding helpers and the keep bits
 // of a row's values.
 #pragma once
 

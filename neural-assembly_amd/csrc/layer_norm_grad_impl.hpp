@@ -1,5 +1,8 @@
-// layer_norm_grad.hip -- the backward pass of layer norm and of its join with the residual
-// add and the counter-based dropout (formulas: layer_norm.hip).
+// layer_norm_grad_impl.hpp -- the backward pass of layer norm and of its join with the residual
+// add and the counter-based dropout (formulas: layer_norm.hip), compiled for each type by
+// layer_norm_grad_f32.hip and layer_norm_grad_f64.hip.
+#pragma once
+
 #include <type_traits>
 
 #include "layer_norm.hpp"
@@ -605,7 +608,7 @@ static int launch_ln_cols(LnGradArgs<T> a, T *dgamma, T *dbeta)
 // Few rows: what the one launch of k_ln_grad_few is for.  By the shape alone, so that equal
 // rows give equal sums whatever else a call asks for.
 constexpr int64_t kFewRows = 512, kFewValues = int64_t(1) << 22;
-static bool few_rows(int64_t rows, int64_t cols) { return rows <= kFewRows && rows * cols <= kFewValues; }
+inline bool few_rows(int64_t rows, int64_t cols) { return rows <= kFewRows && rows * cols <= kFewValues; }
 
 template <typename T, int MODE, int NT, int VPT>
 static int launch_ln_grad_rows(const LnGradArgs<T> &a0, T *dgamma, T *dbeta)
@@ -683,12 +686,5 @@ int launch_ln_grad(const LnGradArgs<T> &a, T *dgamma, T *dbeta)
         });
     return check_launch();
 }
-
-template int launch_ln_grad<float, LN_PLAIN>(const LnGradArgs<float> &, float *, float *);
-template int launch_ln_grad<float, LN_ADD>(const LnGradArgs<float> &, float *, float *);
-template int launch_ln_grad<float, LN_DROP>(const LnGradArgs<float> &, float *, float *);
-template int launch_ln_grad<double, LN_PLAIN>(const LnGradArgs<double> &, double *, double *);
-template int launch_ln_grad<double, LN_ADD>(const LnGradArgs<double> &, double *, double *);
-template int launch_ln_grad<double, LN_DROP>(const LnGradArgs<double> &, double *, double *);
 
 }  // namespace nh
