@@ -144,6 +144,68 @@ struct LnGradArgs {
 template <typename T, int MODE>
 int launch_ln_grad(const LnGradArgs<T> &a, T *dgamma, T *dbeta);
 
-constexpr int kLnWide = 1024;  // lanes of the kernels for rows wider than the registers
+// ---- rows wider than a group's registers -------------------------------------------------
+
+constexpr int kLnWide = 1024;  // lanes of their blocks
+
+// W values side by side: a 16-byte access at the element's own alignment, or one element.
+template <typename T, int W>
+struct Pack {
+    T v[W];
+    NH_DEV static Pack load(const T *p)
+    {
+        Pack r;
+        if constexpr (W == 1) {
+            r.v[0] = *p;
+        } else {
+            const typename VecU<T>::type u = *reinterpret_cast<const typename VecU<T>::type *>(p);
+#pragma unroll
+            for (int j = 0; j < W; j++) r.v[j] = u[j];
+        }
+        return r;
+    }
+    NH_DEV void store(T *p) const
+    {
+        if constexpr (W == 1) {
+            *p = v[0];
+        } else {
+            typename Vec16<T>::type u;
+#pragma unroll
+            for (int j = 0; j < W; j++) u[j] = v[j];
+            *reinterpret_cast<typename VecU<T>::type *>(p) = u;
+        }
+    }
+};
+
+// The row's columns by a block of kLnWide lanes, four vectors in flight each, then the
+// values past the vectors: use(width, first column, load(width, first column)).
+template <typename T, typename L, typename F>
+NH_DEV void walk_row(int64_t cols, L load, F use)
+{
+    constexpr int VN = Vec16<T>::n, UN = 4;
+    using W = std::integral_constant<int, VN>;
+    const int64_t ncv = cols / VN;
+    for (int64_t q = threadIdx.x; q < ncv; q += UN * kLnWide) {
+        decltype(load(W{}, q)) v[UN];
+#pragma unroll
+        for (int u = 0; u < UN; u++)
+            if (q + u * kLnWide < ncv) v[u] = load(W{}, (q + u * kLnWide) * VN);
+#pragma unroll
+        for (int u = 0; u < UN; u++)
+            if (q + u * kLnWide < ncv) use(W{}, (q + u * kLnWide) * VN, v[u]);
+    }
+    const int64_t c = ncv * VN + threadIdx.x;
+    if (c < cols) use(std::integral_constant<int, 1>{}, c, load(std::integral_constant<int, 1>{}, c));
+}
+
+// Keep bits of the W elements from flat index i, element j at bit j.
+template <int W>
+NH_DEV uint32_t keep_at(int64_t i, const DropKey &key)
+{
+    const int o = int(i & 7);
+    uint32_t m = keep_in_order(keep_mask(uint64_t(i) / 8, key)) >> o;
+    if (o + W > 8) m |= keep_in_order(keep_mask(uint64_t(i) / 8 + 1, key)) << (8 - o);
+    return m;
+}
 
 }  // namespace nh
