@@ -213,7 +213,8 @@ __global__ __launch_bounds__((LnPlan<T, NT, VPT, MODE>::NB), (LnPlan<T, NT, VPT,
 // Rows wider than a block's registers, in three walks of a block: h and its sum, the
 // centred squares, y.  How much of the row the caches keep between the walks bounds it
 // (f32 [335, 100000] 100 us, 177 us joined with dropout and h stored; a copy of the same
-// bytes 43 and 86; element by element it took 2 to 3 times as long).
+// bytes 43 and 86; element by element it took 178 and 410, and f32 [127, 262147] 390, now
+// 132).
 template <typename T, int MODE>
 __global__ __launch_bounds__(kLnWide) void k_ln_wide(LnArgs<T> a, int64_t r_base)
 {
