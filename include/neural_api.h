@@ -383,8 +383,9 @@ int neural_counter_dropout_backward(NeuralTensor *grad_in, const NeuralTensor *g
  * Backward, from the saved mean and rstd: xh = (in - mean) rstd, w = grad_out
  * gamma, grad_in = rstd (w - mean_C(w) - xh mean_C(w xh)), grad_gamma = sum over
  * rows of grad_out xh, grad_beta = sum over rows of grad_out.  Any output may be NULL, not all.
- * grad_in may be grad_out or in.  The sums' order depends on the shape and the device
- * alone: equal calls give equal bits.
+ * grad_in may be grad_out or in.  The sums over rows are in double; what a group of
+ * rows leaves of them is rounded to the dtype, and the result.  Their order depends on
+ * the shape and the device alone: equal calls give equal bits.
  *
  * Joined with what precedes it in a transformer's sublayer: hidden = residual +
  * dropout(in) and the norm of hidden, in one pass.  hidden has the bits of neural_add(residual,

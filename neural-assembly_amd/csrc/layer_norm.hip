@@ -11,7 +11,7 @@
 //             dgamma = sum_rows dy xh; dbeta = sum_rows dy
 //
 // Everything between the loads and the stores is in double, f32 rows rounded once
-// per output; mean and rstd are stored in the rows' type (the mean's rounding
+// per output (dgamma and dbeta once more for what each block leaves of them); mean and rstd are stored in the rows' type (the mean's rounding
 // moves xh by what half an ulp of an input of the mean's size would).  The
 // variance is taken from the centred values, which are still in registers.
 //

@@ -10,15 +10,16 @@
 namespace nh {
 
 // How a group's lanes hold a row of the backward pass, and how many groups a CU
-// holds.  NT lanes, VPT vectors each.  Up to 4 vectors: gamma and the sums of dgamma and dbeta
-// (in double) in registers.  5 to 8: the sums in LDS, in the rows' type (128 KB at
-// most), and gamma too where it fits beside them, else in registers: a load of it
-// for each row would wait for the next row's loads, which are older.  More: no
-// sums (k_ln_cols takes them), gamma from the L2.
+// holds.  NT lanes, VPT vectors each.  The sums of dgamma and dbeta over the rows are in
+// double in every form: up to 4 vectors both in registers, and gamma; 5 to 8 vectors in LDS
+// (128 KB at most: f64 rows both, f32 rows dgamma's, with dbeta's in registers), and gamma too
+// where it fits beside them, else in registers: a load of it for each row would wait for the next
+// row's loads, which are older.  16 vectors: no sums (k_ln_cols takes them), gamma from the L2.
 template <typename T, int NT, int VPT>
 struct LnGradPlan {
     static constexpr int NB = NT < 256 ? 256 : NT, RPB = NB / NT;
-    static constexpr bool kRegs = VPT <= 4;                            // sums
+    static constexpr bool kRegs = VPT <= 4;                            // both sums in registers
+    static constexpr bool kSplit = !kRegs && VPT <= 8 && sizeof(T) == 4;  // dbeta's in registers, dgamma's in LDS
     static constexpr bool kGammaRegs = VPT <= 4 || VPT == 7 || VPT == 8;
     static constexpr bool kGammaLds = VPT == 5 || VPT == 6;            // 144 KB with the sums
     // Two rows in turn, not copied from one to the other, which waits for the second's
@@ -47,6 +48,14 @@ struct LnGradPlan {
 // The block's groups fold theirs through LDS and the block leaves one row of
 // partials, in the rows' type (the rounding of one of some hundred terms of a sum that is
 // itself rounded so).  `block` of `blocks`.
+//
+// f32 rows of 8193 to 16387 values have one block's sums of 256 KB: dgamma's take 128 KB of LDS
+// and dbeta's 64 registers a lane, which leaves none for a second row where gamma is in
+// registers too (7 and 8 vectors, the joined forms' 6): there a vector of the next row is
+// loaded as soon as this row's has been used for the last time, and dh behind the row's sums.
+// (Both sums in LDS as floats, rounded every row, and the next row in registers: [2048, 16384]
+// 84.3 us, now 85.8, joined 155, now 148; [2396, 14000] 88.4, now 92.3, joined 159, now 149;
+// narrower alike; but 80 rows a block lost 11 u in dbeta, now 2 u.)
 template <typename T, int NT, int VPT, int MODE, bool SUMS, bool PAST>
 NH_DEV void ln_grad_rows(const LnGradArgs<T> &a, int64_t block, int64_t blocks)
 {
@@ -57,11 +66,17 @@ NH_DEV void ln_grad_rows(const LnGradArgs<T> &a, int64_t block, int64_t blocks)
     using S = RowStream<T, PAST>;
     using Plan = LnGradPlan<T, NT, VPT>;
     constexpr int VN = Vec16<T>::n, RPB = Plan::RPB;
-    constexpr bool LS = SUMS && !Plan::kRegs, RS = SUMS && Plan::kRegs;
+    using D2 = typename Vec16<double>::type;
+    constexpr bool SS = SUMS && Plan::kSplit, RS = SUMS && Plan::kRegs, LS = SUMS && !SS && !RS;
+    constexpr bool RB = RS || SS;  // dbeta's sums in registers
+    static_assert(!LS || sizeof(T) == 8, "the sums are in double");
     __shared__ double lds_s[2][G::kWaves], lds_q[2][G::kWaves];
     __shared__ uint8_t lds_keep[2][MODE == LN_DROP ? RPB : 1][MODE == LN_DROP ? K::kBytes : 1];
     __shared__ V lds_g[LS ? VPT : 1][LS ? NT : 1], lds_b[LS ? VPT : 1][LS ? NT : 1];
-    const int lane = threadIdx.x % NT, sub = threadIdx.x / NT;
+    __shared__ D2 lds_split[SS ? VPT : 1][SS ? VN / 2 : 1][SS ? NT : 1];
+    // (a block of one row: a uniform row saves the address registers that SS is short of; the
+    // other forms are no faster for it, joined [16384, 4096] 232 us, without 230.5)
+    const int lane = threadIdx.x % NT, sub = SS && RPB == 1 ? 0 : threadIdx.x / NT;
     const int64_t cols = a.cols;
     const RowCut<T> cut(cols);
     const auto in_row = [&](int k) { return k < Plan::F || lane + k * NT < cut.ncv; };
@@ -88,12 +103,17 @@ NH_DEV void ln_grad_rows(const LnGradArgs<T> &a, int64_t block, int64_t blocks)
     };
     T gt = T(1);
     if (a.gamma && has_t) gt = a.gamma[cut.sc(lane)];
-    double sg[RS ? VPT : 1][VN], sb[RS ? VPT : 1][VN], sgt = 0.0, sbt = 0.0;
+    double sg[RS ? VPT : 1][VN], sb[RB ? VPT : 1][VN], sgt = 0.0, sbt = 0.0;
 #pragma unroll
     for (int k = 0; k < VPT; k++) {
         if constexpr (RS) {
 #pragma unroll
             for (int j = 0; j < VN; j++) sg[k][j] = sb[k][j] = 0.0;
+        } else if constexpr (SS) {
+#pragma unroll
+            for (int j = 0; j < VN; j++) sb[k][j] = 0.0;
+#pragma unroll
+            for (int i = 0; i < VN / 2; i++) lds_split[k][i][lane] = D2{0.0, 0.0};  // a lane's own slots
         } else if constexpr (LS) {
             V z;
 #pragma unroll
@@ -107,38 +127,47 @@ NH_DEV void ln_grad_rows(const LnGradArgs<T> &a, int64_t block, int64_t blocks)
         V x[VPT], dy[VPT];
         T xt, dyt, mean, rstd;
     };
-    const auto load = [&](Row &w, int64_t r) {
-        const int64_t at = r * cols;
+    const auto load_x = [&](Row &w, int64_t at, int k) {
+        if (in_row(k)) w.x[k] = S::load(reinterpret_cast<const U *>(a.h + at) + lane + k * NT);
+    };
+    const auto load_dy = [&](Row &w, int64_t at, int k) {
+        if (in_row(k)) w.dy[k] = S::load(reinterpret_cast<const U *>(a.dy + at) + lane + k * NT);
+    };
+    const auto load_scalars = [&](Row &w, int64_t r) {
         w.mean = a.mean[r];
         w.rstd = a.rstd[r];
-#pragma unroll
-        for (int k = 0; k < VPT; k++)
-            if (in_row(k)) w.x[k] = S::load(reinterpret_cast<const U *>(a.h + at) + lane + k * NT);
-#pragma unroll
-        for (int k = 0; k < VPT; k++)
-            if (in_row(k)) w.dy[k] = S::load(reinterpret_cast<const U *>(a.dy + at) + lane + k * NT);
         if (has_t) {
-            w.xt = a.h[at + cut.sc(lane)];
-            w.dyt = a.dy[at + cut.sc(lane)];
+            w.xt = a.h[r * cols + cut.sc(lane)];
+            w.dyt = a.dy[r * cols + cut.sc(lane)];
         }
+    };
+    const auto load = [&](Row &w, int64_t r) {
+        const int64_t at = r * cols;
+#pragma unroll
+        for (int k = 0; k < VPT; k++) load_x(w, at, k);
+#pragma unroll
+        for (int k = 0; k < VPT; k++) load_dy(w, at, k);
+        load_scalars(w, r);
     };
     const int64_t step = blocks * RPB;
     int64_t r = block * RPB + sub;
+    // kReload: no registers for two rows; a vector of the next row is loaded where this row's
+    // has been used for the last time.
+    constexpr bool kReload = SS && (Plan::kGammaRegs || (MODE != LN_PLAIN && VPT == 6));
     // Work on row r in w; `ahead`: the next row's loads are issued here, into next.
     const auto work = [&](Row &w, Row &next, int64_t r, int odd, bool ahead) {
         const int64_t at = r * cols;
         constexpr bool kEarly = MODE != LN_PLAIN && VPT <= 8;  // dh fits beside x and dy
         V dh[kEarly ? VPT : 1];
         T dht = T(0);
-        if constexpr (MODE != LN_PLAIN) {
-            if (a.dh) {
+        const auto load_dh = [&] {
+            if (!a.dh) return;
 #pragma unroll
-                for (int k = 0; k < (kEarly ? VPT : 0); k++)
-                    if (in_row(k))
-                        dh[k] = S::load(reinterpret_cast<const U *>(a.dh + at) + lane + k * NT);
-                if (has_t) dht = a.dh[at + cut.sc(lane)];
-            }
-        }
+            for (int k = 0; k < (kEarly ? VPT : 0); k++)
+                if (in_row(k)) dh[k] = S::load(reinterpret_cast<const U *>(a.dh + at) + lane + k * NT);
+            if (has_t) dht = a.dh[at + cut.sc(lane)];
+        };
+        if constexpr (MODE != LN_PLAIN && !kReload) load_dh();
         if (ahead && r + step < a.rows) load(next, r + step);
         const double mean = double(w.mean), rstd = double(w.rstd);
         K keep;
@@ -156,9 +185,13 @@ NH_DEV void ln_grad_rows(const LnGradArgs<T> &a, int64_t block, int64_t blocks)
             if (in_row(k)) {
                 const V gk = gamma_of(k);
                 V vg, vb;
+                D2 vd[SS ? VN / 2 : 1];
                 if constexpr (LS) {
                     vg = lds_g[k][lane];
                     vb = lds_b[k][lane];
+                } else if constexpr (SS) {
+#pragma unroll
+                    for (int i = 0; i < VN / 2; i++) vd[i] = lds_split[k][i][lane];
                 }
 #pragma unroll
                 for (int j = 0; j < VN; j++) {
@@ -167,8 +200,12 @@ NH_DEV void ln_grad_rows(const LnGradArgs<T> &a, int64_t block, int64_t blocks)
                         sums(w.x[k][j], w.dy[k][j], gk[j], ag, ab);
                         vg[j] = T(ag);
                         vb[j] = T(ab);
+                    } else if constexpr (SS) {
+                        double ag = vd[j / 2][j % 2];
+                        sums(w.x[k][j], w.dy[k][j], gk[j], ag, sb[k][j]);
+                        vd[j / 2][j % 2] = ag;
                     } else {
-                        sums(w.x[k][j], w.dy[k][j], gk[j], sg[RS ? k : 0][j], sb[RS ? k : 0][j]);
+                        sums(w.x[k][j], w.dy[k][j], gk[j], sg[RS ? k : 0][j], sb[RB ? k : 0][j]);
                     }
                 }
                 if constexpr (RS) {
@@ -182,8 +219,16 @@ NH_DEV void ln_grad_rows(const LnGradArgs<T> &a, int64_t block, int64_t blocks)
                     lds_b[k][lane] = vb;
                     asm volatile("" : "+v"(s), "+v"(q) : : "memory");  // one vector's terms in registers at a time
                 }
+                if constexpr (SS) {
+#pragma unroll
+                    for (int i = 0; i < VN / 2; i++) lds_split[k][i][lane] = vd[i];
+#pragma unroll
+                    for (int j = 0; j < VN; j++) asm volatile("" : "+v"(sb[k][j]));
+                    asm volatile("" : "+v"(s), "+v"(q) : : "memory");
+                }
             }
         if (has_t) sums(w.xt, w.dyt, gt, sgt, sbt);
+        if constexpr (MODE != LN_PLAIN && kReload) load_dh();
         // both sums over the row by one exchange
         const auto add = [](double p, double t) { return p + t; };
         s = G::part(s, add);
@@ -207,8 +252,10 @@ NH_DEV void ln_grad_rows(const LnGradArgs<T> &a, int64_t block, int64_t blocks)
             const double xh = (double(xv) - mean) * rstd, wv = double(dyv) * double(gv);
             return T(rstd * (__builtin_fma(-xh, c2, wv - c1)));
         };
+        const int64_t after = (r + step) * cols;
+        const bool again = kReload && r + step < a.rows;
 #pragma unroll
-        for (int k = 0; k < VPT; k++)
+        for (int k = 0; k < VPT; k++) {
             if ((MODE != LN_PLAIN || a.dx) && in_row(k)) {
                 hide(w.x[k]);
                 hide(w.dy[k]);
@@ -234,6 +281,11 @@ NH_DEV void ln_grad_rows(const LnGradArgs<T> &a, int64_t block, int64_t blocks)
                 if (MODE == LN_PLAIN || a.dx)
                     S::store(o, reinterpret_cast<U *>(a.dx + at) + lane + k * NT);
             }
+            if (again) {
+                load_x(w, after, k);
+                load_dy(w, after, k);
+            }
+        }
         if (has_t) {
             const int64_t i = at + cut.sc(lane);
             T o = grad(w.xt, w.dyt, gt);
@@ -244,10 +296,13 @@ NH_DEV void ln_grad_rows(const LnGradArgs<T> &a, int64_t block, int64_t blocks)
             if constexpr (MODE == LN_DROP) o = dropped<T>(o, scale, keep.tail, 0);
             if (a.dx) a.dx[i] = o;
         }
+        if (again) load_scalars(w, r + step);
     };
     Row w;
     if (r < a.rows) load(w, r);
-    if constexpr (Plan::turns(MODE)) {
+    if constexpr (kReload) {
+        for (int odd = 0; r < a.rows; r += step, odd ^= 1) work(w, w, r, odd, false);
+    } else if constexpr (Plan::turns(MODE)) {
         Row v;
         while (r < a.rows) {
             work(w, v, r, 0, true);
@@ -281,7 +336,7 @@ NH_DEV void ln_grad_rows(const LnGradArgs<T> &a, int64_t block, int64_t blocks)
                     } else {
 #pragma unroll
                         for (int j = 0; j < VN; j++) {
-                            og[j] = T(sg[k][j]);
+                            og[j] = T(SS ? lds_split[k][SS ? j / 2 : 0][lane][j % 2] : sg[RS ? k : 0][j]);
                             ob[j] = T(sb[k][j]);
                         }
                     }

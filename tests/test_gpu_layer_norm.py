@@ -710,3 +710,36 @@ def test_modules_train_together(pn, rng, dt):
     assert all(not np.array_equal(b, p.numpy()) for b, p in zip(before, ps))
     with pytest.raises(ValueError):
         pre(pn.Tensor.zeros([3, cols + 1], code))
+
+
+@pytest.mark.parametrize("dt,cols", [(np.float32, c) for c in (8200, 10300, 12300, 14341, 16391, 20000)] +
+                         [(np.float64, c) for c in (4200, 6150, 7200, 12003)])
+def test_wide_forms_of_many_rows(pn, rng, dt, cols):
+    """More rows than the one launch of few rows takes and than two for each block, at every
+    number of vectors a lane past four, alone and joined."""
+    _check_all(pn, rng, 530, cols, dt)
+
+
+@pytest.mark.parametrize("rows,cols", [(20001, 5000), (20000, 8200), (20000, 10300), (20001, 13001), (20000, 16384),
+                                       (9000, 20000)])
+def test_column_sums_of_one_sign(pn, rows, cols):
+    """f32 terms of one sign, 35 to 80 rows to a block's sums: dgamma and dbeta carry the
+    rounding of the partials and of the result, u each, whatever the rows (sums in double:
+    (rows + 8) 2^-53 beside them).  mean 0 and rstd 1, so xh is x itself."""
+    import torch
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(rows + cols)
+    x = torch.rand(rows, cols, device="cuda", generator=gen) + 0.5
+    dy = torch.full((rows, cols), 0.1, device="cuda")
+    m, r = torch.zeros(rows, device="cuda"), torch.ones(rows, device="cuda")
+    dg, db = torch.empty(cols, device="cuda"), torch.empty(cols, device="cuda")
+    T = pn.Tensor.from_torch
+    t = [T(v) for v in (dg, db, dy, x, m, r)]
+    torch.cuda.synchronize()
+    assert pn.core._lib.neural_layer_norm_backward(None, t[0]._ptr, t[1]._ptr, t[2]._ptr, t[3]._ptr, None, t[4]._ptr,
+                                                   t[5]._ptr) == 0
+    pn.synchronize()
+    d = dy[0].double()
+    lim = 1.01 * (2 * ref.U[np.dtype(np.float32)] + (rows + 8) * ref.D)
+    for got, want in ((dg, d * x.double().sum(0)), (db, d * rows)):
+        assert float(((got.double() - want).abs() / want).max()) <= lim
