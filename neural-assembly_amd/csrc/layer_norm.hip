@@ -10,10 +10,11 @@
 //             reaches h besides]; dresidual = d, dx = dropout's map of d;
 //             dgamma = sum_rows dy xh; dbeta = sum_rows dy
 //
-// Everything between the loads and the stores is in double, f32 rows rounded once
-// per output (dgamma and dbeta once more for what each block leaves of them); mean and rstd are stored in the rows' type (the mean's rounding
-// moves xh by what half an ulp of an input of the mean's size would).  The
-// variance is taken from the centred values, which are still in registers.
+// Everything between the loads and the stores is in double, f32 rows rounded once per
+// output (dgamma and dbeta once more for what each block leaves of them); mean and rstd
+// are stored in the rows' type (the mean's rounding moves xh by what half an ulp of an
+// input of the mean's size would).  The variance is taken from the centred values, which
+// are still in registers.
 //
 // A row is held by one group of lanes, part of a wave to a block of 1024, at any
 // width and alignment (RowCut), so each tensor is read once and written once.
