@@ -378,13 +378,17 @@ struct LnCall {
     }
 };
 
-// Outputs share no bytes with each other or with an input, except that an output
-// may be one of the first `in_place` inputs itself (tensors of the rows' shape).
+// Outputs share no bytes with each other or with an input, except that one of the first
+// kRowOuts outputs may be one of the first `row_ins` inputs itself: those are the tensors
+// of the rows' shape.  (Of one row, or one column, the others have as many values: the
+// column sums are written beside the rows that are still read.)
+constexpr ptrdiff_t kRowOuts = 2;
 static int check_apart(std::initializer_list<NeuralTensor *> outs, std::initializer_list<const NeuralTensor *> ins,
-                       size_t in_place)
+                       size_t row_ins)
 {
     for (auto o = outs.begin(); o != outs.end(); ++o) {
         if (!*o) continue;
+        const size_t in_place = o - outs.begin() < kRowOuts ? row_ins : 0;
         for (auto p = o + 1; p != outs.end(); ++p)
             if (tensors_may_overlap(*o, *p)) return set_error(NEURAL_ERR_INVALID_ARGUMENT);
         size_t k = 0;

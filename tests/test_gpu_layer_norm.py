@@ -743,3 +743,35 @@ def test_column_sums_of_one_sign(pn, rows, cols):
     lim = 1.01 * (2 * ref.U[np.dtype(np.float32)] + (rows + 8) * ref.D)
     for got, want in ((dg, d * x.double().sum(0)), (db, d * rows)):
         assert float(((got.double() - want).abs() / want).max()) <= lim
+
+
+@pytest.mark.parametrize("cols", [6, 3000, 40000, 70001])
+def test_refusals_of_one_row_or_column(pn, cols):
+    """Where a row's tensors have as many values as gamma's gradient (one row), or as the
+    statistics (one column), only the outputs of the rows' shape may replace an input."""
+    E, lib, T = pn.NeuralError, pn.core._lib, pn.Tensor
+    k, jk = lib.neural_layer_norm_backward, lib.neural_dropout_add_layer_norm_backward
+    x, dy, dh, dx, g = (T.ones([1, cols]) for _ in range(5))
+    m, r = T.zeros([1]), T.ones([1])
+    X, DY, DH, DX, G, M, R = (t._ptr for t in (x, dy, dh, dx, g, m, r))
+    for over in (X, DY):
+        for also in (DX, over, None):
+            assert k(also, over, None, DY, X, G, M, R) == E.INVALID_ARGUMENT
+            assert k(also, None, over, DY, X, G, M, R) == E.INVALID_ARGUMENT
+    for over in (X, DY, DH):
+        assert jk(DX, None, over, None, DY, DH, X, G, M, R, 0.0, None) == E.INVALID_ARGUMENT
+        assert jk(None, DX, None, over, DY, DH, X, G, M, R, 0.0, None) == E.INVALID_ARGUMENT
+    c, res, o, h = (T.ones([cols, 1]) for _ in range(4))
+    s = T.zeros([cols])
+    C, RES, O, H, S = (t._ptr for t in (c, res, o, h, s))
+    f, jf = lib.neural_layer_norm_forward, lib.neural_dropout_add_layer_norm_forward
+    assert f(O, C, None, None, EPS, C, S) == E.INVALID_ARGUMENT
+    assert f(O, C, None, None, EPS, S, C) == E.INVALID_ARGUMENT
+    for over in (C, RES):
+        assert jf(O, H, C, RES, None, None, 0.0, None, EPS, over, S) == E.INVALID_ARGUMENT
+        assert jf(O, H, C, RES, None, None, 0.0, None, EPS, S, over) == E.INVALID_ARGUMENT
+    for t in (x, dy, dh, dx, g, c, res, o, h):
+        assert (t.numpy() == 1).all()
+    # in place is still taken
+    assert k(DY, DX, DH, DY, X, G, M, R) == 0 and f(C, C, None, None, EPS, S, None) == 0
+    assert not c.numpy().any()
