@@ -393,7 +393,8 @@ static int check_apart(std::initializer_list<NeuralTensor *> outs, std::initiali
             if (tensors_may_overlap(*o, *p)) return set_error(NEURAL_ERR_INVALID_ARGUMENT);
         size_t k = 0;
         for (const NeuralTensor *i : ins) {
-            const bool itself = k++ < in_place && i && i->data == (*o)->data && numel(i) == numel(*o);
+            const bool itself = k++ < in_place && i && (i->data == (*o)->data || i->dev == (*o)->dev) &&
+                                numel(i) == numel(*o);
             if (!itself && tensors_may_overlap(*o, i)) return set_error(NEURAL_ERR_INVALID_ARGUMENT);
         }
     }

@@ -761,11 +761,11 @@ bool nh::tensors_may_overlap(const NeuralTensor *a, const NeuralTensor *b)
     span_of(a, &alo, &ahi);
     span_of(b, &blo, &bhi);
     if (ahi <= alo || bhi <= blo) return false;
-    const uintptr_t a0 = reinterpret_cast<uintptr_t>(a->data) + uintptr_t(alo);
-    const uintptr_t a1 = reinterpret_cast<uintptr_t>(a->data) + uintptr_t(ahi);
-    const uintptr_t b0 = reinterpret_cast<uintptr_t>(b->data) + uintptr_t(blo);
-    const uintptr_t b1 = reinterpret_cast<uintptr_t>(b->data) + uintptr_t(bhi);
-    return a0 < b1 && b0 < a1;
+    const auto meet = [&](const void *pa, const void *pb) {
+        const uintptr_t a0 = reinterpret_cast<uintptr_t>(pa), b0 = reinterpret_cast<uintptr_t>(pb);
+        return a0 + uintptr_t(alo) < b0 + uintptr_t(bhi) && b0 + uintptr_t(blo) < a0 + uintptr_t(ahi);
+    };
+    return meet(a->data, b->data) || meet(a->dev, b->dev);
 }
 
 extern "C" {

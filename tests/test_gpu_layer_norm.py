@@ -10,7 +10,7 @@ import numpy as np
 import pytest
 
 import sublayer_ref as ref
-from conftest import GPU, same_bits
+from conftest import GPU, keep, same_bits
 
 pytestmark = GPU
 
@@ -775,3 +775,42 @@ def test_refusals_of_one_row_or_column(pn, cols):
     # in place is still taken
     assert k(DY, DX, DH, DY, X, G, M, R) == 0 and f(C, C, None, None, EPS, S, None) == 0
     assert not c.numpy().any()
+
+
+def test_tensors_over_a_device_address(pn, rng):
+    """A tensor made over an owned tensor's device address is the same memory: refused
+    where outputs may not meet it, and in place where they may replace it."""
+    E, lib = pn.NeuralError, pn.core._lib
+    rows, cols = 6, 50
+
+    def over(t, shape, skip=0):
+        return keep(pn.Tensor._wrap(lib.neural_tensor_from_buffer(
+            t.device_ptr + 4 * skip, (ctypes.c_uint64 * len(shape))(*shape), len(shape), 0, None)))
+
+    c = _case(rng, rows, cols, np.float32)
+    want = _forward(pn, c["x"], c["g"], c["b"])
+    grads = _backward(pn, c["dy"], c["x"], c["g"], want[1], want[2])
+    x, dy, g, b, m, r = (pn.Tensor.from_numpy(v) for v in (c["x"], c["dy"], c["g"], c["b"], want[1], want[2]))
+    y, dg = pn.Tensor.zeros([rows, cols]), pn.Tensor.zeros([cols])
+    wide = pn.Tensor.ones([rows + 1, cols])
+    low, high = over(wide, [rows, cols]), over(wide, [rows, cols], 1)
+    k, f, d = lib.neural_layer_norm_backward, lib.neural_layer_norm_forward, lib.neural_counter_dropout_forward
+    key = _key(pn, 1, 1)
+    assert k(y._ptr, over(g, [cols]), None, dy._ptr, x._ptr, g._ptr, m._ptr, r._ptr) == E.INVALID_ARGUMENT
+    assert k(y._ptr, None, over(x, [cols], 7), dy._ptr, x._ptr, g._ptr, m._ptr, r._ptr) == E.INVALID_ARGUMENT
+    assert k(y._ptr, dg._ptr, over(dg, [cols]), dy._ptr, x._ptr, g._ptr, m._ptr, r._ptr) == E.INVALID_ARGUMENT
+    assert f(high, low, None, None, EPS, None, None) == E.INVALID_ARGUMENT
+    assert f(over(wide, [rows, cols], 1), over(wide, [rows, cols]), None, None, EPS, None,
+             None) == E.INVALID_ARGUMENT
+    assert d(high, low, 0.5, key) == E.INVALID_ARGUMENT
+    assert d(over(wide, [rows, cols + 1], 1), over(wide, [rows, cols + 1]), 0.5, key) == E.INVALID_ARGUMENT
+    assert (wide.numpy() == 1).all() and not y.numpy().any()
+    same_bits(g.numpy(), c["g"])
+    px, pd = over(x, [rows, cols]), over(dy, [rows, cols])
+    assert k(pd, dg._ptr, None, dy._ptr, x._ptr, g._ptr, m._ptr, r._ptr) == 0
+    same_bits(dy.numpy(), grads[0])
+    same_bits(dg.numpy(), grads[1])
+    assert f(px, x._ptr, g._ptr, b._ptr, EPS, None, None) == 0
+    same_bits(x.numpy(), want[0])
+    assert d(x._ptr, px, 0.25, key) == 0
+    same_bits(x.numpy(), ref.dropout(want[0], 0.25, 1, 1))
