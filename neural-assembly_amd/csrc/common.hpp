@@ -187,14 +187,14 @@ inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // f32 activations +2-6 %).
 constexpr int64_t kMaxGridBlocks = (int64_t(1) << 24) - 1;
 // Kernels that give each block (or wave) its own rows take `rows` in launches
-// of at most kMaxGridBlocks blocks of `rpb` rows each: launch(blocks, first
-// row) once per such range.  (A row loop inside those kernels raised their
-// register counts, e.g. 62 -> 96 VGPRs for the f32 log-softmax over rows of
-// 1024, so the loop is on the host.)
+// of blocks of `rpb` rows and `lanes` lanes each, below 2^32 lanes a launch:
+// launch(blocks, first row) once per such range.  (A row loop inside those
+// kernels raised their register counts, e.g. 62 -> 96 VGPRs for the f32
+// log-softmax over rows of 1024, so the loop is on the host.)
 template <typename L>
-void for_row_launches(int64_t rows, int64_t rpb, L launch)
+void for_row_launches(int64_t rows, int64_t rpb, int64_t lanes, L launch)
 {
-    const int64_t per = kMaxGridBlocks * rpb;
+    const int64_t per = (((int64_t(1) << 32) - 1) / lanes) * rpb;
     for (int64_t base = 0; base < rows; base += per) {
         const int64_t n = rows - base < per ? rows - base : per;
         launch(unsigned(ceil_div(n, rpb)), base);

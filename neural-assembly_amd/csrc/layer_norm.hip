@@ -297,7 +297,7 @@ static void launch_ln_rows(const LnArgs<T> &a)
             const int64_t most = int64_t(num_cus()) * Plan::kPerCu, need = ceil_div(a.rows, int64_t(Plan::RPB));
             launch(unsigned(need < most ? need : most), 0);
         } else {
-            for_row_launches(a.rows, Plan::RPB, launch);
+            for_row_launches(a.rows, Plan::RPB, Plan::NB, launch);
         }
     });
 }
@@ -330,7 +330,7 @@ static int launch_ln(const LnArgs<T> &a)
     else if (ncv <= 1024 * 8) launch_ln_rows<T, MODE, 1024, 8>(a);
     else if (ncv <= 1024 * 16) launch_ln_rows<T, MODE, 1024, 16>(a);
     else
-        for_row_launches(a.rows, 1, [&](unsigned g, int64_t base) {
+        for_row_launches(a.rows, 1, kLnWide, [&](unsigned g, int64_t base) {
             NH_LAUNCH((k_ln_wide<T, MODE>), dim3(g), dim3(kLnWide), 0, stream(), a, base);
         });
     return check_launch();

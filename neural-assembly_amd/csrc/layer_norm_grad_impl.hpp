@@ -480,14 +480,14 @@ __global__ __launch_bounds__((LnGradPlan<T, NT, VPT>::NB)) void k_ln_grad_few(Ln
 // 46.7 with 16.
 template <typename T>
 __global__ __launch_bounds__(1024) void k_ln_fold(const T *__restrict__ part, int64_t n, int64_t cols,
-                                                  T *__restrict__ dgamma, T *__restrict__ dbeta)
+                                                  T *__restrict__ dgamma, T *__restrict__ dbeta, int64_t c_base)
 {
     using V = typename Vec16<T>::type;
     using U = typename VecU<T>::type;
     constexpr int VN = Vec16<T>::n, C = 32, L = C / VN, S = 1024 / L, UN = 4, TPC = 1024 / C;
     __shared__ double sh[S][C + 1];  // (read by columns below: no two lanes on a bank)
     const int vl = threadIdx.x % L, st = threadIdx.x / L;
-    const int64_t width = 2 * cols, c = int64_t(blockIdx.x) * C + vl * VN;
+    const int64_t width = 2 * cols, c0 = c_base + int64_t(blockIdx.x) * C, c = c0 + vl * VN;
     double s[VN];
 #pragma unroll
     for (int j = 0; j < VN; j++) s[j] = 0.0;
@@ -521,7 +521,7 @@ __global__ __launch_bounds__(1024) void k_ln_fold(const T *__restrict__ part, in
 #pragma unroll
     for (int i = 0; i < S / TPC; i++) t += sh[part_of + i * TPC][e];
     t = RowGrp<TPC>::sum(t, nullptr);
-    const int64_t at = int64_t(blockIdx.x) * C + e;
+    const int64_t at = c0 + e;
     if (part_of == 0 && at < width) {
         T *out = at < cols ? dgamma : dbeta;
         if (out) out[at < cols ? at : at - cols] = T(t);
@@ -531,8 +531,9 @@ __global__ __launch_bounds__(1024) void k_ln_fold(const T *__restrict__ part, in
 template <typename T>
 static void launch_ln_fold(const T *part, int64_t n, int64_t cols, T *dgamma, T *dbeta)
 {
-    NH_LAUNCH((k_ln_fold<T>), dim3(unsigned(ceil_div(2 * cols, 32))), dim3(1024), 0, stream(), part, n,
-              cols, dgamma, dbeta);
+    for_row_launches(2 * cols, 32, 1024, [&](unsigned g, int64_t base) {
+        NH_LAUNCH((k_ln_fold<T>), dim3(g), dim3(1024), 0, stream(), part, n, cols, dgamma, dbeta, base);
+    });
 }
 
 // Rows wider than a block's registers: the row's sums, then the outputs, reading
@@ -597,14 +598,14 @@ __global__ __launch_bounds__(kLnWide) void k_ln_grad_wide(LnGradArgs<T> a, int64
 // Column sums beside a row pass that cannot hold them: 64 lanes of VN columns a block, the
 // rows of its chunk by 8 waves, four in flight each.
 template <typename T>
-__global__ __launch_bounds__(512) void k_ln_cols(LnGradArgs<T> a, int64_t chunk)
+__global__ __launch_bounds__(512) void k_ln_cols(LnGradArgs<T> a, int64_t chunk, int64_t c_base)
 {
     using V = typename Vec16<T>::type;
     using U = typename VecU<T>::type;
     constexpr int VN = Vec16<T>::n, W = 8, UN = 4;
     __shared__ double sh[W][2 * VN][64];
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const int64_t cols = a.cols, c = (int64_t(blockIdx.x) * 64 + lane) * VN;
+    const int64_t cols = a.cols, c = c_base + (int64_t(blockIdx.x) * 64 + lane) * VN;
     const int64_t r0 = int64_t(blockIdx.y) * chunk, r1 = r0 + chunk < a.rows ? r0 + chunk : a.rows;
     const bool whole = c + VN <= cols;
     double s[2 * VN];
@@ -682,7 +683,9 @@ static int launch_ln_cols(LnGradArgs<T> a, T *dgamma, T *dbeta)
     Partials part;
     NH_TRY(part.open(size_t(chunks) * 2 * size_t(a.cols) * sizeof(T)));
     a.part = static_cast<T *>(part.p);
-    NH_LAUNCH((k_ln_cols<T>), dim3(unsigned(gx), unsigned(chunks)), dim3(512), 0, stream(), a, chunk);
+    for_row_launches(a.cols, 64 * Vec16<T>::n, 512, [&](unsigned g, int64_t base) {
+        NH_LAUNCH((k_ln_cols<T>), dim3(g, unsigned(chunks)), dim3(512), 0, stream(), a, chunk, base);
+    });
     launch_ln_fold(a.part, chunks, a.cols, dgamma, dbeta);
     return check_launch();
 }
@@ -763,7 +766,7 @@ int launch_ln_grad(const LnGradArgs<T> &a, T *dgamma, T *dbeta)
     // the columns first: the row pass may write over what they read
     if (dgamma || dbeta) NH_TRY(launch_ln_cols(a, dgamma, dbeta));
     if (a.dx || a.dres)
-        for_row_launches(a.rows, 1, [&](unsigned g, int64_t base) {
+        for_row_launches(a.rows, 1, kLnWide, [&](unsigned g, int64_t base) {
             NH_LAUNCH((k_ln_grad_wide<T, MODE>), dim3(g), dim3(kLnWide), 0, stream(), a, base);
         });
     return check_launch();

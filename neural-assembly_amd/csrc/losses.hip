@@ -442,7 +442,7 @@ static void launch_ce_rows(const T *x, const CeArgs &a)
 {
     constexpr int W = NT == 512 ? 4 : (NT <= 64 && sizeof(T) == 8 && MODE == CE_LS_FWD && VPT <= 8 ? 5 : 1);
     constexpr int block = NT < 256 ? 256 : NT;
-    for_row_launches(a.rows, block / NT, [&](unsigned g, int64_t base) {
+    for_row_launches(a.rows, block / NT, block, [&](unsigned g, int64_t base) {
         if constexpr (NT <= 64) {
             if (a.cols == int64_t(NT) * VPT * Vec16<T>::n) {
                 // (the tensor loss, which stores nothing, wants it from 8 vectors: f32
@@ -483,7 +483,7 @@ static int launch_ce(const T *x, const CeArgs &a)
     else if (ncv <= 512 * 25) launch_ce_rows<T, MODE, 512, 16, 9>(x, a);
     else if (ncv <= 1024 * 24) launch_ce_rows<T, MODE, 1024, 24>(x, a);
     else
-        for_row_launches(a.rows, 1, [&](unsigned g, int64_t base) {
+        for_row_launches(a.rows, 1, kCeWide, [&](unsigned g, int64_t base) {
             NH_LAUNCH((k_ce_stream<T, MODE>), dim3(g), dim3(kCeWide), 0, stream(), x, a, base);
         });
     return check_launch();

@@ -229,8 +229,8 @@ __global__ __launch_bounds__(kSmWide) void k_softmax_stream(const T *__restrict_
 template <typename T, bool LOG, int NT, int VPT>
 static void launch_rows(const T *x, T *y, int64_t rows, int64_t cols)
 {
-    for_row_launches(rows, NT < kSmBlock ? kSmBlock / NT : 1, [&](unsigned g, int64_t base) {
-        constexpr int block = NT < kSmBlock ? kSmBlock : NT;
+    constexpr int block = NT < kSmBlock ? kSmBlock : NT;
+    for_row_launches(rows, block / NT, block, [&](unsigned g, int64_t base) {
         if constexpr (NT <= 64 && sizeof(T) == 4) {
             if (cols == int64_t(NT) * VPT * Vec16<T>::n) {
                 NH_LAUNCH((k_softmax_rows<T, LOG, NT, VPT, true>), dim3(g), dim3(block), VPT >= 4 ? kFullRowsLds : 0,
@@ -278,7 +278,7 @@ static int launch_softmax(const T *x, T *y, int64_t rows, int64_t cols)
     else if (ncv <= 1024 * 16) launch_rows<T, LOG, 1024, 16>(x, y, rows, cols);
     else if (ncv <= 1024 * 24) launch_rows<T, LOG, 1024, 24>(x, y, rows, cols);
     else
-        for_row_launches(rows, 1, [&](unsigned g, int64_t base) {
+        for_row_launches(rows, 1, kSmWide, [&](unsigned g, int64_t base) {
             NH_LAUNCH((k_softmax_stream<T, LOG>), dim3(g), dim3(kSmWide), 0, stream(), x, y, cols, base);
         });
     return check_launch();

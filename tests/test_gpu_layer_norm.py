@@ -814,3 +814,62 @@ def test_tensors_over_a_device_address(pn, rng):
     same_bits(x.numpy(), want[0])
     assert d(x._ptr, px, 0.25, key) == 0
     same_bits(x.numpy(), ref.dropout(want[0], 0.25, 1, 1))
+
+
+def _room(pn, need):
+    import torch
+    torch.cuda.empty_cache()
+    pn.core._lib.neural_hip_empty_cache()
+    if torch.cuda.mem_get_info()[0] < need + (4 << 30):
+        pytest.skip("not enough free device memory")
+
+
+@pytest.mark.parametrize("cols,rows_too", [((1 << 26) + 5, True), ((1 << 31) + 13, False)])
+def test_gradients_past_a_grid_of_columns(pn, cols, rows_too):
+    """One row so wide that the column sums' blocks (of 1024 lanes, 32 columns; of 512,
+    256 columns) have more lanes than one launch may: exact, of small whole numbers."""
+    import torch
+    _room(pn, 4 * cols * 10)
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(3)
+    x, dy = (torch.empty(1, cols, device="cuda").random_(0, 7, generator=gen).sub_(3) for _ in range(2))
+    dx = torch.full((1, cols), 9.0, device="cuda") if rows_too else None
+    dg, db = torch.full((cols,), 9.0, device="cuda"), torch.full((cols,), 9.0, device="cuda")
+    m, r = torch.zeros(1, device="cuda"), torch.ones(1, device="cuda")
+    T = pn.Tensor.from_torch
+    DX, DG, DB, DY, X, M, R = (T(v) if v is not None else None for v in (dx, dg, db, dy, x, m, r))
+    torch.cuda.synchronize()
+    assert pn.core._lib.neural_layer_norm_backward(_p(DX), DG._ptr, DB._ptr, DY._ptr, X._ptr, None, M._ptr,
+                                                   R._ptr) == 0
+    pn.synchronize()
+    assert torch.equal(db, dy[0]) and torch.equal(dg, (dy * x)[0])
+    if rows_too:
+        w, xd = dy.double(), x.double()
+        want = w - w.mean() - xd * (w * xd).mean()
+        # whole sums below 2^53; under 16 roundings of values below 100, and the result's
+        assert bool(((dx.double() - want).abs() <= 100 * 16 * ref.D + 2.0 ** -24 * want.abs()).all())
+    torch.cuda.empty_cache()
+
+
+def test_rows_past_a_grid_of_wide_blocks(pn):
+    """2^22 rows and more of a block of 1024 lanes each (137 GB, in place): the first rows,
+    those around the second launch's first, and the last."""
+    import torch
+    rows, cols = (1 << 22) + 5, 8196
+    _room(pn, 4 * rows * cols)
+    one = torch.arange(cols, device="cuda", dtype=torch.float32) % 11 - 5
+    x = one.repeat(rows, 1)
+    y0 = one.repeat(1, 1)
+    T = pn.Tensor.from_torch
+    X, Y0 = T(x), T(y0)
+    torch.cuda.synchronize()
+    f = pn.core._lib.neural_layer_norm_forward
+    assert f(Y0._ptr, Y0._ptr, None, None, EPS, None, None) == 0
+    assert f(X._ptr, X._ptr, None, None, EPS, None, None) == 0
+    pn.synchronize()
+    assert not torch.equal(y0[0], one)
+    pick = torch.cat([torch.arange(3, device="cuda"), torch.arange((1 << 22) - 4, rows, device="cuda"),
+                      torch.arange(0, rows, 65521, device="cuda")])
+    assert bool((x[pick] == y0).all())
+    del X, x
+    torch.cuda.empty_cache()
