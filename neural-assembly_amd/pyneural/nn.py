@@ -16,6 +16,7 @@ sublayer, in one pass), each with its backward pass.
 """
 
 import ctypes
+import itertools
 
 import numpy as np
 
@@ -266,18 +267,35 @@ def dropout_seed(seed: int) -> None:
     _check_error(_lib.neural_dropout_seed(ctypes.c_uint32(seed & 0xFFFFFFFF)), "dropout seed")
 
 
+_counter_seeds = itertools.count(1 << 32)  # of the modules that are given none
+
+
+def counter_dropout_seed(seed: int) -> None:
+    """Position the seeds that CounterDropout and DropoutAddLayerNorm modules
+    take where they are given none: the k-th module made from here on, from 0, takes
+    (seed + 1) 2^32 + k (a process starts as with seed 0).  Processes that train
+    one model together each pass a number of their own, or they drop the same
+    elements."""
+    global _counter_seeds
+    if not 0 <= seed < (1 << 32) - 1:
+        raise ValueError(f"seed must be in [0, 2^32 - 2], got {seed}")
+    _counter_seeds = itertools.count((seed + 1) << 32)
+
+
 class CounterDropout(Module):
     """Inverted dropout whose mask is a function of the element's index, ``seed``
     and the number of the call (neural_counter_dropout_forward; the offset of
     call k is ``offset + k``): none is stored, and ``backward`` makes the last
-    forward's again.  float32 and float64; identity in eval mode."""
+    forward's again.  Without a ``seed`` each module takes one of its own
+    (``counter_dropout_seed``): equal seeds and calls drop the same elements.
+    float32 and float64; identity in eval mode."""
 
-    def __init__(self, p: float = 0.5, seed: int = 0, offset: int = 0):
+    def __init__(self, p: float = 0.5, seed: int = None, offset: int = 0):
         super().__init__()
         if not 0.0 <= p <= 1.0:
             raise ValueError(f"Dropout probability must be in [0, 1], got {p}")
         self.p = p
-        self.seed = seed
+        self.seed = next(_counter_seeds) if seed is None else seed
         self.offset = offset  # of the next call
         self._last = None     # (p, key) of the last forward
 
@@ -375,7 +393,7 @@ class DropoutAddLayerNorm(LayerNorm):
     returns those of x and residual."""
 
     def __init__(self, num_features: int, p: float = 0.1, eps: float = 1e-5, dtype: int = NeuralDtype.FLOAT32,
-                 seed: int = 0, offset: int = 0):
+                 seed: int = None, offset: int = 0):
         super().__init__(num_features, eps, dtype)
         self.dropout = CounterDropout(p, seed, offset)
 

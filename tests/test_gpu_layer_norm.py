@@ -873,3 +873,13 @@ def test_rows_past_a_grid_of_wide_blocks(pn):
     assert bool((x[pick] == y0).all())
     del X, x
     torch.cuda.empty_cache()
+
+
+def test_default_modules_drop_apart(pn):
+    """Two sublayers' ends built alike drop different elements in the same step."""
+    x, z = pn.Tensor.ones([40, 50]), pn.Tensor.zeros([40, 50])
+    a, b = (pn.DropoutAddLayerNorm(50, 0.5) for _ in range(2))
+    ha, hb = (m(x, z)[1].numpy() for m in (a, b))
+    # 2000 independent pairs of halves: equal in 1000 +- 22 of them
+    assert 800 < int((ha == hb).sum()) < 1200
+    same_bits(ha, ref.dropout(np.ones((40, 50), np.float32), 0.5, a.dropout.seed, 0))
