@@ -300,9 +300,7 @@ class CounterDropout(Module):
         self._last = None     # (p, key) of the last forward
 
     def _next(self):
-        p, key = (self.p, DropoutKeyC(self.seed, self.offset)) if self.training else (0.0, DropoutKeyC(0, 0))
-        self._last = (p, key)
-        return p, key
+        return (self.p, DropoutKeyC(self.seed, self.offset)) if self.training else (0.0, DropoutKeyC(0, 0))
 
     def _took(self):
         if self.training:
@@ -315,6 +313,7 @@ class CounterDropout(Module):
         _check_error(_lib.neural_counter_dropout_forward(out._ptr, src._ptr, p, ctypes.byref(key)),
                      "counter dropout forward")
         self._took()
+        self._last = (p, key)
         return out
 
     def backward(self, grad_output: Tensor) -> Tensor:
@@ -333,8 +332,9 @@ class CounterDropout(Module):
 
 class LayerNorm(Module):
     """(x - mean) / sqrt(var + eps) * gamma + beta over the last dimension
-    (neural_layer_norm_forward).  ``backward`` returns the input's gradient and
-    leaves those of gamma and beta in their ``grad``."""
+    (neural_layer_norm_forward).  ``backward`` is that of the last forward, whose
+    input it reads again (so that must still hold its values): it returns the
+    input's gradient and leaves those of gamma and beta in their ``grad``."""
 
     def __init__(self, num_features: int, eps: float = 1e-5, dtype: int = NeuralDtype.FLOAT32):
         super().__init__()
@@ -389,8 +389,9 @@ class DropoutAddLayerNorm(LayerNorm):
     dropout(x), out = norm(hidden) (neural_dropout_add_layer_norm_forward);
     dropout as CounterDropout's, none in eval mode.  ``forward`` returns (out,
     hidden): a block that normalises first hands ``hidden`` on as its residual
-    stream.  ``backward`` takes the gradients of both (that of hidden may be None) and
-    returns those of x and residual."""
+    stream.  ``backward``, of the last forward, reads that ``hidden`` again (not to
+    be changed in place before it), takes the gradients of both (that of hidden may
+    be None) and returns those of x and residual."""
 
     def __init__(self, num_features: int, p: float = 0.1, eps: float = 1e-5, dtype: int = NeuralDtype.FLOAT32,
                  seed: int = None, offset: int = 0):
@@ -411,18 +412,17 @@ class DropoutAddLayerNorm(LayerNorm):
                                                         rstd._ptr)
         _check_error(rc, "dropout + add + layer norm forward")
         self.dropout._took()
-        self._saved = (hidden, mean, rstd)
+        self._saved = (hidden, mean, rstd, p, key)
         return out, hidden
 
     def backward(self, grad_output: Tensor, grad_hidden: Tensor = None):
         if self._saved is None:
             raise RuntimeError("DropoutAddLayerNorm.backward called before forward")
-        hidden, mean, rstd = self._saved
+        hidden, mean, rstd, p, key = self._saved
         go = grad_output.contiguous()
         gh = grad_hidden.contiguous() if grad_hidden is not None else None
         gi, gr = Tensor.create(hidden.shape, hidden.dtype), Tensor.create(hidden.shape, hidden.dtype)
         dgamma, dbeta = self._grads()
-        p, key = self.dropout._last
         rc = _lib.neural_dropout_add_layer_norm_backward(gi._ptr, gr._ptr, dgamma._ptr, dbeta._ptr, go._ptr,
                                                          gh._ptr if gh is not None else None, hidden._ptr,
                                                          self.gamma._ptr, mean._ptr, rstd._ptr, p, ctypes.byref(key))

@@ -883,3 +883,28 @@ def test_default_modules_drop_apart(pn):
     # 2000 independent pairs of halves: equal in 1000 +- 22 of them
     assert 800 < int((ha == hb).sum()) < 1200
     same_bits(ha, ref.dropout(np.ones((40, 50), np.float32), 0.5, a.dropout.seed, 0))
+
+
+def test_a_failed_forward_changes_no_mask(pn, rng):
+    """Neither the mask that backward makes again nor the next forward's; and another use
+    of the joined module's dropout is a call of its own."""
+    T, cols = pn.Tensor.from_numpy, 33
+    c = _case(rng, 7, cols, np.float32)
+    one = np.ones(cols, np.float32)
+    x, res, dy, dh = (T(c[k]) for k in ("x", "res", "dy", "dh"))
+    end = pn.DropoutAddLayerNorm(cols, 0.4, seed=3)
+    h = end(x, res)[1].numpy()
+    _, mean, rstd = _forward(pn, h, one, 0 * one)
+    want = _joined_grad(pn, {**c, "g": one}, h, mean, rstd, 0.4, _key(pn, 3, 0))
+    with pytest.raises(pn.NeuralException):
+        end(x, T(c["res"][:3]))
+    end.dropout(x)
+    for a, w in zip(end.backward(dy, dh), want):
+        same_bits(a.numpy(), w)
+    same_bits(end(x, res)[1].numpy(), c["res"] + ref.dropout(c["x"], 0.4, 3, 2))  # after calls 0 and 1
+    drop = pn.CounterDropout(0.5, seed=1)
+    drop(x)
+    drop.p = 2.0
+    with pytest.raises(pn.NeuralException):
+        drop(x)
+    same_bits(drop.backward(dy).numpy(), ref.dropout(c["dy"], 0.5, 1, 0))
