@@ -356,9 +356,10 @@ class LayerNorm(Module):
         return Tensor.create([rows], x.dtype), Tensor.create([rows], x.dtype)
 
     def _grads(self):
-        self.gamma.grad = Tensor.create([self.num_features], self.gamma.dtype)
-        self.beta.grad = Tensor.create([self.num_features], self.beta.dtype)
-        return self.gamma.grad, self.beta.grad
+        return tuple(Tensor.create([self.num_features], t.dtype) for t in self.parameters())
+
+    def _keep_grads(self, grads):  # of a backward that succeeded
+        self.gamma.grad, self.beta.grad = grads
 
     def forward(self, x: Tensor) -> Tensor:
         src = x.contiguous()
@@ -378,6 +379,7 @@ class LayerNorm(Module):
         dgamma, dbeta = self._grads()
         _check_error(_lib.neural_layer_norm_backward(gi._ptr, dgamma._ptr, dbeta._ptr, go._ptr, x._ptr,
                                                      self.gamma._ptr, mean._ptr, rstd._ptr), "layer norm backward")
+        self._keep_grads((dgamma, dbeta))
         return gi
 
     def __repr__(self) -> str:
@@ -427,6 +429,7 @@ class DropoutAddLayerNorm(LayerNorm):
                                                          gh._ptr if gh is not None else None, hidden._ptr,
                                                          self.gamma._ptr, mean._ptr, rstd._ptr, p, ctypes.byref(key))
         _check_error(rc, "dropout + add + layer norm backward")
+        self._keep_grads((dgamma, dbeta))
         return gi, gr
 
     def __repr__(self) -> str:

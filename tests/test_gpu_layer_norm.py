@@ -908,3 +908,22 @@ def test_a_failed_forward_changes_no_mask(pn, rng):
     with pytest.raises(pn.NeuralException):
         drop(x)
     same_bits(drop.backward(dy).numpy(), ref.dropout(c["dy"], 0.5, 1, 0))
+
+
+def test_a_failed_backward_leaves_the_gradients(pn, rng):
+    T, cols = pn.Tensor.from_numpy, 33
+    c = _case(rng, 7, cols, np.float32)
+    x, res, dy = (T(c[k]) for k in ("x", "res", "dy"))
+    end, norm = pn.DropoutAddLayerNorm(cols, 0.4, seed=3), pn.LayerNorm(cols)
+    end(x, res)
+    end.backward(dy)
+    dg, db = end.gamma.grad.numpy(), end.beta.grad.numpy()
+    for bad in (lambda: end.backward(T(c["dy"][:3])), lambda: end.backward(dy, T(c["dh"][:3]))):
+        with pytest.raises(pn.NeuralException):
+            bad()
+        same_bits(end.gamma.grad.numpy(), dg)
+        same_bits(end.beta.grad.numpy(), db)
+    norm(x)
+    with pytest.raises(pn.NeuralException):
+        norm.backward(T(c["dy"][:3]))
+    assert norm.gamma.grad is None and norm.beta.grad is None
