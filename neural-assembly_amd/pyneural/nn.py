@@ -297,7 +297,7 @@ class CounterDropout(Module):
         self.p = p
         self.seed = next(_counter_seeds) if seed is None else seed
         self.offset = offset  # of the next call
-        self._last = None     # (p, key) of the last forward
+        self._last = None     # (p, key, elements) of the last forward
 
     def _next(self):
         return (self.p, DropoutKeyC(self.seed, self.offset)) if self.training else (0.0, DropoutKeyC(0, 0))
@@ -313,13 +313,15 @@ class CounterDropout(Module):
         _check_error(_lib.neural_counter_dropout_forward(out._ptr, src._ptr, p, ctypes.byref(key)),
                      "counter dropout forward")
         self._took()
-        self._last = (p, key)
+        self._last = (p, key, x.numel)
         return out
 
     def backward(self, grad_output: Tensor) -> Tensor:
         if self._last is None:
             raise RuntimeError("CounterDropout.backward called before forward")
-        p, key = self._last
+        p, key, numel = self._last
+        if grad_output.numel != numel:
+            raise ValueError(f"expected a gradient of {numel} elements, got shape {grad_output.shape}")
         go = grad_output.contiguous()
         gi = Tensor.create(grad_output.shape, grad_output.dtype)
         _check_error(_lib.neural_counter_dropout_backward(gi._ptr, go._ptr, p, ctypes.byref(key)),

@@ -927,3 +927,13 @@ def test_a_failed_backward_leaves_the_gradients(pn, rng):
     with pytest.raises(pn.NeuralException):
         norm.backward(T(c["dy"][:3]))
     assert norm.gamma.grad is None and norm.beta.grad is None
+
+
+def test_a_dropout_gradient_has_the_forward_elements(pn, rng):
+    x = rng.normal(0, 1, (5, 8)).astype(np.float32)
+    drop = pn.CounterDropout(0.5, seed=1)
+    drop(pn.Tensor.from_numpy(x))
+    for n in (3, 6):
+        with pytest.raises(ValueError):
+            drop.backward(pn.Tensor.from_numpy(np.ones((n, 8), np.float32)))
+    same_bits(drop.backward(pn.Tensor.from_numpy(x.reshape(40))).numpy(), ref.dropout(x, 0.5, 1, 0).reshape(40))
