@@ -660,7 +660,12 @@ struct Partials {
     bool keep = false;
     int open(size_t bytes)
     {
-        keep = stream_recording();
+        hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+        if (const hipError_t e = hipStreamIsCapturing(stream(), &status)) {  // nothing is launched then
+            (void)hipGetLastError();
+            return hip_fail(e);
+        }
+        keep = status != hipStreamCaptureStatusNone;
         p = keep ? dev_alloc_own(bytes) : dev_alloc(bytes);
         return p ? NEURAL_OK : set_error(NEURAL_ERR_OUT_OF_MEMORY);
     }

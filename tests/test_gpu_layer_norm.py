@@ -937,3 +937,50 @@ def test_a_dropout_gradient_has_the_forward_elements(pn, rng):
         with pytest.raises(ValueError):
             drop.backward(pn.Tensor.from_numpy(np.ones((n, 8), np.float32)))
     same_bits(drop.backward(pn.Tensor.from_numpy(x.reshape(40))).numpy(), ref.dropout(x, 0.5, 1, 0).reshape(40))
+
+
+def _hip():
+    """The HIP runtime that this process has loaded."""
+    with open("/proc/self/maps") as f:
+        return ctypes.CDLL(next(line.split()[-1] for line in f if "libamdhip64" in line))
+
+
+def _alloc_counts(pn):
+    a, m = ctypes.c_ulonglong(), ctypes.c_ulonglong()
+    assert pn.core._lib.neural_hip_alloc_stats(ctypes.byref(a), ctypes.byref(m)) == 0
+    return a.value, m.value
+
+
+def test_a_stream_that_cannot_be_asked(pn, rng):
+    """The null stream while a blocking stream is being captured cannot say whether it is
+    captured itself: the call answers so, without memory or launches, and the
+    capture goes on."""
+    hip, lib, T = _hip(), pn.core._lib, pn.Tensor
+    c = _case(rng, 600, 100, np.float32)  # more than the rows of a call that needs no memory
+    _, mean, rstd = _forward(pn, c["x"], c["g"], c["b"])
+    want = _backward(pn, c["dy"], c["x"], c["g"], mean, rstd)
+    t = [T.from_numpy(v) for v in (c["dy"], c["x"], c["g"], mean, rstd)]
+    dg, db = T.zeros([100]), T.zeros([100])
+    args = [None, dg._ptr, db._ptr] + [v._ptr for v in t]
+    pn.set_stream(None)
+    own = ctypes.c_void_p(lib.neural_hip_get_stream())
+    graph, asked = ctypes.c_void_p(), ctypes.c_int()
+    pn.synchronize()
+    try:
+        pn.set_stream(0)
+        assert hip.hipStreamBeginCapture(own, 2) == 0
+        cannot = hip.hipStreamIsCapturing(None, ctypes.byref(asked)) != 0
+        hip.hipGetLastError()
+        if cannot:
+            before = _alloc_counts(pn)
+            assert lib.neural_layer_norm_backward(*args) == pn.NeuralError.INTERNAL
+            assert _alloc_counts(pn) == before
+        assert hip.hipStreamEndCapture(own, ctypes.byref(graph)) == 0
+        assert hip.hipGraphDestroy(graph) == 0
+    finally:
+        pn.set_stream(None)
+    assert cannot, "the null stream could be asked"
+    assert not dg.numpy().any()
+    assert lib.neural_layer_norm_backward(*args) == 0
+    same_bits(dg.numpy(), want[1])
+    same_bits(db.numpy(), want[2])
