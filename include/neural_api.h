@@ -400,7 +400,8 @@ int neural_counter_dropout_backward(NeuralTensor *grad_in, const NeuralTensor *g
  *
  * Where a gradient of gamma or beta is asked for, the call takes device memory for
  * partial sums from the library's cache; while the stream is being captured, memory of
- * the graph's own, held until the process ends, so graphs may replay side by side.
+ * the graph's own (one block, of its largest call), so graphs may replay side by side.
+ * neural_hip_release_graph_memory gives it back.
  *
  * Errors: NULL_POINTER, DTYPE_MISMATCH, DIM_MISMATCH (a 0-d tensor), SHAPE_MISMATCH,
  * INVALID_ARGUMENT (non-contiguous tensors, eps negative or not finite, p or key as
@@ -704,6 +705,14 @@ void *neural_hip_get_stream(void);
 int   neural_hip_synchronize(void);
 /* Release cached device blocks back to the driver. */
 int   neural_hip_empty_cache(void);
+/* NEW: give back the device memory of captured calls whose graphs have been destroyed,
+ * with all graphs and executable graphs made of them (such memory is held otherwise, as
+ * a graph may be replayed at any time); waits for the device.  HIP may let go of a
+ * destroyed graph only after its last replay: what it still holds is left for the next
+ * call.  An executable graph that took a captured graph's calls by hipGraphExecUpdate holds
+ * no reference to it: destroy the captured graph after the executable one, or
+ * do not call this in between.  NEURAL_ERR_INTERNAL while the stream is being captured. */
+int   neural_hip_release_graph_memory(void);
 /* Device ordinal, compute-unit count and device name of the active GPU. */
 int   neural_hip_device_info(int *ordinal, int *num_cus, char *name, int name_len);
 

@@ -97,10 +97,12 @@ int          hip_fail(hipError_t e);     // maps a HIP error to NEURAL_ERR_* and
 
 void        *dev_alloc(size_t bytes);    // caching allocator (stream-ordered reuse)
 void         dev_free(void *p);
-// Device memory that no cache hands out again, for a launch that is being
-// captured into a graph: the graph may be replayed at any time, so its memory is
-// its own until the process ends.  Allocates during a capture of any mode.
-void        *dev_alloc_own(size_t bytes);
+// Device memory for a launch that is being captured (the active stream is): the
+// graph may be replayed at any time, so the memory is its own, and no cache hands it
+// out again.  One capture's launches, which follow each other on the stream, share a
+// block where it is large enough for each.  Held until neural_hip_release_graph_memory
+// finds the graph and all that was made of it destroyed.  Works in a capture of any mode.
+int          graph_alloc(size_t bytes, void **p);
 
 // Per-runtime device workspace for multi-block reductions: partial results
 // plus a self-resetting completion counter (the last block sets it back to 0).

@@ -652,9 +652,8 @@ __global__ __launch_bounds__(512) void k_ln_cols(LnGradArgs<T> a, int64_t chunk,
 }
 
 // Device memory for the partials of one call.  A call that is being captured
-// has a block of its own, which stays with the graph (it is not given back:
-// the graph may be replayed whenever, beside any other); otherwise the block
-// returns to the cache once the launches that use it are enqueued.
+// has the graph's (which may be replayed whenever, beside any other); otherwise
+// the block returns to the cache once the launches that use it are enqueued.
 struct Partials {
     void *p = nullptr;
     bool keep = false;
@@ -666,7 +665,8 @@ struct Partials {
             return hip_fail(e);
         }
         keep = status != hipStreamCaptureStatusNone;
-        p = keep ? dev_alloc_own(bytes) : dev_alloc(bytes);
+        if (keep) return graph_alloc(bytes, &p);
+        p = dev_alloc(bytes);
         return p ? NEURAL_OK : set_error(NEURAL_ERR_OUT_OF_MEMORY);
     }
     ~Partials()

@@ -204,19 +204,95 @@ void dev_free(void *p)
     r.live.erase(it);
 }
 
-void *dev_alloc_own(size_t bytes)
+// A block of graph_alloc.  `gone` is set by the destructor of a HIP user object that the
+// captured graph, and every graph and executable graph made of it, holds a reference to.
+// HIP may call it from any thread with locks of its own held: it does nothing else.
+namespace {
+struct GraphBlock {
+    void              *p;
+    size_t             bytes;
+    unsigned long long capture;
+    hipStream_t        stream;
+    std::atomic<bool>  gone{false};
+    GraphBlock        *next;
+};
+std::mutex g_graph_mu;  // the list; no HIP call is made under it
+GraphBlock *g_graph_blocks = nullptr;
+void graph_block_gone(void *b) { static_cast<GraphBlock *>(b)->gone.store(true, std::memory_order_release); }
+}  // namespace
+
+int graph_alloc(size_t bytes, void **p)
 {
     g_dev_allocs.fetch_add(1, std::memory_order_relaxed);
-    g_hip_mallocs.fetch_add(1, std::memory_order_relaxed);
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    unsigned long long id = 0;
+    hipGraph_t graph = nullptr;
+    const hipError_t e = hipStreamGetCaptureInfo_v2(stream(), &status, &id, &graph, nullptr, nullptr);
+    if (e != hipSuccess || status != hipStreamCaptureStatusActive) {
+        (void)hipGetLastError();
+        return hip_fail(e != hipSuccess ? e : hipErrorStreamCaptureInvalidated);
+    }
+    {
+        std::lock_guard<std::mutex> g(g_graph_mu);
+        for (GraphBlock *b = g_graph_blocks; b; b = b->next)
+            if (b->capture == id && b->stream == stream() && b->bytes >= bytes) {
+                *p = b->p;
+                return NEURAL_OK;
+            }
+    }
+    GraphBlock *b = new (std::nothrow) GraphBlock{};
+    if (!b) return set_error(NEURAL_ERR_OUT_OF_MEMORY);
     hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
     const bool relaxed = hipThreadExchangeStreamCaptureMode(&mode) == hipSuccess;
-    void *p = nullptr;
-    if (hipMalloc(&p, bytes ? bytes : 1) != hipSuccess) {
+    g_hip_mallocs.fetch_add(1, std::memory_order_relaxed);
+    const bool got = hipMalloc(&b->p, bytes ? bytes : 1) == hipSuccess;
+    // (without the user object the block is simply held until the process ends)
+    hipUserObject_t object = nullptr;
+    if (!got || hipUserObjectCreate(&object, b, graph_block_gone, 1, hipUserObjectNoDestructorSync) != hipSuccess ||
+        hipGraphRetainUserObject(graph, object, 1, hipGraphUserObjectMove) != hipSuccess)
         (void)hipGetLastError();
-        p = nullptr;
-    }
     if (relaxed) (void)hipThreadExchangeStreamCaptureMode(&mode);
-    return p;
+    if (!got) {
+        delete b;
+        return set_error(NEURAL_ERR_OUT_OF_MEMORY);
+    }
+    b->bytes = bytes;
+    b->capture = id;
+    b->stream = stream();
+    std::lock_guard<std::mutex> g(g_graph_mu);
+    b->next = g_graph_blocks;
+    g_graph_blocks = b;
+    *p = b->p;
+    return NEURAL_OK;
+}
+
+static int release_graph_blocks()
+{
+    GraphBlock *gone = nullptr;
+    {
+        std::lock_guard<std::mutex> g(g_graph_mu);
+        for (GraphBlock **at = &g_graph_blocks; *at;) {
+            GraphBlock *b = *at;
+            if (b->gone.load(std::memory_order_acquire)) {
+                *at = b->next;
+                b->next = gone;
+                gone = b;
+            } else {
+                at = &b->next;
+            }
+        }
+    }
+    hipError_t e = hipSuccess;
+    while (gone) {
+        GraphBlock *b = gone;
+        gone = b->next;
+        const hipError_t f = hipFree(b->p);  // waits for the device first
+        if (f != hipSuccess) e = f;
+        delete b;
+    }
+    if (e == hipSuccess) return set_error(NEURAL_OK);
+    (void)hipGetLastError();
+    return hip_fail(e);
 }
 
 bool is_device_ptr(const void *p)
@@ -1141,6 +1217,13 @@ int neural_hip_empty_cache(void)
     std::lock_guard<std::mutex> g(r.mu);
     release_cache_locked(r);
     return set_error(NEURAL_OK);
+}
+
+int neural_hip_release_graph_memory(void)
+{
+    NH_TRY(ensure_init());
+    if (stream_recording()) return set_error(NEURAL_ERR_INTERNAL);
+    return release_graph_blocks();
 }
 
 int neural_hip_device_info(int *ordinal, int *cus, char *name, int name_len)

@@ -12,7 +12,7 @@ transforms.Normalize / MinMaxScale / Compose / compute_stats; tensor_ops.*.
 """
 
 from .core import (NeuralError, NeuralDtype, NeuralException, init, shutdown, version, get_last_error,
-                   get_error_message, clear_error, set_stream, synchronize, device_info)
+                   get_error_message, clear_error, set_stream, synchronize, release_graph_memory, device_info)
 from .tensor import Tensor, zeros, ones, tensor
 from . import nn, activations, optim, quantize, training, tensor_ops, checkpoint, transforms
 from .nn import (ReLU, Sigmoid, Softmax, LogSoftmax, Tanh, CrossEntropyLoss, LabelSmoothingCrossEntropy, Dropout,

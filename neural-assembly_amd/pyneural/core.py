@@ -308,6 +308,7 @@ _SIGS = {
     "neural_hip_get_stream": (_vp, []),
     "neural_hip_synchronize": (_i, []),
     "neural_hip_empty_cache": (_i, []),
+    "neural_hip_release_graph_memory": (_i, []),
     "neural_hip_device_info": (_i, [_ip, _ip, ctypes.c_char_p, _i]),
 }
 
@@ -373,6 +374,12 @@ def set_stream(stream_handle) -> None:
 
 def synchronize() -> None:
     _check_error(_lib.neural_hip_synchronize(), "synchronize")
+
+
+def release_graph_memory() -> None:
+    """Give back the device memory of captured calls whose graphs, and all that
+    was made of them, have been destroyed (neural_hip_release_graph_memory)."""
+    _check_error(_lib.neural_hip_release_graph_memory(), "release_graph_memory")
 
 
 def device_info() -> dict:

@@ -984,3 +984,101 @@ def test_a_stream_that_cannot_be_asked(pn, rng):
     assert lib.neural_layer_norm_backward(*args) == 0
     same_bits(dg.numpy(), want[1])
     same_bits(db.numpy(), want[2])
+
+
+def _captured_grads(pn, torch, stream, cases):
+    """A graph of the gradients of several norms in a row: the graph, its calls' (outputs,
+    wanted, tensors), and how many hipMallocs the library made while it was captured."""
+    lib, T = pn.core._lib, pn.Tensor
+    calls = []
+    for c in cases:
+        _, mean, rstd = _forward(pn, c["x"], c["g"], c["b"])
+        want = _backward(pn, c["dy"], c["x"], c["g"], mean, rstd)
+        ins = [torch.from_numpy(v).cuda() for v in (c["dy"], c["x"], c["g"], mean, rstd)]
+        outs = [torch.zeros_like(v) for v in (ins[1], ins[2], ins[2])]
+        calls.append((outs, want, [T.from_torch(v) for v in outs + ins]))
+    pn.set_stream(stream.cuda_stream)
+    torch.cuda.synchronize()
+    before = _alloc_counts(pn)[1]
+
+    def step():
+        for _, _, t in calls:
+            assert lib.neural_layer_norm_backward(*[v._ptr for v in t]) == 0
+
+    graph = _graph_of(torch, stream, step)
+    made = _alloc_counts(pn)[1] - before
+    pn.set_stream(None)
+    return graph, calls, made
+
+
+def _replayed(torch, replay, calls):
+    for _ in range(2):
+        for outs, _, _ in calls:
+            [o.fill_(9.0) for o in outs]
+        torch.cuda.synchronize()
+        replay()
+        torch.cuda.synchronize()
+        for outs, want, _ in calls:
+            for o, w in zip(outs, want):
+                same_bits(o.cpu().numpy(), w)
+
+
+def test_memory_of_captured_calls(pn, rng):
+    """A capture's gradients share a block, a wider one behind them has its own; the memory
+    stays while the graph lives and is given back when it is gone."""
+    import gc
+    import time
+    import torch
+    s = torch.cuda.Stream()
+    case = lambda rows, cols: _case(rng, rows, cols, np.float32)  # noqa: E731
+    try:
+        _captured_grads(pn, torch, s, [case(600, 50)])  # whatever torch and HIP allocate once
+        graph, calls, made = _captured_grads(pn, torch, s, [case(3000, 4096) for _ in range(3)])  # 16.8 MB of partials
+        assert made == 1
+        other, more, made = _captured_grads(pn, torch, s, [case(3000, 500), case(3000, 2048), case(2000, 300)])
+        assert made == 2
+        _replayed(torch, graph.replay, calls)
+        _replayed(torch, other.replay, more)
+        pn.release_graph_memory()  # both live: nothing of theirs
+        x = torch.full((64 << 20,), 3.0, device="cuda")  # would take what had been freed
+
+        def both():
+            with torch.cuda.stream(s):
+                graph.replay()
+            other.replay()
+
+        _replayed(torch, both, calls + more)
+        assert bool((x == 3).all())
+        had = torch.cuda.mem_get_info()[0]
+        del graph, both
+        gc.collect()
+        for _ in range(100):  # HIP lets go of a destroyed graph in its own time
+            torch.cuda.synchronize()
+            pn.release_graph_memory()
+            got = torch.cuda.mem_get_info()[0] - had
+            if got >= 16 << 20:
+                break
+            time.sleep(0.02)
+        assert 16 << 20 <= got < 48 << 20, got  # one block for the three calls
+        _replayed(torch, other.replay, more)
+    finally:
+        pn.set_stream(None)
+        pn.release_graph_memory()
+
+
+def test_graph_memory_is_not_released_in_a_capture(pn, rng):
+    import torch
+    s = torch.cuda.Stream()
+    y = torch.zeros(8, device="cuda")
+    try:
+        pn.set_stream(s.cuda_stream)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=s):
+            assert pn.core._lib.neural_hip_release_graph_memory() == pn.NeuralError.INTERNAL
+            y.add_(1)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert bool((y == 1).all())
+    finally:
+        pn.set_stream(None)
+    assert pn.core._lib.neural_hip_release_graph_memory() == 0
