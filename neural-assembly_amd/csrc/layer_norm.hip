@@ -289,7 +289,7 @@ template <typename T, int MODE, int NT, int VPT>
 static void launch_ln_rows(const LnArgs<T> &a)
 {
     using Plan = LnPlan<T, NT, VPT, MODE>;
-    with_stream<T, NT, VPT>(a.cols, [&](auto past) {
+    with_stream<T, NT>(a.cols, [&](auto past) {
         const auto launch = [&](unsigned g, int64_t base) {
             NH_LAUNCH((k_ln_rows<T, NT, VPT, MODE, decltype(past)::value>), dim3(g), dim3(Plan::NB), 0, stream(), a, base);
         };

@@ -43,8 +43,9 @@ NH_DEV double rsqrt_d(double v)
 // How a group's vectors of a row are read and written: past the caches (NT, each
 // byte is used once), except where one access of a wave leaves parts of 64-byte
 // blocks to the next, which then are fetched, and written, twice: f32 [838860, 40] 114 us ->
-// 62.6, [335544, 100] 61.0 -> 52.3, [86037, 390] 60.9 -> 53.1 (rows of whole blocks the
-// other way: [349525, 96] 49.8, 52.2 through the caches, [83886, 400] 47.8, 51.8).
+// 59.5, [335544, 100] 61.0 -> 55.5, [86037, 390] 60.9 -> 54.0 (rows of whole blocks the
+// other way, when both were measured: [349525, 96] 49.8, 52.2 through the caches, [83886, 400]
+// 47.8, 51.8; now 47.1 and 49.5).
 template <typename T, bool PAST>
 struct RowStream {
     using V = typename Vec16<T>::type;
@@ -61,16 +62,14 @@ struct RowStream {
     }
 };
 
-// run(std::bool_constant<PAST>) for groups of NT lanes of VPT vectors.
-template <typename T, int NT, int VPT, typename R>
+// run(std::bool_constant<PAST>) for groups of NT lanes.
+template <typename T, int NT, typename R>
 auto with_stream(int64_t cols, R run)
 {
     if constexpr (NT >= 64) {
         return run(std::true_type{});
     } else {
-        if constexpr (NT > 4 || VPT == 1) {
-            if (cols * int64_t(sizeof(T)) % 64 == 0) return run(std::true_type{});
-        }
+        if (cols * int64_t(sizeof(T)) % 64 == 0) return run(std::true_type{});
         return run(std::false_type{});
     }
 }

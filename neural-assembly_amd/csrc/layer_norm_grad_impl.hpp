@@ -726,7 +726,7 @@ static int launch_ln_grad_rows(const LnGradArgs<T> &a0, T *dgamma, T *dbeta)
     // as many blocks as the CUs hold at once, no more than rows
     const int64_t most = int64_t(num_cus()) * Plan::kPerCu;
     const int64_t nb = need < most ? need : most;
-    return with_stream<T, NT, VPT>(a.cols, [&](auto past) -> int {
+    return with_stream<T, NT>(a.cols, [&](auto past) -> int {
         constexpr bool kPast = decltype(past)::value;
         if constexpr (VPT <= 8) {
             if (sums) {
