@@ -36,10 +36,10 @@ struct LnGradPlan {
 };
 
 // Bound by HBM: three streams (the joined forms five), and for the listed widths within
-// 10% of a copy of the same bytes: f32 [16384, 4096] 135 us where the copy takes 134, and 4.9
-// for the partials' fold (k_ln_fold); joined 224 and 4.9 (225); [200000, 96] 39.8 and 4.6 (38).
-// f64 rows of an odd width, whose accesses straddle one 128-byte line in eight: 39.9 and
-// 5.4 at [4096, 2049] (33).
+// 10% of a copy of the same bytes: f32 [16384, 4096] 136 us where the copy takes 134, and 4.9
+// for the partials' fold (k_ln_fold); joined 221 and 4.7 (225); [200000, 96] 40.2 and 4.5 (38).
+// f64 rows of an odd width, whose accesses straddle one 128-byte line in eight: 40.2 and
+// 5.3 at [4096, 2049] (33).
 //
 // Groups of NT lanes walk the rows, r = group, group + groups, ...: each tensor
 // read once, the next row's loads issued before this one is worked on, the row's
@@ -54,7 +54,7 @@ struct LnGradPlan {
 // registers too (7 and 8 vectors, the joined forms' 6): there a vector of the next row is
 // loaded as soon as this row's has been used for the last time, and dh behind the row's sums.
 // (Both sums in LDS as floats, rounded every row, and the next row in registers: [2048, 16384]
-// 84.3 us, now 85.8, joined 155, now 148; [2396, 14000] 88.4, now 92.3, joined 159, now 149;
+// 84.5 us, now 85.6, joined 154, now 150; [2396, 14000] 88.2, now 92.0, joined 159, now 151;
 // narrower alike; but 80 rows a block lost 11 u in dbeta, now 2 u.)
 template <typename T, int NT, int VPT, int MODE, bool SUMS, bool PAST>
 NH_DEV void ln_grad_rows(const LnGradArgs<T> &a, int64_t block, int64_t blocks)
@@ -74,9 +74,8 @@ NH_DEV void ln_grad_rows(const LnGradArgs<T> &a, int64_t block, int64_t blocks)
     __shared__ uint8_t lds_keep[2][MODE == LN_DROP ? RPB : 1][MODE == LN_DROP ? K::kBytes : 1];
     __shared__ V lds_g[LS ? VPT : 1][LS ? NT : 1], lds_b[LS ? VPT : 1][LS ? NT : 1];
     __shared__ D2 lds_split[SS ? VPT : 1][SS ? VN / 2 : 1][SS ? NT : 1];
-    // (a block of one row: a uniform row saves the address registers that SS is short of; the
-    // other forms are no faster for it, joined [16384, 4096] 232 us, without 230.5)
-    const int lane = threadIdx.x % NT, sub = SS && RPB == 1 ? 0 : threadIdx.x / NT;
+    // (a block of one row: a uniform row saves the address registers that SS is short of)
+    const int lane = threadIdx.x % NT, sub = RPB == 1 ? 0 : threadIdx.x / NT;
     const int64_t cols = a.cols;
     const RowCut<T> cut(cols);
     const auto in_row = [&](int k) { return k < Plan::F || lane + k * NT < cut.ncv; };
@@ -133,21 +132,26 @@ NH_DEV void ln_grad_rows(const LnGradArgs<T> &a, int64_t block, int64_t blocks)
     const auto load_dy = [&](Row &w, int64_t at, int k) {
         if (in_row(k)) w.dy[k] = S::load(reinterpret_cast<const U *>(a.dy + at) + lane + k * NT);
     };
-    const auto load_scalars = [&](Row &w, int64_t r) {
+    // first, since loads return in order and the row's work begins with them (behind the row's
+    // others: [512, 4096] 9.3 us, 8.9 so)
+    const auto load_stats = [&](Row &w, int64_t r) {
         w.mean = a.mean[r];
         w.rstd = a.rstd[r];
+    };
+    const auto load_tail = [&](Row &w, int64_t at) {
         if (has_t) {
-            w.xt = a.h[r * cols + cut.sc(lane)];
-            w.dyt = a.dy[r * cols + cut.sc(lane)];
+            w.xt = a.h[at + cut.sc(lane)];
+            w.dyt = a.dy[at + cut.sc(lane)];
         }
     };
     const auto load = [&](Row &w, int64_t r) {
         const int64_t at = r * cols;
+        load_stats(w, r);
 #pragma unroll
         for (int k = 0; k < VPT; k++) load_x(w, at, k);
 #pragma unroll
         for (int k = 0; k < VPT; k++) load_dy(w, at, k);
-        load_scalars(w, r);
+        load_tail(w, at);
     };
     const int64_t step = blocks * RPB;
     int64_t r = block * RPB + sub;
@@ -254,6 +258,7 @@ NH_DEV void ln_grad_rows(const LnGradArgs<T> &a, int64_t block, int64_t blocks)
         };
         const int64_t after = (r + step) * cols;
         const bool again = kReload && r + step < a.rows;
+        if (again) load_stats(w, r + step);
 #pragma unroll
         for (int k = 0; k < VPT; k++) {
             if ((MODE != LN_PLAIN || a.dx) && in_row(k)) {
@@ -296,7 +301,7 @@ NH_DEV void ln_grad_rows(const LnGradArgs<T> &a, int64_t block, int64_t blocks)
             if constexpr (MODE == LN_DROP) o = dropped<T>(o, scale, keep.tail, 0);
             if (a.dx) a.dx[i] = o;
         }
-        if (again) load_scalars(w, r + step);
+        if (again) load_tail(w, after);
     };
     Row w;
     if (r < a.rows) load(w, r);
