@@ -400,8 +400,8 @@ int neural_counter_dropout_backward(NeuralTensor *grad_in, const NeuralTensor *g
  *
  * Where a gradient of gamma or beta is asked for, the call takes device memory for
  * partial sums from the library's cache; while the stream is being captured, memory of
- * the graph's own (one block, of its largest call), so graphs may replay side by side.
- * neural_hip_release_graph_memory gives it back.
+ * the graph's own, which its calls share as far as the first is large enough, so graphs
+ * may replay side by side.  neural_hip_release_graph_memory gives it back.
  *
  * Errors: NULL_POINTER, DTYPE_MISMATCH, DIM_MISMATCH (a 0-d tensor), SHAPE_MISMATCH,
  * INVALID_ARGUMENT (non-contiguous tensors, eps negative or not finite, p or key as

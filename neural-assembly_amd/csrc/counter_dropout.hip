@@ -97,7 +97,8 @@ static int counter_dropout_api(NeuralTensor *out, const NeuralTensor *in, double
     const int64_t n = numel(in);
     if (numel(out) != n) return set_error(NEURAL_ERR_SHAPE_MISMATCH);
     if (!is_contiguous(in) || !is_contiguous(out)) return set_error(NEURAL_ERR_INVALID_ARGUMENT);
-    if (tensors_may_overlap(out, in) && out->data != in->data && out->dev != in->dev) return set_error(NEURAL_ERR_INVALID_ARGUMENT);
+    if (tensors_may_overlap(out, in) && out->data != in->data && out->dev != in->dev)
+        return set_error(NEURAL_ERR_INVALID_ARGUMENT);
     DropArgs a;
     NH_TRY(drop_args(p, key, a));
     if (n == 0) return set_error(NEURAL_OK);
