@@ -482,17 +482,18 @@ __global__ __launch_bounds__((LnGradPlan<T, NT, VPT>::NB)) void k_ln_grad_few(Ln
 // Column sums of the partials: [n][2 cols] -> dgamma, dbeta.  A block of 1024 lanes
 // takes 32 columns, the partials by 128 (f64 64) streams of four in flight.  f32
 // [4096, 1024] in all 15.9 us with 64 columns, 15.3 with 32; f64 [4096, 2049] 45.3 with 32,
-// 46.7 with 16.
+// 46.7 with 16.  b_base: the launch's first block, not its first column, which the compiler
+// would not know to be even: f64 [15360, 34] joined 10.9 us, 10.35 so.
 template <typename T>
 __global__ __launch_bounds__(1024) void k_ln_fold(const T *__restrict__ part, int64_t n, int64_t cols,
-                                                  T *__restrict__ dgamma, T *__restrict__ dbeta, int64_t c_base)
+                                                  T *__restrict__ dgamma, T *__restrict__ dbeta, int64_t b_base)
 {
     using V = typename Vec16<T>::type;
     using U = typename VecU<T>::type;
     constexpr int VN = Vec16<T>::n, C = 32, L = C / VN, S = 1024 / L, UN = 4, TPC = 1024 / C;
     __shared__ double sh[S][C + 1];  // (read by columns below: no two lanes on a bank)
     const int vl = threadIdx.x % L, st = threadIdx.x / L;
-    const int64_t width = 2 * cols, c0 = c_base + int64_t(blockIdx.x) * C, c = c0 + vl * VN;
+    const int64_t width = 2 * cols, c0 = (b_base + int64_t(blockIdx.x)) * C, c = c0 + vl * VN;
     double s[VN];
 #pragma unroll
     for (int j = 0; j < VN; j++) s[j] = 0.0;
@@ -536,7 +537,7 @@ __global__ __launch_bounds__(1024) void k_ln_fold(const T *__restrict__ part, in
 template <typename T>
 static void launch_ln_fold(const T *part, int64_t n, int64_t cols, T *dgamma, T *dbeta)
 {
-    for_row_launches(2 * cols, 32, 1024, [&](unsigned g, int64_t base) {
+    for_row_launches(ceil_div(2 * cols, 32), 1, 1024, [&](unsigned g, int64_t base) {
         NH_LAUNCH((k_ln_fold<T>), dim3(g), dim3(1024), 0, stream(), part, n, cols, dgamma, dbeta, base);
     });
 }
@@ -601,16 +602,16 @@ __global__ __launch_bounds__(kLnWide) void k_ln_grad_wide(LnGradArgs<T> a, int64
 }
 
 // Column sums beside a row pass that cannot hold them: 64 lanes of VN columns a block, the
-// rows of its chunk by 8 waves, four in flight each.
+// rows of its chunk by 8 waves, four in flight each.  b_base: as k_ln_fold's.
 template <typename T>
-__global__ __launch_bounds__(512) void k_ln_cols(LnGradArgs<T> a, int64_t chunk, int64_t c_base)
+__global__ __launch_bounds__(512) void k_ln_cols(LnGradArgs<T> a, int64_t chunk, int64_t b_base)
 {
     using V = typename Vec16<T>::type;
     using U = typename VecU<T>::type;
     constexpr int VN = Vec16<T>::n, W = 8, UN = 4;
     __shared__ double sh[W][2 * VN][64];
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const int64_t cols = a.cols, c = c_base + (int64_t(blockIdx.x) * 64 + lane) * VN;
+    const int64_t cols = a.cols, c = ((b_base + int64_t(blockIdx.x)) * 64 + lane) * VN;
     const int64_t r0 = int64_t(blockIdx.y) * chunk, r1 = r0 + chunk < a.rows ? r0 + chunk : a.rows;
     const bool whole = c + VN <= cols;
     double s[2 * VN];
@@ -693,7 +694,7 @@ static int launch_ln_cols(LnGradArgs<T> a, T *dgamma, T *dbeta)
     Partials part;
     NH_TRY(part.open(size_t(chunks) * 2 * size_t(a.cols) * sizeof(T)));
     a.part = static_cast<T *>(part.p);
-    for_row_launches(a.cols, 64 * Vec16<T>::n, 512, [&](unsigned g, int64_t base) {
+    for_row_launches(gx, 1, 512, [&](unsigned g, int64_t base) {
         NH_LAUNCH((k_ln_cols<T>), dim3(g, unsigned(chunks)), dim3(512), 0, stream(), a, chunk, base);
     });
     launch_ln_fold(a.part, chunks, a.cols, dgamma, dbeta);
