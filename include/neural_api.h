@@ -422,6 +422,96 @@ int neural_dropout_add_layer_norm_backward(NeuralTensor *grad_in, NeuralTensor *
                                            const NeuralTensor *mean, const NeuralTensor *rstd, double p,
                                            const NeuralDropoutKey *key);
 
+/* ---- RMS norm and 8-bit rows (NEW) ----------------------------------------------
+ * No counterpart in the reference.  Rows over the last dimension of contiguous f32 / f64
+ * tensors of any rank >= 1; all tensors of a call have one dtype.
+ *
+ * neural_rms_norm_forward: h = in, or in + residual (residual may be NULL; rounded to the
+ * dtype as neural_add), rstd = 1 / sqrt(sum h^2 / C + eps), out = h rstd gamma (gamma: C
+ * values, NULL: 1), in double, rounded once per value.  hidden: h, for the residual stream
+ * and the backward call (NULL where neither follows, and where residual is NULL: h is in
+ * then); rstd: one value per row, for the backward call (may be NULL).  out or hidden may be
+ * in or residual.  A row whose sum of squares is not finite is NaN.
+ *
+ * neural_rms_norm_backward, from the saved rstd: xh = hidden rstd, w = grad_out gamma,
+ * grad_in = rstd (w - xh mean_C(w xh)) [rounded, + grad_hidden, the gradient that reaches
+ * hidden along the residual stream; may be NULL]: the gradient of in, and of residual.
+ * grad_gamma = sum over rows of grad_out xh, summed in double; what a group of rows leaves of
+ * it is rounded to the dtype.  The order goes by the shape and the device alone: equal calls
+ * give equal bits.  grad_in or grad_gamma may be NULL, not both.  grad_in may be grad_out,
+ * grad_hidden or hidden.  Where grad_gamma is asked for, the call takes device memory for
+ * partial sums, as neural_layer_norm_backward.
+ *
+ * Rows in 8 bits: for a row of values w, a = max |w|, code = 127 w / a rounded to the nearest
+ * whole number, halves away from zero (decided exactly), and scale = a / 127 in the dtype: a
+ * code stands for code * scale.  A row of zeros has codes and scale 0; a row that holds NaN or
+ * an infinity has codes 0 and scale NaN.  Row r's codes begin at codes + r * stride (stride >=
+ * C, in bytes; host or device memory); bytes between the rows are left as they are.
+ *   neural_quantize_rows: w = in.
+ *   neural_rms_norm_forward_q8: w = h gamma and scale = a rstd / 127, the codes of the norm's
+ *   output (before its rounding to the dtype); otherwise as neural_rms_norm_forward.
+ *
+ * neural_linear_q8: out[m, n] = act(scale[m] w_scale[n] sum_k codes[m, k] w_codes[n, k] +
+ * bias[n]) + residual[m, n], out [.., N] of M rows, the weights by output channel: row n's k
+ * codes at w_codes + n * w_stride (from neural_quantize_rows, or any int8 values).  The sum is
+ * exact; its scaling and the bias are taken in double and rounded to the dtype, then the
+ * activation as neural_bias_add_act takes it (act, alpha: there), then the residual is added.
+ * bias, residual: may be NULL; out may be residual.  1 <= k <= 131071 (a sum stays below
+ * 2^31; more: NEURAL_ERR_TENSOR_TOO_LARGE).  Any strides and addresses are taken; codes and
+ * weights at 16-byte aligned addresses with strides that are multiples of 16 are read in place,
+ * others are copied first.
+ *
+ * Errors: NULL_POINTER, DTYPE_MISMATCH, DIM_MISMATCH (a 0-d tensor), SHAPE_MISMATCH,
+ * INVALID_ARGUMENT (non-contiguous tensors, eps negative or not finite, a stride less than the
+ * row, k < 1, an unknown act, hidden without residual, outputs that overlap an input, other
+ * than as allowed, or each other). */
+int neural_rms_norm_forward(NeuralTensor *out, NeuralTensor *hidden, const NeuralTensor *in,
+                            const NeuralTensor *residual, const NeuralTensor *gamma, double eps,
+                            NeuralTensor *rstd);
+int neural_rms_norm_backward(NeuralTensor *grad_in, NeuralTensor *grad_gamma, const NeuralTensor *grad_out,
+                             const NeuralTensor *grad_hidden, const NeuralTensor *hidden,
+                             const NeuralTensor *gamma, const NeuralTensor *rstd);
+int neural_rms_norm_forward_q8(int8_t *codes, int64_t stride, NeuralTensor *scale, NeuralTensor *hidden,
+                               const NeuralTensor *in, const NeuralTensor *residual, const NeuralTensor *gamma,
+                               double eps);
+int neural_quantize_rows(int8_t *codes, int64_t stride, NeuralTensor *scale, const NeuralTensor *in);
+int neural_linear_q8(NeuralTensor *out, const int8_t *codes, int64_t stride, const NeuralTensor *scale,
+                     const int8_t *w_codes, int64_t w_stride, const NeuralTensor *w_scale, int64_t k,
+                     const NeuralTensor *bias, int act, double alpha, const NeuralTensor *residual);
+
+/* ---- Log probabilities of given tokens (NEW) ---------------------------------------
+ * No counterpart in the reference.  logits [.., V] contiguous, f32 or f64, V < 2^31; one token
+ * per row.  z = logits / temperature, lse = log sum_v exp z_v, p = exp(z - lse).
+ *
+ * Forward, every output one value per row in the logits' dtype, any of them NULL, not all:
+ * logprob = z[token] - lse, entropy = -sum p log p (a term of p = 0 is 0), lse (for the
+ * backward call), and the k (0 to 64) largest logits, equal ones by index: top_ids [rows, k]
+ * int64 (host or device memory) and top_logprobs [rows, k] (either may be NULL).
+ * A logit of -inf is a masked one: it is no alternative, and where fewer than k are left the
+ * rest is id -1, log probability -inf.  A row with all logits masked has lse and logprob
+ * -inf and entropy 0.  A row with NaN or +inf has NaN, ids -1.
+ * tokens: int64, one per row, host or device memory; NULL where logprob is not asked for.  A
+ * negative token: the row is not used (padding), its logits are not read: logprob, entropy and
+ * lse 0, ids -1, alternatives' log probabilities -inf.  A token >= V: logprob NaN.
+ *
+ * Backward, from the saved lse and entropy: grad_logits = (g (1[v = token] - p) - e p (log p +
+ * entropy)) / temperature, g and e the gradients of logprob and entropy (one value per row;
+ * either may be NULL, not both; entropy may be NULL without e).  0 in a row that is not used or
+ * has all logits masked; NaN where g is given and the token >= V.  grad_logits may be logits.
+ *
+ * Where a row is split over several blocks the forward call takes device memory for their
+ * partial results, as neural_layer_norm_backward does.
+ * Errors: NULL_POINTER, DTYPE_MISMATCH, DIM_MISMATCH (a 0-d tensor), SHAPE_MISMATCH,
+ * TENSOR_TOO_LARGE, INVALID_ARGUMENT (non-contiguous tensors, k outside [0, 64], a temperature
+ * that is not positive and finite, outputs that overlap an input, other than as allowed, or each
+ * other). */
+int neural_token_logprobs_forward(NeuralTensor *logprob, NeuralTensor *entropy, NeuralTensor *lse,
+                                  int64_t *top_ids, NeuralTensor *top_logprobs, int64_t k,
+                                  const NeuralTensor *logits, const int64_t *tokens, double temperature);
+int neural_token_logprobs_backward(NeuralTensor *grad_logits, const NeuralTensor *g, const NeuralTensor *e,
+                                   const NeuralTensor *logits, const int64_t *tokens, const NeuralTensor *lse,
+                                   const NeuralTensor *entropy, double temperature);
+
 /* ---- 2-D f64 tensor ops: neural_api.h:1273-1305, tensor_ops.c:15-148 ---------- */
 int tensor_concat_2d(const double *a, const double *b, int64_t rows_a, int64_t cols_a,
                      int64_t rows_b, int64_t cols_b, int64_t axis, double *out,

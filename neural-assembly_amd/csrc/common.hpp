@@ -172,6 +172,10 @@ bool         is_contiguous(const NeuralTensor *t);
 // element spans (through the strides) whose addresses intersect, on the host or
 // on the device (a tensor over an owned tensor's device address).
 bool         tensors_may_overlap(const NeuralTensor *a, const NeuralTensor *b);
+// The same for a raw buffer (host or device memory) and a tensor; false where either is null.
+bool         raw_may_overlap(const void *p, size_t bytes, const NeuralTensor *t);
+// ... and for two raw buffers.
+bool         raws_may_overlap(const void *p, size_t pbytes, const void *q, size_t qbytes);
 int          check_tensor(const NeuralTensor *t);   // null / dtype validation
 // Make the device copy current and return its element-0 address.
 int          dev_read(const NeuralTensor *t, const void **p);

@@ -19,9 +19,9 @@
 // A row is held by one group of lanes, part of a wave to a block of 1024, at any
 // width and alignment (RowCut), so each tensor is read once and written once.
 #include <cmath>
-#include <initializer_list>
 
 #include "layer_norm.hpp"
+#include "row_call.hpp"
 
 namespace nh {
 
@@ -338,92 +338,6 @@ static int launch_ln(const LnArgs<T> &a)
 
 // ---- arguments -----------------------------------------------------------------------------
 
-// A call's tensors, checked before anything runs: rows of the last dimension
-// of `like`, in its type.  Optional tensors may be null.
-struct LnCall {
-    const NeuralTensor *like;
-    int64_t rows = 0, cols = 0;
-
-    int open(const NeuralTensor *t)
-    {
-        like = t;
-        NH_TRY(check_tensor(t));
-        if (t->ndim < 1) return set_error(NEURAL_ERR_DIM_MISMATCH);
-        cols = t->shape[t->ndim - 1];
-        rows = cols > 0 ? numel(t) / cols : 0;
-        return is_contiguous(t) ? NEURAL_OK : set_error(NEURAL_ERR_INVALID_ARGUMENT);
-    }
-    int type(const NeuralTensor *t) const
-    {
-        NH_TRY(check_tensor(t));
-        return t->dtype == like->dtype ? NEURAL_OK : set_error(NEURAL_ERR_DTYPE_MISMATCH);
-    }
-    // the shape of `like`
-    int same(const NeuralTensor *t) const
-    {
-        if (!t) return NEURAL_OK;
-        NH_TRY(type(t));
-        if (t->ndim != like->ndim) return set_error(NEURAL_ERR_SHAPE_MISMATCH);
-        for (int64_t i = 0; i < t->ndim; i++)
-            if (t->shape[i] != like->shape[i]) return set_error(NEURAL_ERR_SHAPE_MISMATCH);
-        return is_contiguous(t) ? NEURAL_OK : set_error(NEURAL_ERR_INVALID_ARGUMENT);
-    }
-    // n values (one per row or per column)
-    int vec(const NeuralTensor *t, int64_t n) const
-    {
-        if (!t) return NEURAL_OK;
-        NH_TRY(type(t));
-        if (numel(t) != n) return set_error(NEURAL_ERR_SHAPE_MISMATCH);
-        return is_contiguous(t) ? NEURAL_OK : set_error(NEURAL_ERR_INVALID_ARGUMENT);
-    }
-};
-
-// Outputs share no bytes with each other or with an input, except that one of the first
-// kRowOuts outputs may be one of the first `row_ins` inputs itself: those are the tensors
-// of the rows' shape.  (Of one row, or one column, the others have as many values: the
-// column sums are written beside the rows that are still read.)
-constexpr ptrdiff_t kRowOuts = 2;
-static int check_apart(std::initializer_list<NeuralTensor *> outs, std::initializer_list<const NeuralTensor *> ins,
-                       size_t row_ins)
-{
-    for (auto o = outs.begin(); o != outs.end(); ++o) {
-        if (!*o) continue;
-        const size_t in_place = o - outs.begin() < kRowOuts ? row_ins : 0;
-        for (auto p = o + 1; p != outs.end(); ++p)
-            if (tensors_may_overlap(*o, *p)) return set_error(NEURAL_ERR_INVALID_ARGUMENT);
-        size_t k = 0;
-        for (const NeuralTensor *i : ins) {
-            const bool itself = k++ < in_place && i && (i->data == (*o)->data || i->dev == (*o)->dev) &&
-                                numel(i) == numel(*o);
-            if (!itself && tensors_may_overlap(*o, i)) return set_error(NEURAL_ERR_INVALID_ARGUMENT);
-        }
-    }
-    return NEURAL_OK;
-}
-
-template <typename T>
-static int read_t(const NeuralTensor *t, const T *&p)
-{
-    const void *v = nullptr;
-    if (t) NH_TRY(dev_read(t, &v));
-    p = static_cast<const T *>(v);
-    return NEURAL_OK;
-}
-template <typename T>
-static int write_t(NeuralTensor *t, T *&p)
-{
-    void *v = nullptr;
-    if (t) NH_TRY(dev_write(t, &v, true));
-    p = static_cast<T *>(v);
-    return NEURAL_OK;
-}
-static int written(std::initializer_list<NeuralTensor *> outs)
-{
-    for (NeuralTensor *t : outs)
-        if (t) NH_TRY(dev_written(t));
-    return set_error(NEURAL_OK);
-}
-
 struct LnTensors {
     NeuralTensor *out, *hidden;
     const NeuralTensor *in, *residual, *gamma, *beta;
@@ -431,7 +345,7 @@ struct LnTensors {
 };
 
 template <typename T>
-static int ln_run(const LnTensors &t, const LnCall &c, double eps, const DropArgs &drop, int mode)
+static int ln_run(const LnTensors &t, const RowCall &c, double eps, const DropArgs &drop, int mode)
 {
     LnArgs<T> a{};
     a.rows = c.rows;
@@ -457,7 +371,7 @@ static int ln_forward(const LnTensors &t, double p, const NeuralDropoutKey *key,
 {
     NH_TRY(ensure_init());
     if (!t.out || !t.in || (joined && !t.residual)) return set_error(NEURAL_ERR_NULL_POINTER);
-    LnCall c;
+    RowCall c;
     NH_TRY(c.open(t.in));
     NH_TRY(c.same(t.out));
     NH_TRY(c.same(t.hidden));
@@ -482,7 +396,7 @@ struct LnGradTensors {
 };
 
 template <typename T>
-static int ln_grad_run(const LnGradTensors &t, const LnCall &c, const DropArgs &drop, int mode)
+static int ln_grad_run(const LnGradTensors &t, const RowCall &c, const DropArgs &drop, int mode)
 {
     LnGradArgs<T> a{};
     a.rows = c.rows;
@@ -510,7 +424,7 @@ static int ln_backward(const LnGradTensors &t, double p, const NeuralDropoutKey 
     NH_TRY(ensure_init());
     if (!t.dy || !t.h || !t.mean || !t.rstd || (!t.dx && !t.dres && !t.dgamma && !t.dbeta))
         return set_error(NEURAL_ERR_NULL_POINTER);
-    LnCall c;
+    RowCall c;
     NH_TRY(c.open(t.h));
     NH_TRY(c.same(t.dy));
     NH_TRY(c.same(t.dh));

@@ -6,6 +6,7 @@
 #include <type_traits>
 
 #include "layer_norm.hpp"
+#include "row_call.hpp"
 
 namespace nh {
 
@@ -656,30 +657,6 @@ __global__ __launch_bounds__(512) void k_ln_cols(LnGradArgs<T> a, int64_t chunk,
         a.part[(int64_t(blockIdx.y) * 2 + w / VN) * cols + c + w % VN] = T(t);
     }
 }
-
-// Device memory for the partials of one call.  A call that is being captured
-// has the graph's (which may be replayed whenever, beside any other); otherwise
-// the block returns to the cache once the launches that use it are enqueued.
-struct Partials {
-    void *p = nullptr;
-    bool keep = false;
-    int open(size_t bytes)
-    {
-        hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
-        if (const hipError_t e = hipStreamIsCapturing(stream(), &status)) {  // nothing is launched then
-            (void)hipGetLastError();
-            return hip_fail(e);
-        }
-        keep = status != hipStreamCaptureStatusNone;
-        if (keep) return graph_alloc(bytes, &p);
-        p = dev_alloc(bytes);
-        return p ? NEURAL_OK : set_error(NEURAL_ERR_OUT_OF_MEMORY);
-    }
-    ~Partials()
-    {
-        if (p && !keep) dev_free(p);
-    }
-};
 
 // Column sums by k_ln_cols and a fold.
 template <typename T>

@@ -844,6 +844,25 @@ bool nh::tensors_may_overlap(const NeuralTensor *a, const NeuralTensor *b)
     return meet(a->data, b->data) || meet(a->dev, b->dev);
 }
 
+bool nh::raws_may_overlap(const void *p, size_t pbytes, const void *q, size_t qbytes)
+{
+    if (!p || !q || !pbytes || !qbytes) return false;
+    const uintptr_t a = reinterpret_cast<uintptr_t>(p), b = reinterpret_cast<uintptr_t>(q);
+    return a < b + qbytes && b < a + pbytes;
+}
+
+bool nh::raw_may_overlap(const void *p, size_t bytes, const NeuralTensor *t)
+{
+    if (!t) return false;
+    int64_t lo, hi;
+    span_of(t, &lo, &hi);
+    if (hi <= lo) return false;
+    const auto meet = [&](const void *q) {
+        return q && raws_may_overlap(p, bytes, static_cast<const char *>(q) + lo, size_t(hi - lo));
+    };
+    return meet(t->data) || meet(t->dev);
+}
+
 extern "C" {
 
 int neural_init(void) { return ensure_init(); }

@@ -5,9 +5,9 @@ implementation of Neural-Assembly's tensor hot path.
 Public names follow the reference package for this path: Tensor, zeros,
 ones, tensor; nn.ReLU/Sigmoid/Softmax/Tanh, nn.CrossEntropyLoss /
 LabelSmoothingCrossEntropy, nn.Dropout (+ dropout_seed), nn.CounterDropout,
-nn.LayerNorm, nn.DropoutAddLayerNorm (+ counter_dropout_seed), fused add_relu /
-bias_add_act; activations.*; Quantizer / QuantParams; optim.SGD/Adam/AdamW; training.NaNDetector / grad_l2_norm /
-clip_grad_norm / clip_grad_value; save_checkpoint / load_checkpoint;
+nn.LayerNorm, nn.DropoutAddLayerNorm (+ counter_dropout_seed), nn.RMSNorm, nn.QuantizedLinear,
+nn.TokenLogProbs, fused add_relu / bias_add_act; activations.*; Quantizer / QuantParams, QuantizedRows;
+optim.SGD/Adam/AdamW; training.NaNDetector / grad_l2_norm / clip_grad_norm / clip_grad_value; save_checkpoint / load_checkpoint;
 transforms.Normalize / MinMaxScale / Compose / compute_stats; tensor_ops.*.
 """
 
@@ -16,11 +16,11 @@ from .core import (NeuralError, NeuralDtype, NeuralException, init, shutdown, ve
 from .tensor import Tensor, zeros, ones, tensor
 from . import nn, activations, optim, quantize, training, tensor_ops, checkpoint, transforms
 from .nn import (ReLU, Sigmoid, Softmax, LogSoftmax, Tanh, CrossEntropyLoss, LabelSmoothingCrossEntropy, Dropout,
-                 CounterDropout, LayerNorm, DropoutAddLayerNorm, dropout_seed, counter_dropout_seed, add_relu,
-                 bias_add_act)
+                 CounterDropout, LayerNorm, DropoutAddLayerNorm, RMSNorm, QuantizedLinear, TokenLogProbs, dropout_seed,
+                 counter_dropout_seed, add_relu, bias_add_act)
 from .activations import GELU, LeakyReLU, ELU, SELU, Swish, Mish, HardSwish, Softplus, HardTanh
 from .optim import SGD, Adam, AdamW
-from .quantize import Quantizer, QuantParams, quantized_matmul
+from .quantize import Quantizer, QuantParams, QuantizedRows, quantized_matmul
 from .training import NaNDetector, grad_l2_norm, clip_grad_norm, clip_grad_value
 from .checkpoint import save_checkpoint, load_checkpoint
 from .transforms import Normalize, MinMaxScale, Compose, compute_stats

@@ -282,6 +282,15 @@ _SIGS = {
     "neural_layer_norm_backward": (_i, [_vp] * 8),
     "neural_dropout_add_layer_norm_forward": (_i, [_vp] * 6 + [_d, _vp, _d, _vp, _vp]),
     "neural_dropout_add_layer_norm_backward": (_i, [_vp] * 10 + [_d, _vp]),
+    # RMS norm and 8-bit rows
+    "neural_rms_norm_forward": (_i, [_vp] * 5 + [_d, _vp]),
+    "neural_rms_norm_backward": (_i, [_vp] * 7),
+    "neural_rms_norm_forward_q8": (_i, [_vp, _i64] + [_vp] * 5 + [_d]),
+    "neural_quantize_rows": (_i, [_vp, _i64, _vp, _vp]),
+    "neural_linear_q8": (_i, [_vp, _vp, _i64, _vp, _vp, _i64, _vp, _i64, _vp, _i, _d, _vp]),
+    # log probabilities of given tokens
+    "neural_token_logprobs_forward": (_i, [_vp] * 5 + [_i64, _vp, _vp, _d]),
+    "neural_token_logprobs_backward": (_i, [_vp] * 7 + [_d]),
     # tensor ops
     "tensor_concat_2d": (_i, [_vp, _vp, _i64, _i64, _i64, _i64, _i64, _vp, _i64p, _i64p]),
     "tensor_split_2d": (_i, [_vp, _i64, _i64, _i64, _i64, _vp, _vp, _i64p, _i64p, _i64p, _i64p]),

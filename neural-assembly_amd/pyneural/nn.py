@@ -12,15 +12,20 @@ and bias_add_act (bias add of nn_layers.asm:472-539 followed by an
 activation, one pass).  Without a reference counterpart: CounterDropout (a mask
 made from a seed and a call number, never stored), LayerNorm and
 DropoutAddLayerNorm (the residual add, dropout and norm that end a transformer's
-sublayer, in one pass), each with its backward pass.
+sublayer, in one pass) and RMSNorm (alone or with the residual add), each with its
+backward pass; RMSNorm.forward_q8 and QuantizedLinear (the norm's output in 8 bits,
+and its product with 8-bit weights); TokenLogProbs (log probabilities of given
+tokens, entropy, alternatives, and their gradient).
 """
 
+import collections
 import ctypes
 import itertools
 
 import numpy as np
 
 from .core import _lib, _check_error, DropoutKeyC, NeuralDtype
+from .quantize import QuantizedRows
 from .tensor import Tensor
 
 
@@ -438,6 +443,184 @@ class DropoutAddLayerNorm(LayerNorm):
         return f"DropoutAddLayerNorm({self.num_features}, p={self.dropout.p}, eps={self.eps})"
 
 
+class RMSNorm(Module):
+    """h / sqrt(mean(h^2) + eps) * gamma over the last dimension, h = x or x +
+    residual (neural_rms_norm_forward).  With a residual, ``forward`` returns (out,
+    h): h goes on as the residual stream.  ``backward``, of the last forward, reads h
+    again (not to be changed in place before it), takes the gradients of out and of h
+    (may be None) and returns that of x, which is also the residual's; it leaves
+    gamma's in its ``grad``."""
+
+    def __init__(self, num_features: int, eps: float = 1e-6, dtype: int = NeuralDtype.FLOAT32):
+        super().__init__()
+        if num_features < 1:
+            raise ValueError(f"num_features must be >= 1, got {num_features}")
+        self.num_features = num_features
+        self.eps = eps
+        self.gamma = Tensor.ones([num_features], dtype)
+        self._saved = None
+
+    def parameters(self):
+        return [self.gamma]
+
+    def _inputs(self, x: Tensor, residual):
+        if not x.shape or x.shape[-1] != self.num_features:
+            raise ValueError(f"expected a last dimension of {self.num_features}, got shape {x.shape}")
+        src = x.contiguous()
+        if residual is None:
+            return src, None, None
+        return src, residual.contiguous(), Tensor.create(x.shape, x.dtype)
+
+    def forward(self, x: Tensor, residual: Tensor = None):
+        src, res, hidden = self._inputs(x, residual)
+        out = Tensor.create(x.shape, x.dtype)
+        rstd = Tensor.create([x.numel // self.num_features], x.dtype)
+        rc = _lib.neural_rms_norm_forward(out._ptr, _ptr(hidden), src._ptr, _ptr(res), self.gamma._ptr, self.eps,
+                                          rstd._ptr)
+        _check_error(rc, "rms norm forward")
+        self._saved = (src if hidden is None else hidden, rstd)
+        return out if hidden is None else (out, hidden)
+
+    def backward(self, grad_output: Tensor, grad_hidden: Tensor = None) -> Tensor:
+        if self._saved is None:
+            raise RuntimeError("RMSNorm.backward called before forward")
+        hidden, rstd = self._saved
+        go = grad_output.contiguous()
+        gh = grad_hidden.contiguous() if grad_hidden is not None else None
+        gi, dgamma = Tensor.create(hidden.shape, hidden.dtype), Tensor.create([self.num_features], self.gamma.dtype)
+        rc = _lib.neural_rms_norm_backward(gi._ptr, dgamma._ptr, go._ptr, _ptr(gh), hidden._ptr, self.gamma._ptr,
+                                           rstd._ptr)
+        _check_error(rc, "rms norm backward")
+        self.gamma.grad = dgamma
+        return gi
+
+    def forward_q8(self, x: Tensor, residual: Tensor = None):
+        """The output in 8 bits, as QuantizedRows (neural_rms_norm_forward_q8), for
+        inference: no backward follows.  With a residual, (rows, h)."""
+        src, res, hidden = self._inputs(x, residual)
+        q = QuantizedRows._empty(x.shape, x.dtype)
+        rc = _lib.neural_rms_norm_forward_q8(q.device_ptr, q.stride, q.scale._ptr, _ptr(hidden), src._ptr, _ptr(res),
+                                             self.gamma._ptr, self.eps)
+        _check_error(rc, "rms norm forward (8 bits)")
+        return q if hidden is None else (q, hidden)
+
+    def __repr__(self) -> str:
+        return f"RMSNorm({self.num_features}, eps={self.eps})"
+
+
+class QuantizedLinear(Module):
+    """act(x W^T + bias) + residual on 8-bit rows (neural_linear_q8): ``weight`` is a
+    Tensor [out_features, in_features], quantized here by output channel, or such
+    QuantizedRows.  ``x``: QuantizedRows, or a Tensor, which is quantized by row."""
+
+    def __init__(self, weight, bias: Tensor = None, activation: str = "none", alpha: float = None):
+        super().__init__()
+        self.weight = weight if isinstance(weight, QuantizedRows) else QuantizedRows(weight)
+        if len(self.weight.shape) != 2:
+            raise ValueError(f"expected a weight of two dimensions, got shape {self.weight.shape}")
+        self.out_features, self.in_features = self.weight.shape
+        self.bias = bias
+        self.activation = activation
+        self._act = ACTIVATIONS[activation]
+        self.alpha = _act_alpha(activation, alpha)
+
+    def forward(self, x, residual: Tensor = None) -> Tensor:
+        q = x if isinstance(x, QuantizedRows) else QuantizedRows(x)
+        if q.cols != self.in_features:
+            raise ValueError(f"expected a last dimension of {self.in_features}, got shape {q.shape}")
+        out = Tensor.create((*q.shape[:-1], self.out_features), q.dtype)
+        res = residual.contiguous() if residual is not None else None
+        w = self.weight
+        rc = _lib.neural_linear_q8(out._ptr, q.device_ptr, q.stride, q.scale._ptr, w.device_ptr, w.stride, w.scale._ptr,
+                                   q.cols, _ptr(self.bias), self._act, self.alpha, _ptr(res))
+        _check_error(rc, "quantized linear")
+        return out
+
+    def __repr__(self) -> str:
+        return f"QuantizedLinear({self.in_features}, {self.out_features}, activation={self.activation})"
+
+
+TokenLogProbsOut = collections.namedtuple("TokenLogProbsOut", "logprob entropy top_ids top_logprobs")
+
+
+class TokenLogProbs(Module):
+    """Log probabilities of one given token per row of logits, the rows' entropy and
+    ``top_k`` likeliest tokens (neural_token_logprobs_forward; its handling of masked
+    logits and of rows that are not used, by a negative token, is this module's).
+    ``tokens``: int64, a numpy array, a torch tensor or an address of host or device
+    memory; without them logprob is None.  ``forward`` returns (logprob, entropy,
+    top_ids, top_logprobs): Tensors of one value per row, an int64 numpy array
+    [rows, top_k] and a Tensor [rows, top_k] (both None where top_k is 0).
+    ``backward``, of the last forward, takes the gradients of logprob and entropy
+    (either may be None), reads logits and tokens again and returns the logits'."""
+
+    def __init__(self, temperature: float = 1.0, top_k: int = 0):
+        super().__init__()
+        if not 0.0 < temperature < float("inf"):
+            raise ValueError(f"temperature must be positive and finite, got {temperature}")
+        if not 0 <= top_k <= 64:
+            raise ValueError(f"top_k must be in [0, 64], got {top_k}")
+        self.temperature = temperature
+        self.top_k = top_k
+        self._saved = None
+
+    def forward(self, logits: Tensor, tokens=None) -> TokenLogProbsOut:
+        src = logits.contiguous()
+        if not src.shape or src.shape[-1] < 1:
+            raise ValueError(f"expected a last dimension of at least 1, got shape {src.shape}")
+        rows = src.numel // src.shape[-1]
+        held, at = _int64_rows(tokens, rows)
+        entropy, lse = Tensor.create([rows], src.dtype), Tensor.create([rows], src.dtype)
+        logprob = Tensor.create([rows], src.dtype) if at is not None else None
+        ids = np.empty((rows, self.top_k), dtype=np.int64) if self.top_k else None
+        top = Tensor.create([rows, self.top_k], src.dtype) if self.top_k else None
+        rc = _lib.neural_token_logprobs_forward(_ptr(logprob), entropy._ptr, lse._ptr,
+                                                ids.ctypes.data if self.top_k else None, _ptr(top), self.top_k,
+                                                src._ptr, at, self.temperature)
+        _check_error(rc, "token log probabilities forward")
+        self._saved = (src, held, at, lse, entropy)
+        return TokenLogProbsOut(logprob, entropy, ids, top)
+
+    def backward(self, grad_logprob: Tensor = None, grad_entropy: Tensor = None) -> Tensor:
+        if self._saved is None:
+            raise RuntimeError("TokenLogProbs.backward called before forward")
+        src, _, at, lse, entropy = self._saved
+        g = grad_logprob.contiguous() if grad_logprob is not None else None
+        e = grad_entropy.contiguous() if grad_entropy is not None else None
+        out = Tensor.create(src.shape, src.dtype)
+        rc = _lib.neural_token_logprobs_backward(out._ptr, _ptr(g), _ptr(e), src._ptr, at, lse._ptr, entropy._ptr,
+                                                 self.temperature)
+        _check_error(rc, "token log probabilities backward")
+        return out
+
+    def __repr__(self) -> str:
+        return f"TokenLogProbs(temperature={self.temperature}, top_k={self.top_k})"
+
+
+def _ptr(t):
+    return t._ptr if t is not None else None
+
+
+def _int64_rows(v, rows: int):
+    """(what keeps them alive, address) of `rows` int64 values."""
+    if v is None or isinstance(v, int):
+        return None, v
+    if isinstance(v, np.ndarray) or not hasattr(v, "data_ptr"):
+        v = np.ascontiguousarray(v)
+        if v.dtype.kind not in "iu":
+            raise ValueError(f"expected whole numbers, got {v.dtype}")
+        v = v.astype(np.int64, copy=False)
+        n, at = v.size, v.ctypes.data
+    else:
+        v = v.contiguous()
+        if str(v.dtype) != "torch.int64":
+            raise ValueError(f"expected int64, got {v.dtype}")
+        n, at = v.numel(), v.data_ptr()
+    if n != rows:
+        raise ValueError(f"expected {rows} tokens, got {n}")
+    return v, at
+
+
 def add_relu(a: Tensor, b: Tensor) -> Tensor:
     """max(0, a + b) in one pass (b broadcasts, e.g. a [.., C] bias)."""
     out = Tensor.create(a.shape, a.dtype)
@@ -449,13 +632,15 @@ ACTIVATIONS = {"none": 0, "relu": 1, "sigmoid": 2, "tanh": 3, "gelu": 4, "leaky_
                "swish": 8, "mish": 9, "hardswish": 10, "softplus": 11, "hardtanh": 12}
 
 
+def _act_alpha(activation: str, alpha):
+    return alpha if alpha is not None else 0.01 if activation == "leaky_relu" else 1.0
+
+
 def bias_add_act(x: Tensor, bias: Tensor, activation: str = "relu", alpha: float = None) -> Tensor:
     """act(x + bias) for x [.., C] and bias [C] in one pass; equal bit for bit
     to the bias add followed by the activation.  alpha defaults to 0.01 for
     leaky_relu and 1.0 for elu (the reference's defaults)."""
-    code = ACTIVATIONS[activation]
-    if alpha is None:
-        alpha = 0.01 if activation == "leaky_relu" else 1.0
+    code, alpha = ACTIVATIONS[activation], _act_alpha(activation, alpha)
     out = Tensor.create(x.shape, x.dtype)
     _check_error(_lib.neural_bias_add_act(out._ptr, x._ptr, bias._ptr, code, ctypes.c_double(alpha)),
                  "bias_add_act")

@@ -8,13 +8,19 @@ or an integer address) and may point to host or device memory: the library
 stages host buffers through HBM.  ``Quantizer(float32=True)`` switches to the
 library's float32 entry points (``*_f32``), which read float32 data and
 produce exactly what the double entry points produce for the same values.
+
+Without a counterpart in the reference: QuantizedRows, the rows of a tensor in 8
+bits with a scale each, in device memory (nn.QuantizedLinear multiplies them).
 """
 
 import ctypes
 from dataclasses import dataclass
 
+import numpy as np
+
 from . import core
-from .core import QuantParamsC, NeuralException, NeuralError
+from .core import QuantParamsC, NeuralDtype, NeuralException, NeuralError, _check_error
+from .tensor import Tensor
 
 
 @dataclass
@@ -135,3 +141,50 @@ def quantized_matmul(a_int8, b_int8, m: int, k: int, n: int, params_a: QuantPara
     if rc != 0:
         raise RuntimeError(f"quantized_matmul of [{m}x{k}] by [{k}x{n}] failed")
     return out
+
+
+class QuantizedRows:
+    """The rows of a tensor (over its last dimension) as int8 codes and one scale
+    per row, in device memory: a code stands for code * scale (neural_quantize_rows).
+    ``QuantizedRows(t)`` quantizes ``t``; nn.RMSNorm.forward_q8 makes one from the
+    norm's output.  Row r's codes begin at ``device_ptr + r * stride``."""
+
+    def __init__(self, t: Tensor):
+        src = t.contiguous()
+        self._allocate(t.shape, t.dtype)
+        rc = core._lib.neural_quantize_rows(self.device_ptr, self.stride, self.scale._ptr, src._ptr)
+        _check_error(rc, "quantize rows")
+
+    @classmethod
+    def _empty(cls, shape, dtype) -> "QuantizedRows":
+        q = cls.__new__(cls)
+        q._allocate(shape, dtype)
+        return q
+
+    def _allocate(self, shape, dtype):
+        if not shape:
+            raise ValueError("QuantizedRows needs at least one dimension")
+        self.shape, self.dtype = tuple(shape), dtype
+        self.cols = self.shape[-1]
+        self.rows = int(np.prod(self.shape[:-1], dtype=np.int64)) if self.cols else 0
+        self.stride = -(-self.cols // 64) * 64  # the product reads such rows in place
+        # bytes, held in a float32 tensor
+        self._codes = Tensor.create([max(self.rows * self.stride // 4, 16)], NeuralDtype.FLOAT32)
+        self.scale = Tensor.create([self.rows], dtype)
+
+    @property
+    def device_ptr(self) -> int:
+        return self._codes.device_ptr
+
+    def codes(self) -> "np.ndarray":
+        """The codes, int8, in the tensor's shape."""
+        raw = self._codes.numpy().view(np.int8)[: self.rows * self.stride].reshape(self.rows, self.stride)
+        return raw[:, : self.cols].reshape(self.shape).copy()
+
+    def numpy(self) -> "np.ndarray":
+        """The values the codes stand for, in the tensor's dtype."""
+        scale = self.scale.numpy()
+        return (self.codes().reshape(self.rows, self.cols) * scale[:, None]).reshape(self.shape)
+
+    def __repr__(self):
+        return f"QuantizedRows(shape={self.shape})"
