@@ -446,7 +446,8 @@ int neural_dropout_add_layer_norm_backward(NeuralTensor *grad_in, NeuralTensor *
  * whole number, halves away from zero (decided exactly), and scale = a / 127 in the dtype: a
  * code stands for code * scale.  A row of zeros has codes and scale 0; a row that holds NaN or
  * an infinity has codes 0 and scale NaN.  Row r's codes begin at codes + r * stride (stride >=
- * C, in bytes; host or device memory); bytes between the rows are left as they are.
+ * C, in bytes) of rows * stride bytes of host or device memory; bytes between the rows are left
+ * as they are.
  *   neural_quantize_rows: w = in.
  *   neural_rms_norm_forward_q8: w = h gamma and scale = a rstd / 127, the codes of the norm's
  *   output (before its rounding to the dtype); otherwise as neural_rms_norm_forward.

@@ -5,6 +5,7 @@
 // elementwise activations do, and the residual is added to its result: two more roundings in
 // f32, each half a unit of values that the f32 elementwise calls would leave as well.
 #include <cmath>
+#include <type_traits>
 
 #include "act_fns.hpp"
 #include "row_call.hpp"
@@ -22,41 +23,32 @@ struct LinArgs {
     double alpha;
 };
 
-// The activation of one value, by neural_bias_add_act's functors.
-NH_DEV float act_of(float z, int act, double alpha)
+// The activation of four values, by neural_bias_add_act's functors: the branch is taken once.
+template <typename T>
+NH_DEV void act4(T (&z)[4], int act, double alpha)
 {
+    const auto each = [&](auto f) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) z[e] = f(z[e]);
+    };
+    constexpr bool F32 = sizeof(T) == 4;
     switch (act) {
-    case NEURAL_ACT_RELU: return FnReluAct{}(z);
-    case NEURAL_ACT_SIGMOID: return ActFn<ASigmoid>{}(z);
-    case NEURAL_ACT_TANH: return TanhF32Fn{}(z);
-    case NEURAL_ACT_GELU: return HeadTailFn<GeluF32>{}(z);
-    case NEURAL_ACT_LEAKY_RELU: return ActFn<ALeaky>{ALeaky{alpha}}(z);
-    case NEURAL_ACT_ELU: return HeadTailFn<EluF32>{EluF32{alpha}}(z);
-    case NEURAL_ACT_SELU: return HeadTailFn<SeluF32>{}(z);
-    case NEURAL_ACT_SWISH: return HeadTailFn<SwishF32>{}(z);
-    case NEURAL_ACT_MISH: return HeadTailFn<MishF32>{}(z);
-    case NEURAL_ACT_HARDSWISH: return HardswishF32Fn{}(z);
-    case NEURAL_ACT_SOFTPLUS: return HeadTailFn<SoftplusF32>{}(z);
-    case NEURAL_ACT_HARDTANH: return ActFn<AHardtanh>{}(z);
-    default: return z;
-    }
-}
-NH_DEV double act_of(double z, int act, double alpha)
-{
-    switch (act) {
-    case NEURAL_ACT_RELU: return FnReluAct{}(z);
-    case NEURAL_ACT_SIGMOID: return ActFn<ASigmoid>{}(z);
-    case NEURAL_ACT_TANH: return ActFn<ATanh>{}(z);
-    case NEURAL_ACT_GELU: return ActFn<AGelu>{}(z);
-    case NEURAL_ACT_LEAKY_RELU: return ActFn<ALeaky>{ALeaky{alpha}}(z);
-    case NEURAL_ACT_ELU: return ActFn<AElu>{AElu{alpha}}(z);
-    case NEURAL_ACT_SELU: return ActFn<ASelu>{}(z);
-    case NEURAL_ACT_SWISH: return ActFn<ASwish>{}(z);
-    case NEURAL_ACT_MISH: return ActFn<AMish>{}(z);
-    case NEURAL_ACT_HARDSWISH: return ActFn<AHardswish>{}(z);
-    case NEURAL_ACT_SOFTPLUS: return ActFn<ASoftplus>{}(z);
-    case NEURAL_ACT_HARDTANH: return ActFn<AHardtanh>{}(z);
-    default: return z;
+    case NEURAL_ACT_NONE: break;
+    case NEURAL_ACT_RELU: each(FnReluAct{}); break;
+    case NEURAL_ACT_SIGMOID: each(ActFn<ASigmoid>{}); break;
+    case NEURAL_ACT_TANH: each(std::conditional_t<F32, TanhF32Fn, ActFn<ATanh>>{}); break;
+    case NEURAL_ACT_GELU: each(std::conditional_t<F32, HeadTailFn<GeluF32>, ActFn<AGelu>>{}); break;
+    case NEURAL_ACT_LEAKY_RELU: each(ActFn<ALeaky>{ALeaky{alpha}}); break;
+    case NEURAL_ACT_ELU:
+        if constexpr (F32) each(HeadTailFn<EluF32>{EluF32{alpha}});
+        else each(ActFn<AElu>{AElu{alpha}});
+        break;
+    case NEURAL_ACT_SELU: each(std::conditional_t<F32, HeadTailFn<SeluF32>, ActFn<ASelu>>{}); break;
+    case NEURAL_ACT_SWISH: each(std::conditional_t<F32, HeadTailFn<SwishF32>, ActFn<ASwish>>{}); break;
+    case NEURAL_ACT_MISH: each(std::conditional_t<F32, HeadTailFn<MishF32>, ActFn<AMish>>{}); break;
+    case NEURAL_ACT_HARDSWISH: each(std::conditional_t<F32, HardswishF32Fn, ActFn<AHardswish>>{}); break;
+    case NEURAL_ACT_SOFTPLUS: each(std::conditional_t<F32, HeadTailFn<SoftplusF32>, ActFn<ASoftplus>>{}); break;
+    default: each(ActFn<AHardtanh>{}); break;
     }
 }
 
@@ -67,56 +59,277 @@ NH_DEV T lin_value(int acc, T sa, T sw, T bias)
     return T(double(acc) * (double(sa) * double(sw)) + double(bias));
 }
 
-// 64 x 64 results a block, 4 x 4 a lane, from tiles of 64 codes in LDS, byte by byte.
-template <typename T>
-__global__ __launch_bounds__(256) void k_lin_tile(LinArgs<T> g, int64_t nbx, int64_t b_base)
+typedef int i32x16 __attribute__((ext_vector_type(16)));
+
+// ---- operands --------------------------------------------------------------------------------
+
+constexpr int64_t kLinMaxLd = int64_t(1) << 22;  // 256 rows of it stay in a 32-bit offset
+
+// Rows of codes copied to rows of `ldd` bytes (a multiple of 16) at an aligned address, the bytes
+// past k zero.  A lane takes 16 bytes.
+__global__ __launch_bounds__(256) void k_lin_pad(const int8_t *__restrict__ src, int64_t ld, int8_t *__restrict__ dst,
+                                                 int64_t ldd, int64_t rows, int64_t k)
 {
-    __shared__ int sa[64][17], sw[64][17];
-    const int tid = threadIdx.x;
-    const int64_t b = b_base + blockIdx.x, m0 = b / nbx * 64, n0 = b % nbx * 64;
-    const int ty = tid / 16, tx = tid % 16;
-    int acc[4][4] = {};
-    for (int64_t k0 = 0; k0 < g.k; k0 += 64) {
+    const int64_t units = ldd / 16, step = int64_t(gridDim.x) * 256;
+    for (int64_t t = int64_t(blockIdx.x) * 256 + threadIdx.x; t < rows * units; t += step) {
+        const int64_t r = t / units, u = t - r * units;
+        const int8_t *p = src + r * ld + 16 * u;
+        i32x4 v;
+        if (16 * u + 16 <= k) {
+            typedef int W __attribute__((ext_vector_type(4), aligned(1)));
+            v = *reinterpret_cast<const W *>(p);
+        } else {
+            int8_t b[16];
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int r = ty + 16 * i;
-            const int64_t k = k0 + 4 * tx;
-            uint32_t va = 0, vw = 0;
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                if (m0 + r < g.m && k + e < g.k) va |= uint32_t(uint8_t(g.a[(m0 + r) * g.lda + k + e])) << (8 * e);
-                if (n0 + r < g.n && k + e < g.k) vw |= uint32_t(uint8_t(g.w[(n0 + r) * g.ldw + k + e])) << (8 * e);
-            }
-            sa[r][tx] = int(va);
-            sw[r][tx] = int(vw);
+            for (int q = 0; q < 16; q++) b[q] = 16 * u + q < k ? p[q] : int8_t(0);
+            __builtin_memcpy(&v, b, 16);
         }
-        __syncthreads();
-#pragma unroll 4
-        for (int q = 0; q < 16; q++)
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-#pragma unroll
-                for (int j = 0; j < 4; j++)
-                    acc[i][j] = __builtin_amdgcn_sdot4(sa[ty + 16 * i][q], sw[tx + 16 * j][q], acc[i][j], false);
-        __syncthreads();
+        *reinterpret_cast<i32x4 *>(dst + r * ldd + 16 * u) = v;
     }
-    for (int i = 0; i < 4; i++)
-        for (int j = 0; j < 4; j++) {
-            const int64_t m = m0 + ty + 16 * i, n = n0 + tx + 16 * j;
-            if (m >= g.m || n >= g.n) continue;
-            T z = act_of(lin_value<T>(acc[i][j], g.sa[m], g.sw[n], g.bias ? g.bias[n] : T(0)), g.act, g.alpha);
-            if (g.res) z = z + g.res[m * g.n + n];
-            g.out[m * g.n + n] = z;
+}
+
+// What lanes fetch in the place of units past the rows' end.
+__device__ const int g_lin_zero[4] = {0, 0, 0, 0};
+
+// 16 bytes per lane from memory straight into LDS: lane l's to `lds` + 16 l (lds: the same for the
+// wave, in bytes).  Two forms of the address: a uniform base and 32 bits per lane, or 64 bits.
+// The counter that the compiler keeps of loads in flight does not know these; the waits are
+// written out where their data is read.
+NH_DEV void lds_load(uint32_t lds, uint32_t at, const int8_t *base)
+{
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(lds), "v"(at), "s"(base) : "memory");
+}
+NH_DEV void lds_load(uint32_t lds, const void *p)
+{
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(lds), "v"(p) : "memory");
+}
+// At most `N` of this wave's loads still in flight and its LDS reads done; then the block's.
+template <int N>
+NH_DEV void wait_and_meet()
+{
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(N) : "memory");
+}
+
+// ---- the product by matrix instructions -------------------------------------------------------
+
+// WM x WN waves, each TM x TN tiles of 32 x 32 results; slices of 64 codes of the block's rows of
+// A and W pass through ST buffers in LDS.
+template <int WM_, int WN_, int TM_, int TN_, int ST_, int PER_SIMD_>
+struct LinShape {
+    static constexpr int WM = WM_, WN = WN_, TM = TM_, TN = TN_, ST = ST_, PER_SIMD = PER_SIMD_;
+    static constexpr int NW = WM * WN, NT = 64 * NW, BM = 32 * WM * TM, BN = 32 * WN * TN;
+    static constexpr int kStage = (BM + BN) * 64, kLoads = (BM + BN) / 16 / NW;  // bytes; 1 KB loads per wave
+    static constexpr int kRow = 32 * TN + 4;                                     // the epilogue's rows of a wave
+    static_assert((BM + BN) / 16 % NW == 0, "whole loads per wave");
+    static_assert(NW * 32 * kRow * 4 + 4 * BM <= ST * kStage, "the epilogue's rows fit the buffers");
+};
+
+// Tile of block `h` of nbm x nbn: the hardware deals blocks to the 8 XCDs in turn, each with its own
+// L2, so each XCD gets consecutive numbers, and those go through groups of G rows of tiles,
+// column by column, so that the blocks of an XCD share few panels of A and W.
+NH_DEV void lin_tile(int64_t h, int64_t nbm, int64_t nbn, int64_t &bm, int64_t &bn)
+{
+    constexpr int64_t G = 8;
+    const int64_t nb = nbm * nbn, x = h & 7, q = nb >> 3, rest = nb & 7;
+    const int64_t L = x * q + (x < rest ? x : rest) + (h >> 3);
+    const int64_t gsz = G * nbn, g = L / gsz, r = L - g * gsz, first = g * G;
+    const int64_t rows = nbm - first < G ? nbm - first : G;
+    bm = first + r % rows;
+    bn = r / rows;
+}
+
+// (A's rows are the second operand: a lane's results are of one row of A and, four at a time,
+// consecutive columns.)
+template <typename T, typename S>
+__global__ __launch_bounds__(S::NT, S::PER_SIMD) void k_lin_mfma(LinArgs<T> g, int64_t nbm, int64_t nbn, int64_t b_base,
+                                                                  int64_t nb_all)
+{
+    constexpr int TM = S::TM, TN = S::TN, ST = S::ST, BM = S::BM, BN = S::BN;
+    __shared__ __attribute__((aligned(1024))) int8_t smem[ST * S::kStage];
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    int64_t bm, bn;
+    lin_tile(b_base + blockIdx.x, nbm, nbn, bm, bn);
+    const int64_t m0 = bm * BM, n0 = bn * BN;
+    const int wr = 32 * TM * (w / S::WN), wc = 32 * TN * (w % S::WN);
+    // LDS rows of 64 bytes, four units of 16; unit u of row r lies at u ^ (r / 2 % 4), so that eight
+    // lanes of a 16-byte read cover the banks once.  A load puts lane l's unit at place l % 4 of row
+    // l / 4 of 16: it fetches unit (l % 4) ^ (row / 2 % 4).
+    const uint32_t lds0 = uint32_t(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) int8_t *)smem));
+    const int lrow = lane >> 2, lunit = (lane & 3) ^ (lane >> 3 & 3);
+    uint32_t at[S::kLoads];
+#pragma unroll
+    for (int q = 0; q < S::kLoads; q++) {
+        const int b = w + q * S::NW, r = 16 * b + lrow;
+        if (16 * b < BM) {
+            const int64_t last = g.m - 1 - m0;
+            at[q] = uint32_t((r < last ? r : last) * g.lda + 16 * lunit);
+        } else {
+            const int64_t last = g.n - 1 - n0, rw = r - BM;
+            at[q] = uint32_t((rw < last ? rw : last) * g.ldw + 16 * lunit);
         }
+    }
+    const int8_t *pa = g.a + m0 * g.lda, *pw = g.w + n0 * g.ldw;
+    const int steps = int((g.k + 63) / 64), whole = int(g.k / 64), units = int((g.k + 15) / 16);
+    const auto issue = [&](int s, int buf) {
+        s = s < steps ? s : steps - 1;  // (past the end: again, so that the count of loads stays)
+        const uint32_t lds = lds0 + buf * S::kStage;
+        if (s < whole) {
+#pragma unroll
+            for (int q = 0; q < S::kLoads; q++) {
+                const int b = w + q * S::NW;
+                lds_load(lds + 1024 * b, at[q], (16 * b < BM ? pa : pw) + int64_t(s) * 64);
+            }
+        } else {
+#pragma unroll
+            for (int q = 0; q < S::kLoads; q++) {
+                const int b = w + q * S::NW;
+                const int8_t *p = (16 * b < BM ? pa : pw) + int64_t(s) * 64 + at[q];
+                lds_load(lds + 1024 * b, 4 * s + lunit < units ? static_cast<const void *>(p) : g_lin_zero);
+            }
+        }
+    };
+    const int frow = lane & 31, fsw = frow >> 1 & 3, hi = lane >> 5;
+    const auto frag = [&](int buf, int row, int c) {
+        return *reinterpret_cast<const i32x4 *>(smem + buf * S::kStage + (row + frow) * 64 + (((2 * c + hi) ^ fsw) * 16));
+    };
+    i32x16 acc[TM][TN];
+#pragma unroll
+    for (int i = 0; i < TM; i++)
+#pragma unroll
+        for (int j = 0; j < TN; j++) acc[i][j] = i32x16{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+    i32x4 fa[2][TM], fw[2][TN];
+    const auto read = [&](int buf, int c) {
+#pragma unroll
+        for (int i = 0; i < TM; i++) fa[c][i] = frag(buf, wr + 32 * i, c);
+#pragma unroll
+        for (int j = 0; j < TN; j++) fw[c][j] = frag(buf, BM + wc + 32 * j, c);
+    };
+    const auto multiply = [&](int c) {
+#pragma unroll
+        for (int i = 0; i < TM; i++)
+#pragma unroll
+            for (int j = 0; j < TN; j++)
+                acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fw[c][j], fa[c][i], acc[i][j], 0, 0, 0);
+    };
+#pragma unroll
+    for (int s = 0; s < ST - 1; s++) issue(s, s);
+    wait_and_meet<S::kLoads *(ST - 2)>();
+    read(0, 0);
+    int cur = 0;
+    for (int s = 0; s < steps; s++) {
+        // Slice s: its first half is in registers.  The buffer that the new loads go to was read
+        // in step s - 1, and every wave's reads of it were done at that step's meeting.
+        read(cur, 1);
+        issue(s + ST - 1, cur == 0 ? ST - 1 : cur - 1);
+        __builtin_amdgcn_sched_barrier(0);
+        multiply(0);
+        __builtin_amdgcn_sched_barrier(0);
+        wait_and_meet<S::kLoads *(ST - 2)>();  // slice s + 1 is there
+        cur = cur + 1 == ST ? 0 : cur + 1;
+        read(cur, 0);
+        __builtin_amdgcn_sched_barrier(0);
+        multiply(1);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    wait_and_meet<0>();
+
+    // The epilogue: a wave's results go through its own part of LDS, 32 rows at a time, so that a
+    // lane has four columns side by side of every fourth (TN = 2) row.  Result v of lane l is
+    // column 8 (v / 4) + 4 (l / 32) + v % 4, row l % 32 of its tile.
+    using V = typename Vec16<T>::type;
+    using U = typename VecU<T>::type;
+    int *rows = reinterpret_cast<int *>(smem) + w * 32 * S::kRow;
+    constexpr int CL = 8 * TN, RPI = 64 / CL;  // lanes per row, rows at once
+    const int cl = lane % CL, rl = lane / CL;
+    const int64_t n = n0 + wc + 4 * cl;
+    T sw[4], bias[4];
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        sw[e] = n + e < g.n ? g.sw[n + e] : T(0);
+        bias[e] = g.bias && n + e < g.n ? g.bias[n + e] : T(0);
+    }
+    const bool full = n + 4 <= g.n;
+#pragma unroll 1
+    for (int i = 0; i < TM; i++) {
+        const auto dump = [&](const i32x16 (&t)[TN]) {
+#pragma unroll
+            for (int j = 0; j < TN; j++)
+#pragma unroll
+                for (int v = 0; v < 16; v += 4)
+                    *reinterpret_cast<i32x4 *>(rows + frow * S::kRow + 32 * j + 2 * v + 4 * hi) =
+                        i32x4{t[j][v], t[j][v + 1], t[j][v + 2], t[j][v + 3]};
+        };
+        if (i == 0) dump(acc[0]);
+        if constexpr (TM > 1) if (i == 1) dump(acc[1]);
+        if constexpr (TM > 2) if (i == 2) dump(acc[2]);
+        if constexpr (TM > 3) if (i == 3) dump(acc[3]);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+        for (int r = rl; r < 32; r += RPI) {
+            const i32x4 c = *reinterpret_cast<const i32x4 *>(rows + r * S::kRow + 4 * cl);
+            const int64_t m = m0 + wr + 32 * i + r;
+            if (m >= g.m || n >= g.n) continue;
+            const T sa = g.sa[m];
+            T z[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) z[e] = lin_value<T>(c[e], sa, sw[e], bias[e]);
+            act4(z, g.act, g.alpha);
+            const int64_t o = m * g.n + n;
+            if (full) {
+                V y[4 / Vec16<T>::n];
+#pragma unroll
+                for (int e = 0; e < 4; e++) y[e / Vec16<T>::n][e % Vec16<T>::n] = z[e];
+#pragma unroll
+                for (int q = 0; q < 4 / Vec16<T>::n; q++) {
+                    if (g.res) y[q] = y[q] + *(reinterpret_cast<const U *>(g.res + o) + q);
+                    *(reinterpret_cast<U *>(g.out + o) + q) = y[q];
+                }
+            } else {
+                for (int e = 0; e < 4; e++)
+                    if (n + e < g.n) g.out[o + e] = g.res ? z[e] + g.res[o + e] : z[e];
+            }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
+template <typename T, typename S>
+static void launch_lin_mfma(const LinArgs<T> &g)
+{
+    const int64_t nbm = ceil_div(g.m, S::BM), nbn = ceil_div(g.n, S::BN);
+    for_row_launches(nbm * nbn, 1, S::NT, [&](unsigned blocks, int64_t base) {
+        NH_LAUNCH((k_lin_mfma<T, S>), dim3(blocks), dim3(S::NT), 0, stream(), g, nbm, nbn, base, nbm * nbn);
+    });
+}
+
+// A's or W's rows for the matrix instructions: in place, or copied to `pad` (lin_pad_bytes).
+static size_t lin_pad_bytes(const int8_t *p, int64_t ld, int64_t rows, int64_t k, bool whole_units)
+{
+    const bool fits = ((reinterpret_cast<uintptr_t>(p) | uintptr_t(ld)) & 15) == 0 && ld < kLinMaxLd;
+    return fits && (!whole_units || (k & 15) == 0) ? 0 : size_t(rows) * size_t((k + 63) / 64 * 64);
+}
+static void lin_pad(const int8_t *&p, int64_t &ld, int64_t rows, int64_t k, int8_t *pad)
+{
+    const int64_t ldd = (k + 63) / 64 * 64, need = ceil_div(rows * (ldd / 16), 256);
+    NH_LAUNCH(k_lin_pad, dim3(unsigned(need < kMaxGridBlocks ? need : kMaxGridBlocks)), dim3(256), 0, stream(), p, ld, pad,
+              ldd, rows, k);
+    p = pad;
+    ld = ldd;
 }
 
 template <typename T>
-static int launch_linear(const LinArgs<T> &g)
+static int launch_linear(LinArgs<T> g)
 {
-    const int64_t nbx = ceil_div(g.n, 64);
-    for_row_launches(nbx * ceil_div(g.m, 64), 1, 256, [&](unsigned blocks, int64_t base) {
-        NH_LAUNCH((k_lin_tile<T>), dim3(blocks), dim3(256), 0, stream(), g, nbx, base);
-    });
+    // (where k ends inside a unit of 16, A's bytes past it must be zeros; W's then do not matter)
+    const size_t ba = lin_pad_bytes(g.a, g.lda, g.m, g.k, true), bw = lin_pad_bytes(g.w, g.ldw, g.n, g.k, false);
+    Partials pad;  // (one block: a captured call's blocks share memory)
+    if (ba + bw) NH_TRY(pad.open(ba + bw));
+    if (ba) lin_pad(g.a, g.lda, g.m, g.k, static_cast<int8_t *>(pad.p));
+    if (bw) lin_pad(g.w, g.ldw, g.n, g.k, static_cast<int8_t *>(pad.p) + ba);
+    if (g.m <= 128) launch_lin_mfma<T, LinShape<2, 2, 1, 2, 4, 2>>(g);
+    else launch_lin_mfma<T, LinShape<2, 2, 4, 2, 3, 2>>(g);
     return check_launch();
 }
 
@@ -172,8 +385,7 @@ static int linear_q8(const LinTensors &t)
     if (numel(t.out) == 0) return set_error(NEURAL_OK);
     if (t.stride > int64_t(kMaxRawCount / uint64_t(c.rows)) || t.w_stride > int64_t(kMaxRawCount / uint64_t(c.cols)))
         return set_error(NEURAL_ERR_TENSOR_TOO_LARGE);
-    const size_t a_bytes = size_t(c.rows - 1) * size_t(t.stride) + size_t(t.k);
-    const size_t w_bytes = size_t(c.cols - 1) * size_t(t.w_stride) + size_t(t.k);
+    const size_t a_bytes = size_t(c.rows) * size_t(t.stride), w_bytes = size_t(c.cols) * size_t(t.w_stride);
     if (raw_may_overlap(t.codes, a_bytes, t.out) || raw_may_overlap(t.w_codes, w_bytes, t.out))
         return set_error(NEURAL_ERR_INVALID_ARGUMENT);
     Staged a, w;

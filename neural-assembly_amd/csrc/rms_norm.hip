@@ -129,12 +129,6 @@ struct RmsTensors {
     int64_t stride;
 };
 
-// The bytes from the first code to the last (rows, cols >= 1).
-static size_t code_bytes(int64_t rows, int64_t cols, int64_t stride)
-{
-    return size_t(rows - 1) * size_t(stride) + size_t(cols);
-}
-
 template <typename T>
 static int rms_run(const RmsTensors &t, const RowCall &c, double eps, int out, Staged &codes)
 {
@@ -180,7 +174,7 @@ static int rms_forward(const RmsTensors &t, double eps, int out)
     Staged codes;
     if (out != RMS_VALUES) {
         if (t.stride > int64_t(kMaxRawCount / uint64_t(c.rows))) return set_error(NEURAL_ERR_TENSOR_TOO_LARGE);
-        const size_t bytes = code_bytes(c.rows, c.cols, t.stride);
+        const size_t bytes = size_t(c.rows) * size_t(t.stride);
         for (const NeuralTensor *u : {static_cast<const NeuralTensor *>(t.hidden), static_cast<const NeuralTensor *>(t.scale),
                                       t.in, t.residual, t.gamma})
             if (raw_may_overlap(t.codes, bytes, u)) return set_error(NEURAL_ERR_INVALID_ARGUMENT);
