@@ -112,16 +112,17 @@ NH_DEV void wait_and_meet()
 
 // ---- the product by matrix instructions -------------------------------------------------------
 
-// WM x WN waves, each TM x TN tiles of 32 x 32 results; slices of 64 codes of the block's rows of
-// A and W pass through ST buffers in LDS.
-template <int WM_, int WN_, int TM_, int TN_, int ST_, int PER_SIMD_>
+// WM x WN waves, each TM x TN tiles of 32 x 32 results; slices of 16 KU codes of the block's rows
+// of A and W pass through ST buffers in LDS.
+template <int WM_, int WN_, int TM_, int TN_, int KU_, int ST_, int PER_SIMD_>
 struct LinShape {
-    static constexpr int WM = WM_, WN = WN_, TM = TM_, TN = TN_, ST = ST_, PER_SIMD = PER_SIMD_;
+    static constexpr int WM = WM_, WN = WN_, TM = TM_, TN = TN_, KU = KU_, ST = ST_, PER_SIMD = PER_SIMD_;
     static constexpr int NW = WM * WN, NT = 64 * NW, BM = 32 * WM * TM, BN = 32 * WN * TN;
-    static constexpr int kStage = (BM + BN) * 64, kLoads = (BM + BN) / 16 / NW;  // bytes; 1 KB loads per wave
-    static constexpr int kRow = 32 * TN + 4;                                     // the epilogue's rows of a wave
-    static_assert((BM + BN) / 16 % NW == 0, "whole loads per wave");
-    static_assert(NW * 32 * kRow * 4 + 4 * BM <= ST * kStage, "the epilogue's rows fit the buffers");
+    static constexpr int kSlice = 16 * KU, kStage = (BM + BN) * kSlice;  // bytes of a row, of a buffer
+    static constexpr int kRows = 64 / KU, kLoads = (BM + BN) / kRows / NW;  // rows a load (1 KB), loads per wave
+    static constexpr int kOut = 32 * TN + 4;                             // the epilogue's rows of a wave
+    static_assert(BM % (kRows * NW) == 0 && BN % (kRows * NW) == 0, "whole loads per wave");
+    static constexpr int kLoadsA = BM / kRows / NW;
 };
 
 // Tile of block `h` of nbm x nbn: the hardware deals blocks to the 8 XCDs in turn, each with its own
@@ -141,57 +142,50 @@ NH_DEV void lin_tile(int64_t h, int64_t nbm, int64_t nbn, int64_t &bm, int64_t &
 // (A's rows are the second operand: a lane's results are of one row of A and, four at a time,
 // consecutive columns.)
 template <typename T, typename S>
-__global__ __launch_bounds__(S::NT, S::PER_SIMD) void k_lin_mfma(LinArgs<T> g, int64_t nbm, int64_t nbn, int64_t b_base,
-                                                                  int64_t nb_all)
+__global__ __launch_bounds__(S::NT, S::PER_SIMD) void k_lin_mfma(LinArgs<T> g, int64_t nbm, int64_t nbn, int64_t b_base)
 {
-    constexpr int TM = S::TM, TN = S::TN, ST = S::ST, BM = S::BM, BN = S::BN;
+    constexpr int TM = S::TM, TN = S::TN, ST = S::ST, KU = S::KU, BM = S::BM, BN = S::BN, C = KU / 2;
+    static_assert(S::NW * 32 * S::kOut * int(sizeof(T)) <= ST * S::kStage, "the epilogue's rows fit the buffers");
     __shared__ __attribute__((aligned(1024))) int8_t smem[ST * S::kStage];
+    __shared__ T par_a[BM], par_w[BN], par_b[BN];
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     int64_t bm, bn;
     lin_tile(b_base + blockIdx.x, nbm, nbn, bm, bn);
     const int64_t m0 = bm * BM, n0 = bn * BN;
     const int wr = 32 * TM * (w / S::WN), wc = 32 * TN * (w % S::WN);
-    // LDS rows of 64 bytes, four units of 16; unit u of row r lies at u ^ (r / 2 % 4), so that eight
-    // lanes of a 16-byte read cover the banks once.  A load puts lane l's unit at place l % 4 of row
-    // l / 4 of 16: it fetches unit (l % 4) ^ (row / 2 % 4).
+    // LDS rows of KU units of 16 bytes; unit u of row r lies at u ^ swz(r), so that the sixteen lanes
+    // of a 16-byte read that go at once cover the 64 banks once.  A load puts lane l's unit at
+    // place l % KU of row l / KU: it fetches the unit that belongs there.
+    const auto swz = [](int r) { return KU == 4 ? r >> 2 & 3 : r >> 1 & 7; };
     const uint32_t lds0 = uint32_t(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) int8_t *)smem));
-    const int lrow = lane >> 2, lunit = (lane & 3) ^ (lane >> 3 & 3);
     uint32_t at[S::kLoads];
+    int unit[S::kLoads];
 #pragma unroll
     for (int q = 0; q < S::kLoads; q++) {
-        const int b = w + q * S::NW, r = 16 * b + lrow;
-        if (16 * b < BM) {
-            const int64_t last = g.m - 1 - m0;
-            at[q] = uint32_t((r < last ? r : last) * g.lda + 16 * lunit);
-        } else {
-            const int64_t last = g.n - 1 - n0, rw = r - BM;
-            at[q] = uint32_t((rw < last ? rw : last) * g.ldw + 16 * lunit);
-        }
+        const bool of_a = q < S::kLoadsA;
+        const int r = (w + (of_a ? q : q - S::kLoadsA) * S::NW) * S::kRows + lane / KU;
+        const int64_t last = of_a ? g.m - 1 - m0 : g.n - 1 - n0;
+        unit[q] = (lane % KU) ^ swz(r);
+        at[q] = uint32_t((r < last ? r : last) * (of_a ? g.lda : g.ldw) + 16 * unit[q]);
     }
     const int8_t *pa = g.a + m0 * g.lda, *pw = g.w + n0 * g.ldw;
-    const int steps = int((g.k + 63) / 64), whole = int(g.k / 64), units = int((g.k + 15) / 16);
+    const int steps = int((g.k + S::kSlice - 1) / S::kSlice), whole = int(g.k / S::kSlice), units = int((g.k + 15) / 16);
     const auto issue = [&](int s, int buf) {
         s = s < steps ? s : steps - 1;  // (past the end: again, so that the count of loads stays)
         const uint32_t lds = lds0 + buf * S::kStage;
+        const int8_t *sa = pa + int64_t(s) * S::kSlice, *sw = pw + int64_t(s) * S::kSlice;
         if (s < whole) {
 #pragma unroll
-            for (int q = 0; q < S::kLoads; q++) {
-                const int b = w + q * S::NW;
-                lds_load(lds + 1024 * b, at[q], (16 * b < BM ? pa : pw) + int64_t(s) * 64);
-            }
+            for (int q = 0; q < S::kLoads; q++) lds_load(lds + 1024 * (w + q * S::NW), at[q], q < S::kLoadsA ? sa : sw);
         } else {
 #pragma unroll
             for (int q = 0; q < S::kLoads; q++) {
-                const int b = w + q * S::NW;
-                const int8_t *p = (16 * b < BM ? pa : pw) + int64_t(s) * 64 + at[q];
-                lds_load(lds + 1024 * b, 4 * s + lunit < units ? static_cast<const void *>(p) : g_lin_zero);
+                const int8_t *p = (q < S::kLoadsA ? sa : sw) + at[q];
+                lds_load(lds + 1024 * (w + q * S::NW), KU * s + unit[q] < units ? static_cast<const void *>(p) : g_lin_zero);
             }
         }
     };
-    const int frow = lane & 31, fsw = frow >> 1 & 3, hi = lane >> 5;
-    const auto frag = [&](int buf, int row, int c) {
-        return *reinterpret_cast<const i32x4 *>(smem + buf * S::kStage + (row + frow) * 64 + (((2 * c + hi) ^ fsw) * 16));
-    };
+    const int frow = lane & 31, fsw = swz(frow), hi = lane >> 5;
     i32x16 acc[TM][TN];
 #pragma unroll
     for (int i = 0; i < TM; i++)
@@ -199,65 +193,97 @@ __global__ __launch_bounds__(S::NT, S::PER_SIMD) void k_lin_mfma(LinArgs<T> g, i
         for (int j = 0; j < TN; j++) acc[i][j] = i32x16{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
     i32x4 fa[2][TM], fw[2][TN];
     const auto read = [&](int buf, int c) {
+        const int8_t *p = smem + buf * S::kStage + frow * S::kSlice + (((2 * c + hi) ^ fsw) * 16);
 #pragma unroll
-        for (int i = 0; i < TM; i++) fa[c][i] = frag(buf, wr + 32 * i, c);
+        for (int i = 0; i < TM; i++) fa[c & 1][i] = *reinterpret_cast<const i32x4 *>(p + (wr + 32 * i) * S::kSlice);
 #pragma unroll
-        for (int j = 0; j < TN; j++) fw[c][j] = frag(buf, BM + wc + 32 * j, c);
+        for (int j = 0; j < TN; j++) fw[c & 1][j] = *reinterpret_cast<const i32x4 *>(p + (BM + wc + 32 * j) * S::kSlice);
     };
     const auto multiply = [&](int c) {
 #pragma unroll
         for (int i = 0; i < TM; i++)
 #pragma unroll
             for (int j = 0; j < TN; j++)
-                acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fw[c][j], fa[c][i], acc[i][j], 0, 0, 0);
+                acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fw[c & 1][j], fa[c & 1][i], acc[i][j], 0, 0, 0);
     };
 #pragma unroll
-    for (int s = 0; s < ST - 1; s++) issue(s, s);
-    wait_and_meet<S::kLoads *(ST - 2)>();
+    for (int s = 0; s < ST; s++) issue(s, s);
+    for (int i = threadIdx.x; i < BM; i += S::NT) par_a[i] = m0 + i < g.m ? g.sa[m0 + i] : T(0);
+    for (int i = threadIdx.x; i < BN; i += S::NT) {
+        par_w[i] = n0 + i < g.n ? g.sw[n0 + i] : T(0);
+        par_b[i] = g.bias && n0 + i < g.n ? g.bias[n0 + i] : T(0);
+    }
+    wait_and_meet<0>();
     read(0, 0);
     int cur = 0;
     for (int s = 0; s < steps; s++) {
-        // Slice s: its first half is in registers.  The buffer that the new loads go to was read
-        // in step s - 1, and every wave's reads of it were done at that step's meeting.
-        read(cur, 1);
-        issue(s + ST - 1, cur == 0 ? ST - 1 : cur - 1);
+        // Slice s, its first chunk of 32 codes in registers already.
+#pragma unroll
+        for (int c = 0; c + 1 < C; c++) {
+            read(cur, c + 1);
+            __builtin_amdgcn_sched_barrier(0);
+            multiply(c);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        // Slice s + 1 is there, and every wave has read all of slice s: its buffer is free.
+        wait_and_meet<S::kLoads *(ST - 2)>();
+        const int next = cur + 1 == ST ? 0 : cur + 1;
+        read(next, 0);
+        issue(s + ST, cur);
         __builtin_amdgcn_sched_barrier(0);
-        multiply(0);
+        multiply(C - 1);
         __builtin_amdgcn_sched_barrier(0);
-        wait_and_meet<S::kLoads *(ST - 2)>();  // slice s + 1 is there
-        cur = cur + 1 == ST ? 0 : cur + 1;
-        read(cur, 0);
-        __builtin_amdgcn_sched_barrier(0);
-        multiply(1);
-        __builtin_amdgcn_sched_barrier(0);
+        cur = next;
     }
     wait_and_meet<0>();
 
     // The epilogue: a wave's results go through its own part of LDS, 32 rows at a time, so that a
-    // lane has four columns side by side of every fourth (TN = 2) row.  Result v of lane l is
-    // column 8 (v / 4) + 4 (l / 32) + v % 4, row l % 32 of its tile.
+    // lane has four columns side by side.  Result v of lane l is column 8 (v / 4) + 4 (l / 32) + v %
+    // 4, row l % 32 of its tile.  Sums lie there as their bits (f32) or as doubles.
     using V = typename Vec16<T>::type;
     using U = typename VecU<T>::type;
-    int *rows = reinterpret_cast<int *>(smem) + w * 32 * S::kRow;
-    constexpr int CL = 8 * TN, RPI = 64 / CL;  // lanes per row, rows at once
+    constexpr int VN = Vec16<T>::n, Q = 4 / VN, CL = 8 * TN, RPI = 64 / CL, NI = 32 / RPI;  // lanes per row, rows at once
+    T *rows = reinterpret_cast<T *>(smem) + w * 32 * S::kOut;
     const int cl = lane % CL, rl = lane / CL;
     const int64_t n = n0 + wc + 4 * cl;
     T sw[4], bias[4];
 #pragma unroll
     for (int e = 0; e < 4; e++) {
-        sw[e] = n + e < g.n ? g.sw[n + e] : T(0);
-        bias[e] = g.bias && n + e < g.n ? g.bias[n + e] : T(0);
+        sw[e] = par_w[wc + 4 * cl + e];
+        bias[e] = par_b[wc + 4 * cl + e];
     }
-    const bool full = n + 4 <= g.n;
+    const bool full = n + 4 <= g.n, act = g.act != NEURAL_ACT_NONE;
+    const auto sums = [&](int r, int (&c)[4]) {
+        const T *p = rows + r * S::kOut + 4 * cl;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            if constexpr (sizeof(T) == 4) c[e] = __float_as_int(p[e]);
+            else c[e] = int(p[e]);
+        }
+    };
 #pragma unroll 1
     for (int i = 0; i < TM; i++) {
+        const int64_t mi = m0 + wr + 32 * i;
+        V res[NI][Q];
+        if (g.res && full) {
+#pragma unroll
+            for (int u = 0; u < NI; u++)
+                if (mi + rl + u * RPI < g.m) {
+#pragma unroll
+                    for (int q = 0; q < Q; q++)
+                        res[u][q] = *(reinterpret_cast<const U *>(g.res + (mi + rl + u * RPI) * g.n + n) + q);
+                }
+        }
         const auto dump = [&](const i32x16 (&t)[TN]) {
 #pragma unroll
             for (int j = 0; j < TN; j++)
 #pragma unroll
-                for (int v = 0; v < 16; v += 4)
-                    *reinterpret_cast<i32x4 *>(rows + frow * S::kRow + 32 * j + 2 * v + 4 * hi) =
-                        i32x4{t[j][v], t[j][v + 1], t[j][v + 2], t[j][v + 3]};
+                for (int v = 0; v < 16; v++) {
+                    T x;
+                    if constexpr (sizeof(T) == 4) x = __int_as_float(t[j][v]);
+                    else x = double(t[j][v]);
+                    rows[frow * S::kOut + 32 * j + 8 * (v / 4) + 4 * hi + v % 4] = x;
+                }
         };
         if (i == 0) dump(acc[0]);
         if constexpr (TM > 1) if (i == 1) dump(acc[1]);
@@ -265,29 +291,63 @@ __global__ __launch_bounds__(S::NT, S::PER_SIMD) void k_lin_mfma(LinArgs<T> g, i
         if constexpr (TM > 3) if (i == 3) dump(acc[3]);
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
-#pragma unroll 1
-        for (int r = rl; r < 32; r += RPI) {
-            const i32x4 c = *reinterpret_cast<const i32x4 *>(rows + r * S::kRow + 4 * cl);
-            const int64_t m = m0 + wr + 32 * i + r;
-            if (m >= g.m || n >= g.n) continue;
-            const T sa = g.sa[m];
-            T z[4];
+        const auto value = [&](int r, T (&z)[4]) {
+            int c[4];
+            sums(r, c);
+            const T sa = par_a[wr + 32 * i + r];
 #pragma unroll
             for (int e = 0; e < 4; e++) z[e] = lin_value<T>(c[e], sa, sw[e], bias[e]);
-            act4(z, g.act, g.alpha);
+        };
+        const auto store = [&](int64_t m, const T (&z)[4]) {
             const int64_t o = m * g.n + n;
-            if (full) {
-                V y[4 / Vec16<T>::n];
+            if (m < g.m && full) {
 #pragma unroll
-                for (int e = 0; e < 4; e++) y[e / Vec16<T>::n][e % Vec16<T>::n] = z[e];
+                for (int q = 0; q < Q; q++) {
+                    V y;
 #pragma unroll
-                for (int q = 0; q < 4 / Vec16<T>::n; q++) {
-                    if (g.res) y[q] = y[q] + *(reinterpret_cast<const U *>(g.res + o) + q);
-                    *(reinterpret_cast<U *>(g.out + o) + q) = y[q];
+                    for (int e = 0; e < VN; e++) y[e] = z[q * VN + e];
+                    __builtin_nontemporal_store(y, reinterpret_cast<U *>(g.out + o) + q);
                 }
-            } else {
+            } else if (m < g.m) {
                 for (int e = 0; e < 4; e++)
-                    if (n + e < g.n) g.out[o + e] = g.res ? z[e] + g.res[o + e] : z[e];
+                    if (n + e < g.n) g.out[o + e] = z[e];
+            }
+        };
+        if (act) {  // one copy of the activations' code, so a loop
+#pragma unroll 1
+            for (int r = rl; r < 32; r += RPI) {
+                T z[4];
+                value(r, z);
+                act4(z, g.act, g.alpha);
+                if (!g.res) {
+                    store(mi + r, z);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) rows[r * S::kOut + 4 * cl + e] = z[e];
+                }
+            }
+        }
+        if (!act || g.res) {
+#pragma unroll
+            for (int u = 0; u < NI; u++) {
+                const int r = rl + u * RPI;
+                const int64_t m = mi + r;
+                T z[4];
+                if (act) {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) z[e] = rows[r * S::kOut + 4 * cl + e];
+                } else {
+                    value(r, z);
+                }
+                if (g.res) {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        T y = res[u][e / VN][e % VN];
+                        if (!full) y = m < g.m && n + e < g.n ? g.res[m * g.n + n + e] : T(0);
+                        z[e] = z[e] + y;
+                    }
+                }
+                store(m, z);
             }
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -300,7 +360,7 @@ static void launch_lin_mfma(const LinArgs<T> &g)
 {
     const int64_t nbm = ceil_div(g.m, S::BM), nbn = ceil_div(g.n, S::BN);
     for_row_launches(nbm * nbn, 1, S::NT, [&](unsigned blocks, int64_t base) {
-        NH_LAUNCH((k_lin_mfma<T, S>), dim3(blocks), dim3(S::NT), 0, stream(), g, nbm, nbn, base, nbm * nbn);
+        NH_LAUNCH((k_lin_mfma<T, S>), dim3(blocks), dim3(S::NT), 0, stream(), g, nbm, nbn, base);
     });
 }
 
@@ -328,8 +388,14 @@ static int launch_linear(LinArgs<T> g)
     if (ba + bw) NH_TRY(pad.open(ba + bw));
     if (ba) lin_pad(g.a, g.lda, g.m, g.k, static_cast<int8_t *>(pad.p));
     if (bw) lin_pad(g.w, g.ldw, g.n, g.k, static_cast<int8_t *>(pad.p) + ba);
-    if (g.m <= 128) launch_lin_mfma<T, LinShape<2, 2, 1, 2, 4, 2>>(g);
-    else launch_lin_mfma<T, LinShape<2, 2, 4, 2, 3, 2>>(g);
+    if constexpr (sizeof(T) == 8) {
+        launch_lin_mfma<T, LinShape<2, 2, 2, 2, 8, 3, 2>>(g);
+    } else {
+        const int64_t large = ceil_div(g.m, 256) * ceil_div(g.n, 256);
+        if (g.m <= 128) launch_lin_mfma<T, LinShape<2, 2, 1, 2, 4, 4, 2>>(g);
+        else if (large >= num_cus() * 5 / 8) launch_lin_mfma<T, LinShape<2, 4, 4, 2, 8, 2, 2>>(g);
+        else launch_lin_mfma<T, LinShape<2, 2, 2, 2, 4, 4, 2>>(g);
+    }
     return check_launch();
 }
 
