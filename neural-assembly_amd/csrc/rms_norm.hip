@@ -17,108 +17,6 @@
 
 namespace nh {
 
-enum { RMS_VALUES = 0, RMS_CODES = 1, ROW_CODES = 2 };
-
-template <typename T>
-struct RmsArgs {
-    const T *x, *res, *gamma;  // res: where it is added; gamma: may be null
-    T *h, *y, *rstd, *scale;   // h, rstd: may be null; y: values; scale: codes
-    int8_t *codes;
-    int64_t stride, rows, cols;
-    double inv_c, eps;
-};
-
-// Codes of W values side by side, as one store.
-template <int W>
-NH_DEV void store_codes(int8_t *p, const int (&c)[W])
-{
-    if constexpr (W == 1) {
-        *p = int8_t(c[0]);
-    } else {
-        typedef int8_t B __attribute__((ext_vector_type(W), aligned(1)));
-        B b;
-#pragma unroll
-        for (int j = 0; j < W; j++) b[j] = int8_t(c[j]);
-        *reinterpret_cast<B *>(p) = b;
-    }
-}
-
-// Maximum over a block, NaN where one value is.
-template <int NT>
-NH_DEV double group_amax(double v, double *lds)
-{
-    const auto comb = [](double a, double b) { return amax_comb(a, b); };
-    return RowGrp<NT>::across(RowGrp<NT>::part(v, comb), lds, comb);
-}
-
-// A block of kLnWide lanes walks a row of any width twice: h, its square sum and its largest
-// |w|, then the outputs.
-template <typename T, bool ADD, int OUT>
-__global__ __launch_bounds__(kLnWide) void k_rms_wide(RmsArgs<T> a, int64_t r_base)
-{
-    using G = RowGrp<kLnWide>;
-    __shared__ double lds_q[G::kWaves], lds_a[G::kWaves];
-    const int64_t r = r_base + blockIdx.x, cols = a.cols, at = r * cols;
-    const auto load = [&](auto w, int64_t c) {
-        constexpr int W = decltype(w)::value;
-        struct {
-            Pack<T, W> x, res, g;
-        } v;
-        v.x = Pack<T, W>::load(a.x + at + c);
-        if constexpr (ADD) v.res = Pack<T, W>::load(a.res + at + c);
-#pragma unroll
-        for (int j = 0; j < W; j++) v.g.v[j] = T(1);
-        if (OUT != ROW_CODES && a.gamma) v.g = Pack<T, W>::load(a.gamma + c);
-        return v;
-    };
-    const auto join = [&](const auto &v, int j) {
-        if constexpr (ADD) return T(v.res.v[j] + v.x.v[j]);
-        else return v.x.v[j];
-    };
-    double q = 0.0, m = 0.0;
-    walk_row<T>(cols, load, [&](auto w, int64_t, const auto &v) {
-        constexpr int W = decltype(w)::value;
-#pragma unroll
-        for (int j = 0; j < W; j++) {
-            const double h = double(join(v, j));
-            if constexpr (OUT != ROW_CODES) q = __builtin_fma(h, h, q);
-            if constexpr (OUT != RMS_VALUES) m = amax_comb(m, __builtin_fabs(h * double(v.g.v[j])));
-        }
-    });
-    double rstd = 1.0;
-    if constexpr (OUT != ROW_CODES) rstd = rms_rstd(G::sum(q, lds_q), a.inv_c, a.eps);
-    if constexpr (OUT != RMS_VALUES) m = group_amax<kLnWide>(m, lds_a);
-    const RowCodes<T> codes(OUT != RMS_VALUES ? m : 0.0);
-    if (threadIdx.x == 0) {
-        if (OUT != ROW_CODES && a.rstd) a.rstd[r] = T(rstd);
-        if (OUT != RMS_VALUES) a.scale[r] = codes.scale(m, rstd);
-    }
-    walk_row<T>(cols, load, [&](auto w, int64_t c, const auto &v) {
-        constexpr int W = decltype(w)::value;
-        Pack<T, W> h, o;
-        int b[W];
-#pragma unroll
-        for (int j = 0; j < W; j++) {
-            h.v[j] = join(v, j);
-            const double hv = double(h.v[j]), g = double(v.g.v[j]);
-            if constexpr (OUT == RMS_VALUES) o.v[j] = T(hv * rstd * g);
-            else b[j] = codes.code(hv * g);
-        }
-        if (ADD && a.h) h.store(a.h + at + c);
-        if constexpr (OUT == RMS_VALUES) o.store(a.y + at + c);
-        else store_codes<W>(a.codes + r * a.stride + c, b);
-    });
-}
-
-template <typename T, bool ADD, int OUT>
-static int launch_rms(const RmsArgs<T> &a)
-{
-    for_row_launches(a.rows, 1, kLnWide, [&](unsigned g, int64_t base) {
-        NH_LAUNCH((k_rms_wide<T, ADD, OUT>), dim3(g), dim3(kLnWide), 0, stream(), a, base);
-    });
-    return check_launch();
-}
-
 // ---- arguments -----------------------------------------------------------------------------
 
 struct RmsTensors {
