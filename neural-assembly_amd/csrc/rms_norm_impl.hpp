@@ -31,29 +31,33 @@ NH_DEV double group_amax(double v, double *lds)
 }
 
 // How a group's lanes hold a row: NT lanes, VPT vectors each, the first F of them whole.
-// kAhead: two rows, one in flight while the other is worked on.  kParams: gamma is loaded before
-// the row's sums, not behind them.
-template <typename T, int NT, int VPT, bool ADD>
+// kAhead: two rows, one in flight while the other is worked on; the resident blocks go by the loads
+// that suit the memory, about 48 KB a CU in flight, and more where rows are read alone (rows to 8
+// bits f32 [16384, 4096] 65.6 us with 3 waves a SIMD, 56.8 with 5, 61.7 with 8; [8192, 8192] 74.8
+// with 2, 59.6 with 3).  kParams: gamma is loaded before the row's sums, not behind them.
+template <typename T, int NT, int VPT, bool ADD, int OUT>
 struct RmsPlan {
     static constexpr int NB = NT < 256 ? 256 : NT, RPB = NB / NT;
     static constexpr bool kAhead = !ADD && NT < 1024;
     static constexpr bool kParams = kAhead || (VPT <= 4 && NT < 1024);
     static constexpr int F = NT < 1024 || VPT <= 4 ? VPT - 1 : VPT / 2;
-    static constexpr int kWaves = !kAhead ? (NT == 1024 ? 4 : 1) : VPT >= 5 ? 2 : VPT >= 3 ? 3 : VPT == 2 ? 5 : 8;
+    static constexpr int kWaves = !kAhead ? (NT == 1024 ? 4 : 1)
+                                  : OUT == ROW_CODES ? (VPT >= 5 ? 3 : VPT >= 3 ? 5 : 8)
+                                                     : (VPT >= 5 ? 2 : VPT >= 3 ? 3 : VPT == 2 ? 5 : 8);
     static constexpr int kPerCu = kWaves * 256 / NB;  // resident blocks
 };
 
 // Groups of NT lanes walk the rows, r = group, group + groups, ...: a row is read once, its
 // square sum and its largest |w| taken from the registers by one exchange.  Bound by HBM.
 template <typename T, int NT, int VPT, bool ADD, int OUT, bool PAST>
-__global__ __launch_bounds__((RmsPlan<T, NT, VPT, ADD>::NB), (RmsPlan<T, NT, VPT, ADD>::kWaves)) void k_rms_rows(
+__global__ __launch_bounds__((RmsPlan<T, NT, VPT, ADD, OUT>::NB), (RmsPlan<T, NT, VPT, ADD, OUT>::kWaves)) void k_rms_rows(
     RmsArgs<T> a, int64_t r_base)
 {
     using V = typename Vec16<T>::type;
     using U = typename VecU<T>::type;
     using G = RowGrp<NT>;
     using S = RowStream<T, PAST>;
-    using Plan = RmsPlan<T, NT, VPT, ADD>;
+    using Plan = RmsPlan<T, NT, VPT, ADD, OUT>;
     constexpr int VN = Vec16<T>::n, RPB = Plan::RPB;
     constexpr bool SUM = OUT != ROW_CODES, MAX = OUT != RMS_VALUES;
     __shared__ double lds_q[2][G::kWaves], lds_m[2][G::kWaves];
@@ -109,6 +113,9 @@ __global__ __launch_bounds__((RmsPlan<T, NT, VPT, ADD>::NB), (RmsPlan<T, NT, VPT
             }
         }
         double q = 0.0, m = 0.0;
+        constexpr bool FMAX = OUT == ROW_CODES && sizeof(T) == 4;  // the values themselves: their maximum in float
+        float mf = 0.0f;
+        bool odd_value = false;  // NaN, which the maximum passes over
         const auto gamma = [&](int k) {
             if constexpr (kParams) {
                 hide(g[k]);
@@ -119,7 +126,12 @@ __global__ __launch_bounds__((RmsPlan<T, NT, VPT, ADD>::NB), (RmsPlan<T, NT, VPT
         };
         const auto take = [&](T h, T gv) {
             if constexpr (SUM) q = __builtin_fma(double(h), double(h), q);
-            if constexpr (MAX) m = amax_comb(m, __builtin_fabs(double(h) * double(gv)));
+            if constexpr (FMAX) {
+                mf = __builtin_fmaxf(mf, __builtin_fabsf(h));
+                odd_value |= h != h;
+            } else if constexpr (MAX) {
+                m = amax_comb(m, __builtin_fabs(double(h) * double(gv)));
+            }
         };
 #pragma unroll
         for (int k = 0; k < VPT; k++)
@@ -130,6 +142,7 @@ __global__ __launch_bounds__((RmsPlan<T, NT, VPT, ADD>::NB), (RmsPlan<T, NT, VPT
                 for (int j = 0; j < VN; j++) take(w.x[k][j], MAX ? gk[j] : T(1));
             }
         if (has_t) take(w.xt, gt);
+        if constexpr (FMAX) m = odd_value ? __builtin_nan("") : double(mf);
         const auto add = [](double x, double y) { return x + y; };
         const auto most = [](double x, double y) { return amax_comb(x, y); };
         if constexpr (SUM) q = G::part(q, add);
@@ -162,7 +175,7 @@ __global__ __launch_bounds__((RmsPlan<T, NT, VPT, ADD>::NB), (RmsPlan<T, NT, VPT
                 if constexpr (MAX) {
                     int c[VN];
 #pragma unroll
-                    for (int j = 0; j < VN; j++) c[j] = codes.code(double(w.x[k][j]) * double(gk[j]));
+                    for (int j = 0; j < VN; j++) c[j] = codes.code(w.x[k][j], gk[j]);
                     store_codes<VN>(a.codes + r * a.stride + int64_t(lane + k * NT) * VN, c);
                 } else {
                     V o;
@@ -173,7 +186,7 @@ __global__ __launch_bounds__((RmsPlan<T, NT, VPT, ADD>::NB), (RmsPlan<T, NT, VPT
             }
         if (has_t) {
             if constexpr (MAX) {
-                const int c[1] = {codes.code(double(w.xt) * double(gt))};
+                const int c[1] = {codes.code(w.xt, gt)};
                 store_codes<1>(a.codes + r * a.stride + cut.sc(lane), c);
             } else {
                 a.y[at + cut.sc(lane)] = T(double(w.xt) * rstd * double(gt));
@@ -246,9 +259,8 @@ __global__ __launch_bounds__(kLnWide) void k_rms_wide(RmsArgs<T> a, int64_t r_ba
 #pragma unroll
         for (int j = 0; j < W; j++) {
             h.v[j] = join(v, j);
-            const double hv = double(h.v[j]), g = double(v.g.v[j]);
-            if constexpr (OUT == RMS_VALUES) o.v[j] = T(hv * rstd * g);
-            else b[j] = codes.code(hv * g);
+            if constexpr (OUT == RMS_VALUES) o.v[j] = T(double(h.v[j]) * rstd * double(v.g.v[j]));
+            else b[j] = codes.code(h.v[j], v.g.v[j]);
         }
         if (ADD && a.h) h.store(a.h + at + c);
         if constexpr (OUT == RMS_VALUES) o.store(a.y + at + c);
@@ -259,7 +271,7 @@ __global__ __launch_bounds__(kLnWide) void k_rms_wide(RmsArgs<T> a, int64_t r_ba
 template <typename T, bool ADD, int OUT, int NT, int VPT>
 static void launch_rms_rows(const RmsArgs<T> &a)
 {
-    using Plan = RmsPlan<T, NT, VPT, ADD>;
+    using Plan = RmsPlan<T, NT, VPT, ADD, OUT>;
     with_stream<T, NT>(a.cols, [&](auto past) {
         const auto launch = [&](unsigned g, int64_t base) {
             NH_LAUNCH((k_rms_rows<T, NT, VPT, ADD, OUT, decltype(past)::value>), dim3(g), dim3(Plan::NB), 0, stream(), a,
