@@ -8,6 +8,7 @@
 // s and t are summed in double: where one token has nearly all the probability, logprob and
 // entropy are as small as the rest of s, which a sum in float would round away beside 1.
 #include <cmath>
+#include <type_traits>
 
 #include "row_call.hpp"
 #include "row_group.hpp"
@@ -16,15 +17,48 @@ namespace nh {
 
 constexpr int kLpMaxTop = 64;
 
-// An alternative: a larger value comes first, of equal ones the lower index.  i < 0: none.
-template <typename T>
-struct LpKey {
-    T v;
-    int i;
-    NH_DEV static LpKey none() { return {-__builtin_inff(), -1}; }
-    NH_DEV bool before(const LpKey &o) const
+// An alternative as one key: of two, the larger key comes first, a larger value, of equal ones (0
+// and -0 too) the lower index.  A key of zero is none, behind all.
+template <typename T> struct LpKey;
+template <>
+struct LpKey<float> {
+    uint64_t k;
+    NH_DEV static LpKey none() { return {0}; }
+    NH_DEV static LpKey of(float v, int i)
     {
-        return i >= 0 && (o.i < 0 || v > o.v || (v == o.v && i < o.i));
+        const int b = __float_as_int(v + 0.0f);
+        return {uint64_t(uint32_t(b) ^ (uint32_t(b >> 31) | 0x80000000u)) << 32 | ~uint32_t(i)};
+    }
+    NH_DEV bool before(const LpKey &o) const { return k > o.k; }
+    NH_DEV bool any() const { return k != 0; }
+    NH_DEV int index() const { return any() ? int(~uint32_t(k)) : -1; }
+    NH_DEV float value() const
+    {
+        const uint32_t o = uint32_t(k >> 32);
+        return any() ? __uint_as_float(o >> 31 ? o ^ 0x80000000u : ~o) : -__builtin_inff();
+    }
+    NH_DEV LpKey of_lane(int off) const { return {uint64_t(__shfl_xor((long long)(k), off, 64))}; }
+};
+template <>
+struct LpKey<double> {
+    uint64_t k;
+    uint64_t i;  // ~index, 0 for none
+    NH_DEV static LpKey none() { return {0, 0}; }
+    NH_DEV static LpKey of(double v, int i)
+    {
+        const int64_t b = __double_as_longlong(v + 0.0);
+        return {uint64_t(b) ^ (uint64_t(b >> 63) | 0x8000000000000000ull), ~uint32_t(i)};
+    }
+    NH_DEV bool before(const LpKey &o) const { return k > o.k || (k == o.k && i > o.i); }
+    NH_DEV bool any() const { return i != 0; }
+    NH_DEV int index() const { return any() ? int(~uint32_t(i)) : -1; }
+    NH_DEV double value() const
+    {
+        return any() ? __longlong_as_double(int64_t(k >> 63 ? k ^ 0x8000000000000000ull : ~k)) : -__builtin_inf();
+    }
+    NH_DEV LpKey of_lane(int off) const
+    {
+        return {uint64_t(__shfl_xor((long long)(k), off, 64)), uint64_t(__shfl_xor((long long)(i), off, 64))};
     }
 };
 
@@ -55,22 +89,7 @@ NH_DEV LpPart lp_join(const LpPart &a, const LpPart &b, double inv_t)
     return {m, a.s * fa + b.s * fb, fa * (a.t + da * a.s) + fb * (b.t + db * b.s)};
 }
 
-// The same over N parts, and over a wave's lanes: one exponential for each.
-template <int N>
-NH_DEV LpPart lp_join_all(const LpPart (&p)[N], double inv_t)
-{
-    LpPart r{p[0].m, 0.0, 0.0};
-#pragma unroll
-    for (int i = 1; i < N; i++) r.m = __builtin_fmax(r.m, p[i].m);
-#pragma unroll
-    for (int i = 0; i < N; i++) {
-        const bool any = p[i].m != -__builtin_inf();
-        const double d = any ? p[i].m - r.m : 0.0, f = any ? exp(d * inv_t) : 0.0;
-        r.s += p[i].s * f;
-        r.t += f * (p[i].t + d * p[i].s);
-    }
-    return r;
-}
+// The same over a wave's lanes: one exponential for each.
 NH_DEV LpPart lp_join_wave(const LpPart &p, double inv_t)
 {
     const double m = RowGrp<64>::max(p.m, nullptr);
@@ -99,9 +118,9 @@ NH_DEV void lp_store(const LpArgs<T> &a, int64_t r, int64_t tok, const LpRow &ro
 template <typename T>
 NH_DEV void lp_store_top(const LpArgs<T> &a, int64_t r, int q, const LpKey<T> &k, const LpRow &row)
 {
-    if (a.top_ids) a.top_ids[r * a.k + q] = row.sound() ? int64_t(k.i) : -1;
+    if (a.top_ids) a.top_ids[r * a.k + q] = row.sound() ? int64_t(k.index()) : -1;
     if (a.top_lp)
-        a.top_lp[r * a.k + q] = !row.sound() ? T(__builtin_nan("")) : k.i < 0 ? -T(__builtin_inf()) : T(row.logprob(double(k.v)));
+        a.top_lp[r * a.k + q] = !row.sound() ? T(__builtin_nan("")) : k.any() ? T(row.logprob(double(k.value()))) : -T(__builtin_inf());
 }
 // A row that is not used, by a group of NT lanes.
 template <typename T, int NT>
@@ -130,107 +149,168 @@ NH_DEV void lp_meet()
     }
 }
 
-template <typename T>
-NH_DEV LpKey<T> lp_first(const LpKey<T> &a, const LpKey<T> &b) { return b.before(a) ? b : a; }
-template <typename T>
-NH_DEV LpKey<T> lp_wave_first(LpKey<T> k)
+// The wave's largest value, NaN passed over, the same in every lane: sixteen lanes by four moves,
+// then one of each sixteen.
+NH_DEV float lp_wave_top(float v)
 {
-#pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) k = lp_first(k, LpKey<T>{__shfl_xor(k.v, off, 64), __shfl_xor(k.i, off, 64)});
-    return k;
+    v = __builtin_fmaxf(v, dpp_f<kDppXor1>(v));
+    v = __builtin_fmaxf(v, dpp_f<kDppXor2>(v));
+    v = __builtin_fmaxf(v, dpp_f<kDppHalfMirror>(v));
+    v = __builtin_fmaxf(v, dpp_f<kDppMirror>(v));
+    const auto of = [&](int lane) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), lane)); };
+    return __builtin_fmaxf(__builtin_fmaxf(of(0), of(16)), __builtin_fmaxf(of(32), of(48)));
 }
+NH_DEV double lp_wave_top(double v) { return RowGrp<64>::max(v, nullptr); }
 
-// LDS of a group that orders alternatives.
+// LDS of a group that orders alternatives: a list of candidates for each of its waves.
 template <typename T, int NT>
 struct LpOrder {
-    static constexpr int kCand = NT == 64 ? 256 : 1024;
-    T v[kCand];
-    int i[kCand];
-    int n;
-    T wave_v[4];
-    int wave_i[4];
-    LpKey<T> out[kLpMaxTop];
+    static constexpr int W = NT / 64, kCand = 256;
+    alignas(16) LpKey<T> key[W][kCand + 2];
+    alignas(16) int n[W];
+    T wave_v[W];
+    LpKey<T> wave_key[W], out[kLpMaxTop];
 };
 
-// The k first of n candidates (n <= kCand, all apart) into o.out: a candidate's place is
-// the number of those before it.
+// The k first of the waves' lists (n[w] <= kCand, all apart) into out: a candidate's place is the
+// number of those before it.  Each wave places its own.
 template <typename T, int NT>
-NH_DEV void lp_rank(LpOrder<T, NT> &o, int n, int k, int lane)
+NH_DEV void lp_rank(LpOrder<T, NT> &o, int k, int lane)
 {
-    for (int q = lane; q < k; q += NT)
-        if (q >= n) o.out[q] = LpKey<T>::none();
-    for (int c = lane; c < n; c += NT) {
-        const LpKey<T> mine{o.v[c], o.i[c]};
+    constexpr int W = NT / 64;
+    const int w = W == 1 ? 0 : lane >> 6, wl = lane & 63;
+    int total = 0;
+#pragma unroll
+    for (int u = 0; u < W; u++) total += o.n[u];
+    for (int q = total + lane; q < k; q += NT) o.out[q] = LpKey<T>::none();
+    for (int c = wl; c < o.n[w]; c += 64) {
+        const LpKey<T> mine = o.key[w][c];
         int place = 0;
-        for (int j = 0; j < n; j++) place += LpKey<T>{o.v[j], o.i[j]}.before(mine) ? 1 : 0;
+#pragma unroll
+        for (int u = 0; u < W; u++)
+#pragma unroll 2
+            for (int j = 0; j < o.n[u]; j += 2) {
+                struct alignas(16) {
+                    LpKey<T> k[2];
+                } pair;
+                pair.k[0] = o.key[u][j];
+                pair.k[1] = o.key[u][j + 1];
+                place += pair.k[0].before(mine) ? 1 : 0;
+                place += pair.k[1].before(mine) ? 1 : 0;
+            }
         if (place < k) o.out[place] = mine;
     }
 }
 
 // The k first keys by k rounds of the group's best key behind the one found before: for rows
-// whose values crowd at the bound (each(f): f(key) for every key of a lane).
+// whose values crowd at the bound (each(f): f(value, index) for every key of a lane).
 template <typename T, int NT, typename E>
-NH_DEV void lp_rounds(LpOrder<T, NT> &o, int k, int lane, E each)
+NH_DEV void lp_rounds(LpOrder<T, NT> &o, int k, int lane, const E &each)
 {
     LpKey<T> last = LpKey<T>::none();
     for (int q = 0; q < k; q++) {
         LpKey<T> best = LpKey<T>::none();
-        if (q == 0 || last.i >= 0)
-            each([&](const LpKey<T> &c) {
-                if (c.before(best) && (q == 0 || last.before(c))) best = c;
-            });
-        best = lp_wave_first(best);
+        each([&](T v, int i) {
+            const LpKey<T> c = LpKey<T>::of(v, i);
+            if (v > -T(__builtin_inf()) && (q == 0 || last.before(c)) && c.before(best)) best = c;
+        });
+        if (q > 0 && !last.any()) best = LpKey<T>::none();
+#pragma unroll
+        for (int off = 32; off >= 1; off >>= 1) {
+            const LpKey<T> u = best.of_lane(off);
+            if (u.before(best)) best = u;
+        }
         if constexpr (NT > 64) {
             __syncthreads();
-            if ((threadIdx.x & 63) == 0) {
-                o.wave_v[threadIdx.x >> 6] = best.v;
-                o.wave_i[threadIdx.x >> 6] = best.i;
-            }
+            if ((lane & 63) == 0) o.wave_key[lane >> 6] = best;
             __syncthreads();
 #pragma unroll
-            for (int w = 0; w < NT / 64; w++) best = lp_first(best, LpKey<T>{o.wave_v[w], o.wave_i[w]});
+            for (int w = 0; w < NT / 64; w++)
+                if (o.wave_key[w].before(best)) best = o.wave_key[w];
         }
         last = best;
         if (lane == 0) o.out[q] = best;
     }
 }
 
-// Where a row is split: its parts' sums and alternatives, [rows][parts] and [rows][parts][k].
+// The k first of a group's keys into o.out.  pop(true) gives the lane's largest value that was not
+// taken yet, of those that stand for its keys, pop(false) looks at it.  With j = k / waves rounded
+// up, the j-th of them over a wave, and the least of that over the waves, is passed by k keys at
+// least; what passes it (some 2 k where values are in no order) each wave collects (pass(bound,
+// take): take(ok, value, index) with the same lanes for all), and it is ordered by counting.
+// What bounds it is one wave's latency, some 7 cycles an instruction.
+template <typename T, int NT, typename P, typename C, typename E>
+NH_DEV void lp_select(LpOrder<T, NT> &o, int k, int lane, P pop, C pass, const E &each)
+{
+    constexpr int W = NT / 64;
+    const int w = W == 1 ? 0 : lane >> 6, wl = lane & 63;
+    const T none = -T(__builtin_inf());
+    T left = pop(false), bound = none;
+    for (int q = 1;; q++) {
+        bound = lp_wave_top(left);
+        if (q * W >= k || bound == none) break;
+        const uint64_t who = __ballot(left == bound);
+        if (wl == int(__builtin_ctzll(who))) left = pop(true);
+    }
+    if constexpr (W > 1) {
+        if (wl == 0) o.wave_v[w] = bound;
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < W; u++) bound = o.wave_v[u] < bound ? o.wave_v[u] : bound;
+    }
+    int n = 0;  // the same in all lanes
+    pass(bound, [&](bool ok, T y, int i) {
+        const uint64_t who = __ballot(ok);
+        if (who) {
+            const int at = n + int(__builtin_amdgcn_mbcnt_hi(uint32_t(who >> 32), __builtin_amdgcn_mbcnt_lo(uint32_t(who), 0)));
+            if (ok && at < o.kCand) o.key[w][at] = LpKey<T>::of(y, i);
+            n += int(__builtin_popcountll(who));
+        }
+    });
+    if (wl == 0) o.n[w] = n;
+    if (wl < 2 && n <= o.kCand) o.key[w][n + wl] = LpKey<T>::none();
+    lp_meet<NT>();
+    bool fits = true;
+#pragma unroll
+    for (int u = 0; u < W; u++) fits &= o.n[u] <= o.kCand;
+    if (fits) lp_rank<T, NT>(o, k, lane);
+    else lp_rounds<T, NT>(o, k, lane, each);
+    lp_meet<NT>();
+}
+
+// Where a row is split: its waves' sums, [rows][parts][4], and its parts' alternatives,
+// [rows][parts][k].
 template <typename T>
 struct LpScratch {
-    LpPart *part;
-    T *v;
-    int *i;
+    LpPart *sums;
+    LpKey<T> *keys;
 };
 
-// A group of NT lanes (a wave, or a block of 256) holds one of `parts` parts of a row in
-// registers, VPT vectors a lane: one read.  Each wave takes its own largest value as the
-// reference of its exponentials.  The k first values of the part: with j = k / waves rounded up,
-// the j-th largest of a wave's lanes' largest values, and the least of those over the waves, is
-// passed by k values at least; what passes it (some 2 k in a random row) is collected and
-// ordered by counting.  Bound by HBM where rows are many.
-template <typename T, int NT, int VPT>
-__global__ __launch_bounds__(256) void k_lp_parts(LpArgs<T> a, LpScratch<T> scratch, int parts, int64_t b_base)
+// A row is cut into parts of 256 lanes, `per` vectors at most, VPT a lane, or of a wave where it is
+// narrow; a group of NT lanes holds one part in registers: one read.  Each wave takes its own largest value as the reference of its exponentials.
+// r_base: the launch's first row.  What bounds it where rows are many: HBM, with vector issue
+// at two thirds (f32: about 16 issue slots a value).
+template <typename T, int NT, int VPT, bool TOP>
+__global__ __launch_bounds__(256, TOP ? 4 : 1) void k_lp_parts(LpArgs<T> a, LpScratch<T> scratch, int parts, int64_t per,
+                                                               int64_t r_base)
 {
     using V = typename Vec16<T>::type;
     using U = typename VecU<T>::type;
     constexpr int VN = Vec16<T>::n, RPB = 256 / NT, W = NT / 64;
-    __shared__ LpPart sh[4];
-    __shared__ LpOrder<T, NT> order[RPB];
+    __shared__ LpPart sh[W];
     const int lane = threadIdx.x % NT, sub = RPB == 1 ? 0 : threadIdx.x / NT;
-    const int64_t unit = (b_base + int64_t(blockIdx.x)) * RPB + sub;
-    const int64_t r = parts == 1 ? unit : unit / parts;
-    const int p = parts == 1 ? 0 : int(unit - r * parts);
+    const int rl = RPB > 1 ? int(blockIdx.x) * RPB + sub : int(blockIdx.x / unsigned(parts));
+    const int p = RPB > 1 ? 0 : int(blockIdx.x) - rl * parts;
+    const int64_t r = r_base + rl;
     if (RPB > 1 && r >= a.rows) return;
     const int64_t tok = a.tokens ? a.tokens[r] : 0;
     if (tok < 0) {
         if (parts == 1) lp_unused<T, NT>(a, r, lane);
         return;
     }
-    // vectors v0 .. v1 of the row, and in the last part the values past them
-    const int64_t cols = a.cols, ncv = cols / VN, per = (ncv + parts - 1) / parts;
-    const int64_t v0 = p * per < ncv ? p * per : ncv, v1 = v0 + per < ncv ? v0 + per : ncv;
-    const int nv = int(v1 - v0), rem = p == parts - 1 ? int(cols - ncv * VN) : 0;
+    // vectors v0 .. of the row, and in the last part the values past them
+    const int64_t cols = a.cols, ncv = cols / VN, v0 = p * per < ncv ? p * per : ncv;
+    const int nv = int(ncv - v0 < per ? ncv - v0 : per), rem = p == parts - 1 ? int(cols - ncv * VN) : 0;
     const T *x = a.x + r * cols;
     const T none = -T(__builtin_inf());
     V v[VPT];
@@ -241,42 +321,57 @@ __global__ __launch_bounds__(256) void k_lp_parts(LpArgs<T> a, LpScratch<T> scra
         if (lane + k * NT < nv) v[k] = __builtin_nontemporal_load(reinterpret_cast<const U *>(x) + v0 + lane + k * NT);
     }
     const T vt = lane < rem ? x[ncv * VN + lane] : none;
-    const auto each = [&](auto f) {  // f(value, its index in the row), in order of the index
+    const int first = int((v0 + lane) * VN);
+    const auto each = [&](auto f) {  // f(value, its index in the row)
 #pragma unroll
         for (int k = 0; k < VPT; k++)
 #pragma unroll
-            for (int j = 0; j < VN; j++) f(v[k][j], int((v0 + lane + k * NT) * VN + j));
-        f(vt, int(ncv * VN + lane));
+            for (int j = 0; j < VN; j++) f(v[k][j], first + k * NT * VN + j);
+        if (rem) f(vt, int(ncv * VN) + lane);
     };
-    T top = none;  // the lane's largest
-    each([&](T y, int) { top = sizeof(T) == 4 ? __builtin_fmaxf(top, y) : __builtin_fmax(top, y); });
+    const auto most = [](T y, T z) {
+        if constexpr (sizeof(T) == 4) return __builtin_fmaxf(y, z);
+        else return __builtin_fmax(y, z);
+    };
+    T top = vt, vmax[VPT];  // the lane's largest, and each vector's
+#pragma unroll
+    for (int k = 0; k < VPT; k++) {
+        vmax[k] = v[k][0];
+#pragma unroll
+        for (int j = 1; j < VN; j++) vmax[k] = most(vmax[k], v[k][j]);
+        top = most(top, vmax[k]);
+    }
     const T m = RowGrp<64>::max(top, nullptr);
     LpPart sum{double(m), 0.0, 0.0};
     const T ref = m == none ? T(0) : m;
     if constexpr (sizeof(T) == 4) {
         // exp(d / T) = 2^(d c), c = log2(e) / T in two floats: the product's rounding error and
-        // the second part go into the result as a factor 1 + error ln 2.
+        // the second part go into the result as a factor 1 + error ln 2.  Four values are added
+        // in float, except where one of them is the largest, whose 1 would swallow the others.
         const double cd = a.inv_t * 1.4426950408889634;
-        const float c = float(cd), c2 = float(cd - double(c)), least = -200.0f / c;  // exp(least / T) = 0
-        const auto term = [&](float y, float &e, float &ed) {
+        const float c = float(cd), c2 = float(cd - double(c));
+        const float least = float(-200.0 * 0.6931471805599453 / a.inv_t);  // exp(least / T) = 0
+        const auto term = [&](float y, float &ed) {
             float d = y - ref;
             d = d < least ? least : d;  // (NaN stays)
             const float h = d * c, lo = __builtin_fmaf(d, c2, __builtin_fmaf(d, c, -h));
-            e = __builtin_amdgcn_exp2f(h);
+            float e = __builtin_amdgcn_exp2f(h);
             e = __builtin_fmaf(e, lo * 0.693147181f, e);
             ed = e * d;
-            sum.s += double(e);
+            return e;
         };
 #pragma unroll
         for (int k = 0; k < VPT; k++) {
-            float e, q[4];
+            float e[4], q[4];
 #pragma unroll
-            for (int j = 0; j < 4; j++) term(v[k][j], e, q[j]);
+            for (int j = 0; j < 4; j++) e[j] = term(v[k][j], q[j]);
             sum.t += double((q[0] + q[1]) + (q[2] + q[3]));
+            if (__ballot(vmax[k] == m)) sum.s += (double(e[0]) + double(e[1])) + (double(e[2]) + double(e[3]));
+            else sum.s += double((e[0] + e[1]) + (e[2] + e[3]));
         }
         if (rem) {  // uniform
-            float e, q;
-            term(vt, e, q);
+            float q;
+            sum.s += double(term(vt, q));
             sum.t += double(q);
         }
     } else {
@@ -288,141 +383,129 @@ __global__ __launch_bounds__(256) void k_lp_parts(LpArgs<T> a, LpScratch<T> scra
     }
     sum.s = wave_dsum(sum.s);
     sum.t = wave_dsum(sum.t);
-    LpOrder<T, NT> &o = order[sub];
-    if (lane == 0) o.n = 0;
-    if constexpr (W > 1) {
-        if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = sum;
-    }
-    if (a.k) {
-        T left = top, bound = none;
-        for (int q = 0; q < (a.k + W - 1) / W; q++) {
-            bound = RowGrp<64>::max(left, nullptr);
-            const uint64_t who = __ballot(left == bound);
-            if (bound == none) break;
-            if ((threadIdx.x & 63) == __builtin_ctzll(who)) left = none;
-        }
-        if (W > 1 && (threadIdx.x & 63) == 0) o.wave_v[threadIdx.x >> 6] = bound;
-        lp_meet<NT>();
-        if constexpr (W > 1) {
+    __shared__ LpOrder<T, NT> order[TOP ? RPB : 1];
+    if constexpr (TOP) {
+        // Alternatives of a wave that are many for its lanes: its vectors stand for their values,
+        // not its lanes (k = 64 of 1000: 26 us, by lanes 171, as too much passed the bound).
+        const bool fine = NT == 64 && a.k > NT / 4;
+        T over = top, scalar = vt;
+        T over_v[VPT];
 #pragma unroll
-            for (int w = 0; w < W; w++) bound = o.wave_v[w] < bound ? o.wave_v[w] : bound;
-        }
-        const auto passes = [&](T y) { return y >= bound && y > none; };
-        int mine = 0;
-        each([&](T y, int) { mine += passes(y) ? 1 : 0; });
-        int before = mine;  // of the wave's lanes up to this one
+        for (int k = 0; k < VPT; k++) over_v[k] = vmax[k];
+        const auto pop = [&](bool next) {
+            if (next) {
+                if (fine) {
+                    bool gone = false;
 #pragma unroll
-        for (int off = 1; off < 64; off <<= 1) {
-            const int u = __shfl_up(before, off, 64);
-            if (int(threadIdx.x & 63) >= off) before += u;
-        }
-        int at = 0;
-        if ((threadIdx.x & 63) == 63) at = atomicAdd(&o.n, before);
-        at = __shfl(at, 63, 64) + before - mine;
-        if (mine)
-            each([&](T y, int i) {
-                if (passes(y)) {
-                    if (at < o.kCand) {
-                        o.v[at] = y;
-                        o.i[at] = i;
+                    for (int k = 0; k < VPT; k++) {
+                        const bool it = !gone && over_v[k] == over;
+                        over_v[k] = it ? none : over_v[k];
+                        gone |= it;
                     }
-                    at++;
+                    scalar = gone ? scalar : none;
+                    over = scalar;
+#pragma unroll
+                    for (int k = 0; k < VPT; k++) over = most(over, over_v[k]);
+                } else {
+                    over = none;
                 }
-            });
-        lp_meet<NT>();
-        const int n = o.n;
-        if (n <= o.kCand) {
-            lp_rank<T, NT>(o, n, a.k, lane);
-        } else {
-            lp_rounds<T, NT>(o, a.k, lane, [&](auto f) {
-                each([&](T y, int i) {
-                    if (y > none) f(LpKey<T>{y, i});
-                });
-            });
-        }
+            }
+            return over;
+        };
+        const auto pass = [&](T bound, auto take) {
+            uint32_t hits = 0;  // the lane's vectors with a value that passes
+#pragma unroll
+            for (int k = 0; k < VPT; k++) hits |= vmax[k] >= bound && vmax[k] > none ? 1u << k : 0u;
+            while (__ballot(hits != 0)) {
+                const int at = __builtin_ctz(hits | 0x80000000u);
+                const bool on = hits != 0;
+                // vector `at` by masks: by a choice of vectors the compiler puts them into memory
+                using I = std::conditional_t<sizeof(T) == 4, uint32_t, uint64_t>;
+                I bits[VN] = {};
+#pragma unroll
+                for (int k = 0; k < VPT; k++) {
+                    const I mask = at == k ? ~I(0) : I(0);
+#pragma unroll
+                    for (int j = 0; j < VN; j++) {
+                        I b;
+                        const T e = v[k][j];
+                        __builtin_memcpy(&b, &e, sizeof(T));
+                        bits[j] |= b & mask;
+                    }
+                }
+                T y[VN];
+                __builtin_memcpy(y, bits, sizeof(bits));
+                hits &= hits - 1;
+#pragma unroll
+                for (int j = 0; j < VN; j++) take(on && y[j] >= bound && y[j] > none, y[j], first + at * (NT * VN) + j);
+            }
+            if (rem) take(vt >= bound && vt > none, vt, int(ncv * VN) + lane);
+        };
+        lp_select<T, NT>(order[sub], a.k, lane, pop, pass, each);
     }
-    lp_meet<NT>();
-    if constexpr (W > 1) sum = lp_join_all(sh, a.inv_t);
+    const LpOrder<T, NT> &o = order[TOP ? sub : 0];
+    const int keys = TOP ? a.k : 0;
     if (parts == 1) {
+        if constexpr (W > 1) {
+            if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = sum;
+            __syncthreads();
+            const int wl = threadIdx.x & 63;
+            sum = lp_join_wave(wl < W ? sh[wl < W ? wl : 0] : LpPart{-__builtin_inf(), 0.0, 0.0}, a.inv_t);
+        }
         const LpRow row(sum, a.inv_t);
         if (lane == 0) lp_store(a, r, tok, row, sum.t);
-        for (int q = lane; q < a.k; q += NT) lp_store_top(a, r, q, o.out[q], row);
+        for (int q = lane; q < keys; q += NT) lp_store_top(a, r, q, o.out[q], row);
     } else {
-        if (lane == 0) scratch.part[unit] = sum;
-        for (int q = lane; q < a.k; q += NT) {
-            scratch.v[unit * a.k + q] = o.out[q].v;
-            scratch.i[unit * a.k + q] = o.out[q].i;
-        }
+        const int64_t unit = r * parts + p;
+        if ((threadIdx.x & 63) == 0) scratch.sums[unit * 4 + (threadIdx.x >> 6)] = sum;
+        for (int q = lane; q < keys; q += NT) scratch.keys[unit * a.k + q] = o.out[q];
     }
 }
 
-// A row's parts joined, NT lanes a row.  The alternatives: the largest of the parts' k-th
-// values is passed by k of all at least.
+// A row's parts joined: NT lanes a row, a wave where no alternatives are asked for.
 template <typename T, int NT>
 __global__ __launch_bounds__(256) void k_lp_join(LpArgs<T> a, LpScratch<T> scratch, int parts, int64_t b_base)
 {
-    constexpr int RPB = 256 / NT, W = NT / 64;
-    __shared__ LpPart sh[4];
-    __shared__ T sh_b[4];
-    __shared__ LpOrder<T, NT> order[1];  // (a wave a row: no alternatives)
+    constexpr int RPB = 256 / NT;
+    __shared__ LpPart sh[1];
     const int lane = threadIdx.x % NT, sub = RPB == 1 ? 0 : threadIdx.x / NT;
     const int64_t r = (b_base + int64_t(blockIdx.x)) * RPB + sub;
     if (RPB > 1 && r >= a.rows) return;
     const int64_t tok = a.tokens ? a.tokens[r] : 0;
     if (tok < 0) return lp_unused<T, NT>(a, r, lane);
     const T none = -T(__builtin_inf());
-    const LpPart *part = scratch.part + r * parts;
-    const T *kv = scratch.v + r * parts * a.k;
-    const int *ki = scratch.i + r * parts * a.k;
     LpPart sum{-__builtin_inf(), 0.0, 0.0};
-    T bound = none;
-    for (int p = lane; p < parts; p += NT) {
-        sum = lp_join(sum, part[p], a.inv_t);
-        if (a.k) {
-            const T b = kv[int64_t(p) * a.k + a.k - 1];
-            bound = b > bound ? b : bound;
-        }
+    const LpPart *sums = scratch.sums + r * parts * 4;
+    if (NT == 64 || lane < 64) {  // one wave, in one order
+        for (int p = lane; p < parts * 4; p += 64) sum = p < 64 ? sums[p] : lp_join(sum, sums[p], a.inv_t);
+        sum = lp_join_wave(sum, a.inv_t);
     }
-    sum = lp_join_wave(sum, a.inv_t);
-    if constexpr (W > 1) {
-        bound = RowGrp<64>::max(bound, nullptr);
-        if ((threadIdx.x & 63) == 0) {
-            sh[threadIdx.x >> 6] = sum;
-            sh_b[threadIdx.x >> 6] = bound;
-        }
-        if (threadIdx.x == 0) order[0].n = 0;
-        __syncthreads();
-        sum = lp_join_all(sh, a.inv_t);
-        bound = sh_b[0];
-#pragma unroll
-        for (int w = 1; w < W; w++) bound = sh_b[w] > bound ? sh_b[w] : bound;
-    }
-    const LpRow row(sum, a.inv_t);
-    if (lane == 0) lp_store(a, r, tok, row, sum.t);
-    if constexpr (W > 1) {
-        if (!a.k) return;
-        LpOrder<T, NT> &o = order[0];
-        const int64_t n_all = int64_t(parts) * a.k;
-        for (int64_t c = lane; c < n_all; c += NT) {
-            const LpKey<T> key{kv[c], ki[c]};
-            if (key.i >= 0 && key.v >= bound) {
-                const int at = atomicAdd(&o.n, 1);  // (any order: they are ordered after)
-                if (at < o.kCand) {
-                    o.v[at] = key.v;
-                    o.i[at] = key.i;
-                }
+    if constexpr (NT == 64) {
+        if (lane == 0) lp_store(a, r, tok, LpRow(sum, a.inv_t), sum.t);
+    } else {
+        __shared__ LpOrder<T, NT> o;
+        if (lane == 0) sh[0] = sum;
+        const int64_t n = int64_t(parts) * a.k;
+        const LpKey<T> *keys = scratch.keys + r * n;
+        const auto each = [&](auto f) {
+            for (int64_t c = lane; c < n; c += NT) f(keys[c].value(), keys[c].index());
+        };
+        T top = none;  // (a place without a value holds none)
+        each([&](T y, int) { top = y > top ? y : top; });
+        const auto pop = [&](bool next) {
+            if (next) top = none;  // a lane's keys by their largest alone
+            return top;
+        };
+        const auto pass = [&](T bound, auto take) {
+            for (int64_t c0 = 0; c0 < n; c0 += NT) {
+                const bool on = c0 + lane < n;
+                const LpKey<T> key = on ? keys[c0 + lane] : LpKey<T>::none();
+                take(key.any() && key.value() >= bound, key.value(), key.index());
             }
-        }
-        __syncthreads();
-        const int n = o.n;
-        if (n <= o.kCand) {
-            lp_rank<T, NT>(o, n, a.k, lane);
-        } else {
-            lp_rounds<T, NT>(o, a.k, lane, [&](auto f) {
-                for (int64_t c = lane; c < n_all; c += NT) f(LpKey<T>{kv[c], ki[c]});
-            });
-        }
-        __syncthreads();
+        };
+        lp_select<T, NT>(o, a.k, lane, pop, pass, each);
+        const LpRow row(sh[0], a.inv_t);
+        if (lane == 0) lp_store(a, r, tok, row, sh[0].t);
         for (int q = lane; q < a.k; q += NT) lp_store_top(a, r, q, o.out[q], row);
     }
 }
@@ -436,45 +519,50 @@ struct LpGradArgs {
     double inv_t;
 };
 
-// What a row's gradient is made of; rows that are not used or have every logit masked: g = e = 0
-// and zero.
+// What a row's gradient is made of: dx = -p (g + e (log p + H)) / T, and + g / T at the token.
+// f32 rows: log2 p = x a + b in double, its exponential to f32's accuracy; f64 rows: log p.  p = 0
+// (a masked logit) leaves 0: log p is held above -inf.
+template <typename T>
 struct LpGradRow {
-    double lse, g, e, h;
+    double a, b, g, e, h;
     int64_t tok;
-    bool zero;
+    bool zero;  // a row that is not used, or with every logit masked
+    NH_DEV LpGradRow(const LpGradArgs<T> &q, int64_t r)
+    {
+        constexpr double L = sizeof(T) == 4 ? 1.4426950408889634 : 1.0;
+        tok = q.tokens ? q.tokens[r] : -2;
+        const double lse = double(q.lse[r]);
+        a = q.inv_t * L;
+        b = -lse * L;
+        g = q.g ? double(q.g[r]) * q.inv_t : 0.0;
+        if (q.g && tok >= q.cols) g = __builtin_nan("");
+        e = q.e ? double(q.e[r]) * q.inv_t : 0.0;
+        h = q.e ? double(q.entropy[r]) : 0.0;
+        zero = (q.tokens && tok < 0) || lse == -__builtin_inf();
+    }
+    NH_DEV T operator()(T x, bool at) const
+    {
+        double p, lp;
+        if constexpr (sizeof(T) == 4) {
+            double t = __builtin_fma(double(x), a, b);
+            t = t < -300.0 ? -300.0 : t;
+            const double n = __builtin_rint(t);
+            p = double(__builtin_ldexpf(__builtin_amdgcn_exp2f(float(t - n)), int(n)));
+            lp = t * 0.6931471805599453;
+        } else {
+            lp = __builtin_fma(x, a, b);
+            lp = lp < -2000.0 ? -2000.0 : lp;
+            p = exp(lp);
+        }
+        const double v = -p * __builtin_fma(e, lp + h, g);
+        return zero ? T(0) : T(at ? v + g : v);
+    }
 };
 
-template <typename T>
-NH_DEV LpGradRow lp_grad_row(const LpGradArgs<T> &a, int64_t r)
-{
-    LpGradRow w;
-    w.tok = a.tokens ? a.tokens[r] : -2;
-    w.lse = double(a.lse[r]);
-    w.g = a.g ? double(a.g[r]) : 0.0;
-    if (a.g && w.tok >= a.cols) w.g = __builtin_nan("");
-    w.e = a.e ? double(a.e[r]) : 0.0;
-    w.h = a.e ? double(a.entropy[r]) : 0.0;
-    w.zero = (a.tokens && w.tok < 0) || w.lse == -__builtin_inf();
-    return w;
-}
-
-// log p in double, its exponential to f32 accuracy for f32 rows, the terms in double.
-template <typename T>
-NH_DEV T lp_grad(T x, bool at, const LpGradRow &w, double inv_t)
-{
-    const double lp = double(x) * inv_t - w.lse;
-    double p;
-    if constexpr (sizeof(T) == 4) p = double(exp_d2f(lp));
-    else p = exp(lp);
-    double v = w.g * ((at ? 1.0 : 0.0) - p);
-    const double ent = w.e * p * (lp + w.h);
-    v -= p == 0.0 ? 0.0 : ent;  // (a masked logit: 0 * -inf)
-    return w.zero ? T(0) : T(v * inv_t);
-}
-
-// Rows of at least kLpFlat values (and f64 rows of half): the tensor as one run of vectors that
-// begin at 128-byte lines of dx, so that stores fill whole lines whatever the rows' width (f32
-// [4096, 50257], whose rows start anywhere).  A block's 1024 vectors lie in two rows at most.
+// Rows of at least kLpFlat f32 values (f64: half): the tensor as one run of vectors that begin at
+// 128-byte lines of dx, so that stores fill whole lines whatever the rows' width (f32 [4096, 50257],
+// whose rows start anywhere).  A block's 1024 vectors lie in two rows at most, mostly in one:
+// its numbers are the same for the block then, and nothing is read for a row of zeros.
 constexpr int64_t kLpFlat = 4096;
 template <typename T>
 __global__ __launch_bounds__(256) void k_lp_grad_flat(LpGradArgs<T> a, int64_t head, int64_t b_base)
@@ -483,35 +571,46 @@ __global__ __launch_bounds__(256) void k_lp_grad_flat(LpGradArgs<T> a, int64_t h
     using U = typename VecU<T>::type;
     constexpr int VN = Vec16<T>::n, P = 4;
     const int64_t n = a.rows * a.cols, nv = (n - head) / VN, q0 = (b_base + int64_t(blockIdx.x)) * 256 * P;
-    const int64_t first = head + q0 * VN, r0 = first / a.cols;  // uniform
-    V x[P];
+    const int64_t first = head + q0 * VN, r0 = first / a.cols, off = first - r0 * a.cols;  // uniform
+    const U *x = reinterpret_cast<const U *>(a.x + head) + q0;
+    U *dx = reinterpret_cast<U *>(a.dx + head) + q0;
+    const int left = nv - q0 < 256 * P ? int(nv - q0) : 256 * P, lane = threadIdx.x;
+    if (r0 < a.rows) {
+        const LpGradRow<T> w0(a, r0);
+        if (off + 256 * P * VN <= a.cols) {
+            const int64_t at = w0.tok - off;  // the token, from the block's first value
+            V v[P];
+            if (!w0.zero) {
 #pragma unroll
-    for (int k = 0; k < P; k++) {
-        const int64_t q = q0 + threadIdx.x + k * 256;
-        if (q < nv) x[k] = __builtin_nontemporal_load(reinterpret_cast<const U *>(a.x + head) + q);
-    }
-    const LpGradRow w0 = lp_grad_row(a, r0 < a.rows ? r0 : a.rows - 1);
-    const LpGradRow w1 = lp_grad_row(a, r0 + 1 < a.rows ? r0 + 1 : a.rows - 1);
-    const int64_t off = first - r0 * a.cols;
-#pragma unroll
-    for (int k = 0; k < P; k++) {
-        const int64_t q = q0 + threadIdx.x + k * 256;
-        if (q < nv) {
-            const int64_t c = off + int64_t(threadIdx.x + k * 256) * VN;
-            V o;
-#pragma unroll
-            for (int j = 0; j < VN; j++) {
-                const bool next = c + j >= a.cols;
-                const int64_t col = next ? c + j - a.cols : c + j;
-                LpGradRow w;
-                w.lse = next ? w1.lse : w0.lse;
-                w.g = next ? w1.g : w0.g;
-                w.e = next ? w1.e : w0.e;
-                w.h = next ? w1.h : w0.h;
-                w.zero = next ? w1.zero : w0.zero;
-                o[j] = lp_grad(x[k][j], col == (next ? w1.tok : w0.tok), w, a.inv_t);
+                for (int k = 0; k < P; k++)
+                    if (lane + k * 256 < left) v[k] = __builtin_nontemporal_load(x + lane + k * 256);
             }
-            __builtin_nontemporal_store(o, reinterpret_cast<U *>(a.dx + head) + q);
+#pragma unroll
+            for (int k = 0; k < P; k++)
+                if (lane + k * 256 < left) {
+                    V o;
+#pragma unroll
+                    for (int j = 0; j < VN; j++) o[j] = w0.zero ? T(0) : w0(v[k][j], false);
+                    if (at / VN == lane + k * 256 && at >= 0 && !w0.zero) {
+#pragma unroll
+                        for (int j = 0; j < VN; j++)
+                            if (j == at % VN) o[j] = w0(v[k][j], true);
+                    }
+                    __builtin_nontemporal_store(o, dx + lane + k * 256);
+                }
+        } else {
+            const LpGradRow<T> w1(a, r0 + 1 < a.rows ? r0 + 1 : r0);
+#pragma unroll
+            for (int k = 0; k < P; k++)
+                if (lane + k * 256 < left) {
+                    const V v = __builtin_nontemporal_load(x + lane + k * 256);
+                    const int64_t c = off + int64_t(lane + k * 256) * VN;
+                    V o;
+#pragma unroll
+                    for (int j = 0; j < VN; j++)
+                        o[j] = c + j < a.cols ? w0(v[j], c + j == w0.tok) : w1(v[j], c + j - a.cols == w1.tok);
+                    __builtin_nontemporal_store(o, dx + lane + k * 256);
+                }
         }
     }
     // the values before the first vector and past the last
@@ -520,8 +619,8 @@ __global__ __launch_bounds__(256) void k_lp_grad_flat(LpGradArgs<T> a, int64_t h
         const int64_t i = int64_t(threadIdx.x) < head ? int64_t(threadIdx.x) : tail + threadIdx.x - head;
         if (i < n) {
             const int64_t r = i / a.cols;
-            const LpGradRow w = lp_grad_row(a, r);
-            a.dx[i] = lp_grad(a.x[i], i - r * a.cols == w.tok, w, a.inv_t);
+            const LpGradRow<T> w(a, r);
+            a.dx[i] = w(a.x[i], i - r * a.cols == w.tok);
         }
     }
 }
@@ -536,7 +635,7 @@ __global__ __launch_bounds__(256) void k_lp_grad_row(LpGradArgs<T> a, int64_t r_
     const int lane = threadIdx.x % NT, sub = RPB == 1 ? 0 : threadIdx.x / NT;
     const int64_t r = r_base + int64_t(blockIdx.x) * RPB + sub;
     if (RPB > 1 && r >= a.rows) return;
-    const LpGradRow w = lp_grad_row(a, r);
+    const LpGradRow<T> w(a, r);
     const T *x = a.x + r * a.cols;
     T *dx = a.dx + r * a.cols;
     const int ncv = int(a.cols / VN), rem = int(a.cols % VN);
@@ -544,46 +643,52 @@ __global__ __launch_bounds__(256) void k_lp_grad_row(LpGradArgs<T> a, int64_t r_
         const V v = *(reinterpret_cast<const U *>(x) + q);
         V o;
 #pragma unroll
-        for (int j = 0; j < VN; j++) o[j] = lp_grad(v[j], int64_t(q) * VN + j == w.tok, w, a.inv_t);
+        for (int j = 0; j < VN; j++) o[j] = w(v[j], int64_t(q) * VN + j == w.tok);
         *(reinterpret_cast<U *>(dx) + q) = o;
     }
     if (lane < rem) {
         const int64_t c = int64_t(ncv) * VN + lane;
-        dx[c] = lp_grad(x[c], c == w.tok, w, a.inv_t);
+        dx[c] = w(x[c], c == w.tok);
     }
 }
 
 template <typename T, int NT, int VPT>
-static void launch_lp_parts(const LpArgs<T> &a, const LpScratch<T> &scratch, int parts)
+static void launch_lp_parts(const LpArgs<T> &a, const LpScratch<T> &scratch, int parts, int64_t per)
 {
-    for_row_launches(a.rows * parts, 256 / NT, 256, [&](unsigned g, int64_t base) {
-        NH_LAUNCH((k_lp_parts<T, NT, VPT>), dim3(g), dim3(256), 0, stream(), a, scratch, parts, base / (256 / NT));
-    });
+    const int64_t rpb = 256 / NT, most = kMaxGridBlocks / parts * rpb;  // rows a launch (parts > 1: rpb is 1)
+    for (int64_t base = 0; base < a.rows; base += most) {
+        const int64_t n = a.rows - base < most ? a.rows - base : most;
+        const dim3 grid(unsigned(ceil_div(n, rpb) * parts));
+        if (a.k) NH_LAUNCH((k_lp_parts<T, NT, VPT, true>), grid, dim3(256), 0, stream(), a, scratch, parts, per, base);
+        else NH_LAUNCH((k_lp_parts<T, NT, VPT, false>), grid, dim3(256), 0, stream(), a, scratch, parts, per, base);
+    }
 }
 
 // By the width alone, so that equal rows have equal results in any batch: a wave up to 256
-// vectors, a block up to 1024, and as many blocks as it takes beyond, joined by a second launch.
+// vectors, 256 lanes up to 2048, and beyond parts of that by blocks of their own, joined by a second
+// launch (one block of 1024 for four parts: [64, 32000] with one alternative 22.9 us, two launches
+// 13.5).
 template <typename T>
 static int launch_lp(const LpArgs<T> &a)
 {
     const int64_t ncv = a.cols / Vec16<T>::n;
     const LpScratch<T> no{};
-    if (ncv <= 64) launch_lp_parts<T, 64, 1>(a, no, 1);
-    else if (ncv <= 128) launch_lp_parts<T, 64, 2>(a, no, 1);
-    else if (ncv <= 256) launch_lp_parts<T, 64, 4>(a, no, 1);
-    else if (ncv <= 512) launch_lp_parts<T, 256, 2>(a, no, 1);
-    else if (ncv <= 1024) launch_lp_parts<T, 256, 4>(a, no, 1);
+    const int parts = int(ceil_div(ncv, 2048));
+    const int64_t per = parts ? ceil_div(ncv, parts) : 0;
+    if (ncv <= 64) launch_lp_parts<T, 64, 1>(a, no, 1, 64);
+    else if (ncv <= 128) launch_lp_parts<T, 64, 2>(a, no, 1, 128);
+    else if (ncv <= 256) launch_lp_parts<T, 64, 4>(a, no, 1, 256);
+    else if (ncv <= 512) launch_lp_parts<T, 256, 2>(a, no, 1, 512);
+    else if (ncv <= 1024) launch_lp_parts<T, 256, 4>(a, no, 1, 1024);
+    else if (ncv <= 2048) launch_lp_parts<T, 256, 8>(a, no, 1, 2048);
     else {
-        const int parts = int(ceil_div(ncv, 1024));
         const size_t units = size_t(a.rows) * size_t(parts), keys = units * size_t(a.k);
         Partials block;
-        NH_TRY(block.open(units * sizeof(LpPart) + keys * (sizeof(T) + sizeof(int))));
-        LpScratch<T> scratch{static_cast<LpPart *>(block.p), nullptr, nullptr};
-        scratch.v = reinterpret_cast<T *>(scratch.part + units);
-        scratch.i = reinterpret_cast<int *>(scratch.v + keys);
-        launch_lp_parts<T, 256, 4>(a, scratch, parts);
-        const int rpb = a.k ? 1 : 4;
-        for_row_launches(a.rows, rpb, 256, [&](unsigned g, int64_t base) {
+        NH_TRY(block.open(units * 4 * sizeof(LpPart) + keys * sizeof(LpKey<T>)));
+        LpScratch<T> scratch{static_cast<LpPart *>(block.p), nullptr};
+        scratch.keys = reinterpret_cast<LpKey<T> *>(scratch.sums + units * 4);
+        launch_lp_parts<T, 256, 8>(a, scratch, parts, per);
+        for_row_launches(a.rows, a.k ? 1 : 4, 256, [&](unsigned g, int64_t base) {
             if (a.k) NH_LAUNCH((k_lp_join<T, 256>), dim3(g), dim3(256), 0, stream(), a, scratch, parts, base);
             else NH_LAUNCH((k_lp_join<T, 64>), dim3(g), dim3(256), 0, stream(), a, scratch, parts, base / 4);
         });
