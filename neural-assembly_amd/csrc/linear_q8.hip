@@ -67,24 +67,30 @@ constexpr int64_t kLinMaxLd = int64_t(1) << 22;  // 256 rows of it stay in a 32-
 
 // Rows of codes copied to rows of `ldd` bytes (a multiple of 16) at an aligned address, the bytes
 // past k zero.  A lane takes 16 bytes.
-__global__ __launch_bounds__(256) void k_lin_pad(const int8_t *__restrict__ src, int64_t ld, int8_t *__restrict__ dst,
-                                                 int64_t ldd, int64_t rows, int64_t k)
+struct LinPad {
+    const int8_t *src;
+    int8_t *dst;
+    int64_t ld, rows;  // rows 0: nothing to copy
+};
+__global__ __launch_bounds__(256) void k_lin_pad(LinPad a, LinPad w, int64_t ldd, int64_t k)
 {
-    const int64_t units = ldd / 16, step = int64_t(gridDim.x) * 256;
-    for (int64_t t = int64_t(blockIdx.x) * 256 + threadIdx.x; t < rows * units; t += step) {
-        const int64_t r = t / units, u = t - r * units;
-        const int8_t *p = src + r * ld + 16 * u;
+    typedef int W __attribute__((ext_vector_type(4), aligned(1)));
+    const int64_t units = ldd / 16, step = int64_t(gridDim.x) * 256, first = a.rows * units;
+    for (int64_t t0 = int64_t(blockIdx.x) * 256 + threadIdx.x; t0 < first + w.rows * units; t0 += step) {
+        const bool of_a = t0 < first;
+        const LinPad &p = of_a ? a : w;
+        const int64_t t = of_a ? t0 : t0 - first, r = t / units, u = t - r * units;
+        const int8_t *src = p.src + r * p.ld + 16 * u;
         i32x4 v;
         if (16 * u + 16 <= k) {
-            typedef int W __attribute__((ext_vector_type(4), aligned(1)));
-            v = *reinterpret_cast<const W *>(p);
+            v = *reinterpret_cast<const W *>(src);
         } else {
             int8_t b[16];
 #pragma unroll
-            for (int q = 0; q < 16; q++) b[q] = 16 * u + q < k ? p[q] : int8_t(0);
+            for (int q = 0; q < 16; q++) b[q] = 16 * u + q < k ? src[q] : int8_t(0);
             __builtin_memcpy(&v, b, 16);
         }
-        *reinterpret_cast<i32x4 *>(dst + r * ldd + 16 * u) = v;
+        *reinterpret_cast<i32x4 *>(p.dst + r * ldd + 16 * u) = v;
     }
 }
 
@@ -139,10 +145,15 @@ NH_DEV void lin_tile(int64_t h, int64_t nbm, int64_t nbn, int64_t &bm, int64_t &
     bn = r / rows;
 }
 
+// Where few tiles meet a long depth, LIN_PART blocks sum a part of it each and leave their
+// registers, and LIN_JOIN blocks add those up and end as LIN_WHOLE ones do.
+enum { LIN_WHOLE = 0, LIN_PART = 1, LIN_JOIN = 2 };
+
 // (A's rows are the second operand: a lane's results are of one row of A and, four at a time,
 // consecutive columns.)
-template <typename T, typename S>
-__global__ __launch_bounds__(S::NT, S::PER_SIMD) void k_lin_mfma(LinArgs<T> g, int64_t nbm, int64_t nbn, int64_t b_base)
+template <typename T, typename S, int MODE>
+__global__ __launch_bounds__(S::NT, S::PER_SIMD) void k_lin_mfma(LinArgs<T> g, int64_t nbm, int64_t nbn, int64_t b_base,
+                                                                  i32x4 *parts, int splits)
 {
     constexpr int TM = S::TM, TN = S::TN, ST = S::ST, KU = S::KU, BM = S::BM, BN = S::BN, C = KU / 2;
     static_assert(S::NW * 32 * S::kOut * int(sizeof(T)) <= ST * S::kStage, "the epilogue's rows fit the buffers");
@@ -150,92 +161,133 @@ __global__ __launch_bounds__(S::NT, S::PER_SIMD) void k_lin_mfma(LinArgs<T> g, i
     __shared__ T par_a[BM], par_w[BN], par_b[BN];
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     int64_t bm, bn;
-    lin_tile(b_base + blockIdx.x, nbm, nbn, bm, bn);
+    const int split = MODE == LIN_PART ? int(blockIdx.x) % splits : 0;
+    const int64_t tile = b_base + (MODE == LIN_PART ? int(blockIdx.x) / splits : int(blockIdx.x));
+    lin_tile(tile, nbm, nbn, bm, bn);
     const int64_t m0 = bm * BM, n0 = bn * BN;
     const int wr = 32 * TM * (w / S::WN), wc = 32 * TN * (w % S::WN);
-    // LDS rows of KU units of 16 bytes; unit u of row r lies at u ^ swz(r), so that the sixteen lanes
-    // of a 16-byte read that go at once cover the 64 banks once.  A load puts lane l's unit at
-    // place l % KU of row l / KU: it fetches the unit that belongs there.
-    const auto swz = [](int r) { return KU == 4 ? r >> 2 & 3 : r >> 1 & 7; };
-    const uint32_t lds0 = uint32_t(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) int8_t *)smem));
-    uint32_t at[S::kLoads];
-    int unit[S::kLoads];
-#pragma unroll
-    for (int q = 0; q < S::kLoads; q++) {
-        const bool of_a = q < S::kLoadsA;
-        const int r = (w + (of_a ? q : q - S::kLoadsA) * S::NW) * S::kRows + lane / KU;
-        const int64_t last = of_a ? g.m - 1 - m0 : g.n - 1 - n0;
-        unit[q] = (lane % KU) ^ swz(r);
-        at[q] = uint32_t((r < last ? r : last) * (of_a ? g.lda : g.ldw) + 16 * unit[q]);
-    }
-    const int8_t *pa = g.a + m0 * g.lda, *pw = g.w + n0 * g.ldw;
-    const int steps = int((g.k + S::kSlice - 1) / S::kSlice), whole = int(g.k / S::kSlice), units = int((g.k + 15) / 16);
-    const auto issue = [&](int s, int buf) {
-        s = s < steps ? s : steps - 1;  // (past the end: again, so that the count of loads stays)
-        const uint32_t lds = lds0 + buf * S::kStage;
-        const int8_t *sa = pa + int64_t(s) * S::kSlice, *sw = pw + int64_t(s) * S::kSlice;
-        if (s < whole) {
-#pragma unroll
-            for (int q = 0; q < S::kLoads; q++) lds_load(lds + 1024 * (w + q * S::NW), at[q], q < S::kLoadsA ? sa : sw);
-        } else {
-#pragma unroll
-            for (int q = 0; q < S::kLoads; q++) {
-                const int8_t *p = (q < S::kLoadsA ? sa : sw) + at[q];
-                lds_load(lds + 1024 * (w + q * S::NW), KU * s + unit[q] < units ? static_cast<const void *>(p) : g_lin_zero);
-            }
+    const int frow = lane & 31, hi = lane >> 5;
+    const auto scales = [&] {
+        for (int i = threadIdx.x; i < BM; i += S::NT) par_a[i] = m0 + i < g.m ? g.sa[m0 + i] : T(0);
+        for (int i = threadIdx.x; i < BN; i += S::NT) {
+            par_w[i] = n0 + i < g.n ? g.sw[n0 + i] : T(0);
+            par_b[i] = g.bias && n0 + i < g.n ? g.bias[n0 + i] : T(0);
         }
     };
-    const int frow = lane & 31, fsw = swz(frow), hi = lane >> 5;
     i32x16 acc[TM][TN];
 #pragma unroll
     for (int i = 0; i < TM; i++)
 #pragma unroll
         for (int j = 0; j < TN; j++) acc[i][j] = i32x16{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
-    i32x4 fa[2][TM], fw[2][TN];
-    const auto read = [&](int buf, int c) {
-        const int8_t *p = smem + buf * S::kStage + frow * S::kSlice + (((2 * c + hi) ^ fsw) * 16);
-#pragma unroll
-        for (int i = 0; i < TM; i++) fa[c & 1][i] = *reinterpret_cast<const i32x4 *>(p + (wr + 32 * i) * S::kSlice);
-#pragma unroll
-        for (int j = 0; j < TN; j++) fw[c & 1][j] = *reinterpret_cast<const i32x4 *>(p + (BM + wc + 32 * j) * S::kSlice);
+    // the block's registers of a part: 16 bytes a lane side by side
+    const auto at_part = [&](int p, int q) {
+        return parts + (((tile - b_base) * splits + p) * S::NW + w) * int64_t(TM * TN * 4 * 64) + q * 64 + lane;
     };
-    const auto multiply = [&](int c) {
+    if constexpr (MODE == LIN_JOIN) {
+        scales();
+#pragma unroll 1
+        for (int p = 0; p < splits; p++)
+#pragma unroll
+            for (int i = 0; i < TM; i++)
+#pragma unroll
+                for (int j = 0; j < TN; j++)
+#pragma unroll
+                    for (int v = 0; v < 4; v++) {
+                        const i32x4 c = *at_part(p, (i * TN + j) * 4 + v);
+#pragma unroll
+                        for (int e = 0; e < 4; e++) acc[i][j][4 * v + e] += c[e];
+                    }
+        __syncthreads();
+    } else {
+        // LDS rows of KU units of 16 bytes; unit u of row r lies at u ^ swz(r), so that the sixteen
+        // lanes of a 16-byte read that go at once cover the 64 banks once.  A load puts lane l's
+        // unit at place l % KU of row l / KU: it fetches the unit that belongs there.
+        const auto swz = [](int r) { return KU == 4 ? r >> 2 & 3 : r >> 1 & 7; };
+        const uint32_t lds0 = uint32_t(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) int8_t *)smem));
+        uint32_t at[S::kLoads];
+        int unit[S::kLoads];
+#pragma unroll
+        for (int q = 0; q < S::kLoads; q++) {
+            const bool of_a = q < S::kLoadsA;
+            const int r = (w + (of_a ? q : q - S::kLoadsA) * S::NW) * S::kRows + lane / KU;
+            const int64_t last = of_a ? g.m - 1 - m0 : g.n - 1 - n0;
+            unit[q] = (lane % KU) ^ swz(r);
+            at[q] = uint32_t((r < last ? r : last) * (of_a ? g.lda : g.ldw) + 16 * unit[q]);
+        }
+        const int8_t *pa = g.a + m0 * g.lda, *pw = g.w + n0 * g.ldw;
+        const int all = int((g.k + S::kSlice - 1) / S::kSlice), whole = int(g.k / S::kSlice), units = int((g.k + 15) / 16);
+        const int begin = MODE == LIN_PART ? all * split / splits : 0;
+        const int steps = MODE == LIN_PART ? all * (split + 1) / splits : all;
+        const auto issue = [&](int s, int buf) {
+            s = s < steps ? s : steps - 1;  // (past the end: again, so that the count of loads stays)
+            const uint32_t lds = lds0 + buf * S::kStage;
+            const int8_t *sa = pa + int64_t(s) * S::kSlice, *sw = pw + int64_t(s) * S::kSlice;
+            if (s < whole) {
+#pragma unroll
+                for (int q = 0; q < S::kLoads; q++) lds_load(lds + 1024 * (w + q * S::NW), at[q], q < S::kLoadsA ? sa : sw);
+            } else {
+#pragma unroll
+                for (int q = 0; q < S::kLoads; q++) {
+                    const int8_t *p = (q < S::kLoadsA ? sa : sw) + at[q];
+                    lds_load(lds + 1024 * (w + q * S::NW),
+                             KU * s + unit[q] < units ? static_cast<const void *>(p) : g_lin_zero);
+                }
+            }
+        };
+        const int fsw = swz(frow);
+        i32x4 fa[2][TM], fw[2][TN];
+        const auto read = [&](int buf, int c) {
+            const int8_t *p = smem + buf * S::kStage + frow * S::kSlice + (((2 * c + hi) ^ fsw) * 16);
+#pragma unroll
+            for (int i = 0; i < TM; i++) fa[c & 1][i] = *reinterpret_cast<const i32x4 *>(p + (wr + 32 * i) * S::kSlice);
+#pragma unroll
+            for (int j = 0; j < TN; j++) fw[c & 1][j] = *reinterpret_cast<const i32x4 *>(p + (BM + wc + 32 * j) * S::kSlice);
+        };
+        const auto multiply = [&](int c) {
+#pragma unroll
+            for (int i = 0; i < TM; i++)
+#pragma unroll
+                for (int j = 0; j < TN; j++)
+                    acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fw[c & 1][j], fa[c & 1][i], acc[i][j], 0, 0, 0);
+        };
+#pragma unroll
+        for (int s = 0; s < ST; s++) issue(begin + s, s);
+        if constexpr (MODE == LIN_WHOLE) scales();
+        wait_and_meet<0>();
+        read(0, 0);
+        int cur = 0;
+        for (int s = begin; s < steps; s++) {
+            // Slice s, its first chunk of 32 codes in registers already.
+#pragma unroll
+            for (int c = 0; c + 1 < C; c++) {
+                read(cur, c + 1);
+                __builtin_amdgcn_sched_barrier(0);
+                multiply(c);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            // Slice s + 1 is there, and every wave has read all of slice s: its buffer is free.
+            wait_and_meet<S::kLoads *(ST - 2)>();
+            const int next = cur + 1 == ST ? 0 : cur + 1;
+            read(next, 0);
+            issue(s + ST, cur);
+            __builtin_amdgcn_sched_barrier(0);
+            multiply(C - 1);
+            __builtin_amdgcn_sched_barrier(0);
+            cur = next;
+        }
+        wait_and_meet<0>();
+    }
+    if constexpr (MODE == LIN_PART) {
 #pragma unroll
         for (int i = 0; i < TM; i++)
 #pragma unroll
             for (int j = 0; j < TN; j++)
-                acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fw[c & 1][j], fa[c & 1][i], acc[i][j], 0, 0, 0);
-    };
 #pragma unroll
-    for (int s = 0; s < ST; s++) issue(s, s);
-    for (int i = threadIdx.x; i < BM; i += S::NT) par_a[i] = m0 + i < g.m ? g.sa[m0 + i] : T(0);
-    for (int i = threadIdx.x; i < BN; i += S::NT) {
-        par_w[i] = n0 + i < g.n ? g.sw[n0 + i] : T(0);
-        par_b[i] = g.bias && n0 + i < g.n ? g.bias[n0 + i] : T(0);
+                for (int v = 0; v < 4; v++)
+                    *at_part(split, (i * TN + j) * 4 + v) =
+                        i32x4{acc[i][j][4 * v], acc[i][j][4 * v + 1], acc[i][j][4 * v + 2], acc[i][j][4 * v + 3]};
+        return;
     }
-    wait_and_meet<0>();
-    read(0, 0);
-    int cur = 0;
-    for (int s = 0; s < steps; s++) {
-        // Slice s, its first chunk of 32 codes in registers already.
-#pragma unroll
-        for (int c = 0; c + 1 < C; c++) {
-            read(cur, c + 1);
-            __builtin_amdgcn_sched_barrier(0);
-            multiply(c);
-            __builtin_amdgcn_sched_barrier(0);
-        }
-        // Slice s + 1 is there, and every wave has read all of slice s: its buffer is free.
-        wait_and_meet<S::kLoads *(ST - 2)>();
-        const int next = cur + 1 == ST ? 0 : cur + 1;
-        read(next, 0);
-        issue(s + ST, cur);
-        __builtin_amdgcn_sched_barrier(0);
-        multiply(C - 1);
-        __builtin_amdgcn_sched_barrier(0);
-        cur = next;
-    }
-    wait_and_meet<0>();
 
     // The epilogue: a wave's results go through its own part of LDS, 32 rows at a time, so that a
     // lane has four columns side by side.  Result v of lane l is column 8 (v / 4) + 4 (l / 32) + v %
@@ -355,48 +407,197 @@ __global__ __launch_bounds__(S::NT, S::PER_SIMD) void k_lin_mfma(LinArgs<T> g, i
     }
 }
 
-template <typename T, typename S>
-static void launch_lin_mfma(const LinArgs<T> &g)
+// ---- few rows ------------------------------------------------------------------------------------
+
+// 16 codes of a row from place k, at any address; zeros past the row's end.
+NH_DEV i32x4 lin_unit(const int8_t *row, int64_t k, int64_t end)
 {
-    const int64_t nbm = ceil_div(g.m, S::BM), nbn = ceil_div(g.n, S::BN);
-    for_row_launches(nbm * nbn, 1, S::NT, [&](unsigned blocks, int64_t base) {
-        NH_LAUNCH((k_lin_mfma<T, S>), dim3(blocks), dim3(S::NT), 0, stream(), g, nbm, nbn, base);
-    });
+    typedef int W __attribute__((ext_vector_type(4), aligned(1)));
+    i32x4 v{0, 0, 0, 0};
+    if (k + 16 <= end) {
+        v = *reinterpret_cast<const W *>(row + k);
+    } else if (k < end) {
+        int8_t b[16];
+#pragma unroll
+        for (int q = 0; q < 16; q++) b[q] = k + q < end ? row[k + q] : int8_t(0);
+        __builtin_memcpy(&v, b, 16);
+    }
+    return v;
 }
 
-// A's or W's rows for the matrix instructions: in place, or copied to `pad` (lin_pad_bytes).
+// Up to 16 rows: the weights are read once and are what the time goes to.  A block takes 16 output
+// channels; its 8 waves share out the depth, each with UN slices of 64 codes in flight from memory
+// to registers, and add up in LDS.  Rows and weights may lie at any address.  1 x 4096 -> 4096 5.3
+// us (a launch alone 3.5; 64 x 64 tiles 11.2), 16 rows 6.6, 1 x 16384 -> 4096 12.6 (5.3 TB/s; 31).
+template <typename T>
+__global__ __launch_bounds__(512) void k_lin_few(LinArgs<T> g, int64_t b_base)
+{
+    constexpr int W = 8, UN = 8;
+    __shared__ i32x4 part[W][64];
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t n0 = (b_base + int64_t(blockIdx.x)) * 16;
+    const int r = lane & 15, u = lane >> 4;
+    const int8_t *pw = g.w + (n0 + r < g.n ? n0 + r : g.n - 1) * g.ldw, *pa = g.a + (r < g.m ? r : g.m - 1) * g.lda;
+    i32x4 acc{0, 0, 0, 0};
+    const int64_t slices = (g.k + 63) / 64, s0 = slices * w / W, s1 = slices * (w + 1) / W;
+    for (int64_t s = s0; s < s1; s += UN) {
+        i32x4 vw[UN], va[UN];
+        const bool inside = (s + UN) * 64 <= g.k && s + UN <= s1;  // uniform
+#pragma unroll
+        for (int q = 0; q < UN; q++) {
+            const int64_t k = (s + q) * 64 + 16 * u, end = inside ? INT64_MAX : s + q < s1 ? g.k : 0;
+            vw[q] = lin_unit(pw, k, end);
+            va[q] = lin_unit(pa, k, end);
+        }
+#pragma unroll
+        for (int q = 0; q < UN; q++) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(vw[q], va[q], acc, 0, 0, 0);
+    }
+    part[w][lane] = acc;
+    __syncthreads();
+    // result v of lane l: row l % 16, channel 4 (l / 16) + v
+    if (w > 0) return;
+#pragma unroll
+    for (int q = 1; q < W; q++) acc += part[q][lane];
+    const int64_t m = r, n = n0 + 4 * u;
+    if (m < g.m && n < g.n) {
+        const T sa = g.sa[m];
+        T z[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            z[e] = n + e < g.n ? lin_value<T>(acc[e], sa, g.sw[n + e], g.bias ? g.bias[n + e] : T(0)) : T(0);
+        act4(z, g.act, g.alpha);
+        const int64_t o = m * g.n + n;
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            if (n + e < g.n) g.out[o + e] = g.res ? z[e] + g.res[o + e] : z[e];
+    }
+}
+
+// ---- the choice --------------------------------------------------------------------------------
+
+// Parts of the depth for few tiles: as many blocks as two a CU, none under 16 slices (2048 codes),
+// and at least 3, as the parts' way through memory and the second launch cost some 4 us: 64 x
+// 16384 -> 4096 32 us whole, 20 in 8 parts; 64 x 4096 -> 4096 11.6 whole, 12.4 in 4; 64 x 4096 ->
+// 16384 14 whole, 18 in 2.
+template <typename S>
+static int lin_splits(int64_t tiles, int64_t k)
+{
+    const int64_t want = int64_t(num_cus()) * 2 / tiles, most = ceil_div(k, S::kSlice) / 16;
+    const int64_t n = want < most ? want : most;
+    return n < 3 ? 1 : int(n);
+}
+
+template <typename T, typename S, bool SPLIT>
+static int launch_lin_mfma(const LinArgs<T> &g, int8_t *scratch, int splits)
+{
+    const int64_t nbm = ceil_div(g.m, S::BM), nbn = ceil_div(g.n, S::BN);
+    i32x4 *parts = reinterpret_cast<i32x4 *>(scratch);
+    if constexpr (SPLIT) {
+        if (splits > 1) {  // (few tiles: one launch each)
+            const unsigned tiles = unsigned(nbm * nbn);
+            NH_LAUNCH((k_lin_mfma<T, S, LIN_PART>), dim3(tiles * unsigned(splits)), dim3(S::NT), 0, stream(), g, nbm, nbn,
+                      int64_t(0), parts, splits);
+            NH_LAUNCH((k_lin_mfma<T, S, LIN_JOIN>), dim3(tiles), dim3(S::NT), 0, stream(), g, nbm, nbn, int64_t(0), parts,
+                      splits);
+            return check_launch();
+        }
+    }
+    for_row_launches(nbm * nbn, 1, S::NT, [&](unsigned blocks, int64_t base) {
+        NH_LAUNCH((k_lin_mfma<T, S, LIN_WHOLE>), dim3(blocks), dim3(S::NT), 0, stream(), g, nbm, nbn, base, parts, 1);
+    });
+    return check_launch();
+}
+
+// Bytes of the copy of A or W that the matrix instructions' loads need, 0: read in place.
 static size_t lin_pad_bytes(const int8_t *p, int64_t ld, int64_t rows, int64_t k, bool whole_units)
 {
     const bool fits = ((reinterpret_cast<uintptr_t>(p) | uintptr_t(ld)) & 15) == 0 && ld < kLinMaxLd;
     return fits && (!whole_units || (k & 15) == 0) ? 0 : size_t(rows) * size_t((k + 63) / 64 * 64);
 }
-static void lin_pad(const int8_t *&p, int64_t &ld, int64_t rows, int64_t k, int8_t *pad)
-{
-    const int64_t ldd = (k + 63) / 64 * 64, need = ceil_div(rows * (ldd / 16), 256);
-    NH_LAUNCH(k_lin_pad, dim3(unsigned(need < kMaxGridBlocks ? need : kMaxGridBlocks)), dim3(256), 0, stream(), p, ld, pad,
-              ldd, rows, k);
-    p = pad;
-    ld = ldd;
-}
 
-template <typename T>
-static int launch_linear(LinArgs<T> g)
+// The product on shape S: copies of what cannot be read in place, parts of the depth where S may be
+// split and has few tiles.
+template <typename T, typename S, bool SPLIT>
+static int launch_lin_shape(LinArgs<T> g)
 {
     // (where k ends inside a unit of 16, A's bytes past it must be zeros; W's then do not matter)
     const size_t ba = lin_pad_bytes(g.a, g.lda, g.m, g.k, true), bw = lin_pad_bytes(g.w, g.ldw, g.n, g.k, false);
-    Partials pad;  // (one block: a captured call's blocks share memory)
-    if (ba + bw) NH_TRY(pad.open(ba + bw));
-    if (ba) lin_pad(g.a, g.lda, g.m, g.k, static_cast<int8_t *>(pad.p));
-    if (bw) lin_pad(g.w, g.ldw, g.n, g.k, static_cast<int8_t *>(pad.p) + ba);
-    if constexpr (sizeof(T) == 8) {
-        launch_lin_mfma<T, LinShape<2, 2, 2, 2, 8, 3, 2>>(g);
-    } else {
-        const int64_t large = ceil_div(g.m, 256) * ceil_div(g.n, 256);
-        if (g.m <= 128) launch_lin_mfma<T, LinShape<2, 2, 1, 2, 4, 4, 2>>(g);
-        else if (large >= num_cus() * 5 / 8) launch_lin_mfma<T, LinShape<2, 4, 4, 2, 8, 2, 2>>(g);
-        else launch_lin_mfma<T, LinShape<2, 2, 2, 2, 4, 4, 2>>(g);
+    const int64_t tiles = ceil_div(g.m, S::BM) * ceil_div(g.n, S::BN);
+    const int splits = SPLIT ? lin_splits<S>(tiles, g.k) : 1;
+    const size_t bp = splits > 1 ? size_t(tiles) * size_t(splits) * size_t(S::BM * S::BN * 4) : 0;
+    Partials block;  // (one: a captured call's blocks share memory)
+    if (bp + ba + bw) NH_TRY(block.open(bp + ba + bw));
+    int8_t *mem = static_cast<int8_t *>(block.p);
+    if (ba + bw) {
+        const int64_t ldd = (g.k + 63) / 64 * 64;
+        const LinPad a{g.a, mem + bp, g.lda, ba ? g.m : 0}, w{g.w, mem + bp + ba, g.ldw, bw ? g.n : 0};
+        const int64_t need = ceil_div((a.rows + w.rows) * (ldd / 16), 256);
+        NH_LAUNCH(k_lin_pad, dim3(unsigned(need < kMaxGridBlocks ? need : kMaxGridBlocks)), dim3(256), 0, stream(), a, w, ldd,
+                  g.k);
+        if (ba) {
+            g.a = a.dst;
+            g.lda = ldd;
+        }
+        if (bw) {
+            g.w = w.dst;
+            g.ldw = ldd;
+        }
     }
-    return check_launch();
+    return launch_lin_mfma<T, S, SPLIT>(g, mem, splits);
+}
+
+// By the cost of each shape, in us for a depth of 4096 as measured here: the most tiles that fall to
+// one CU at what one costs it alone, or all tiles at what they cost when every CU works.  A small
+// tile answers sooner where there are few of them, a large one reads less for each product:
+// 300 x 4096 -> 4096 15 us on 64 x 64 tiles, 25 on 128 x 128, 54 on 256 x 256; 1024 rows 33, 27,
+// 54; 2048 rows 58, 42, 55 and 40 on 128 x 256; 4096 rows 110, 93, 71 on 256 x 256.
+struct LinCost {
+    double per_cu, fixed, all;  // all: per 64 x 64 of results
+};
+template <typename S>
+static double lin_cost(int64_t m, int64_t n, const LinCost &c)
+{
+    const int64_t tiles = ceil_div(m, S::BM) * ceil_div(n, S::BN);
+    const double alone = c.fixed + c.per_cu * double(ceil_div(tiles, num_cus()));
+    const double all = c.all * double(tiles) * double(S::BM * S::BN / 4096) * (256.0 / num_cus());
+    return alone > all ? alone : all;
+}
+
+template <typename T>
+static int launch_linear(const LinArgs<T> &g)
+{
+    // (wider, 64 x 64 tiles stream better: 1 x 4096 -> 16384 15.9 us, 13.3 by tiles)
+    if (g.m <= 16 && ceil_div(g.n, 16) <= int64_t(num_cus()) * 2) {
+        for_row_launches(ceil_div(g.n, 16), 1, 512, [&](unsigned blocks, int64_t base) {
+            NH_LAUNCH((k_lin_few<T>), dim3(blocks), dim3(512), 0, stream(), g, base);
+        });
+        return check_launch();
+    }
+    using S64 = LinShape<2, 2, 1, 1, 8, 3, 2>;
+    if constexpr (sizeof(T) == 8) {  // (its epilogue takes twice the LDS: two shapes)
+        using S128 = LinShape<2, 2, 2, 2, 8, 3, 1>;
+        return ceil_div(g.m, 128) * ceil_div(g.n, 128) >= 2 * num_cus() ? launch_lin_shape<T, S128, false>(g)
+                                                                       : launch_lin_shape<T, S64, true>(g);
+    } else {
+        using S128x64 = LinShape<2, 2, 2, 1, 8, 3, 2>;
+        using S128 = LinShape<2, 2, 2, 2, 8, 2, 2>;
+        using S128x256 = LinShape<2, 4, 2, 2, 8, 3, 2>;
+        using S256 = LinShape<2, 4, 4, 2, 8, 2, 2>;
+        const double cost[] = {lin_cost<S64>(g.m, g.n, {7.0, 4.0, 0.028}), lin_cost<S128x64>(g.m, g.n, {10.0, 8.0, 0.025}),
+                               lin_cost<S128>(g.m, g.n, {17.0, 9.0, 0.0205}),
+                               lin_cost<S128x256>(g.m, g.n, {34.0, 5.0, 0.0194}),
+                               lin_cost<S256>(g.m, g.n, {50.0, 4.0, 0.0173})};
+        int best = 0;
+        for (int i = 1; i < 5; i++)
+            if (cost[i] < cost[best]) best = i;
+        switch (best) {
+        case 0: return launch_lin_shape<T, S64, true>(g);
+        case 1: return launch_lin_shape<T, S128x64, false>(g);
+        case 2: return launch_lin_shape<T, S128, false>(g);
+        case 3: return launch_lin_shape<T, S128x256, false>(g);
+        default: return launch_lin_shape<T, S256, false>(g);
+        }
+    }
 }
 
 // ---- arguments -----------------------------------------------------------------------------

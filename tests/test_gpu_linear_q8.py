@@ -127,6 +127,19 @@ def test_larger(pn, rng, m, k, n):
 
 
 @pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("m,k,n", [(16, 100, 8192), (16, 100, 8193), (17, 6143, 70), (17, 6145, 70), (33, 8192, 65), (64, 8209, 130),
+                                   (100, 20000, 300), (20, 131071, 33), (512, 300, 4096), (513, 300, 4097), (1024, 272, 4096),
+                                   (1100, 272, 4100), (2048, 272, 4096), (2049, 129, 4097), (4096, 130, 4096), (4000, 64, 4200)])
+def test_forms(pn, rng, dt, m, k, n):
+    """Sizes around the changes of form: few rows, depth in parts, every tile; epilogue and copies of
+    each."""
+    c = _case(rng, m, k, n, dt)
+    _check(pn, c)
+    ld = -(-k // 16) * 16
+    _check(pn, c, res=False, lda=ld, ldw=ld)
+
+
+@pytest.mark.parametrize("dt", DT)
 @pytest.mark.parametrize("act", range(13))
 def test_activations(pn, rng, dt, act):
     """Every activation, with every part of the epilogue there or not, over the values that the
@@ -266,7 +279,7 @@ def test_refusals(pn):
     assert not t.cpu().numpy().any()
 
 
-@pytest.mark.parametrize("m,k,n", [(1, 700, 500), (40, 1001, 300), (500, 1001, 300)])
+@pytest.mark.parametrize("m,k,n", [(1, 700, 500), (40, 1001, 300), (40, 8209, 300), (500, 1001, 300)])
 def test_graphs_and_streams(pn, rng, m, k, n):
     """Two captured products on two streams (unaligned rows, which are copied first: each graph
     its own memory), replayed at once, with eager calls in between."""
