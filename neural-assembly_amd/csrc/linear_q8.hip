@@ -66,31 +66,36 @@ typedef int i32x16 __attribute__((ext_vector_type(16)));
 constexpr int64_t kLinMaxLd = int64_t(1) << 22;  // 256 rows of it stay in a 32-bit offset
 
 // Rows of codes copied to rows of `ldd` bytes (a multiple of 16) at an aligned address, the bytes
-// past k zero.  A lane takes 16 bytes.
+// past k zero.  A wave takes 64 units of 16 bytes of a row.
 struct LinPad {
     const int8_t *src;
     int8_t *dst;
     int64_t ld, rows;  // rows 0: nothing to copy
 };
-__global__ __launch_bounds__(256) void k_lin_pad(LinPad a, LinPad w, int64_t ldd, int64_t k)
+__global__ __launch_bounds__(256) void k_lin_pad(LinPad a, LinPad w, int ldd, int k)
 {
     typedef int W __attribute__((ext_vector_type(4), aligned(1)));
-    const int64_t units = ldd / 16, step = int64_t(gridDim.x) * 256, first = a.rows * units;
-    for (int64_t t0 = int64_t(blockIdx.x) * 256 + threadIdx.x; t0 < first + w.rows * units; t0 += step) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t parts = (ldd / 16 + 63) / 64;
+    const int64_t first = a.rows * parts, end = first + w.rows * parts;
+    for (int64_t t0 = int64_t(blockIdx.x) * 4 + wave; t0 < end; t0 += int64_t(gridDim.x) * 4) {
         const bool of_a = t0 < first;
         const LinPad &p = of_a ? a : w;
-        const int64_t t = of_a ? t0 : t0 - first, r = t / units, u = t - r * units;
-        const int8_t *src = p.src + r * p.ld + 16 * u;
+        const uint64_t t = t0 - (of_a ? 0 : first);
+        const int64_t r = t >> 32 ? t / parts : uint32_t(t) / parts;
+        const int at = 16 * (64 * int(t - r * parts) + lane);
+        if (at >= ldd) continue;
+        const int8_t *src = p.src + r * p.ld + at;
         i32x4 v;
-        if (16 * u + 16 <= k) {
+        if (at + 16 <= k) {
             v = *reinterpret_cast<const W *>(src);
         } else {
             int8_t b[16];
 #pragma unroll
-            for (int q = 0; q < 16; q++) b[q] = 16 * u + q < k ? src[q] : int8_t(0);
+            for (int q = 0; q < 16; q++) b[q] = at + q < k ? src[q] : int8_t(0);
             __builtin_memcpy(&v, b, 16);
         }
-        *reinterpret_cast<i32x4 *>(p.dst + r * ldd + 16 * u) = v;
+        *reinterpret_cast<i32x4 *>(p.dst + r * ldd + at) = v;
     }
 }
 
@@ -531,9 +536,9 @@ static int launch_lin_shape(LinArgs<T> g)
     if (ba + bw) {
         const int64_t ldd = (g.k + 63) / 64 * 64;
         const LinPad a{g.a, mem + bp, g.lda, ba ? g.m : 0}, w{g.w, mem + bp + ba, g.ldw, bw ? g.n : 0};
-        const int64_t need = ceil_div((a.rows + w.rows) * (ldd / 16), 256);
-        NH_LAUNCH(k_lin_pad, dim3(unsigned(need < kMaxGridBlocks ? need : kMaxGridBlocks)), dim3(256), 0, stream(), a, w, ldd,
-                  g.k);
+        const int64_t need = ceil_div((a.rows + w.rows) * ceil_div(ldd, 1024), 4);
+        NH_LAUNCH(k_lin_pad, dim3(unsigned(need < kMaxGridBlocks ? need : kMaxGridBlocks)), dim3(256), 0, stream(), a, w,
+                  int(ldd), int(g.k));
         if (ba) {
             g.a = a.dst;
             g.lda = ldd;
