@@ -458,9 +458,10 @@ int neural_dropout_add_layer_norm_backward(NeuralTensor *grad_in, NeuralTensor *
  * exact; its scaling and the bias are taken in double and rounded to the dtype, then the
  * activation as neural_bias_add_act takes it (act, alpha: there), then the residual is added.
  * bias, residual: may be NULL; out may be residual.  1 <= k <= 131071 (a sum stays below
- * 2^31; more: NEURAL_ERR_TENSOR_TOO_LARGE).  Any strides and addresses are taken; codes and
- * weights at 16-byte aligned addresses with strides that are multiples of 16 are read in place,
- * others are copied first.
+ * 2^31; more: NEURAL_ERR_TENSOR_TOO_LARGE).  Any strides and addresses are taken; rows at
+ * 16-byte aligned addresses with strides that are multiples of 16 are read fastest.  For others,
+ * where there are more than a few rows, and for long depths with few results the call takes
+ * device memory, as neural_layer_norm_backward.
  *
  * Errors: NULL_POINTER, DTYPE_MISMATCH, DIM_MISMATCH (a 0-d tensor), SHAPE_MISMATCH,
  * INVALID_ARGUMENT (non-contiguous tensors, eps negative or not finite, a stride less than the

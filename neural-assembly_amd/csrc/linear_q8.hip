@@ -21,6 +21,7 @@ struct LinArgs {
     int64_t m, n, k;
     int act;
     double alpha;
+    bool cut;  // k ends inside a unit of 16 bytes of A's rows, and other bytes follow it
 };
 
 // The activation of four values, by neural_bias_add_act's functors: the branch is taken once.
@@ -99,6 +100,22 @@ __global__ __launch_bounds__(256) void k_lin_pad(LinPad a, LinPad w, int ldd, in
     }
 }
 
+// 16 codes of a row from place k, at any address; zeros past the row's end.
+NH_DEV i32x4 lin_unit(const int8_t *row, int64_t k, int64_t end)
+{
+    typedef int W __attribute__((ext_vector_type(4), aligned(1)));
+    i32x4 v{0, 0, 0, 0};
+    if (k + 16 <= end) {
+        v = *reinterpret_cast<const W *>(row + k);
+    } else if (k < end) {
+        int8_t b[16];
+#pragma unroll
+        for (int q = 0; q < 16; q++) b[q] = k + q < end ? row[k + q] : int8_t(0);
+        __builtin_memcpy(&v, b, 16);
+    }
+    return v;
+}
+
 // What lanes fetch in the place of units past the rows' end.
 __device__ const int g_lin_zero[4] = {0, 0, 0, 0};
 
@@ -134,6 +151,7 @@ struct LinShape {
     static constexpr int kOut = 32 * TN + 4;                             // the epilogue's rows of a wave
     static_assert(BM % (kRows * NW) == 0 && BN % (kRows * NW) == 0, "whole loads per wave");
     static constexpr int kLoadsA = BM / kRows / NW;
+    static constexpr bool kCut = TM * TN == 1;  // (of larger tiles the registers for it would spill)
 };
 
 // Tile of block `h` of nbm x nbn: the hardware deals blocks to the 8 XCDs in turn, each with its own
@@ -223,20 +241,35 @@ __global__ __launch_bounds__(S::NT, S::PER_SIMD) void k_lin_mfma(LinArgs<T> g, i
         const int all = int((g.k + S::kSlice - 1) / S::kSlice), whole = int(g.k / S::kSlice), units = int((g.k + 15) / 16);
         const int begin = MODE == LIN_PART ? all * split / splits : 0;
         const int steps = MODE == LIN_PART ? all * (split + 1) / splits : all;
+        // past the end: a slice again, so that the count of loads stays
+        const int past = S::kCut && steps - begin > 1 ? steps - 2 : steps - 1;
         const auto issue = [&](int s, int buf) {
-            s = s < steps ? s : steps - 1;  // (past the end: again, so that the count of loads stays)
+            s = s < steps ? s : past;
             const uint32_t lds = lds0 + buf * S::kStage;
             const int8_t *sa = pa + int64_t(s) * S::kSlice, *sw = pw + int64_t(s) * S::kSlice;
             if (s < whole) {
 #pragma unroll
                 for (int q = 0; q < S::kLoads; q++) lds_load(lds + 1024 * (w + q * S::NW), at[q], q < S::kLoadsA ? sa : sw);
-            } else {
+                return;
+            }
+            // Where k ends inside a unit of A's rows in place, they go through registers, which
+            // leave out what lies behind it (W's is then multiplied by zeros).  All loads before
+            // have then ended.
+            const bool inside = S::kCut && g.cut;
+            if (inside) {
 #pragma unroll
-                for (int q = 0; q < S::kLoads; q++) {
-                    const int8_t *p = (q < S::kLoadsA ? sa : sw) + at[q];
-                    lds_load(lds + 1024 * (w + q * S::NW),
-                             KU * s + unit[q] < units ? static_cast<const void *>(p) : g_lin_zero);
+                for (int q = 0; q < S::kLoadsA; q++) {
+                    const i32x4 v = lin_unit(sa + at[q] - 16 * unit[q], 16 * unit[q], g.k - int64_t(s) * S::kSlice);
+                    *reinterpret_cast<i32x4 *>(smem + buf * S::kStage + 1024 * (w + q * S::NW) + 16 * lane) = v;
                 }
+                asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
+            }
+#pragma unroll
+            for (int q = 0; q < S::kLoads; q++) {
+                if (inside && q < S::kLoadsA) continue;
+                const int8_t *p = (q < S::kLoadsA ? sa : sw) + at[q];
+                lds_load(lds + 1024 * (w + q * S::NW),
+                         KU * s + unit[q] < units ? static_cast<const void *>(p) : g_lin_zero);
             }
         };
         const int fsw = swz(frow);
@@ -414,22 +447,6 @@ __global__ __launch_bounds__(S::NT, S::PER_SIMD) void k_lin_mfma(LinArgs<T> g, i
 
 // ---- few rows ------------------------------------------------------------------------------------
 
-// 16 codes of a row from place k, at any address; zeros past the row's end.
-NH_DEV i32x4 lin_unit(const int8_t *row, int64_t k, int64_t end)
-{
-    typedef int W __attribute__((ext_vector_type(4), aligned(1)));
-    i32x4 v{0, 0, 0, 0};
-    if (k + 16 <= end) {
-        v = *reinterpret_cast<const W *>(row + k);
-    } else if (k < end) {
-        int8_t b[16];
-#pragma unroll
-        for (int q = 0; q < 16; q++) b[q] = k + q < end ? row[k + q] : int8_t(0);
-        __builtin_memcpy(&v, b, 16);
-    }
-    return v;
-}
-
 // Up to 16 rows: the weights are read once and are what the time goes to.  A block takes 16 output
 // channels; its 8 waves share out the depth, each with UN slices of 64 codes in flight from memory
 // to registers, and add up in LDS.  Rows and weights may lie at any address.  1 x 4096 -> 4096 5.3
@@ -492,49 +509,28 @@ static int lin_splits(int64_t tiles, int64_t k)
     return n < 3 ? 1 : int(n);
 }
 
-template <typename T, typename S, bool SPLIT>
-static int launch_lin_mfma(const LinArgs<T> &g, int8_t *scratch, int splits)
+// Rows that go straight to LDS, without a copy.
+static bool lin_in_place(const int8_t *p, int64_t ld)
 {
-    const int64_t nbm = ceil_div(g.m, S::BM), nbn = ceil_div(g.n, S::BN);
-    i32x4 *parts = reinterpret_cast<i32x4 *>(scratch);
-    if constexpr (SPLIT) {
-        if (splits > 1) {  // (few tiles: one launch each)
-            const unsigned tiles = unsigned(nbm * nbn);
-            NH_LAUNCH((k_lin_mfma<T, S, LIN_PART>), dim3(tiles * unsigned(splits)), dim3(S::NT), 0, stream(), g, nbm, nbn,
-                      int64_t(0), parts, splits);
-            NH_LAUNCH((k_lin_mfma<T, S, LIN_JOIN>), dim3(tiles), dim3(S::NT), 0, stream(), g, nbm, nbn, int64_t(0), parts,
-                      splits);
-            return check_launch();
-        }
-    }
-    for_row_launches(nbm * nbn, 1, S::NT, [&](unsigned blocks, int64_t base) {
-        NH_LAUNCH((k_lin_mfma<T, S, LIN_WHOLE>), dim3(blocks), dim3(S::NT), 0, stream(), g, nbm, nbn, base, parts, 1);
-    });
-    return check_launch();
+    return ((reinterpret_cast<uintptr_t>(p) | uintptr_t(ld)) & 15) == 0 && ld < kLinMaxLd;
 }
 
-// Bytes of the copy of A or W that the matrix instructions' loads need, 0: read in place.
-static size_t lin_pad_bytes(const int8_t *p, int64_t ld, int64_t rows, int64_t k, bool whole_units)
-{
-    const bool fits = ((reinterpret_cast<uintptr_t>(p) | uintptr_t(ld)) & 15) == 0 && ld < kLinMaxLd;
-    return fits && (!whole_units || (k & 15) == 0) ? 0 : size_t(rows) * size_t((k + 63) / 64 * 64);
-}
-
-// The product on shape S: copies of what cannot be read in place, parts of the depth where S may be
-// split and has few tiles.
-template <typename T, typename S, bool SPLIT>
+// The product on shape S: copies of what does not go straight to LDS (through registers, as few
+// rows do, 577 x 1001 -> 3001 in f64 took 22 us for 17), long depths in parts where S is SMALL.
+template <typename T, typename S, bool SMALL>
 static int launch_lin_shape(LinArgs<T> g)
 {
-    // (where k ends inside a unit of 16, A's bytes past it must be zeros; W's then do not matter)
-    const size_t ba = lin_pad_bytes(g.a, g.lda, g.m, g.k, true), bw = lin_pad_bytes(g.w, g.ldw, g.n, g.k, false);
-    const int64_t tiles = ceil_div(g.m, S::BM) * ceil_div(g.n, S::BN);
-    const int splits = SPLIT ? lin_splits<S>(tiles, g.k) : 1;
-    const size_t bp = splits > 1 ? size_t(tiles) * size_t(splits) * size_t(S::BM * S::BN * 4) : 0;
+    const int64_t nbm = ceil_div(g.m, S::BM), nbn = ceil_div(g.n, S::BN), ldd = (g.k + 63) / 64 * 64;
+    g.cut = (g.k & 15) != 0 && lin_in_place(g.a, g.lda);
+    const size_t ba = lin_in_place(g.a, g.lda) && (S::kCut || !g.cut) ? 0 : size_t(g.m) * size_t(ldd);
+    const size_t bw = lin_in_place(g.w, g.ldw) ? 0 : size_t(g.n) * size_t(ldd);
+    const int splits = SMALL ? lin_splits<S>(nbm * nbn, g.k) : 1;
+    const size_t bp = splits > 1 ? size_t(nbm * nbn) * size_t(splits) * size_t(S::BM * S::BN * 4) : 0;
     Partials block;  // (one: a captured call's blocks share memory)
     if (bp + ba + bw) NH_TRY(block.open(bp + ba + bw));
     int8_t *mem = static_cast<int8_t *>(block.p);
+    i32x4 *parts = reinterpret_cast<i32x4 *>(mem);
     if (ba + bw) {
-        const int64_t ldd = (g.k + 63) / 64 * 64;
         const LinPad a{g.a, mem + bp, g.lda, ba ? g.m : 0}, w{g.w, mem + bp + ba, g.ldw, bw ? g.n : 0};
         const int64_t need = ceil_div((a.rows + w.rows) * ceil_div(ldd, 1024), 4);
         NH_LAUNCH(k_lin_pad, dim3(unsigned(need < kMaxGridBlocks ? need : kMaxGridBlocks)), dim3(256), 0, stream(), a, w,
@@ -548,7 +544,20 @@ static int launch_lin_shape(LinArgs<T> g)
             g.ldw = ldd;
         }
     }
-    return launch_lin_mfma<T, S, SPLIT>(g, mem, splits);
+    if constexpr (SMALL) {
+        if (splits > 1) {  // (few tiles: one launch each)
+            const unsigned tiles = unsigned(nbm * nbn);
+            NH_LAUNCH((k_lin_mfma<T, S, LIN_PART>), dim3(tiles * unsigned(splits)), dim3(S::NT), 0, stream(), g, nbm, nbn,
+                      int64_t(0), parts, splits);
+            NH_LAUNCH((k_lin_mfma<T, S, LIN_JOIN>), dim3(tiles), dim3(S::NT), 0, stream(), g, nbm, nbn, int64_t(0), parts,
+                      splits);
+            return check_launch();
+        }
+    }
+    for_row_launches(nbm * nbn, 1, S::NT, [&](unsigned blocks, int64_t base) {
+        NH_LAUNCH((k_lin_mfma<T, S, LIN_WHOLE>), dim3(blocks), dim3(S::NT), 0, stream(), g, nbm, nbn, base, parts, 1);
+    });
+    return check_launch();
 }
 
 // By the cost of each shape, in us for a depth of 4096 as measured here: the most tiles that fall to
@@ -582,7 +591,7 @@ static int launch_linear(const LinArgs<T> &g)
     if constexpr (sizeof(T) == 8) {  // (its epilogue takes twice the LDS: two shapes)
         using S128 = LinShape<2, 2, 2, 2, 8, 3, 1>;
         return ceil_div(g.m, 128) * ceil_div(g.n, 128) >= 2 * num_cus() ? launch_lin_shape<T, S128, false>(g)
-                                                                       : launch_lin_shape<T, S64, true>(g);
+                                                                        : launch_lin_shape<T, S64, true>(g);
     } else {
         using S128x64 = LinShape<2, 2, 2, 1, 8, 3, 2>;
         using S128 = LinShape<2, 2, 2, 2, 8, 2, 2>;
