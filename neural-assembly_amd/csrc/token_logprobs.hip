@@ -287,9 +287,11 @@ struct LpScratch {
 };
 
 // A row is cut into parts of 256 lanes, `per` vectors at most, VPT a lane, or of a wave where it is
-// narrow; a group of NT lanes holds one part in registers: one read.  Each wave takes its own largest value as the reference of its exponentials.
+// narrow; a group of NT lanes holds one part in registers: one read.  Each wave takes its own
+// largest value as the reference of its exponentials.
 // r_base: the launch's first row.  What bounds it where rows are many: HBM, with vector issue
-// at two thirds (f32: about 16 issue slots a value).
+// at two thirds (f32: about 16 issue slots a value; [4096, 50257] 145 us, a copy's rate 137); with
+// alternatives the latency of ordering them (k = 1: 230 us, 20: 269).
 template <typename T, int NT, int VPT, bool TOP>
 __global__ __launch_bounds__(256, TOP ? 4 : 1) void k_lp_parts(LpArgs<T> a, LpScratch<T> scratch, int parts, int64_t per,
                                                                int64_t r_base)
@@ -386,8 +388,9 @@ __global__ __launch_bounds__(256, TOP ? 4 : 1) void k_lp_parts(LpArgs<T> a, LpSc
     __shared__ LpOrder<T, NT> order[TOP ? RPB : 1];
     if constexpr (TOP) {
         // Alternatives of a wave that are many for its lanes: its vectors stand for their values,
-        // not its lanes (k = 64 of 1000: 26 us, by lanes 171, as too much passed the bound).
-        const bool fine = NT == 64 && a.k > NT / 4;
+        // not its lanes (64 rows of 1000, k = 64: 20 us, by lanes 53, as too much passes the bound;
+        // k = 40: 13 both; k = 24: 9.7 and 8.7).
+        const bool fine = NT == 64 && a.k > 40;
         T over = top, scalar = vt;
         T over_v[VPT];
 #pragma unroll
@@ -666,8 +669,8 @@ static void launch_lp_parts(const LpArgs<T> &a, const LpScratch<T> &scratch, int
 
 // By the width alone, so that equal rows have equal results in any batch: a wave up to 256
 // vectors, 256 lanes up to 2048, and beyond parts of that by blocks of their own, joined by a second
-// launch (one block of 1024 for four parts: [64, 32000] with one alternative 22.9 us, two launches
-// 13.5).
+// launch (one block of 1024 for four parts: [64, 32000] with one alternative 22.9 us, where two
+// launches then took 13.5; now 11.6).
 template <typename T>
 static int launch_lp(const LpArgs<T> &a)
 {
