@@ -24,13 +24,13 @@ struct LinArgs {
     bool cut;  // k ends inside a unit of 16 bytes of A's rows, and other bytes follow it
 };
 
-// The activation of four values, by neural_bias_add_act's functors: the branch is taken once.
-template <typename T>
-NH_DEV void act4(T (&z)[4], int act, double alpha)
+// The activation of N values, by neural_bias_add_act's functors: the branch is taken once.
+template <typename T, int N>
+NH_DEV void act_all(T (&z)[N], int act, double alpha)
 {
     const auto each = [&](auto f) {
 #pragma unroll
-        for (int e = 0; e < 4; e++) z[e] = f(z[e]);
+        for (int e = 0; e < N; e++) z[e] = f(z[e]);
     };
     constexpr bool F32 = sizeof(T) == 4;
     switch (act) {
@@ -174,6 +174,10 @@ enum { LIN_WHOLE = 0, LIN_PART = 1, LIN_JOIN = 2 };
 
 // (A's rows are the second operand: a lane's results are of one row of A and, four at a time,
 // consecutive columns.)
+// What bounds it, at 8192 x 4096 -> 16384 on 256 x 256 tiles (541 us, 2.03 POP/s): 54 us of a tile's
+// 67 are its products, at the clock that the power leaves (2.5 POP/s); then all CUs store a tile at
+// once, 11 us at the memory's rate, with the scaling beside it.  gelu adds 6, in vector issue.  The
+// stores straight from the registers, 32 bytes of a row at a time, took 818 us in all.
 template <typename T, typename S, int MODE>
 __global__ __launch_bounds__(S::NT, S::PER_SIMD) void k_lin_mfma(LinArgs<T> g, int64_t nbm, int64_t nbn, int64_t b_base,
                                                                   i32x4 *parts, int splits)
@@ -342,6 +346,7 @@ __global__ __launch_bounds__(S::NT, S::PER_SIMD) void k_lin_mfma(LinArgs<T> g, i
         sw[e] = par_w[wc + 4 * cl + e];
         bias[e] = par_b[wc + 4 * cl + e];
     }
+    constexpr int UA = TM * TN == 1 ? 4 : TM * TN <= 4 ? 2 : 1;  // rows of a turn, as registers allow
     const bool full = n + 4 <= g.n, act = g.act != NEURAL_ACT_NONE;
     const auto sums = [&](int r, int (&c)[4]) {
         const T *p = rows + r * S::kOut + 4 * cl;
@@ -405,15 +410,23 @@ __global__ __launch_bounds__(S::NT, S::PER_SIMD) void k_lin_mfma(LinArgs<T> g, i
         };
         if (act) {  // one copy of the activations' code, so a loop
 #pragma unroll 1
-            for (int r = rl; r < 32; r += RPI) {
-                T z[4];
-                value(r, z);
-                act4(z, g.act, g.alpha);
-                if (!g.res) {
-                    store(mi + r, z);
-                } else {
+            for (int r = rl; r < 32; r += UA * RPI) {
+                T z[UA][4], zz[4 * UA];
 #pragma unroll
-                    for (int e = 0; e < 4; e++) rows[r * S::kOut + 4 * cl + e] = z[e];
+                for (int q = 0; q < UA; q++) value(r + q * RPI, z[q]);
+#pragma unroll
+                for (int q = 0; q < 4 * UA; q++) zz[q] = z[q / 4][q % 4];
+                act_all(zz, g.act, g.alpha);
+#pragma unroll
+                for (int q = 0; q < 4 * UA; q++) z[q / 4][q % 4] = zz[q];
+#pragma unroll
+                for (int q = 0; q < UA; q++) {
+                    if (!g.res) {
+                        store(mi + r + q * RPI, z[q]);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; e++) rows[(r + q * RPI) * S::kOut + 4 * cl + e] = z[q][e];
+                    }
                 }
             }
         }
@@ -487,7 +500,7 @@ __global__ __launch_bounds__(512) void k_lin_few(LinArgs<T> g, int64_t b_base)
 #pragma unroll
         for (int e = 0; e < 4; e++)
             z[e] = n + e < g.n ? lin_value<T>(acc[e], sa, g.sw[n + e], g.bias ? g.bias[n + e] : T(0)) : T(0);
-        act4(z, g.act, g.alpha);
+        act_all(z, g.act, g.alpha);
         const int64_t o = m * g.n + n;
 #pragma unroll
         for (int e = 0; e < 4; e++)

@@ -48,7 +48,9 @@ struct RmsPlan {
 };
 
 // Groups of NT lanes walk the rows, r = group, group + groups, ...: a row is read once, its
-// square sum and its largest |w| taken from the registers by one exchange.  Bound by HBM.
+// square sum and its largest |w| taken from the registers by one exchange.  Bound by HBM: f32
+// [16384, 4096] 85 us, with the residual 175, and to 8 bits 131 (a copy of as many bytes 83, 176,
+// 140); [65536, 1000] 92, 177, 132 (84, 171, 136); [4096, 16384] 94, 190, 152 (86, 176, 140).
 template <typename T, int NT, int VPT, bool ADD, int OUT, bool PAST>
 __global__ __launch_bounds__((RmsPlan<T, NT, VPT, ADD, OUT>::NB), (RmsPlan<T, NT, VPT, ADD, OUT>::kWaves)) void k_rms_rows(
     RmsArgs<T> a, int64_t r_base)
@@ -211,7 +213,8 @@ __global__ __launch_bounds__((RmsPlan<T, NT, VPT, ADD, OUT>::NB), (RmsPlan<T, NT
 }
 
 // Rows wider than a block's registers: two walks of a block, h, its square sum and its
-// largest |w|, then the outputs.
+// largest |w|, then the outputs (f32 [670, 100000] 148 us, with the residual 302, where a copy of
+// the tensors once takes 85 and 175).
 template <typename T, bool ADD, int OUT>
 __global__ __launch_bounds__(kLnWide) void k_rms_wide(RmsArgs<T> a, int64_t r_base)
 {
