@@ -289,8 +289,8 @@ struct LpScratch {
 // A row is cut into parts of 256 lanes, `per` vectors at most, VPT a lane, or of a wave where it is
 // narrow; a group of NT lanes holds one part in registers: one read.  Each wave takes its own
 // largest value as the reference of its exponentials.
-// r_base: the launch's first row.  What bounds it where rows are many: HBM, with vector issue
-// at two thirds (f32: about 16 issue slots a value; [4096, 50257] 145 us, a copy's rate 137); with
+// r_base: the launch's first row.  What bounds it where rows are many: the vector units, with HBM
+// close behind (f32: about 16 issue slots a value; [4096, 50257] 145 us, a copy's rate 137); with
 // alternatives the latency of ordering them (k = 1: 230 us, 20: 269).
 template <typename T, int NT, int VPT, bool TOP>
 __global__ __launch_bounds__(256, TOP ? 4 : 1) void k_lp_parts(LpArgs<T> a, LpScratch<T> scratch, int parts, int64_t per,
