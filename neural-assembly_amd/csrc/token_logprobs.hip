@@ -109,9 +109,14 @@ struct LpRow {
 };
 
 template <typename T>
-NH_DEV void lp_store(const LpArgs<T> &a, int64_t r, int64_t tok, const LpRow &row, double t)
+NH_DEV T lp_logit(const LpArgs<T> &a, int64_t r, int64_t tok)
 {
-    if (a.logprob) a.logprob[r] = tok < a.cols ? T(row.logprob(double(a.x[r * a.cols + tok]))) : T(__builtin_nan(""));
+    return a.logprob && tok < a.cols ? a.x[r * a.cols + tok] : T(0);
+}
+template <typename T>
+NH_DEV void lp_store(const LpArgs<T> &a, int64_t r, int64_t tok, T logit, const LpRow &row, double t)
+{
+    if (a.logprob) a.logprob[r] = tok < a.cols ? T(row.logprob(double(logit))) : T(__builtin_nan(""));
     if (a.entropy) a.entropy[r] = T(row.entropy(t));
     if (a.lse) a.lse[r] = T(row.lse());
 }
@@ -456,7 +461,7 @@ __global__ __launch_bounds__(256, TOP ? 4 : 1) void k_lp_parts(LpArgs<T> a, LpSc
             sum = lp_join_wave(wl < W ? sh[wl < W ? wl : 0] : LpPart{-__builtin_inf(), 0.0, 0.0}, a.inv_t);
         }
         const LpRow row(sum, a.inv_t);
-        if (lane == 0) lp_store(a, r, tok, row, sum.t);
+        if (lane == 0) lp_store(a, r, tok, lp_logit(a, r, tok), row, sum.t);
         for (int q = lane; q < keys; q += NT) lp_store_top(a, r, q, o.out[q], row);
     } else {
         const int64_t unit = r * parts + p;
@@ -465,34 +470,45 @@ __global__ __launch_bounds__(256, TOP ? 4 : 1) void k_lp_parts(LpArgs<T> a, LpSc
     }
 }
 
-// A row's parts joined: NT lanes a row, a wave where no alternatives are asked for.
+// A row's parts joined: NT lanes a row, a wave where no alternatives are asked for.  What the
+// parts left comes from the other dies' caches: all of it is asked for first.
 template <typename T, int NT>
 __global__ __launch_bounds__(256) void k_lp_join(LpArgs<T> a, LpScratch<T> scratch, int parts, int64_t b_base)
 {
-    constexpr int RPB = 256 / NT;
-    __shared__ LpPart sh[1];
+    constexpr int RPB = 256 / NT, HELD = NT == 64 ? 1 : 4;
     const int lane = threadIdx.x % NT, sub = RPB == 1 ? 0 : threadIdx.x / NT;
     const int64_t r = (b_base + int64_t(blockIdx.x)) * RPB + sub;
     if (RPB > 1 && r >= a.rows) return;
+    const LpPart empty{-__builtin_inf(), 0.0, 0.0};
+    const LpPart *sums = scratch.sums + r * parts * 4;
+    LpPart sum = (NT == 64 || lane < 64) && lane < parts * 4 ? sums[lane] : empty;
+    const int64_t n = int64_t(parts) * a.k;
+    const LpKey<T> *keys = scratch.keys + r * n;
+    LpKey<T> held[HELD];  // the first of a lane's keys
+    if constexpr (NT > 64) {
+#pragma unroll
+        for (int q = 0; q < HELD; q++) held[q] = lane + q * NT < n ? keys[lane + q * NT] : LpKey<T>::none();
+    }
     const int64_t tok = a.tokens ? a.tokens[r] : 0;
     if (tok < 0) return lp_unused<T, NT>(a, r, lane);
-    const T none = -T(__builtin_inf());
-    LpPart sum{-__builtin_inf(), 0.0, 0.0};
-    const LpPart *sums = scratch.sums + r * parts * 4;
+    const T logit = lp_logit(a, r, tok);
     if (NT == 64 || lane < 64) {  // one wave, in one order
-        for (int p = lane; p < parts * 4; p += 64) sum = p < 64 ? sums[p] : lp_join(sum, sums[p], a.inv_t);
+        for (int p = lane + 64; p < parts * 4; p += 64) sum = lp_join(sum, sums[p], a.inv_t);
         sum = lp_join_wave(sum, a.inv_t);
     }
     if constexpr (NT == 64) {
-        if (lane == 0) lp_store(a, r, tok, LpRow(sum, a.inv_t), sum.t);
+        if (lane == 0) lp_store(a, r, tok, logit, LpRow(sum, a.inv_t), sum.t);
     } else {
+        __shared__ LpPart sh[1];
         __shared__ LpOrder<T, NT> o;
         if (lane == 0) sh[0] = sum;
-        const int64_t n = int64_t(parts) * a.k;
-        const LpKey<T> *keys = scratch.keys + r * n;
         const auto each = [&](auto f) {
-            for (int64_t c = lane; c < n; c += NT) f(keys[c].value(), keys[c].index());
+#pragma unroll
+            for (int q = 0; q < HELD; q++)
+                if (lane + q * NT < n) f(held[q].value(), held[q].index());
+            for (int64_t c = lane + HELD * NT; c < n; c += NT) f(keys[c].value(), keys[c].index());
         };
+        const T none = -T(__builtin_inf());
         T top = none;  // (a place without a value holds none)
         each([&](T y, int) { top = y > top ? y : top; });
         const auto pop = [&](bool next) {
@@ -500,15 +516,15 @@ __global__ __launch_bounds__(256) void k_lp_join(LpArgs<T> a, LpScratch<T> scrat
             return top;
         };
         const auto pass = [&](T bound, auto take) {
-            for (int64_t c0 = 0; c0 < n; c0 += NT) {
-                const bool on = c0 + lane < n;
-                const LpKey<T> key = on ? keys[c0 + lane] : LpKey<T>::none();
-                take(key.any() && key.value() >= bound, key.value(), key.index());
-            }
+            const auto one = [&](const LpKey<T> &key) { take(key.any() && key.value() >= bound, key.value(), key.index()); };
+#pragma unroll
+            for (int q = 0; q < HELD; q++)
+                if (q * NT < n) one(held[q]);
+            for (int64_t c0 = HELD * NT; c0 < n; c0 += NT) one(c0 + lane < n ? keys[c0 + lane] : LpKey<T>::none());
         };
         lp_select<T, NT>(o, a.k, lane, pop, pass, each);
         const LpRow row(sh[0], a.inv_t);
-        if (lane == 0) lp_store(a, r, tok, row, sh[0].t);
+        if (lane == 0) lp_store(a, r, tok, logit, row, sh[0].t);
         for (int q = lane; q < a.k; q += NT) lp_store_top(a, r, q, o.out[q], row);
     }
 }
