@@ -8,6 +8,7 @@
 // s and t are summed in double: where one token has nearly all the probability, logprob and
 // entropy are as small as the rest of s, which a sum in float would round away beside 1.
 #include <cmath>
+#include <limits>
 #include <type_traits>
 
 #include "row_call.hpp"
@@ -178,32 +179,35 @@ struct LpOrder {
 };
 
 // The k first of the waves' lists (n[w] <= kCand, all apart) into out: a candidate's place is the
-// number of those before it.  Each wave places its own.
+// number of those before it.  Each wave places its own, four lanes to a candidate, which share
+// the lists.
 template <typename T, int NT>
 NH_DEV void lp_rank(LpOrder<T, NT> &o, int k, int lane)
 {
-    constexpr int W = NT / 64;
-    const int w = W == 1 ? 0 : lane >> 6, wl = lane & 63;
+    constexpr int W = NT / 64, STEP = W == 1 ? 8 : 2;
+    const int w = W == 1 ? 0 : lane >> 6, quad = lane & 3, list = W == 1 ? 0 : quad;
     int total = 0;
 #pragma unroll
     for (int u = 0; u < W; u++) total += o.n[u];
     for (int q = total + lane; q < k; q += NT) o.out[q] = LpKey<T>::none();
-    for (int c = wl; c < o.n[w]; c += 64) {
-        const LpKey<T> mine = o.key[w][c];
+    const int n = o.n[list], own = o.n[w];
+    for (int c0 = 0; c0 < own; c0 += 16) {
+        const int c = c0 + ((lane & 63) >> 2);
+        const LpKey<T> mine = o.key[w][c < own ? c : own];
         int place = 0;
-#pragma unroll
-        for (int u = 0; u < W; u++)
-#pragma unroll 2
-            for (int j = 0; j < o.n[u]; j += 2) {
-                struct alignas(16) {
-                    LpKey<T> k[2];
-                } pair;
-                pair.k[0] = o.key[u][j];
-                pair.k[1] = o.key[u][j + 1];
-                place += pair.k[0].before(mine) ? 1 : 0;
-                place += pair.k[1].before(mine) ? 1 : 0;
-            }
-        if (place < k) o.out[place] = mine;
+#pragma unroll 4
+        for (int j = W == 1 ? 2 * quad : 0; j < n; j += STEP) {
+            struct alignas(16) {
+                LpKey<T> k[2];
+            } pair;
+            pair.k[0] = o.key[list][j];
+            pair.k[1] = o.key[list][j + 1];
+            place += pair.k[0].before(mine) ? 1 : 0;
+            place += pair.k[1].before(mine) ? 1 : 0;
+        }
+        place += dpp_i<kDppXor1>(place);
+        place += dpp_i<kDppXor2>(place);
+        if (quad == 0 && c < own && place < k) o.out[place] = mine;
     }
 }
 
@@ -241,11 +245,11 @@ NH_DEV void lp_rounds(LpOrder<T, NT> &o, int k, int lane, const E &each)
 // The k first of a group's keys into o.out.  pop(true) gives the lane's largest value that was not
 // taken yet, of those that stand for its keys, pop(false) looks at it.  With j = k / waves rounded
 // up, the j-th of them over a wave, and the least of that over the waves, is passed by k keys at
-// least; what passes it (some 2 k where values are in no order) each wave collects (pass(bound,
-// take): take(ok, value, index) with the same lanes for all), and it is ordered by counting.
+// least; what passes it (some 2 k where values are in no order) each wave collects, lane by lane
+// (emit(least, f): f(value, index) for the lane's keys from least on), and it is ordered by counting.
 // What bounds it is one wave's latency, some 7 cycles an instruction.
 template <typename T, int NT, typename P, typename C, typename E>
-NH_DEV void lp_select(LpOrder<T, NT> &o, int k, int lane, P pop, C pass, const E &each)
+NH_DEV void lp_select(LpOrder<T, NT> &o, int k, int lane, P pop, C emit, const E &each)
 {
     constexpr int W = NT / 64;
     const int w = W == 1 ? 0 : lane >> 6, wl = lane & 63;
@@ -263,15 +267,15 @@ NH_DEV void lp_select(LpOrder<T, NT> &o, int k, int lane, P pop, C pass, const E
 #pragma unroll
         for (int u = 0; u < W; u++) bound = o.wave_v[u] < bound ? o.wave_v[u] : bound;
     }
-    int n = 0;  // the same in all lanes
-    pass(bound, [&](bool ok, T y, int i) {
-        const uint64_t who = __ballot(ok);
-        if (who) {
-            const int at = n + int(__builtin_amdgcn_mbcnt_hi(uint32_t(who >> 32), __builtin_amdgcn_mbcnt_lo(uint32_t(who), 0)));
-            if (ok && at < o.kCand) o.key[w][at] = LpKey<T>::of(y, i);
-            n += int(__builtin_popcountll(who));
-        }
-    });
+    const T least = bound == none ? -std::numeric_limits<T>::max() : bound;
+    int own = 0, at = 0, n = 0;  // the lane's, those of the lanes before, the wave's
+    each([&](T y, int) { own += y >= least ? 1 : 0; });
+    for (int b = 0; __ballot(own >> b); b++) {
+        const uint64_t who = __ballot(own >> b & 1);
+        at += int(__builtin_amdgcn_mbcnt_hi(uint32_t(who >> 32), __builtin_amdgcn_mbcnt_lo(uint32_t(who), 0))) << b;
+        n += int(__builtin_popcountll(who)) << b;
+    }
+    if (n <= o.kCand) emit(least, [&](T y, int i) { o.key[w][at++] = LpKey<T>::of(y, i); });
     if (wl == 0) o.n[w] = n;
     if (wl < 2 && n <= o.kCand) o.key[w][n + wl] = LpKey<T>::none();
     lp_meet<NT>();
@@ -420,36 +424,17 @@ __global__ __launch_bounds__(256, TOP ? 4 : 1) void k_lp_parts(LpArgs<T> a, LpSc
             }
             return over;
         };
-        const auto pass = [&](T bound, auto take) {
-            uint32_t hits = 0;  // the lane's vectors with a value that passes
+        const auto emit = [&](T least, auto f) {
 #pragma unroll
-            for (int k = 0; k < VPT; k++) hits |= vmax[k] >= bound && vmax[k] > none ? 1u << k : 0u;
-            while (__ballot(hits != 0)) {
-                const int at = __builtin_ctz(hits | 0x80000000u);
-                const bool on = hits != 0;
-                // vector `at` by masks: by a choice of vectors the compiler puts them into memory
-                using I = std::conditional_t<sizeof(T) == 4, uint32_t, uint64_t>;
-                I bits[VN] = {};
+            for (int k = 0; k < VPT; k++)
+                if (vmax[k] >= least) {
 #pragma unroll
-                for (int k = 0; k < VPT; k++) {
-                    const I mask = at == k ? ~I(0) : I(0);
-#pragma unroll
-                    for (int j = 0; j < VN; j++) {
-                        I b;
-                        const T e = v[k][j];
-                        __builtin_memcpy(&b, &e, sizeof(T));
-                        bits[j] |= b & mask;
-                    }
+                    for (int j = 0; j < VN; j++)
+                        if (v[k][j] >= least) f(v[k][j], first + k * NT * VN + j);
                 }
-                T y[VN];
-                __builtin_memcpy(y, bits, sizeof(bits));
-                hits &= hits - 1;
-#pragma unroll
-                for (int j = 0; j < VN; j++) take(on && y[j] >= bound && y[j] > none, y[j], first + at * (NT * VN) + j);
-            }
-            if (rem) take(vt >= bound && vt > none, vt, int(ncv * VN) + lane);
+            if (vt >= least) f(vt, int(ncv * VN) + lane);
         };
-        lp_select<T, NT>(order[sub], a.k, lane, pop, pass, each);
+        lp_select<T, NT>(order[sub], a.k, lane, pop, emit, each);
     }
     const LpOrder<T, NT> &o = order[TOP ? sub : 0];
     const int keys = TOP ? a.k : 0;
@@ -484,10 +469,11 @@ __global__ __launch_bounds__(256) void k_lp_join(LpArgs<T> a, LpScratch<T> scrat
     LpPart sum = (NT == 64 || lane < 64) && lane < parts * 4 ? sums[lane] : empty;
     const int64_t n = int64_t(parts) * a.k;
     const LpKey<T> *keys = scratch.keys + r * n;
-    LpKey<T> held[HELD];  // the first of a lane's keys
+    const int turn = (lane & 63) * (NT / 64) + lane / 64;  // few keys go to all waves
+    LpKey<T> held[HELD];                                  // the first of a lane's keys
     if constexpr (NT > 64) {
 #pragma unroll
-        for (int q = 0; q < HELD; q++) held[q] = lane + q * NT < n ? keys[lane + q * NT] : LpKey<T>::none();
+        for (int q = 0; q < HELD; q++) held[q] = turn + q * NT < n ? keys[turn + q * NT] : LpKey<T>::none();
     }
     const int64_t tok = a.tokens ? a.tokens[r] : 0;
     if (tok < 0) return lp_unused<T, NT>(a, r, lane);
@@ -505,8 +491,8 @@ __global__ __launch_bounds__(256) void k_lp_join(LpArgs<T> a, LpScratch<T> scrat
         const auto each = [&](auto f) {
 #pragma unroll
             for (int q = 0; q < HELD; q++)
-                if (lane + q * NT < n) f(held[q].value(), held[q].index());
-            for (int64_t c = lane + HELD * NT; c < n; c += NT) f(keys[c].value(), keys[c].index());
+                if (turn + q * NT < n) f(held[q].value(), held[q].index());
+            for (int64_t c = turn + HELD * NT; c < n; c += NT) f(keys[c].value(), keys[c].index());
         };
         const T none = -T(__builtin_inf());
         T top = none;  // (a place without a value holds none)
@@ -515,14 +501,12 @@ __global__ __launch_bounds__(256) void k_lp_join(LpArgs<T> a, LpScratch<T> scrat
             if (next) top = none;  // a lane's keys by their largest alone
             return top;
         };
-        const auto pass = [&](T bound, auto take) {
-            const auto one = [&](const LpKey<T> &key) { take(key.any() && key.value() >= bound, key.value(), key.index()); };
-#pragma unroll
-            for (int q = 0; q < HELD; q++)
-                if (q * NT < n) one(held[q]);
-            for (int64_t c0 = HELD * NT; c0 < n; c0 += NT) one(c0 + lane < n ? keys[c0 + lane] : LpKey<T>::none());
+        const auto emit = [&](T least, auto f) {
+            each([&](T y, int i) {
+                if (y >= least) f(y, i);
+            });
         };
-        lp_select<T, NT>(o, a.k, lane, pop, pass, each);
+        lp_select<T, NT>(o, a.k, lane, pop, emit, each);
         const LpRow row(sh[0], a.inv_t);
         if (lane == 0) lp_store(a, r, tok, logit, row, sh[0].t);
         for (int q = lane; q < a.k; q += NT) lp_store_top(a, r, q, o.out[q], row);
