@@ -299,10 +299,11 @@ struct LpScratch {
 // narrow; a group of NT lanes holds one part in registers: one read.  Each wave takes its own
 // largest value as the reference of its exponentials.
 // r_base: the launch's first row.  What bounds it where rows are many: the vector units, with HBM
-// close behind (f32: about 16 issue slots a value; [4096, 50257] 145 us, a copy's rate 137); with
-// alternatives the latency of ordering them (k = 1: 230 us, 20: 269).
+// close behind (f32: about 16 issue slots a value; [4096, 50257] 140 us, a copy's rate 137); with
+// alternatives the latency of ordering them (k = 1: 210 us, 20: 253, 64: 377; with four waves a
+// SIMD, for which nine registers are spilled, 231, 257 and 347).
 template <typename T, int NT, int VPT, bool TOP>
-__global__ __launch_bounds__(256, TOP ? 4 : 1) void k_lp_parts(LpArgs<T> a, LpScratch<T> scratch, int parts, int64_t per,
+__global__ __launch_bounds__(256, TOP ? 3 : 1) void k_lp_parts(LpArgs<T> a, LpScratch<T> scratch, int parts, int64_t per,
                                                                int64_t r_base)
 {
     using V = typename Vec16<T>::type;
