@@ -465,7 +465,8 @@ int neural_dropout_add_layer_norm_backward(NeuralTensor *grad_in, NeuralTensor *
  *
  * Errors: NULL_POINTER, DTYPE_MISMATCH, DIM_MISMATCH (a 0-d tensor), SHAPE_MISMATCH,
  * INVALID_ARGUMENT (non-contiguous tensors, eps negative or not finite, a stride less than the
- * row, k < 1, an unknown act, hidden without residual, outputs that overlap an input, other
+ * row, k < 1, an unknown act, hidden without residual, codes in host memory in a captured call,
+ * outputs that overlap an input, other
  * than as allowed, or each other). */
 int neural_rms_norm_forward(NeuralTensor *out, NeuralTensor *hidden, const NeuralTensor *in,
                             const NeuralTensor *residual, const NeuralTensor *gamma, double eps,
@@ -505,7 +506,7 @@ int neural_linear_q8(NeuralTensor *out, const int8_t *codes, int64_t stride, con
  * partial results, as neural_layer_norm_backward does.
  * Errors: NULL_POINTER, DTYPE_MISMATCH, DIM_MISMATCH (a 0-d tensor), SHAPE_MISMATCH,
  * TENSOR_TOO_LARGE, INVALID_ARGUMENT (non-contiguous tensors, k outside [0, 64], a temperature
- * that is not positive and finite, outputs that overlap an input, other than as allowed, or each
+ * outside [1e-10, 1e10], tokens or top_ids in host memory in a captured call, outputs that overlap an input, other than as allowed, or each
  * other). */
 int neural_token_logprobs_forward(NeuralTensor *logprob, NeuralTensor *entropy, NeuralTensor *lse,
                                   int64_t *top_ids, NeuralTensor *top_logprobs, int64_t k,

@@ -683,8 +683,8 @@ static int linear_q8(const LinTensors &t)
     if (raw_may_overlap(t.codes, a_bytes, t.out) || raw_may_overlap(t.w_codes, w_bytes, t.out))
         return set_error(NEURAL_ERR_INVALID_ARGUMENT);
     Staged a, w;
-    NH_TRY(a.open(t.codes, a_bytes, true));
-    NH_TRY(w.open(t.w_codes, w_bytes, true));
+    NH_TRY(open_raw(a, t.codes, a_bytes, true));
+    NH_TRY(open_raw(w, t.w_codes, w_bytes, true));
     NH_TRY((t.out->dtype == NEURAL_DTYPE_FLOAT32 ? lin_run<float>(t, c, a, w) : lin_run<double>(t, c, a, w)));
     NH_TRY(a.finish(false));
     NH_TRY(w.finish(false));

@@ -77,7 +77,7 @@ static int rms_forward(const RmsTensors &t, double eps, int out)
                                       t.in, t.residual, t.gamma})
             if (raw_may_overlap(t.codes, bytes, u)) return set_error(NEURAL_ERR_INVALID_ARGUMENT);
         // (host memory between the rows comes back as it was)
-        NH_TRY(codes.open(t.codes, bytes, t.stride > c.cols));
+        NH_TRY(open_raw(codes, t.codes, bytes, t.stride > c.cols));
     }
     return t.in->dtype == NEURAL_DTYPE_FLOAT32 ? rms_run<float>(t, c, eps, out, codes)
                                                : rms_run<double>(t, c, eps, out, codes);

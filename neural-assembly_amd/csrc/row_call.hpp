@@ -94,6 +94,14 @@ inline int written(std::initializer_list<NeuralTensor *> outs)
     return set_error(NEURAL_OK);
 }
 
+// A call's buffer that is no tensor, in host or device memory.  Host memory is copied now, which
+// a captured call cannot do again when it is replayed: it is refused before anything is recorded.
+inline int open_raw(Staged &s, const void *p, size_t bytes, bool upload)
+{
+    if (!is_device_ptr(p) && stream_recording()) return set_error(NEURAL_ERR_INVALID_ARGUMENT);
+    return s.open(p, bytes, upload);
+}
+
 // Device memory for the partials of one call.  A call that is being captured
 // has the graph's (which may be replayed whenever, beside any other); otherwise
 // the block returns to the cache once the launches that use it are enqueued.

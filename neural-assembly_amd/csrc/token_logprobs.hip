@@ -735,7 +735,8 @@ struct LpTensors {
     const int64_t *tokens;
 };
 
-static bool lp_temperature(double t) { return t > 0.0 && t < __builtin_inf() && 1.0 / t < __builtin_inf(); }
+// (f32 rows have 1 / T and differences of logits times their weight in float)
+static bool lp_temperature(double t) { return t >= 1e-10 && t <= 1e10; }
 
 template <typename T>
 static int lp_run(const LpTensors &t, const RowCall &c, double temperature, const Staged &tokens, const Staged &ids)
@@ -783,8 +784,8 @@ static int lp_forward(LpTensors t, double temperature)
             return set_error(NEURAL_ERR_INVALID_ARGUMENT);
     if (raws_may_overlap(t.top_ids, id_bytes, t.tokens, tok_bytes)) return set_error(NEURAL_ERR_INVALID_ARGUMENT);
     Staged tokens, ids;
-    if (t.tokens) NH_TRY(tokens.open(t.tokens, tok_bytes, true));
-    if (t.top_ids) NH_TRY(ids.open(t.top_ids, id_bytes, false));
+    if (t.tokens) NH_TRY(open_raw(tokens, t.tokens, tok_bytes, true));
+    if (t.top_ids) NH_TRY(open_raw(ids, t.top_ids, id_bytes, false));
     NH_TRY((t.logits->dtype == NEURAL_DTYPE_FLOAT32 ? lp_run<float>(t, c, temperature, tokens, ids)
                                                     : lp_run<double>(t, c, temperature, tokens, ids)));
     if (t.top_ids) NH_TRY(ids.finish(true));
@@ -836,7 +837,7 @@ static int lp_backward(const LpGradTensors &t, double temperature)
     const size_t tok_bytes = size_t(c.rows) * 8;
     if (raw_may_overlap(t.tokens, tok_bytes, t.dx)) return set_error(NEURAL_ERR_INVALID_ARGUMENT);
     Staged tokens;
-    if (t.tokens) NH_TRY(tokens.open(t.tokens, tok_bytes, true));
+    if (t.tokens) NH_TRY(open_raw(tokens, t.tokens, tok_bytes, true));
     NH_TRY((t.logits->dtype == NEURAL_DTYPE_FLOAT32 ? lp_grad_run<float>(t, c, temperature, tokens)
                                                     : lp_grad_run<double>(t, c, temperature, tokens)));
     if (t.tokens) NH_TRY(tokens.finish(false));

@@ -556,8 +556,8 @@ class TokenLogProbs(Module):
 
     def __init__(self, temperature: float = 1.0, top_k: int = 0):
         super().__init__()
-        if not 0.0 < temperature < float("inf"):
-            raise ValueError(f"temperature must be positive and finite, got {temperature}")
+        if not 1e-10 <= temperature <= 1e10:
+            raise ValueError(f"temperature must be in [1e-10, 1e10], got {temperature}")
         if not 0 <= top_k <= 64:
             raise ValueError(f"top_k must be in [0, 64], got {top_k}")
         self.temperature = temperature

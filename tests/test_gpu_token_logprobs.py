@@ -198,6 +198,18 @@ def test_extreme_logits(pn, rng, dt):
         _check(pn, y, tokens, 6, temperature)
 
 
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("temperature", [1e-10, 1e10])
+def test_extreme_temperatures(pn, rng, dt, temperature):
+    """The largest and smallest, with logits of their size, and with ordinary ones that are all
+    alike beside the largest; masked ones among them."""
+    x, tokens = _case(rng, 6, 777, dt, masked=0.3, unused=0)
+    got = _check(pn, x * dt(temperature), tokens, 6, temperature)
+    assert not np.isnan(got["logprob"]).any()
+    if temperature > 1:
+        _check(pn, x, tokens, 6, temperature)
+
+
 def test_outputs_left_out(pn, rng):
     """Every output alone has the bits that it has beside the others; no tokens: every row used."""
     for rows, V in ((5, 300), (5, 40000), (400, 2000)):
@@ -319,7 +331,7 @@ def test_refusals(pn):
     assert with_(f, ok, _6=None) == E.NULL_POINTER and with_(f, ok, _7=None) == E.NULL_POINTER
     assert f(None, None, None, None, None, 3, x._ptr, tok.data_ptr(), 1.0) == E.NULL_POINTER
     assert f(None, None, None, ids.data_ptr(), top._ptr, 0, x._ptr, tok.data_ptr(), 1.0) == E.NULL_POINTER
-    for t in (0.0, -1.0, float("nan"), float("inf"), 1e-320):
+    for t in (0.0, -1.0, float("nan"), float("inf"), 1e-320, 9e-11, 1.1e10):
         assert with_(f, ok, _8=t) == E.INVALID_ARGUMENT and with_(k, gk, _7=t) == E.INVALID_ARGUMENT
     for n in (-1, 65):
         assert with_(f, ok, _5=n) == E.INVALID_ARGUMENT
@@ -393,6 +405,44 @@ def test_graphs_and_streams(pn, rng, rows, V):
                 tok.copy_(torch.randint(-1, V, (rows,), device="cuda"))
             lib.neural_hip_empty_cache()
             torch.cuda.synchronize()
+    finally:
+        pn.set_stream(None)
+
+
+def test_host_memory_while_capturing(pn, rng):
+    """Tokens, ids and codes in host memory are refused in a captured call, which goes on."""
+    import torch
+    lib, T = pn.core._lib, pn.Tensor
+    x, lp, dx = torch.randn(3, 100, device="cuda"), torch.zeros(3, device="cuda"), torch.zeros(3, 100, device="cuda")
+    dev = torch.tensor([1, 2, 3], device="cuda")
+    tok, ids, codes = np.array([1, 2, 3]), np.full((3, 2), 7), np.full((3, 100), 7, np.int8)
+    w, hw, sw = torch.ones(100, 100, dtype=torch.int8, device="cuda"), np.ones((100, 100), np.int8), torch.ones(100, device="cuda")
+    X, LP, DX, SW = (T.from_torch(v) for v in (x, lp, dx, sw))
+    want = torch.log_softmax(x.double(), 1)[[0, 1, 2], [1, 2, 3]].cpu().numpy()
+    s = torch.cuda.Stream()
+    pn.set_stream(s.cuda_stream)
+    try:
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=s):
+            rcs = [lib.neural_token_logprobs_forward(LP._ptr, None, None, None, None, 0, X._ptr, tok.ctypes.data, 1.0),
+                   lib.neural_token_logprobs_forward(LP._ptr, None, None, ids.ctypes.data, None, 2, X._ptr, dev.data_ptr(), 1.0),
+                   lib.neural_token_logprobs_backward(DX._ptr, LP._ptr, None, X._ptr, tok.ctypes.data, LP._ptr, None, 1.0),
+                   lib.neural_quantize_rows(codes.ctypes.data, 100, LP._ptr, X._ptr),
+                   lib.neural_rms_norm_forward_q8(codes.ctypes.data, 100, LP._ptr, None, X._ptr, None, None, 0.1),
+                   lib.neural_linear_q8(DX._ptr, codes.ctypes.data, 100, LP._ptr, w.data_ptr(), 100, SW._ptr, 100, None, 0,
+                                        0.0, None),
+                   lib.neural_linear_q8(DX._ptr, w.data_ptr(), 100, LP._ptr, hw.ctypes.data, 100, SW._ptr, 100, None, 0,
+                                        0.0, None)]
+            assert lib.neural_token_logprobs_forward(LP._ptr, None, None, None, None, 0, X._ptr, dev.data_ptr(), 1.0) == 0
+        assert rcs == [pn.NeuralError.INVALID_ARGUMENT] * 7, rcs
+        for _ in range(2):
+            lp.zero_()
+            torch.cuda.synchronize()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert np.abs(lp.cpu().numpy() - want).max() < 1e-5
+        assert (ids == 7).all() and (codes == 7).all()
     finally:
         pn.set_stream(None)
 

@@ -32,7 +32,7 @@ def test_module_arguments():
     from pyneural import nn
     with pytest.raises(ValueError):
         pn.RMSNorm(0)
-    for bad in (0.0, -1.0, float("inf"), float("nan")):
+    for bad in (0.0, -1.0, 9e-11, 1.1e10, float("inf"), float("nan")):
         with pytest.raises(ValueError):
             pn.TokenLogProbs(temperature=bad)
     for k in (-1, 65):
