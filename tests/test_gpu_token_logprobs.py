@@ -416,7 +416,8 @@ def test_host_memory_while_capturing(pn, rng):
     x, lp, dx = torch.randn(3, 100, device="cuda"), torch.zeros(3, device="cuda"), torch.zeros(3, 100, device="cuda")
     dev = torch.tensor([1, 2, 3], device="cuda")
     tok, ids, codes = np.array([1, 2, 3]), np.full((3, 2), 7), np.full((3, 100), 7, np.int8)
-    w, hw, sw = torch.ones(100, 100, dtype=torch.int8, device="cuda"), np.ones((100, 100), np.int8), torch.ones(100, device="cuda")
+    w, hw = torch.ones(100, 100, dtype=torch.int8, device="cuda"), np.ones((100, 100), np.int8)
+    sw = torch.ones(100, device="cuda")
     X, LP, DX, SW = (T.from_torch(v) for v in (x, lp, dx, sw))
     want = torch.log_softmax(x.double(), 1)[[0, 1, 2], [1, 2, 3]].cpu().numpy()
     s = torch.cuda.Stream()
@@ -426,7 +427,8 @@ def test_host_memory_while_capturing(pn, rng):
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph, stream=s):
             rcs = [lib.neural_token_logprobs_forward(LP._ptr, None, None, None, None, 0, X._ptr, tok.ctypes.data, 1.0),
-                   lib.neural_token_logprobs_forward(LP._ptr, None, None, ids.ctypes.data, None, 2, X._ptr, dev.data_ptr(), 1.0),
+                   lib.neural_token_logprobs_forward(LP._ptr, None, None, ids.ctypes.data, None, 2, X._ptr,
+                                                     dev.data_ptr(), 1.0),
                    lib.neural_token_logprobs_backward(DX._ptr, LP._ptr, None, X._ptr, tok.ctypes.data, LP._ptr, None, 1.0),
                    lib.neural_quantize_rows(codes.ctypes.data, 100, LP._ptr, X._ptr),
                    lib.neural_rms_norm_forward_q8(codes.ctypes.data, 100, LP._ptr, None, X._ptr, None, None, 0.1),
