@@ -102,7 +102,10 @@ NH_DEV LpPart lp_join_wave(const LpPart &p, double inv_t)
 // A row's results from its sums.
 struct LpRow {
     double m, inv_t, s, ls;  // m: 0 where every logit is masked
-    NH_DEV LpRow(const LpPart &p, double it) : m(p.m == -__builtin_inf() ? 0.0 : p.m), inv_t(it), s(p.s), ls(log(p.s)) {}
+    NH_DEV static LpRow of(const LpPart &p, double it)
+    {
+        return {p.m == -__builtin_inf() ? 0.0 : p.m, it, p.s, log(p.s)};
+    }
     NH_DEV bool sound() const { return s == s; }
     NH_DEV double logprob(double x) const { return s == 0.0 ? -__builtin_inf() : (x - m) * inv_t - ls; }
     NH_DEV double lse() const { return m * inv_t + ls; }
@@ -177,6 +180,16 @@ struct LpOrder {
     T wave_v[W];
     LpKey<T> wave_key[W], out[kLpMaxTop];
 };
+
+// Whether every wave's candidates fit its list.
+template <typename T, int NT>
+NH_DEV bool lp_fits(const LpOrder<T, NT> &o)
+{
+    bool fits = true;
+#pragma unroll
+    for (int u = 0; u < NT / 64; u++) fits &= o.n[u] <= o.kCand;
+    return fits;
+}
 
 // The k first of the waves' lists (n[w] <= kCand, all apart) into out: a candidate's place is the
 // number of those before it.  Each wave places its own, four lanes to a candidate, which share
@@ -279,12 +292,26 @@ NH_DEV void lp_select(LpOrder<T, NT> &o, int k, int lane, P pop, C emit, const E
     if (wl == 0) o.n[w] = n;
     if (wl < 2 && n <= o.kCand) o.key[w][n + wl] = LpKey<T>::none();
     lp_meet<NT>();
-    bool fits = true;
-#pragma unroll
-    for (int u = 0; u < W; u++) fits &= o.n[u] <= o.kCand;
-    if (fits) lp_rank<T, NT>(o, k, lane);
+    if (lp_fits(o)) lp_rank<T, NT>(o, k, lane);
     else lp_rounds<T, NT>(o, k, lane, each);
     lp_meet<NT>();
+}
+
+// What the other waves of a block do meanwhile: they meet as often.  first() runs beside the lists'
+// making, then() beside their ordering.
+template <typename T, int NT, typename F, typename G>
+NH_DEV void lp_beside(const LpOrder<T, NT> &o, int k, const F &first, const G &then)
+{
+    __syncthreads();  // the bounds
+    first();
+    __syncthreads();  // the lists
+    then();
+    if (!lp_fits(o))
+        for (int q = 0; q < k; q++) {  // lp_rounds
+            __syncthreads();
+            __syncthreads();
+        }
+    __syncthreads();  // the order
 }
 
 // Where a row is split: its waves' sums, [rows][parts][4], and its parts' alternatives,
@@ -302,14 +329,21 @@ struct LpScratch {
 // close behind (f32: about 16 issue slots a value; [4096, 50257] 140 us, a copy's rate 137); with
 // alternatives the latency of ordering them (k = 1: 210 us, 20: 253, 64: 377; with four waves a
 // SIMD, for which nine registers are spilled, 231, 257 and 347).
-template <typename T, int NT, int VPT, bool TOP>
-__global__ __launch_bounds__(256, TOP ? 3 : 1) void k_lp_parts(LpArgs<T> a, LpScratch<T> scratch, int parts, int64_t per,
-                                                               int64_t r_base)
+enum { LP_SUMS = 0, LP_TOP = 1, LP_TOP_BESIDE = 2 };  // alternatives too, by the same waves or by others
+constexpr int lp_lanes(int nt, int mode) { return mode == LP_TOP_BESIDE ? 2 * nt : nt < 256 ? 256 : nt; }
+template <typename T, int NT, int VPT, int MODE>
+__global__ __launch_bounds__(lp_lanes(NT, MODE), (MODE == LP_SUMS ? 1 : 3)) void k_lp_parts(LpArgs<T> a, LpScratch<T> scratch,
+                                                                                         int parts, int64_t per,
+                                                                                         int64_t r_base)
 {
+    constexpr bool TOP = MODE != LP_SUMS, TWO = MODE == LP_TOP_BESIDE;
     using V = typename Vec16<T>::type;
     using U = typename VecU<T>::type;
     constexpr int VN = Vec16<T>::n, RPB = 256 / NT, W = NT / 64;
     __shared__ LpPart sh[W];
+    __shared__ LpRow row_of;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const bool sums = !TWO || wave < W, tops = TOP && (!TWO || wave >= W);
     const int lane = threadIdx.x % NT, sub = RPB == 1 ? 0 : threadIdx.x / NT;
     const int rl = RPB > 1 ? int(blockIdx.x) * RPB + sub : int(blockIdx.x / unsigned(parts));
     const int p = RPB > 1 ? 0 : int(blockIdx.x) - rl * parts;
@@ -317,7 +351,7 @@ __global__ __launch_bounds__(256, TOP ? 3 : 1) void k_lp_parts(LpArgs<T> a, LpSc
     if (RPB > 1 && r >= a.rows) return;
     const int64_t tok = a.tokens ? a.tokens[r] : 0;
     if (tok < 0) {
-        if (parts == 1) lp_unused<T, NT>(a, r, lane);
+        if (parts == 1 && sums) lp_unused<T, NT>(a, r, lane);
         return;
     }
     // vectors v0 .. of the row, and in the last part the values past them
@@ -353,50 +387,63 @@ __global__ __launch_bounds__(256, TOP ? 3 : 1) void k_lp_parts(LpArgs<T> a, LpSc
         for (int j = 1; j < VN; j++) vmax[k] = most(vmax[k], v[k][j]);
         top = most(top, vmax[k]);
     }
-    const T m = RowGrp<64>::max(top, nullptr);
-    LpPart sum{double(m), 0.0, 0.0};
-    const T ref = m == none ? T(0) : m;
-    if constexpr (sizeof(T) == 4) {
-        // exp(d / T) = 2^(d c), c = log2(e) / T in two floats: the product's rounding error and
-        // the second part go into the result as a factor 1 + error ln 2.  Four values are added
-        // in float, except where one of them is the largest, whose 1 would swallow the others.
-        const double cd = a.inv_t * 1.4426950408889634;
-        const float c = float(cd), c2 = float(cd - double(c));
-        const float least = float(-200.0 * 0.6931471805599453 / a.inv_t);  // exp(least / T) = 0
-        const auto term = [&](float y, float &ed) {
-            float d = y - ref;
-            d = d < least ? least : d;  // (NaN stays)
-            const float h = d * c, lo = __builtin_fmaf(d, c2, __builtin_fmaf(d, c, -h));
-            float e = __builtin_amdgcn_exp2f(h);
-            e = __builtin_fmaf(e, lo * 0.693147181f, e);
-            ed = e * d;
-            return e;
-        };
+    LpPart sum;
+    const auto add = [&] {
+        const T m = RowGrp<64>::max(top, nullptr);
+        sum = {double(m), 0.0, 0.0};
+        const T ref = m == none ? T(0) : m;
+        if constexpr (sizeof(T) == 4) {
+            // exp(d / T) = 2^(d c), c = log2(e) / T in two floats: the product's rounding error and
+            // the second part go into the result as a factor 1 + error ln 2.  Four values are added
+            // in float, except where one of them is the largest, whose 1 would swallow the others.
+            const double cd = a.inv_t * 1.4426950408889634;
+            const float c = float(cd), c2 = float(cd - double(c));
+            const float least = float(-200.0 * 0.6931471805599453 / a.inv_t);  // exp(least / T) = 0
+            const auto term = [&](float y, float &ed) {
+                float d = y - ref;
+                d = d < least ? least : d;  // (NaN stays)
+                const float h = d * c, lo = __builtin_fmaf(d, c2, __builtin_fmaf(d, c, -h));
+                float e = __builtin_amdgcn_exp2f(h);
+                e = __builtin_fmaf(e, lo * 0.693147181f, e);
+                ed = e * d;
+                return e;
+            };
 #pragma unroll
-        for (int k = 0; k < VPT; k++) {
-            float e[4], q[4];
+            for (int k = 0; k < VPT; k++) {
+                float e[4], q[4];
 #pragma unroll
-            for (int j = 0; j < 4; j++) e[j] = term(v[k][j], q[j]);
-            sum.t += double((q[0] + q[1]) + (q[2] + q[3]));
-            if (__ballot(vmax[k] == m)) sum.s += (double(e[0]) + double(e[1])) + (double(e[2]) + double(e[3]));
-            else sum.s += double((e[0] + e[1]) + (e[2] + e[3]));
+                for (int j = 0; j < 4; j++) e[j] = term(v[k][j], q[j]);
+                sum.t += double((q[0] + q[1]) + (q[2] + q[3]));
+                if (__ballot(vmax[k] == m)) sum.s += (double(e[0]) + double(e[1])) + (double(e[2]) + double(e[3]));
+                else sum.s += double((e[0] + e[1]) + (e[2] + e[3]));
+            }
+            if (rem) {  // uniform
+                float q;
+                sum.s += double(term(vt, q));
+                sum.t += double(q);
+            }
+        } else {
+            each([&](T y, int) {
+                const double d = y - ref, e = exp(d * a.inv_t);
+                sum.s += e;
+                sum.t += d * a.inv_t < -2000.0 ? 0.0 : e * d;
+            });
         }
-        if (rem) {  // uniform
-            float q;
-            sum.s += double(term(vt, q));
-            sum.t += double(q);
-        }
-    } else {
-        each([&](T y, int) {
-            const double d = y - ref, e = exp(d * a.inv_t);
-            sum.s += e;
-            sum.t += d * a.inv_t < -2000.0 ? 0.0 : e * d;
-        });
-    }
-    sum.s = wave_dsum(sum.s);
-    sum.t = wave_dsum(sum.t);
+        sum.s = wave_dsum(sum.s);
+        sum.t = wave_dsum(sum.t);
+    };
+    if (!TWO) add();
     __shared__ LpOrder<T, NT> order[TOP ? RPB : 1];
-    if constexpr (TOP) {
+    const auto finish = [&] {  // a row of one part, by the first wave that sums
+        if constexpr (W > 1) sum = lp_join_wave(lane < W ? sh[lane < W ? lane : 0] : LpPart{-__builtin_inf(), 0.0, 0.0}, a.inv_t);
+        const LpRow row = LpRow::of(sum, a.inv_t);
+        if (lane == 0) lp_store(a, r, tok, lp_logit(a, r, tok), row, sum.t);
+        return row;
+    };
+    const auto leave = [&] {  // a wave's sums
+        if ((threadIdx.x & 63) == 0) (parts == 1 ? sh : scratch.sums + (r * parts + p) * W)[wave % W] = sum;
+    };
+    if constexpr (TOP) if (tops) {
         // Alternatives of a wave that are many for its lanes: its vectors stand for their values,
         // not its lanes (64 rows of 1000, k = 64: 20 us, by lanes 53, as too much passes the bound;
         // k = 40: 13 both; k = 24: 9.7 and 8.7).
@@ -438,57 +485,88 @@ __global__ __launch_bounds__(256, TOP ? 3 : 1) void k_lp_parts(LpArgs<T> a, LpSc
         lp_select<T, NT>(order[sub], a.k, lane, pop, emit, each);
     }
     const LpOrder<T, NT> &o = order[TOP ? sub : 0];
-    const int keys = TOP ? a.k : 0;
-    if (parts == 1) {
-        if constexpr (W > 1) {
-            if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = sum;
-            __syncthreads();
-            const int wl = threadIdx.x & 63;
-            sum = lp_join_wave(wl < W ? sh[wl < W ? wl : 0] : LpPart{-__builtin_inf(), 0.0, 0.0}, a.inv_t);
-        }
-        const LpRow row(sum, a.inv_t);
-        if (lane == 0) lp_store(a, r, tok, lp_logit(a, r, tok), row, sum.t);
-        for (int q = lane; q < keys; q += NT) lp_store_top(a, r, q, o.out[q], row);
-    } else {
-        const int64_t unit = r * parts + p;
-        if ((threadIdx.x & 63) == 0) scratch.sums[unit * 4 + (threadIdx.x >> 6)] = sum;
-        for (int q = lane; q < keys; q += NT) scratch.keys[unit * a.k + q] = o.out[q];
+    if constexpr (TWO) {
+        if (sums)
+            lp_beside<T, NT>(
+                o, a.k,
+                [&] {
+                    add();
+                    leave();
+                },
+                [&] {
+                    if (parts == 1 && wave == 0) {
+                        const LpRow row = finish();
+                        if (lane == 0) row_of = row;
+                    }
+                });
+        if (tops && parts == 1)
+            for (int q = lane; q < a.k; q += NT) lp_store_top(a, r, q, o.out[q], row_of);
+    } else if (W > 1 || parts > 1) {
+        leave();
+    }
+    if (parts > 1) {
+        if (tops)
+            for (int q = lane; q < a.k; q += NT) scratch.keys[(r * parts + p) * a.k + q] = o.out[q];
+        return;
+    }
+    if constexpr (!TWO) {
+        if constexpr (W > 1) __syncthreads();
+        if (W > 1 && wave > 0) return;
+        const LpRow row = finish();
+        if constexpr (TOP)
+            for (int q = lane; q < a.k; q += NT) lp_store_top(a, r, q, o.out[q], row);
     }
 }
 
 // A row's parts joined: NT lanes a row, a wave where no alternatives are asked for.  What the
 // parts left comes from the other dies' caches: all of it is asked for first.
 template <typename T, int NT>
-__global__ __launch_bounds__(256) void k_lp_join(LpArgs<T> a, LpScratch<T> scratch, int parts, int64_t b_base)
+__global__ __launch_bounds__(NT == 64 ? 256 : NT + 64) void k_lp_join(LpArgs<T> a, LpScratch<T> scratch, int parts, int64_t b_base)
 {
     constexpr int RPB = 256 / NT, HELD = NT == 64 ? 1 : 4;
+    const bool tops = NT > 64 && threadIdx.x < NT;  // NT > 64: the last wave joins the sums beside
     const int lane = threadIdx.x % NT, sub = RPB == 1 ? 0 : threadIdx.x / NT;
     const int64_t r = (b_base + int64_t(blockIdx.x)) * RPB + sub;
     if (RPB > 1 && r >= a.rows) return;
     const LpPart empty{-__builtin_inf(), 0.0, 0.0};
     const LpPart *sums = scratch.sums + r * parts * 4;
-    LpPart sum = (NT == 64 || lane < 64) && lane < parts * 4 ? sums[lane] : empty;
+    LpPart sum = !tops && lane < parts * 4 ? sums[lane] : empty;
     const int64_t n = int64_t(parts) * a.k;
     const LpKey<T> *keys = scratch.keys + r * n;
     const int turn = (lane & 63) * (NT / 64) + lane / 64;  // few keys go to all waves
     LpKey<T> held[HELD];                                  // the first of a lane's keys
-    if constexpr (NT > 64) {
+    if (tops) {
 #pragma unroll
         for (int q = 0; q < HELD; q++) held[q] = turn + q * NT < n ? keys[turn + q * NT] : LpKey<T>::none();
     }
     const int64_t tok = a.tokens ? a.tokens[r] : 0;
-    if (tok < 0) return lp_unused<T, NT>(a, r, lane);
-    const T logit = lp_logit(a, r, tok);
-    if (NT == 64 || lane < 64) {  // one wave, in one order
+    if (tok < 0) {
+        if (NT == 64 || tops) lp_unused<T, NT>(a, r, lane);
+        return;
+    }
+    const auto join = [&] {  // one wave, in one order
+        const T logit = lp_logit(a, r, tok);
         for (int p = lane + 64; p < parts * 4; p += 64) sum = lp_join(sum, sums[p], a.inv_t);
         sum = lp_join_wave(sum, a.inv_t);
-    }
+        const LpRow row = LpRow::of(sum, a.inv_t);
+        if (lane == 0) lp_store(a, r, tok, logit, row, sum.t);
+        return row;
+    };
     if constexpr (NT == 64) {
-        if (lane == 0) lp_store(a, r, tok, logit, LpRow(sum, a.inv_t), sum.t);
+        join();
     } else {
-        __shared__ LpPart sh[1];
+        __shared__ LpRow row_of;
         __shared__ LpOrder<T, NT> o;
-        if (lane == 0) sh[0] = sum;
+        if (!tops) {
+            lp_beside<T, NT>(
+                o, a.k,
+                [&] {
+                    const LpRow row = join();
+                    if (lane == 0) row_of = row;
+                },
+                [] {});
+            return;
+        }
         const auto each = [&](auto f) {
 #pragma unroll
             for (int q = 0; q < HELD; q++)
@@ -508,9 +586,7 @@ __global__ __launch_bounds__(256) void k_lp_join(LpArgs<T> a, LpScratch<T> scrat
             });
         };
         lp_select<T, NT>(o, a.k, lane, pop, emit, each);
-        const LpRow row(sh[0], a.inv_t);
-        if (lane == 0) lp_store(a, r, tok, logit, row, sh[0].t);
-        for (int q = lane; q < a.k; q += NT) lp_store_top(a, r, q, o.out[q], row);
+        for (int q = lane; q < a.k; q += NT) lp_store_top(a, r, q, o.out[q], row_of);
     }
 }
 
@@ -656,22 +732,30 @@ __global__ __launch_bounds__(256) void k_lp_grad_row(LpGradArgs<T> a, int64_t r_
     }
 }
 
+// No more blocks than CUs: other waves find the alternatives beside the sums, the same bits ([1,
+// 8192], k = 20: 7.4 -> 5.9 us, [64, 32000] 13.2 -> 12.0; with more blocks the waves are missed:
+// [512, 32000] 29 -> 50).
 template <typename T, int NT, int VPT>
 static void launch_lp_parts(const LpArgs<T> &a, const LpScratch<T> &scratch, int parts, int64_t per)
 {
-    const int64_t rpb = 256 / NT, most = kMaxGridBlocks / parts * rpb;  // rows a launch (parts > 1: rpb is 1)
+    const int64_t rpb = NT < 256 ? 256 / NT : 1, most = kMaxGridBlocks / 2 / parts * rpb;  // rows a launch
     for (int64_t base = 0; base < a.rows; base += most) {
         const int64_t n = a.rows - base < most ? a.rows - base : most;
         const dim3 grid(unsigned(ceil_div(n, rpb) * parts));
-        if (a.k) NH_LAUNCH((k_lp_parts<T, NT, VPT, true>), grid, dim3(256), 0, stream(), a, scratch, parts, per, base);
-        else NH_LAUNCH((k_lp_parts<T, NT, VPT, false>), grid, dim3(256), 0, stream(), a, scratch, parts, per, base);
+        const auto go = [&](auto kernel, int mode) {
+            NH_LAUNCH(kernel, grid, dim3(unsigned(lp_lanes(NT, mode))), 0, stream(), a, scratch, parts, per, base);
+        };
+        if constexpr (NT > 64) {
+            if (a.k && int(grid.x) <= num_cus()) {
+                go(k_lp_parts<T, NT, VPT, LP_TOP_BESIDE>, LP_TOP_BESIDE);
+                continue;
+            }
+        }
+        if (a.k) go(k_lp_parts<T, NT, VPT, LP_TOP>, LP_TOP);
+        else go(k_lp_parts<T, NT, VPT, LP_SUMS>, LP_SUMS);
     }
 }
 
-// By the width alone, so that equal rows have equal results in any batch: a wave up to 256
-// vectors, 256 lanes up to 2048, and beyond parts of that by blocks of their own, joined by a second
-// launch (one block of 1024 for four parts: [64, 32000] with one alternative 22.9 us, where two
-// launches then took 13.5; now 11.6).
 template <typename T>
 static int launch_lp(const LpArgs<T> &a)
 {
@@ -692,8 +776,8 @@ static int launch_lp(const LpArgs<T> &a)
         LpScratch<T> scratch{static_cast<LpPart *>(block.p), nullptr};
         scratch.keys = reinterpret_cast<LpKey<T> *>(scratch.sums + units * 4);
         launch_lp_parts<T, 256, 8>(a, scratch, parts, per);
-        for_row_launches(a.rows, a.k ? 1 : 4, 256, [&](unsigned g, int64_t base) {
-            if (a.k) NH_LAUNCH((k_lp_join<T, 256>), dim3(g), dim3(256), 0, stream(), a, scratch, parts, base);
+        for_row_launches(a.rows, a.k ? 1 : 4, 256 + 64, [&](unsigned g, int64_t base) {
+            if (a.k) NH_LAUNCH((k_lp_join<T, 256>), dim3(g), dim3(256 + 64), 0, stream(), a, scratch, parts, base);
             else NH_LAUNCH((k_lp_join<T, 64>), dim3(g), dim3(256), 0, stream(), a, scratch, parts, base / 4);
         });
         return check_launch();
