@@ -322,19 +322,20 @@ struct LpScratch {
     LpKey<T> *keys;
 };
 
+// Sums alone, alternatives by the waves that sum, or by as many others beside them.
+enum { LP_SUMS = 0, LP_TOP = 1, LP_TOP_BESIDE = 2 };
+constexpr int lp_lanes(int nt, int mode) { return mode == LP_TOP_BESIDE ? 2 * nt : nt < 256 ? 256 : nt; }
+
 // A row is cut into parts of 256 lanes, `per` vectors at most, VPT a lane, or of a wave where it is
 // narrow; a group of NT lanes holds one part in registers: one read.  Each wave takes its own
 // largest value as the reference of its exponentials.
 // r_base: the launch's first row.  What bounds it where rows are many: the vector units, with HBM
 // close behind (f32: about 16 issue slots a value; [4096, 50257] 140 us, a copy's rate 137); with
-// alternatives the latency of ordering them (k = 1: 210 us, 20: 253, 64: 377; with four waves a
-// SIMD, for which nine registers are spilled, 231, 257 and 347).
-enum { LP_SUMS = 0, LP_TOP = 1, LP_TOP_BESIDE = 2 };  // alternatives too, by the same waves or by others
-constexpr int lp_lanes(int nt, int mode) { return mode == LP_TOP_BESIDE ? 2 * nt : nt < 256 ? 256 : nt; }
+// alternatives the latency of ordering them (k = 1: 212 us, 20: 256, 64: 383; with four waves a
+// SIMD, for which nine registers were spilled, 231, 257 and 347).
 template <typename T, int NT, int VPT, int MODE>
-__global__ __launch_bounds__(lp_lanes(NT, MODE), (MODE == LP_SUMS ? 1 : 3)) void k_lp_parts(LpArgs<T> a, LpScratch<T> scratch,
-                                                                                         int parts, int64_t per,
-                                                                                         int64_t r_base)
+__global__ __launch_bounds__(lp_lanes(NT, MODE), (MODE == LP_SUMS ? 1 : 3)) void k_lp_parts(
+    LpArgs<T> a, LpScratch<T> scratch, int parts, int64_t per, int64_t r_base)
 {
     constexpr bool TOP = MODE != LP_SUMS, TWO = MODE == LP_TOP_BESIDE;
     using V = typename Vec16<T>::type;
@@ -732,9 +733,9 @@ __global__ __launch_bounds__(256) void k_lp_grad_row(LpGradArgs<T> a, int64_t r_
     }
 }
 
-// No more blocks than CUs: other waves find the alternatives beside the sums, the same bits ([1,
-// 8192], k = 20: 7.4 -> 5.9 us, [64, 32000] 13.2 -> 12.0; with more blocks the waves are missed:
-// [512, 32000] 29 -> 50).
+// Where there are no more blocks than CUs other waves find the alternatives, with the same result
+// ([1, 8192], k = 20: 5.8 us, 7.4 by the waves that sum; [64, 32000] 11.8, 13.2); with more the waves
+// are missed ([512, 32000] 50 us, 29).
 template <typename T, int NT, int VPT>
 static void launch_lp_parts(const LpArgs<T> &a, const LpScratch<T> &scratch, int parts, int64_t per)
 {

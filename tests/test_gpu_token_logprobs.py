@@ -210,6 +210,24 @@ def test_extreme_temperatures(pn, rng, dt, temperature):
         _check(pn, x, tokens, 6, temperature)
 
 
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("V", [1000, 1111, 4099, 9000])
+def test_rows_in_any_batch(pn, rng, dt, V):
+    """A row has the bits of its batch of three in one of 600, which other forms take: values in no
+    order, all alike, and mostly masked."""
+    x, tokens = _case(rng, 600, V, dt)
+    x[1] = 0.25
+    x[2, rng.random(V) < 0.99] = -np.inf
+    x[3] = np.where(rng.random(V) < 0.5, 1, 2)
+    for k in (1, 20, 64):
+        whole = _forward(pn, x, tokens, k)
+        for r in (0, 2, 597):
+            part = _forward(pn, x[r:r + 3], tokens[r:r + 3], k)
+            for n in ("logprob", "entropy", "lse", "top"):
+                same_bits(part[n], whole[n][r:r + 3])
+            assert np.array_equal(part["ids"], whole["ids"][r:r + 3])
+
+
 def test_outputs_left_out(pn, rng):
     """Every output alone has the bits that it has beside the others; no tokens: every row used."""
     for rows, V in ((5, 300), (5, 40000), (400, 2000)):
