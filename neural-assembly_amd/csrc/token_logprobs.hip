@@ -757,6 +757,10 @@ static void launch_lp_parts(const LpArgs<T> &a, const LpScratch<T> &scratch, int
     }
 }
 
+// By the width alone, so that equal rows have equal results in any batch: a wave up to 256
+// vectors, 256 lanes up to 2048, and beyond parts of that by blocks of their own, joined by a second
+// launch (one block of 1024 for four parts: [64, 32000] with one alternative 22.9 us, where two
+// launches then took 13.5; now 9.8).
 template <typename T>
 static int launch_lp(const LpArgs<T> &a)
 {
