@@ -100,21 +100,43 @@ __global__ __launch_bounds__(256) void k_lin_pad(LinPad a, LinPad w, int ldd, in
     }
 }
 
-// 16 codes of a row from place k, at any address; zeros past the row's end.
-NH_DEV i32x4 lin_unit(const int8_t *row, int64_t k, int64_t end)
-{
-    typedef int W __attribute__((ext_vector_type(4), aligned(1)));
-    i32x4 v{0, 0, 0, 0};
-    if (k + 16 <= end) {
-        v = *reinterpret_cast<const W *>(row + k);
-    } else if (k < end) {
-        int8_t b[16];
+// 16 codes of a row from place k (a multiple of 16) on, zeros past the row's end: what is loaded, and
+// what that makes.  A row at a multiple of 4 bytes is loaded as it lies.  Of others (BYTES) the
+// words that its bytes lie in are loaded, and shifted: loads of 16 bytes from odd addresses take
+// several times as long (16 x 4097 -> 4096 18.6 us, by words 10.7).  No word is loaded of which
+// no byte is the row's.
+template <bool BYTES>
+struct LinUnit {
+    i32x4 v;
+    int last, shift;  // BYTES: the fifth word, and where in the first one the row's bytes begin
+    NH_DEV void load(const int8_t *row, int64_t k, int64_t end)
+    {
+        typedef int W __attribute__((ext_vector_type(4), aligned(4)));
+        shift = BYTES ? int(reinterpret_cast<uintptr_t>(row) & 3) : 0;
+        v = i32x4{0, 0, 0, 0};
+        last = 0;
+        if (k + 16 <= end) {
+            const int *p = reinterpret_cast<const int *>(row + k - shift);
+            v = *reinterpret_cast<const W *>(p);
+            if constexpr (BYTES) last = p[shift ? 4 : 3];
+        } else if (k < end) {
+            int8_t b[16];
 #pragma unroll
-        for (int q = 0; q < 16; q++) b[q] = k + q < end ? row[k + q] : int8_t(0);
-        __builtin_memcpy(&v, b, 16);
+            for (int q = 0; q < 16; q++) b[q] = k + q < end ? row[k + q] : int8_t(0);
+            __builtin_memcpy(&v, b, 16);
+            shift = 0;
+        }
     }
-    return v;
-}
+    NH_DEV i32x4 codes() const
+    {
+        if constexpr (!BYTES) return v;
+        i32x4 r;
+#pragma unroll
+        for (int q = 0; q < 4; q++)
+            r[q] = int(__builtin_amdgcn_alignbyte(uint32_t(q < 3 ? v[q < 3 ? q + 1 : 3] : last), uint32_t(v[q]), shift));
+        return r;
+    }
+};
 
 // What lanes fetch in the place of units past the rows' end.
 __device__ const int g_lin_zero[4] = {0, 0, 0, 0};
@@ -263,8 +285,9 @@ __global__ __launch_bounds__(S::NT, S::PER_SIMD) void k_lin_mfma(LinArgs<T> g, i
             if (inside) {
 #pragma unroll
                 for (int q = 0; q < S::kLoadsA; q++) {
-                    const i32x4 v = lin_unit(sa + at[q] - 16 * unit[q], 16 * unit[q], g.k - int64_t(s) * S::kSlice);
-                    *reinterpret_cast<i32x4 *>(smem + buf * S::kStage + 1024 * (w + q * S::NW) + 16 * lane) = v;
+                    LinUnit<false> u;
+                    u.load(sa + at[q] - 16 * unit[q], 16 * unit[q], g.k - int64_t(s) * S::kSlice);
+                    *reinterpret_cast<i32x4 *>(smem + buf * S::kStage + 1024 * (w + q * S::NW) + 16 * lane) = u.codes();
                 }
                 asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
             }
@@ -464,7 +487,7 @@ __global__ __launch_bounds__(S::NT, S::PER_SIMD) void k_lin_mfma(LinArgs<T> g, i
 // channels; its 8 waves share out the depth, each with UN slices of 64 codes in flight from memory
 // to registers, and add up in LDS.  Rows and weights may lie at any address.  1 x 4096 -> 4096 5.3
 // us (a launch alone 3.5; 64 x 64 tiles 11.2), 16 rows 6.6, 1 x 16384 -> 4096 12.6 (5.3 TB/s; 31).
-template <typename T>
+template <typename T, bool BYTES>
 __global__ __launch_bounds__(512) void k_lin_few(LinArgs<T> g, int64_t b_base)
 {
     constexpr int W = 8, UN = 8;
@@ -476,16 +499,16 @@ __global__ __launch_bounds__(512) void k_lin_few(LinArgs<T> g, int64_t b_base)
     i32x4 acc{0, 0, 0, 0};
     const int64_t slices = (g.k + 63) / 64, s0 = slices * w / W, s1 = slices * (w + 1) / W;
     for (int64_t s = s0; s < s1; s += UN) {
-        i32x4 vw[UN], va[UN];
+        LinUnit<BYTES> vw[UN], va[UN];
         const bool inside = (s + UN) * 64 <= g.k && s + UN <= s1;  // uniform
 #pragma unroll
         for (int q = 0; q < UN; q++) {
             const int64_t k = (s + q) * 64 + 16 * u, end = inside ? INT64_MAX : s + q < s1 ? g.k : 0;
-            vw[q] = lin_unit(pw, k, end);
-            va[q] = lin_unit(pa, k, end);
+            vw[q].load(pw, k, end);
+            va[q].load(pa, k, end);
         }
 #pragma unroll
-        for (int q = 0; q < UN; q++) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(vw[q], va[q], acc, 0, 0, 0);
+        for (int q = 0; q < UN; q++) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(vw[q].codes(), va[q].codes(), acc, 0, 0, 0);
     }
     part[w][lane] = acc;
     __syncthreads();
@@ -522,6 +545,13 @@ static int lin_splits(int64_t tiles, int64_t k)
     return n < 3 ? 1 : int(n);
 }
 
+// Rows that all begin at multiples of 4 bytes.
+template <typename T>
+static bool lin_words(const LinArgs<T> &g)
+{
+    return ((reinterpret_cast<uintptr_t>(g.a) | reinterpret_cast<uintptr_t>(g.w) | uintptr_t(g.lda) | uintptr_t(g.ldw)) & 3) == 0;
+}
+
 // Rows that go straight to LDS, without a copy.
 static bool lin_in_place(const int8_t *p, int64_t ld)
 {
@@ -529,7 +559,7 @@ static bool lin_in_place(const int8_t *p, int64_t ld)
 }
 
 // The product on shape S: copies of what does not go straight to LDS (through registers, as few
-// rows do, 577 x 1001 -> 3001 in f64 took 22 us for 17), long depths in parts where S is SMALL.
+// rows do, 577 x 1001 -> 3001 in f64 took 22 us for 17; by words, three slices ahead, 24), long depths in parts where S is SMALL.
 template <typename T, typename S, bool SMALL>
 static int launch_lin_shape(LinArgs<T> g)
 {
@@ -593,10 +623,13 @@ static double lin_cost(int64_t m, int64_t n, const LinCost &c)
 template <typename T>
 static int launch_linear(const LinArgs<T> &g)
 {
-    // (wider, 64 x 64 tiles stream better: 1 x 4096 -> 16384 15.9 us, 13.3 by tiles)
-    if (g.m <= 16 && ceil_div(g.n, 16) <= int64_t(num_cus()) * 2) {
+    // (wider, 64 x 64 tiles stream better what they do not copy: 1 x 4096 -> 16384 15.9 us, 13.3 by
+    // tiles; 16 rows of 4100 codes -> 16000 22.9 us, 35.5 with a copy of the weights; one of 4097
+    // 28.8 and 34.8)
+    if (g.m <= 16 && (ceil_div(g.n, 16) <= int64_t(num_cus()) * 2 || !lin_in_place(g.w, g.ldw))) {
         for_row_launches(ceil_div(g.n, 16), 1, 512, [&](unsigned blocks, int64_t base) {
-            NH_LAUNCH((k_lin_few<T>), dim3(blocks), dim3(512), 0, stream(), g, base);
+            if (lin_words(g)) NH_LAUNCH((k_lin_few<T, false>), dim3(blocks), dim3(512), 0, stream(), g, base);
+            else NH_LAUNCH((k_lin_few<T, true>), dim3(blocks), dim3(512), 0, stream(), g, base);
         });
         return check_launch();
     }
