@@ -559,7 +559,8 @@ static bool lin_in_place(const int8_t *p, int64_t ld)
 }
 
 // The product on shape S: copies of what does not go straight to LDS (through registers, as few
-// rows do, 577 x 1001 -> 3001 in f64 took 22 us for 17; by words, three slices ahead, 24), long depths in parts where S is SMALL.
+// rows do, 577 x 1001 -> 3001 in f64 took 22 us for 17; by words, three slices ahead, 24), long depths
+// in parts where S is SMALL.
 template <typename T, typename S, bool SMALL>
 static int launch_lin_shape(LinArgs<T> g)
 {
