@@ -612,9 +612,11 @@ def _int64_rows(v, rows: int):
         v = v.astype(np.int64, copy=False)
         n, at = v.size, v.ctypes.data
     else:
-        v = v.contiguous()
         if str(v.dtype) != "torch.int64":
             raise ValueError(f"expected int64, got {v.dtype}")
+        if v.is_cuda and not v.is_contiguous():  # torch would copy them on its stream, not the library's
+            raise ValueError("expected contiguous tokens in device memory")
+        v = v.contiguous()
         n, at = v.numel(), v.data_ptr()
     if n != rows:
         raise ValueError(f"expected {rows} tokens, got {n}")

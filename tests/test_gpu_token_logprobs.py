@@ -467,6 +467,18 @@ def test_host_memory_while_capturing(pn, rng):
         pn.set_stream(None)
 
 
+def test_strided_tokens(pn, rng):
+    """In host memory they are copied; in device memory refused, as torch's copy would be on a stream
+    of its own."""
+    import torch
+    x, _ = _case(rng, 3, 50, np.float32)
+    m, tok = pn.TokenLogProbs(), torch.tensor([4, 0, 7, 0, 9, 0])
+    got = m(pn.Tensor.from_numpy(x), tok[::2]).logprob.numpy()
+    same_bits(got, _forward(pn, x, np.array([4, 7, 9]))["logprob"])
+    with pytest.raises(ValueError):
+        m(pn.Tensor.from_numpy(x), tok.cuda()[::2])
+
+
 def test_threads(pn, rng):
     import threading
     cases = [_case(rng, 3 + i, 20011 + 7000 * i, np.float32) for i in range(4)]
