@@ -483,8 +483,8 @@ __global__ __launch_bounds__(S::NT, S::PER_SIMD) void k_lin_mfma(LinArgs<T> g, i
 
 // ---- few rows ------------------------------------------------------------------------------------
 
-// Up to 16 rows: the weights are read once and are what the time goes to.  A block takes 16 output
-// channels; its 8 waves share out the depth, each with UN slices of 64 codes in flight from memory
+// Up to 16 rows, or groups of 16: the weights are read once a group and are what the time goes to.  A
+// block takes 16 output channels; its 8 waves share out the depth, each with UN slices of 64 codes in flight from memory
 // to registers, and add up in LDS.  Rows and weights may lie at any address.  1 x 4096 -> 4096 5.3
 // us (a launch alone 3.5; 64 x 64 tiles 11.2), 16 rows 6.6, 1 x 16384 -> 4096 12.6 (5.3 TB/s; 31).
 template <typename T, bool BYTES>
@@ -494,8 +494,8 @@ __global__ __launch_bounds__(512) void k_lin_few(LinArgs<T> g, int64_t b_base)
     __shared__ i32x4 part[W][64];
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int64_t n0 = (b_base + int64_t(blockIdx.x)) * 16;
-    const int r = lane & 15, u = lane >> 4;
-    const int8_t *pw = g.w + (n0 + r < g.n ? n0 + r : g.n - 1) * g.ldw, *pa = g.a + (r < g.m ? r : g.m - 1) * g.lda;
+    const int r = lane & 15, u = lane >> 4, m = 16 * int(blockIdx.y) + r;
+    const int8_t *pw = g.w + (n0 + r < g.n ? n0 + r : g.n - 1) * g.ldw, *pa = g.a + (m < g.m ? m : g.m - 1) * g.lda;
     i32x4 acc{0, 0, 0, 0};
     const int64_t slices = (g.k + 63) / 64, s0 = slices * w / W, s1 = slices * (w + 1) / W;
     for (int64_t s = s0; s < s1; s += UN) {
@@ -512,11 +512,11 @@ __global__ __launch_bounds__(512) void k_lin_few(LinArgs<T> g, int64_t b_base)
     }
     part[w][lane] = acc;
     __syncthreads();
-    // result v of lane l: row l % 16, channel 4 (l / 16) + v
+    // result v of lane l: row l % 16 of the block's, channel 4 (l / 16) + v
     if (w > 0) return;
 #pragma unroll
     for (int q = 1; q < W; q++) acc += part[q][lane];
-    const int64_t m = r, n = n0 + 4 * u;
+    const int64_t n = n0 + 4 * u;
     if (m < g.m && n < g.n) {
         const T sa = g.sa[m];
         T z[4];
@@ -624,13 +624,19 @@ static double lin_cost(int64_t m, int64_t n, const LinCost &c)
 template <typename T>
 static int launch_linear(const LinArgs<T> &g)
 {
-    // (wider, 64 x 64 tiles stream better what they do not copy: 1 x 4096 -> 16384 15.9 us, 13.3 by
-    // tiles; 16 rows of 4100 codes -> 16000 22.9 us, 35.5 with a copy of the weights; one of 4097
-    // 28.8 and 34.8)
-    if (g.m <= 16 && (ceil_div(g.n, 16) <= int64_t(num_cus()) * 2 || !lin_in_place(g.w, g.ldw))) {
-        for_row_launches(ceil_div(g.n, 16), 1, 512, [&](unsigned blocks, int64_t base) {
-            if (lin_words(g)) NH_LAUNCH((k_lin_few<T, false>), dim3(blocks), dim3(512), 0, stream(), g, base);
-            else NH_LAUNCH((k_lin_few<T, true>), dim3(blocks), dim3(512), 0, stream(), g, base);
+    // Up to 16 rows (wider, 64 x 64 tiles stream better what they do not copy: 1 x 4096 -> 16384 15.9
+    // us, 13.3 by tiles; 16 rows of 4100 codes -> 16000 22.9 us, 35.5 with a copy of the weights; one of
+    // 4097 28.8 and 34.8), and more in groups of 16 where that is still few blocks and spares the copy
+    // (64 x 1001 -> 1000 5.8 us, 9.6 with it; 32 x 4097 -> 4096 19.0, 22.7, 64 35.3, 23.3; 64 x 4100 ->
+    // 4096 22.0, 23.2; 17 x 16001 -> 1000 24.8, 21.8).
+    const int64_t blocks_n = ceil_div(g.n, 16), groups = ceil_div(g.m, 16), cus = num_cus();
+    const bool copied = !lin_in_place(g.w, g.ldw);
+    if (groups == 1 ? blocks_n <= 2 * cus || copied
+                    : copied && g.k <= 8192 && groups * blocks_n <= (lin_words(g) ? 4 : 2) * cus) {
+        for_row_launches(blocks_n, 1, 512 * groups, [&](unsigned blocks, int64_t base) {
+            const dim3 grid(blocks, unsigned(groups));
+            if (lin_words(g)) NH_LAUNCH((k_lin_few<T, false>), grid, dim3(512), 0, stream(), g, base);
+            else NH_LAUNCH((k_lin_few<T, true>), grid, dim3(512), 0, stream(), g, base);
         });
         return check_launch();
     }

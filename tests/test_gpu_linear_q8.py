@@ -140,6 +140,17 @@ def test_forms(pn, rng, dt, m, k, n):
 
 
 @pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("ld", [1001, 1002, 1004])
+@pytest.mark.parametrize("m,n", [(16, 8200), (17, 1000), (33, 700), (64, 100), (97, 1000), (129, 33), (500, 17), (32, 4096),
+                                 (48, 4100)])
+def test_unaligned_groups(pn, rng, dt, ld, m, n):
+    """Rows at strides of 1, 2 and 4 bytes' alignment in groups of 16, from an odd address too."""
+    c = _case(rng, m, 1001, n, dt)
+    _check(pn, c, act=8, lda=ld, ldw=ld)
+    _check(pn, c, res=False, lda=ld, ldw=ld, shift=3)
+
+
+@pytest.mark.parametrize("dt", DT)
 @pytest.mark.parametrize("act", range(13))
 def test_activations(pn, rng, dt, act):
     """Every activation, with every part of the epilogue there or not, over the values that the
