@@ -497,10 +497,13 @@ int neural_linear_q8(NeuralTensor *out, const int8_t *codes, int64_t stride, con
  * negative token: the row is not used (padding), its logits are not read: logprob, entropy and
  * lse 0, ids -1, alternatives' log probabilities -inf.  A token >= V: logprob NaN.
  *
- * Backward, from the saved lse and entropy: grad_logits = (g (1[v = token] - p) - e p (log p +
- * entropy)) / temperature, g and e the gradients of logprob and entropy (one value per row;
- * either may be NULL, not both; entropy may be NULL without e).  0 in a row that is not used or
- * has all logits masked; NaN where g is given and the token >= V.  grad_logits may be logits.
+ * Backward, from the forward call's lse and entropy of the same logits and temperature: grad_logits
+ * = (g (1[v = token] - p) - e p (log p + entropy)) / temperature, g and e the gradients of logprob
+ * and entropy (one value per row; either may be NULL, not both; entropy may be NULL without e).
+ * Where |lse| < 64 p is exp(z - lse): lse's rounding to f32 leaves at most 2^-19 of p.  Other rows
+ * (low temperatures, large logits) are summed again and take about twice the time.  0 in a row that
+ * is not used or has all logits masked; NaN where g is given and the token >= V.  grad_logits may
+ * be logits.
  *
  * Where a row is split over several blocks the forward call takes device memory for their
  * partial results, as neural_layer_norm_backward does.

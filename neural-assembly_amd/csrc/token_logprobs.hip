@@ -600,17 +600,23 @@ struct LpGradArgs {
     double inv_t;
 };
 
+// Where |lse| is below this, log p = x / T - lse from the saved lse: its rounding to f32 leaves at most
+// 2^-19 of p.  Beyond it the rounding grows with |lse|, which low temperatures and large logits make as
+// large as any number (past f32's range at T = 1e-10), so such rows are summed anew.
+constexpr double kLpNear = 64.0;
+
 // What a row's gradient is made of: dx = -p (g + e (log p + H)) / T, and + g / T at the token.
 // f32 rows: log2 p = x a + b in double, its exponential to f32's accuracy; f64 rows: log p.  p = 0
 // (a masked logit) leaves 0: log p is held above -inf.
 template <typename T>
 struct LpGradRow {
+    static constexpr double L = sizeof(T) == 4 ? 1.4426950408889634 : 1.0;
     double a, b, g, e, h;
     int64_t tok;
     bool zero;  // a row that is not used, or with every logit masked
+    bool far;   // lp_far_row's: whether all logits are masked, too, shows there
     NH_DEV LpGradRow(const LpGradArgs<T> &q, int64_t r)
     {
-        constexpr double L = sizeof(T) == 4 ? 1.4426950408889634 : 1.0;
         tok = q.tokens ? q.tokens[r] : -2;
         const double lse = double(q.lse[r]);
         a = q.inv_t * L;
@@ -619,31 +625,104 @@ struct LpGradRow {
         if (q.g && tok >= q.cols) g = __builtin_nan("");
         e = q.e ? double(q.e[r]) * q.inv_t : 0.0;
         h = q.e ? double(q.entropy[r]) : 0.0;
-        zero = (q.tokens && tok < 0) || lse == -__builtin_inf();
+        zero = q.tokens && tok < 0;
+        far = !zero && __builtin_fabs(lse) >= kLpNear;
     }
-    NH_DEV T operator()(T x, bool at) const
+    // p of its logarithm t (base 2 for f32 rows); lp: log p.
+    NH_DEV static double prob(double t, double &lp)
     {
-        double p, lp;
         if constexpr (sizeof(T) == 4) {
-            double t = __builtin_fma(double(x), a, b);
             t = t < -300.0 ? -300.0 : t;
             const double n = __builtin_rint(t);
-            p = double(__builtin_ldexpf(__builtin_amdgcn_exp2f(float(t - n)), int(n)));
             lp = t * 0.6931471805599453;
+            return double(__builtin_ldexpf(__builtin_amdgcn_exp2f(float(t - n)), int(n)));
         } else {
-            lp = __builtin_fma(x, a, b);
-            lp = lp < -2000.0 ? -2000.0 : lp;
-            p = exp(lp);
+            lp = t < -2000.0 ? -2000.0 : t;
+            return exp(lp);
         }
+    }
+    NH_DEV T operator()(double x, bool at) const
+    {
+        double lp;
+        const double p = prob(__builtin_fma(x, a, b), lp);
         const double v = -p * __builtin_fma(e, lp + h, g);
         return zero ? T(0) : T(at ? v + g : v);
     }
 };
 
+// A far row by NT lanes in two walks, UN vectors a lane in flight: its sums, s = sum exp((x - m) / T)
+// by the lane's largest logit m so far (factors in double where it rises, so that they add no error),
+// then the gradient of log p = (x - m) / T - log s.  One group does the whole row, as dx may be the
+// logits.
+template <typename T, int NT>
+NH_DEV void lp_far_row(const LpGradArgs<T> &q, LpGradRow<T> w, int64_t r, int lane)
+{
+    using V = typename Vec16<T>::type;
+    using U = typename VecU<T>::type;
+    using G = RowGrp<NT>;
+    constexpr int VN = Vec16<T>::n, UN = 4;
+    __shared__ double lds[2][G::kWaves];
+    const U *x = reinterpret_cast<const U *>(q.x + r * q.cols);
+    U *dx = reinterpret_cast<U *>(q.dx + r * q.cols);
+    const int ncv = int(q.cols / VN), rem = int(q.cols % VN);
+    const int64_t c = int64_t(ncv) * VN + lane;  // the value past the vectors
+    const T none = -T(__builtin_inf());
+    const T xt = lane < rem ? q.x[r * q.cols + c] : none;
+    T m = none;
+    double s = 0.0, lp;
+    for (int k0 = lane; k0 < ncv + NT; k0 += UN * NT) {  // (NT more: a turn at least, for xt)
+        V v[UN];
+        T top = k0 == lane ? xt : none;
+#pragma unroll
+        for (int u = 0; u < UN; u++) {
+#pragma unroll
+            for (int j = 0; j < VN; j++) v[u][j] = none;
+            if (k0 + u * NT < ncv) v[u] = x[k0 + u * NT];
+        }
+#pragma unroll
+        for (int u = 0; u < UN; u++)
+#pragma unroll
+            for (int j = 0; j < VN; j++) top = v[u][j] > top ? v[u][j] : top;
+        if (top > m) {
+            if (m != none) s *= exp((double(m) - double(top)) * q.inv_t);
+            m = top;
+        }
+        if (m == none) continue;
+        const auto term = [&](T y) { s += w.prob((double(y) - double(m)) * w.a, lp); };
+#pragma unroll
+        for (int u = 0; u < UN; u++)
+#pragma unroll
+            for (int j = 0; j < VN; j++) term(v[u][j]);
+        if (k0 == lane) term(xt);
+    }
+    if constexpr (NT > 64) __syncthreads();  // (a block may have two such rows)
+    const double most = G::max(double(m), lds[0]);
+    w.zero = most == -__builtin_inf();
+    s = G::sum(m == none ? 0.0 : s * exp((double(m) - most) * q.inv_t), lds[1]);
+    const double ref = w.zero ? 0.0 : most;
+    w.b = -log(s) * w.L;
+    for (int k0 = lane; k0 < ncv; k0 += UN * NT) {
+        V v[UN];
+#pragma unroll
+        for (int u = 0; u < UN; u++)
+            if (k0 + u * NT < ncv) v[u] = x[k0 + u * NT];
+#pragma unroll
+        for (int u = 0; u < UN; u++)
+            if (k0 + u * NT < ncv) {
+                V o;
+#pragma unroll
+                for (int j = 0; j < VN; j++) o[j] = w(double(v[u][j]) - ref, int64_t(k0 + u * NT) * VN + j == w.tok);
+                dx[k0 + u * NT] = o;
+            }
+    }
+    if (lane < rem) q.dx[r * q.cols + c] = w(double(xt) - ref, c == w.tok);
+}
+
 // Rows of at least kLpFlat f32 values (f64: half): the tensor as one run of vectors that begin at
 // 128-byte lines of dx, so that stores fill whole lines whatever the rows' width (f32 [4096, 50257],
-// whose rows start anywhere).  A block's 1024 vectors lie in two rows at most, mostly in one:
-// its numbers are the same for the block then, and nothing is read for a row of zeros.
+// whose rows start anywhere: 268 us, a copy of as many bytes 276; with all rows far 498).  A block's
+// 1024 vectors lie in two rows at most, mostly in one: its numbers are the same for the block then, and
+// nothing is read for a row that is not used.
 constexpr int64_t kLpFlat = 4096;
 template <typename T>
 __global__ __launch_bounds__(256) void k_lp_grad_flat(LpGradArgs<T> a, int64_t head, int64_t b_base)
@@ -658,7 +737,8 @@ __global__ __launch_bounds__(256) void k_lp_grad_flat(LpGradArgs<T> a, int64_t h
     const int left = nv - q0 < 256 * P ? int(nv - q0) : 256 * P, lane = threadIdx.x;
     if (r0 < a.rows) {
         const LpGradRow<T> w0(a, r0);
-        if (off + 256 * P * VN <= a.cols) {
+        const bool one = off + 256 * P * VN <= a.cols;
+        if (one && !w0.far) {
             const int64_t at = w0.tok - off;  // the token, from the block's first value
             V v[P];
             if (!w0.zero) {
@@ -679,20 +759,33 @@ __global__ __launch_bounds__(256) void k_lp_grad_flat(LpGradArgs<T> a, int64_t h
                     }
                     __builtin_nontemporal_store(o, dx + lane + k * 256);
                 }
-        } else {
+        } else if (!one) {
             const LpGradRow<T> w1(a, r0 + 1 < a.rows ? r0 + 1 : r0);
 #pragma unroll
             for (int k = 0; k < P; k++)
                 if (lane + k * 256 < left) {
-                    const V v = __builtin_nontemporal_load(x + lane + k * 256);
                     const int64_t c = off + int64_t(lane + k * 256) * VN;
-                    V o;
+                    if (!w0.far && !w1.far) {
+                        const V v = __builtin_nontemporal_load(x + lane + k * 256);
+                        V o;
 #pragma unroll
-                    for (int j = 0; j < VN; j++)
-                        o[j] = c + j < a.cols ? w0(v[j], c + j == w0.tok) : w1(v[j], c + j - a.cols == w1.tok);
-                    __builtin_nontemporal_store(o, dx + lane + k * 256);
+                        for (int j = 0; j < VN; j++)
+                            o[j] = c + j < a.cols ? w0(v[j], c + j == w0.tok) : w1(v[j], c + j - a.cols == w1.tok);
+                        __builtin_nontemporal_store(o, dx + lane + k * 256);
+                    } else {  // the values of the row that is not far
+                        const T *xs = reinterpret_cast<const T *>(x + lane + k * 256);
+                        T *dxs = reinterpret_cast<T *>(dx + lane + k * 256);
+                        for (int j = 0; j < VN; j++) {
+                            const bool second = c + j >= a.cols;
+                            if (second ? w1.far : w0.far) continue;
+                            dxs[j] = second ? w1(xs[j], c + j - a.cols == w1.tok) : w0(xs[j], c + j == w0.tok);
+                        }
+                    }
                 }
+            if (w1.far && r0 + 1 < a.rows) lp_far_row<T, 256>(a, w1, r0 + 1, lane);
         }
+        // a far row is the block's in which it begins (row 0: the first's)
+        if (w0.far && (off == 0 || first == head)) lp_far_row<T, 256>(a, w0, r0, lane);
     }
     // the values before the first vector and past the last
     if (b_base + int64_t(blockIdx.x) == 0 && threadIdx.x < 64) {
@@ -701,7 +794,7 @@ __global__ __launch_bounds__(256) void k_lp_grad_flat(LpGradArgs<T> a, int64_t h
         if (i < n) {
             const int64_t r = i / a.cols;
             const LpGradRow<T> w(a, r);
-            a.dx[i] = w(a.x[i], i - r * a.cols == w.tok);
+            if (!w.far) a.dx[i] = w(a.x[i], i - r * a.cols == w.tok);
         }
     }
 }
@@ -717,6 +810,10 @@ __global__ __launch_bounds__(256) void k_lp_grad_row(LpGradArgs<T> a, int64_t r_
     const int64_t r = r_base + int64_t(blockIdx.x) * RPB + sub;
     if (RPB > 1 && r >= a.rows) return;
     const LpGradRow<T> w(a, r);
+    if (w.far) {
+        lp_far_row<T, NT>(a, w, r, lane);
+        return;
+    }
     const T *x = a.x + r * a.cols;
     T *dx = a.dx + r * a.cols;
     const int ncv = int(a.cols / VN), rem = int(a.cols % VN);

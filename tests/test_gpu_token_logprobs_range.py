@@ -1,0 +1,141 @@
+"""Token log probabilities over the whole range of temperatures and logits: the gradient against
+a softmax in long double from the logits alone, not from the saved log-sum-exp."""
+
+import numpy as np
+import pytest
+
+import serving_ref as ref
+from conftest import GPU, same_bits
+from sublayer_ref import D, U, within
+from test_gpu_token_logprobs import _backward, _forward
+
+pytestmark = GPU
+
+DT = [np.float32, np.float64]
+L = np.longdouble
+
+
+def _grad_of_logits(x, tokens, g, e, temperature):
+    """The gradient, and its bound for a call from the lse and entropy that forward leaves.
+
+    s is off by es of itself (serving_ref.logprobs: each exponential to 8 u, each term's rounding in
+    double).  log p = (x - m) / T - log s: off by es and by 4 D of its terms.  Where |lse| < 64 it may be
+    x / T - lse instead, with lse rounded to the type: u |lse| more.  p: its exponential, 8 u, beside
+    that; the entropy: the forward call's bound; then as serving_ref.logprobs_grad."""
+    rows, V = x.shape
+    u, inv = U[x.dtype], 1 / L(temperature)
+    with np.errstate(all="ignore"):
+        xl = x.astype(L)
+        m = xl.max(1, keepdims=True)
+        masked = np.isneginf(m)
+        d = np.where(masked, L(0), xl - np.where(masked, L(0), m)) * inv
+        p = np.exp(d)
+        p = np.where(np.isneginf(xl), L(0), p)
+        dz = np.where(np.isneginf(d), L(0), d)
+        s = p.sum(1, keepdims=True)
+        mine = np.where(dz == 0, L(0), p)
+        es = u * (mine * (8 + np.abs(dz))).sum(1, keepdims=True) / s + (V + 8) * D * 2
+        ls = np.log(s)
+        lse = m * inv + ls
+        p, lp = p / s, dz - ls
+        want, bound = ref.logprobs(x, tokens, 0, temperature)
+        h, bh = want["entropy"][:, None], bound["entropy"][:, None]
+        at = (np.arange(V) == tokens[:, None]).astype(L)
+        gl = np.zeros((rows, 1), L) if g is None else g.astype(L)[:, None]
+        el = np.zeros((rows, 1), L) if e is None else e.astype(L)[:, None]
+        lz = np.where(p == 0, L(0), lp + h)
+        grad = (gl * (at - p) - el * p * lz) * inv
+        off = es + 4 * D * (np.abs(dz) + np.abs(ls))
+        off = off + np.where(np.abs(lse) < 65, u * np.abs(lse) + 4 * D * (np.abs(m * inv) + np.abs(dz) + np.abs(lse)), 0)
+        dp = np.where(p == 0, L(0), p * (8 * u + off))
+        dl = off + bh + u * np.abs(lz)
+        err = np.abs(gl) * (dp + 2 * u * np.abs(at - p)) + np.abs(el) * (dp * np.abs(lz) + p * dl + 3 * u * p * np.abs(lz))
+        tiny = ref.tiny_of(x.dtype) * (1 + inv) * (1 + np.abs(gl) + np.abs(el) * (1 + np.abs(lz)))
+        limit = 1.02 * inv * err + 2 * u * np.abs(grad) + 4 * tiny
+        zero = masked | (tokens < 0)[:, None]
+    return np.where(zero, L(0), grad), np.where(zero, L(0), limit)
+
+
+def _rows(rng, V, dt, temperature):
+    """Rows whose lse lies anywhere: sure ones with the likeliest token and another, ties, rivals within
+    a few temperatures, masks, rows that are not used, large and huge logits of both signs."""
+    x = rng.normal(0, 2.5, (14, V))
+    tokens = rng.integers(0, V, 14)
+    top = rng.integers(0, V, 14)
+    x[np.arange(14), top] += 22.7
+    tokens[0] = top[0]
+    x[2, tokens[2]] = x[2, top[2]]
+    near = rng.integers(0, V, 9)
+    x[3, near] = x[3, top[3]] - temperature * np.arange(9) / 2
+    tokens[3] = near[1]
+    x[4] = np.clip(temperature * rng.normal(0, 2.5, V), -1e30, 1e30)
+    x[5, rng.random(V) < 0.9] = -np.inf
+    tokens[5] = int(np.argmax(x[5]))
+    x[6] = -np.inf
+    tokens[7] = -1
+    x[8] = 1e5 * rng.normal(0, 1, V)
+    tokens[8] = int(np.argmax(x[8]))
+    x[9] = 1e30 * rng.normal(0, 1, V)
+    tokens[9] = int(np.argmax(x[9]))
+    x[10] = -1e30
+    x[11] = rng.normal(0, 1, V)
+    x[12] = -300.0 + x[12]
+    tokens[12] = top[12]
+    return x.astype(dt), tokens.astype(np.int64)
+
+
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("V", [3, 300, 1000, 2000, 4096, 5003, 40001])
+@pytest.mark.parametrize("temperature", [1e-10, 1e-6, 1e-4, 1e-3, 0.01, 0.3, 1.0, 30.0, 1e4, 1e10])
+def test_gradient_of_the_logits(pn, rng, dt, V, temperature):
+    x, tokens = _rows(rng, V, dt, temperature)
+    got = _forward(pn, x, tokens, 0, temperature)
+    g, e = rng.normal(0, 1, 14).astype(dt), rng.normal(0, 1, 14).astype(dt)
+    for a, b in ((g, None), (None, e), (g, e)):
+        dx = _backward(pn, x, tokens, a, b, got["lse"], got["entropy"], temperature)
+        want, bound = _grad_of_logits(x, tokens, a, b, temperature)
+        within(dx, want, bound, "dx")
+    assert not dx[[6, 7]].any()
+
+
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("V", [300, 2000, 4096, 4097, 5003, 40001])
+@pytest.mark.parametrize("shift", [0, 1, 5])
+def test_gradient_over_the_logits(pn, rng, dt, V, shift):
+    """In place, from any address, rows of both kinds side by side: the bits of a gradient elsewhere,
+    and nothing beside it touched."""
+    import torch
+    temperature, rows = 0.01, 14
+    x, tokens = _rows(rng, V, dt, temperature)
+    x[::3] *= dt(0.01)  # |lse| < 64 in every third row
+    got = _forward(pn, x, tokens, 0, temperature)
+    near = np.abs(got["lse"]) < 64
+    assert near.any() and not near.all()
+    g, e = rng.normal(0, 1, rows).astype(dt), rng.normal(0, 1, rows).astype(dt)
+    want = _backward(pn, x, tokens, g, e, got["lse"], got["entropy"], temperature)
+    big = torch.full((x.size + 64,), 5, dtype=torch.float32 if dt == np.float32 else torch.float64, device="cuda")
+    view = big[16 + shift:16 + shift + x.size].view(x.shape)
+    view.copy_(torch.from_numpy(x))
+    T = pn.Tensor
+    X, tok = T.from_torch(view), torch.from_numpy(tokens).cuda()
+    t = [T.from_numpy(v) for v in (g, e, got["lse"], got["entropy"])]
+    torch.cuda.synchronize()
+    assert pn.core._lib.neural_token_logprobs_backward(X._ptr, t[0]._ptr, t[1]._ptr, X._ptr, tok.data_ptr(), t[2]._ptr,
+                                                       t[3]._ptr, temperature) == 0
+    pn.synchronize()
+    same_bits(view.cpu().numpy(), want)
+    assert bool((big[:16 + shift] == 5).all()) and bool((big[16 + shift + x.size:] == 5).all())
+
+
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("temperature", [1e-6, 1e-3, 0.7])
+def test_gradient_of_a_sure_token_by_module(pn, rng, dt, temperature):
+    """The likeliest token's own gradient is g (1 - p) / T: nothing where nothing else is likely."""
+    x, tokens = _rows(rng, 1000, dt, temperature)
+    x, tokens = x[:1].copy(), tokens[:1]
+    m = pn.TokenLogProbs(temperature=temperature)
+    m(pn.Tensor.from_numpy(x), tokens)
+    g = np.ones(1, dt)
+    dx = m.backward(pn.Tensor.from_numpy(g)).numpy()
+    want, bound = _grad_of_logits(x, tokens, g, None, temperature)
+    within(dx, want, bound, "dx")
