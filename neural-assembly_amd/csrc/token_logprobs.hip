@@ -80,6 +80,13 @@ struct LpPart {
     double m, s, t;
 };
 
+// A part's t moved by d, times f = exp(d / T).  Where f is 0 nothing of it is left, but d s may lie past
+// double's range (logits at its lowest value as masks).  NaN stays.
+NH_DEV double lp_moved(const LpPart &p, double d, double f)
+{
+    return f == 0.0 ? f * p.t : f * (p.t + d * p.s);
+}
+
 // The sums of two parts by the larger m.  A part without values (m -inf) has s = t = 0, or NaN
 // where it holds NaN, which stays.
 NH_DEV LpPart lp_join(const LpPart &a, const LpPart &b, double inv_t)
@@ -87,7 +94,7 @@ NH_DEV LpPart lp_join(const LpPart &a, const LpPart &b, double inv_t)
     const double none = -__builtin_inf(), m = __builtin_fmax(a.m, b.m);
     const double da = a.m == none ? 0.0 : a.m - m, db = b.m == none ? 0.0 : b.m - m;
     const double fa = a.m == none ? 0.0 : exp(da * inv_t), fb = b.m == none ? 0.0 : exp(db * inv_t);
-    return {m, a.s * fa + b.s * fb, fa * (a.t + da * a.s) + fb * (b.t + db * b.s)};
+    return {m, a.s * fa + b.s * fb, lp_moved(a, da, fa) + lp_moved(b, db, fb)};
 }
 
 // The same over a wave's lanes: one exponential for each.
@@ -96,7 +103,7 @@ NH_DEV LpPart lp_join_wave(const LpPart &p, double inv_t)
     const double m = RowGrp<64>::max(p.m, nullptr);
     const bool any = p.m != -__builtin_inf();
     const double d = any ? p.m - m : 0.0, f = any ? exp(d * inv_t) : 0.0;
-    return {m, wave_dsum(p.s * f), wave_dsum(f * (p.t + d * p.s))};
+    return {m, wave_dsum(p.s * f), wave_dsum(lp_moved(p, d, f))};
 }
 
 // A row's results from its sums.

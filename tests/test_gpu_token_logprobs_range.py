@@ -139,3 +139,34 @@ def test_gradient_of_a_sure_token_by_module(pn, rng, dt, temperature):
     dx = m.backward(pn.Tensor.from_numpy(g)).numpy()
     want, bound = _grad_of_logits(x, tokens, g, None, temperature)
     within(dx, want, bound, "dx")
+
+
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("V", [3, 300, 513, 700, 3000, 5003, 20011, 40001])
+@pytest.mark.parametrize("temperature", [0.5, 1.0, 1e10])
+def test_masks_of_the_lowest_value(pn, rng, dt, V, temperature):
+    """Logits ruled out by the type's lowest value, or others far from the largest, in whole waves and
+    parts: sums, alternatives, and the gradient."""
+    low = np.finfo(dt).min
+    x, tokens = _rows(rng, V, dt, 1.0)
+    x[9:11] = x[3:5]
+    tokens[9:11] = V // 2
+    keep = {r: rng.integers(0, V, 3) for r in range(9)}
+    for r, at in keep.items():
+        row = np.full(V, (low, low / 2, -1e300 if dt == np.float64 else -1e30)[r % 3], dt)
+        row[at], row[tokens[r]] = x[r, at], x[r, tokens[r]]
+        x[r] = row
+    x[6] = low
+    x[11] = np.where(np.arange(V) < V // 2, low, -np.inf)
+    x[11, V - 1] = 2.0
+    got = _forward(pn, x, tokens, 5, temperature)
+    want, bound = ref.logprobs(x, tokens, 5, temperature)
+    for n in ("logprob", "entropy", "lse", "top"):
+        with np.errstate(all="ignore"):
+            rounded = want[n].astype(dt)
+        within(got[n], np.where(np.isinf(rounded), rounded, want[n]), bound[n], n)  # (past the type's range)
+    assert np.array_equal(got["ids"], want["ids"]) and not np.isnan(got["entropy"]).any()
+    g, e = rng.normal(0, 1, 14).astype(dt), rng.normal(0, 1, 14).astype(dt)
+    dx = _backward(pn, x, tokens, g, e, got["lse"], got["entropy"], temperature)
+    want, bound = _grad_of_logits(x, tokens, g, e, temperature)
+    within(dx, want, bound, "dx")
