@@ -431,7 +431,7 @@ int neural_dropout_add_layer_norm_backward(NeuralTensor *grad_in, NeuralTensor *
  * values, NULL: 1), in double, rounded once per value.  hidden: h, for the residual stream
  * and the backward call (NULL where neither follows, and where residual is NULL: h is in
  * then); rstd: one value per row, for the backward call (may be NULL).  out or hidden may be
- * in or residual.  A row whose sum of squares is not finite is NaN.
+ * in or residual.  A row whose sum of squares is not finite is NaN, and so is one of zeros with eps 0.
  *
  * neural_rms_norm_backward, from the saved rstd: xh = hidden rstd, w = grad_out gamma,
  * grad_in = rstd (w - xh mean_C(w xh)) [rounded, + grad_hidden, the gradient that reaches

@@ -63,10 +63,12 @@ struct RowCodes {
         const int i = whole(__builtin_fabs(w));
         return live ? (w < 0.0 ? -i : i) : 0;
     }
-    // scale of codes that stand for w * by
+    // scale of codes that stand for w * by.  A row of zeros has 0, also where `by` is infinite (the norm
+    // of one with eps = 0).
     NH_DEV T scale(double a0, double by) const
     {
         if (!(a0 < __builtin_inf())) return T(__builtin_nan(""));
+        if (a0 == 0.0 && by == by) return T(0);
         return T(a / 127.0 * by / up);
     }
 };
