@@ -114,7 +114,11 @@ struct LpRow {
         return {p.m == -__builtin_inf() ? 0.0 : p.m, it, p.s, log(p.s)};
     }
     NH_DEV bool sound() const { return s == s; }
-    NH_DEV double logprob(double x) const { return s == 0.0 ? -__builtin_inf() : (x - m) * inv_t - ls; }
+    // (halves: the difference of two f64 logits may pass double's range where that over T does not)
+    NH_DEV double logprob(double x) const
+    {
+        return s == 0.0 ? -__builtin_inf() : (0.5 * x - 0.5 * m) * (2.0 * inv_t) - ls;
+    }
     NH_DEV double lse() const { return m * inv_t + ls; }
     NH_DEV double entropy(double t) const { return s == 0.0 ? 0.0 : ls - t * inv_t / s; }
 };

@@ -170,3 +170,24 @@ def test_masks_of_the_lowest_value(pn, rng, dt, V, temperature):
     dx = _backward(pn, x, tokens, g, e, got["lse"], got["entropy"], temperature)
     want, bound = _grad_of_logits(x, tokens, g, e, temperature)
     within(dx, want, bound, "dx")
+
+
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("V", [40, 700, 40001])
+@pytest.mark.parametrize("temperature", [2.0, 50.0, 1e10])
+def test_differences_past_the_range(pn, rng, dt, V, temperature):
+    """Logits of both signs near the type's largest value: (x - m) / T is within its range where x - m
+    is not."""
+    big = dt(0.9) * np.finfo(dt).max
+    x = (rng.uniform(-1, 1, (6, V)) * big).astype(dt)
+    x[:, V // 3] = big
+    tokens = np.argmin(x, 1)
+    tokens[4:] = np.argmax(x[4:], 1)
+    x[3, 1:] = -big
+    x[3, V // 3] = big
+    got = _forward(pn, x, tokens, 7, temperature)
+    want, bound = ref.logprobs(x, tokens, 7, temperature)
+    assert np.isfinite(got["logprob"]).all()
+    for n in ("logprob", "entropy", "lse", "top"):
+        within(got[n], want[n], bound[n], n)
+    assert np.array_equal(got["ids"], want["ids"])
