@@ -488,7 +488,8 @@ int neural_linear_q8(NeuralTensor *out, const int8_t *codes, int64_t stride, con
  *
  * Forward, every output one value per row in the logits' dtype, any of them NULL, not all:
  * logprob = z[token] - lse, entropy = -sum p log p (a term of p = 0 is 0), lse (for the
- * backward call), and the k (0 to 64) largest logits, equal ones by index: top_ids [rows, k]
+ * backward call; a tensor of four values per row takes what that call needs of it: lse, m = max
+ * logit, log sum_v exp((logit_v - m) / temperature), entropy), and the k (0 to 64) largest logits, equal ones by index: top_ids [rows, k]
  * int64 (host or device memory) and top_logprobs [rows, k] (either may be NULL).
  * A logit of -inf is a masked one: it is no alternative, and where fewer than k are left the
  * rest is id -1, log probability -inf.  A row with all logits masked has lse and logprob
@@ -499,11 +500,12 @@ int neural_linear_q8(NeuralTensor *out, const int8_t *codes, int64_t stride, con
  *
  * Backward, from the forward call's lse and entropy of the same logits and temperature: grad_logits
  * = (g (1[v = token] - p) - e p (log p + entropy)) / temperature, g and e the gradients of logprob
- * and entropy (one value per row; either may be NULL, not both; entropy may be NULL without e).
- * Where |lse| < 64 p is exp(z - lse): lse's rounding to f32 leaves at most 2^-19 of p.  Other rows
- * (low temperatures, large logits) are summed again and take about twice the time.  0 in a row that
- * is not used or has all logits masked; NaN where g is given and the token >= V.  grad_logits may
- * be logits.
+ * and entropy (one value per row; either may be NULL, not both).  entropy may be NULL without e, and
+ * with lse of four values per row, whose fourth is taken.  Where |lse| < 64 p is exp(z - lse): lse's
+ * rounding to f32 leaves at most 2^-19 of p.  Other rows (low temperatures, large logits) take m and
+ * the log of their sum from lse's four values; with one they are summed again, in twice the time, and
+ * in more where they are few and wide.  0 in a row that is not used or has all logits masked; NaN
+ * where g is given and the token >= V.  grad_logits may be logits.
  *
  * Where a row is split over several blocks the forward call takes device memory for their
  * partial results, as neural_layer_norm_backward does.

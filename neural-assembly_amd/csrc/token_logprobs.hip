@@ -3,7 +3,7 @@
 //
 //   z = x / temperature; with m = max x and d = x - m: s = sum exp(d / T), t = sum exp(d / T) d / T;
 //   lse = m / T + log s; logprob = (x_t - m) / T - log s; entropy = log s - t / s
-//   gradient: (g (1_t - p) - e p (log p + H)) / T, p = exp(z - lse)
+//   gradient: (g (1_t - p) - e p (log p + H)) / T, log p = z - lse, or (x - m) / T - log s
 //
 // s and t are summed in double: where one token has nearly all the probability, logprob and
 // entropy are as small as the rest of s, which a sum in float would round away beside 1.
@@ -71,6 +71,7 @@ struct LpArgs {
     int64_t *top_ids;                     // or null
     int64_t rows, cols;
     int k;
+    bool four;  // lse holds four values a row: lse, m, log s, entropy
     double inv_t;
 };
 
@@ -133,7 +134,13 @@ NH_DEV void lp_store(const LpArgs<T> &a, int64_t r, int64_t tok, T logit, const 
 {
     if (a.logprob) a.logprob[r] = tok < a.cols ? T(row.logprob(double(logit))) : T(__builtin_nan(""));
     if (a.entropy) a.entropy[r] = T(row.entropy(t));
-    if (a.lse) a.lse[r] = T(row.lse());
+    if (a.lse && a.four) {
+        const T v[4] = {T(row.lse()), T(row.m), T(row.ls), T(row.entropy(t))};
+#pragma unroll
+        for (int q = 0; q < 4; q++) a.lse[4 * r + q] = v[q];
+    } else if (a.lse) {
+        a.lse[r] = T(row.lse());
+    }
 }
 template <typename T>
 NH_DEV void lp_store_top(const LpArgs<T> &a, int64_t r, int q, const LpKey<T> &k, const LpRow &row)
@@ -149,7 +156,8 @@ NH_DEV void lp_unused(const LpArgs<T> &a, int64_t r, int lane)
     if (lane == 0) {
         if (a.logprob) a.logprob[r] = T(0);
         if (a.entropy) a.entropy[r] = T(0);
-        if (a.lse) a.lse[r] = T(0);
+        if (a.lse)
+            for (int q = 0; q < (a.four ? 4 : 1); q++) a.lse[(a.four ? 4 : 1) * r + q] = T(0);
     }
     for (int q = lane; q < a.k; q += NT) {
         if (a.top_ids) a.top_ids[r * a.k + q] = -1;
@@ -608,12 +616,14 @@ struct LpGradArgs {
     const int64_t *tokens;               // or null
     T *dx;
     int64_t rows, cols;
+    bool four;  // lse holds four values a row
     double inv_t;
 };
 
 // Where |lse| is below this, log p = x / T - lse from the saved lse: its rounding to f32 leaves at most
 // 2^-19 of p.  Beyond it the rounding grows with |lse|, which low temperatures and large logits make as
-// large as any number (past f32's range at T = 1e-10), so such rows are summed anew.
+// large as any number (past f32's range at T = 1e-10): such rows take (x - m) / T - log s, from the four
+// values that the forward call left of them, or are summed anew.
 constexpr double kLpNear = 64.0;
 
 // What a row's gradient is made of: dx = -p (g + e (log p + H)) / T, and + g / T at the token.
@@ -622,22 +632,31 @@ constexpr double kLpNear = 64.0;
 template <typename T>
 struct LpGradRow {
     static constexpr double L = sizeof(T) == 4 ? 1.4426950408889634 : 1.0;
-    double a, b, g, e, h;
+    double a, b, ref, g, e, h;
     int64_t tok;
     bool zero;  // a row that is not used, or with every logit masked
     bool far;   // lp_far_row's: whether all logits are masked, too, shows there
     NH_DEV LpGradRow(const LpGradArgs<T> &q, int64_t r)
     {
         tok = q.tokens ? q.tokens[r] : -2;
-        const double lse = double(q.lse[r]);
+        const T *saved = q.lse + (q.four ? 4 * r : r);
+        const double lse = double(saved[0]);
         a = q.inv_t * L;
         b = -lse * L;
+        ref = 0.0;
         g = q.g ? double(q.g[r]) * q.inv_t : 0.0;
         if (q.g && tok >= q.cols) g = __builtin_nan("");
         e = q.e ? double(q.e[r]) * q.inv_t : 0.0;
-        h = q.e ? double(q.entropy[r]) : 0.0;
+        h = q.e ? double(q.four ? saved[3] : q.entropy[r]) : 0.0;
         zero = q.tokens && tok < 0;
         far = !zero && __builtin_fabs(lse) >= kLpNear;
+        if (far && q.four) {
+            far = false;
+            const double ls = double(saved[2]);
+            ref = double(saved[1]);
+            b = -ls * L;
+            zero = ls == -__builtin_inf();
+        }
     }
     // p of its logarithm t (base 2 for f32 rows); lp: log p.
     NH_DEV static double prob(double t, double &lp)
@@ -652,10 +671,10 @@ struct LpGradRow {
             return exp(lp);
         }
     }
-    NH_DEV T operator()(double x, bool at) const
+    NH_DEV T operator()(T x, bool at) const
     {
         double lp;
-        const double p = prob(__builtin_fma(x, a, b), lp);
+        const double p = prob(__builtin_fma(double(x) - ref, a, b), lp);
         const double v = -p * __builtin_fma(e, lp + h, g);
         return zero ? T(0) : T(at ? v + g : v);
     }
@@ -710,7 +729,7 @@ NH_DEV void lp_far_row(const LpGradArgs<T> &q, LpGradRow<T> w, int64_t r, int la
     const double most = G::max(double(m), lds[0]);
     w.zero = most == -__builtin_inf();
     s = G::sum(m == none ? 0.0 : s * exp((double(m) - most) * q.inv_t), lds[1]);
-    const double ref = w.zero ? 0.0 : most;
+    w.ref = w.zero ? 0.0 : most;
     w.b = -log(s) * w.L;
     for (int k0 = lane; k0 < ncv; k0 += UN * NT) {
         V v[UN];
@@ -722,18 +741,18 @@ NH_DEV void lp_far_row(const LpGradArgs<T> &q, LpGradRow<T> w, int64_t r, int la
             if (k0 + u * NT < ncv) {
                 V o;
 #pragma unroll
-                for (int j = 0; j < VN; j++) o[j] = w(double(v[u][j]) - ref, int64_t(k0 + u * NT) * VN + j == w.tok);
+                for (int j = 0; j < VN; j++) o[j] = w(v[u][j], int64_t(k0 + u * NT) * VN + j == w.tok);
                 dx[k0 + u * NT] = o;
             }
     }
-    if (lane < rem) q.dx[r * q.cols + c] = w(double(xt) - ref, c == w.tok);
+    if (lane < rem) q.dx[r * q.cols + c] = w(xt, c == w.tok);
 }
 
 // Rows of at least kLpFlat f32 values (f64: half): the tensor as one run of vectors that begin at
 // 128-byte lines of dx, so that stores fill whole lines whatever the rows' width (f32 [4096, 50257],
-// whose rows start anywhere: 268 us, a copy of as many bytes 276; with all rows far 498).  A block's
-// 1024 vectors lie in two rows at most, mostly in one: its numbers are the same for the block then, and
-// nothing is read for a row that is not used.
+// whose rows start anywhere: 268 us, a copy of as many bytes 276; with all rows far 498, 267 from four
+// values; one far row of 131072 70 us and 4.1).  A block's 1024 vectors lie in two rows at most, mostly
+// in one: its numbers are the same for the block then, and nothing is read for a row that is not used.
 constexpr int64_t kLpFlat = 4096;
 template <typename T>
 __global__ __launch_bounds__(256) void k_lp_grad_flat(LpGradArgs<T> a, int64_t head, int64_t b_base)
@@ -935,6 +954,13 @@ struct LpTensors {
 // (f32 rows have 1 / T and differences of logits times their weight in float)
 static bool lp_temperature(double t) { return t >= 1e-10 && t <= 1e10; }
 
+// lse of one value a row, or four.
+static bool lp_four(const NeuralTensor *lse, const RowCall &c) { return lse && numel(lse) != c.rows; }
+static int lp_check_lse(const NeuralTensor *lse, const RowCall &c)
+{
+    return c.vec(lse, lse && numel(lse) == 4 * c.rows ? 4 * c.rows : c.rows);
+}
+
 template <typename T>
 static int lp_run(const LpTensors &t, const RowCall &c, double temperature, const Staged &tokens, const Staged &ids)
 {
@@ -942,6 +968,7 @@ static int lp_run(const LpTensors &t, const RowCall &c, double temperature, cons
     a.rows = c.rows;
     a.cols = c.cols;
     a.k = int(t.k);
+    a.four = lp_four(t.lse, c);
     a.inv_t = 1.0 / temperature;
     a.tokens = static_cast<const int64_t *>(tokens.dev);
     a.top_ids = static_cast<int64_t *>(ids.dev);
@@ -969,7 +996,7 @@ static int lp_forward(LpTensors t, double temperature)
     NH_TRY(c.open(t.logits));
     NH_TRY(c.vec(t.logprob, c.rows));
     NH_TRY(c.vec(t.entropy, c.rows));
-    NH_TRY(c.vec(t.lse, c.rows));
+    NH_TRY(lp_check_lse(t.lse, c));
     NH_TRY(c.vec(t.top_lp, c.rows * t.k));
     if (!lp_temperature(temperature)) return set_error(NEURAL_ERR_INVALID_ARGUMENT);
     if (c.cols >= int64_t(1) << 31) return set_error(NEURAL_ERR_TENSOR_TOO_LARGE);
@@ -1003,6 +1030,7 @@ static int lp_grad_run(const LpGradTensors &t, const RowCall &c, double temperat
     LpGradArgs<T> a{};
     a.rows = c.rows;
     a.cols = c.cols;
+    a.four = lp_four(t.lse, c);
     a.inv_t = 1.0 / temperature;
     a.tokens = static_cast<const int64_t *>(tokens.dev);
     NH_TRY(read_t(t.logits, a.x));
@@ -1018,15 +1046,15 @@ static int lp_grad_run(const LpGradTensors &t, const RowCall &c, double temperat
 static int lp_backward(const LpGradTensors &t, double temperature)
 {
     NH_TRY(ensure_init());
-    if (!t.dx || !t.logits || !t.lse || (!t.g && !t.e) || (t.g && !t.tokens) || (t.e && !t.entropy))
-        return set_error(NEURAL_ERR_NULL_POINTER);
+    if (!t.dx || !t.logits || !t.lse || (!t.g && !t.e) || (t.g && !t.tokens)) return set_error(NEURAL_ERR_NULL_POINTER);
     RowCall c;
     NH_TRY(c.open(t.logits));
     NH_TRY(c.same(t.dx));
     NH_TRY(c.vec(t.g, c.rows));
     NH_TRY(c.vec(t.e, c.rows));
-    NH_TRY(c.vec(t.lse, c.rows));
+    NH_TRY(lp_check_lse(t.lse, c));
     NH_TRY(c.vec(t.entropy, c.rows));
+    if (t.e && !t.entropy && !lp_four(t.lse, c)) return set_error(NEURAL_ERR_NULL_POINTER);
     if (!lp_temperature(temperature)) return set_error(NEURAL_ERR_INVALID_ARGUMENT);
     if (c.cols >= int64_t(1) << 31) return set_error(NEURAL_ERR_TENSOR_TOO_LARGE);
     NH_TRY(check_apart({t.dx}, {t.logits, t.g, t.e, t.lse, t.entropy}, 1));

@@ -551,8 +551,11 @@ class TokenLogProbs(Module):
     memory; without them logprob is None.  ``forward`` returns (logprob, entropy,
     top_ids, top_logprobs): Tensors of one value per row, an int64 numpy array
     [rows, top_k] and a Tensor [rows, top_k] (both None where top_k is 0).
-    ``backward``, of the last forward, takes the gradients of logprob and entropy
-    (either may be None), reads logits and tokens again and returns the logits'."""
+    ``backward``, of the last forward and its temperature, takes the gradients of logprob
+    and entropy (either may be None), reads logits and tokens again (not to be changed in
+    place before it) and returns the logits'.  The ids come to the host with the forward
+    call, which waits for them; code under graph capture passes device memory to the entry
+    point."""
 
     def __init__(self, temperature: float = 1.0, top_k: int = 0):
         super().__init__()
@@ -570,26 +573,26 @@ class TokenLogProbs(Module):
             raise ValueError(f"expected a last dimension of at least 1, got shape {src.shape}")
         rows = src.numel // src.shape[-1]
         held, at = _int64_rows(tokens, rows)
-        entropy, lse = Tensor.create([rows], src.dtype), Tensor.create([rows], src.dtype)
+        entropy, saved = Tensor.create([rows], src.dtype), Tensor.create([rows, 4], src.dtype)
         logprob = Tensor.create([rows], src.dtype) if at is not None else None
         ids = np.empty((rows, self.top_k), dtype=np.int64) if self.top_k else None
         top = Tensor.create([rows, self.top_k], src.dtype) if self.top_k else None
-        rc = _lib.neural_token_logprobs_forward(_ptr(logprob), entropy._ptr, lse._ptr,
+        rc = _lib.neural_token_logprobs_forward(_ptr(logprob), entropy._ptr, saved._ptr,
                                                 ids.ctypes.data if self.top_k else None, _ptr(top), self.top_k,
                                                 src._ptr, at, self.temperature)
         _check_error(rc, "token log probabilities forward")
-        self._saved = (src, held, at, lse, entropy)
+        self._saved = (src, held, at, saved, self.temperature)
         return TokenLogProbsOut(logprob, entropy, ids, top)
 
     def backward(self, grad_logprob: Tensor = None, grad_entropy: Tensor = None) -> Tensor:
         if self._saved is None:
             raise RuntimeError("TokenLogProbs.backward called before forward")
-        src, _, at, lse, entropy = self._saved
+        src, _, at, saved, temperature = self._saved
         g = grad_logprob.contiguous() if grad_logprob is not None else None
         e = grad_entropy.contiguous() if grad_entropy is not None else None
         out = Tensor.create(src.shape, src.dtype)
-        rc = _lib.neural_token_logprobs_backward(out._ptr, _ptr(g), _ptr(e), src._ptr, at, lse._ptr, entropy._ptr,
-                                                 self.temperature)
+        rc = _lib.neural_token_logprobs_backward(out._ptr, _ptr(g), _ptr(e), src._ptr, at, saved._ptr, None,
+                                                 temperature)
         _check_error(rc, "token log probabilities backward")
         return out
 

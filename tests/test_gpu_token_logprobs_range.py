@@ -15,8 +15,9 @@ DT = [np.float32, np.float64]
 L = np.longdouble
 
 
-def _grad_of_logits(x, tokens, g, e, temperature):
-    """The gradient, and its bound for a call from the lse and entropy that forward leaves.
+def _grad_of_logits(x, tokens, g, e, temperature, four=False):
+    """The gradient, and its bound for a call from the lse and entropy that forward leaves (four: from
+    its four values, log s rounded to the type: u log s more).
 
     s is off by es of itself (serving_ref.logprobs: each exponential to 8 u, each term's rounding in
     double).  log p = (x - m) / T - log s: off by es and by 4 D of its terms.  Where |lse| < 64 it may be
@@ -45,7 +46,7 @@ def _grad_of_logits(x, tokens, g, e, temperature):
         el = np.zeros((rows, 1), L) if e is None else e.astype(L)[:, None]
         lz = np.where(p == 0, L(0), lp + h)
         grad = (gl * (at - p) - el * p * lz) * inv
-        off = es + 4 * D * (np.abs(dz) + np.abs(ls))
+        off = es + 4 * D * (np.abs(dz) + np.abs(ls)) + (u * np.abs(ls) if four else 0)
         off = off + np.where(np.abs(lse) < 65, u * np.abs(lse) + 4 * D * (np.abs(m * inv) + np.abs(dz) + np.abs(lse)), 0)
         dp = np.where(p == 0, L(0), p * (8 * u + off))
         dl = off + bh + u * np.abs(lz)
@@ -137,7 +138,7 @@ def test_gradient_of_a_sure_token_by_module(pn, rng, dt, temperature):
     m(pn.Tensor.from_numpy(x), tokens)
     g = np.ones(1, dt)
     dx = m.backward(pn.Tensor.from_numpy(g)).numpy()
-    want, bound = _grad_of_logits(x, tokens, g, None, temperature)
+    want, bound = _grad_of_logits(x, tokens, g, None, temperature, True)
     within(dx, want, bound, "dx")
 
 
@@ -191,3 +192,77 @@ def test_differences_past_the_range(pn, rng, dt, V, temperature):
     for n in ("logprob", "entropy", "lse", "top"):
         within(got[n], want[n], bound[n], n)
     assert np.array_equal(got["ids"], want["ids"])
+
+
+@pytest.mark.parametrize("dt", DT)
+def test_module_between_the_calls(pn, rng, dt):
+    """What a caller does to the returned entropy and to the module's temperature between forward and
+    backward does not reach the gradient."""
+    T = pn.Tensor
+    x, tokens = _rows(rng, 600, dt, 0.8)
+    g, e = T.from_numpy(rng.normal(0, 1, 14).astype(dt)), T.from_numpy(rng.normal(0, 1, 14).astype(dt))
+    m = pn.TokenLogProbs(temperature=0.8)
+    m(T.from_numpy(x), tokens)
+    want = m.backward(g, e).numpy()
+    o = m(T.from_numpy(x), tokens)
+    o.entropy.fill(7.0)
+    o.logprob.fill(7.0)
+    m.temperature = 3.0
+    same_bits(m.backward(g, e).numpy(), want)
+
+
+def _four(pn, x, tokens, temperature):
+    """lse of four values per row, alone."""
+    import torch
+    T = pn.Tensor
+    X, tok = T.from_numpy(x), torch.from_numpy(tokens).cuda()
+    saved = T.create([x.shape[0], 4], X.dtype)
+    torch.cuda.synchronize()
+    assert pn.core._lib.neural_token_logprobs_forward(None, None, saved._ptr, None, None, 0, X._ptr, tok.data_ptr(),
+                                                      temperature) == 0
+    return saved.numpy()
+
+
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("V", [3, 300, 2000, 4096, 5003, 40001])
+@pytest.mark.parametrize("temperature", [1e-10, 1e-4, 0.01, 1.0, 1e10])
+def test_four_saved_values(pn, rng, dt, V, temperature):
+    """What they hold; the gradient from them, with the bits that one value gives where |lse| < 64."""
+    x, tokens = _rows(rng, V, dt, temperature)
+    got = _forward(pn, x, tokens, 0, temperature)
+    four = _four(pn, x, tokens, temperature)
+    same_bits(four[:, 0], got["lse"])
+    same_bits(four[:, 3], got["entropy"])
+    used = tokens >= 0
+    top = x.max(1)
+    masked = np.isneginf(top)
+    assert np.array_equal(four[used, 1], np.where(masked, dt(0), top)[used]) and not four[~used].any()
+    assert np.isneginf(four[masked & used, 2]).all() and np.isfinite(four[~masked, 2]).all()
+    g, e = rng.normal(0, 1, 14).astype(dt), rng.normal(0, 1, 14).astype(dt)
+    near = np.abs(got["lse"]) < 64
+    for a, b in ((g, None), (None, e), (g, e)):
+        one = _backward(pn, x, tokens, a, b, got["lse"], got["entropy"], temperature)
+        dx = _backward(pn, x, tokens, a, b, four, None, temperature)
+        same_bits(dx[near], one[near])
+        want, bound = _grad_of_logits(x, tokens, a, b, temperature, True)
+        within(dx, want, bound, "dx")
+
+
+def test_four_saved_values_refused(pn):
+    """Counts other than one and four a row, and no entropy beside one."""
+    E, lib, T = pn.NeuralError, pn.core._lib, pn.Tensor
+    x, dx, g, tok = T.zeros([3, 9]), T.zeros([3, 9]), T.zeros([3]), np.zeros(3, np.int64)
+    forward, backward = lib.neural_token_logprobs_forward, lib.neural_token_logprobs_backward
+    for n in (0, 1, 6, 9, 13):
+        s = T.create([n])
+        assert forward(None, None, s._ptr, None, None, 0, x._ptr, tok.ctypes.data, 1.0) == E.SHAPE_MISMATCH
+        assert backward(dx._ptr, g._ptr, None, x._ptr, tok.ctypes.data, s._ptr, None, 1.0) == E.SHAPE_MISMATCH
+    one, four, five = T.zeros([3]), T.zeros([3, 4]), T.zeros([5])
+    assert backward(dx._ptr, g._ptr, g._ptr, x._ptr, tok.ctypes.data, one._ptr, None, 1.0) == E.NULL_POINTER
+    assert backward(dx._ptr, g._ptr, g._ptr, x._ptr, tok.ctypes.data, four._ptr, five._ptr, 1.0) == E.SHAPE_MISMATCH
+    assert forward(None, four._ptr, None, None, None, 0, x._ptr, tok.ctypes.data, 1.0) == E.SHAPE_MISMATCH
+    assert forward(None, None, x._ptr, None, None, 0, x._ptr, tok.ctypes.data, 1.0) == E.SHAPE_MISMATCH
+    for v in (four, dx, g):
+        assert not v.numpy().any()
+    assert forward(None, None, four._ptr, None, None, 0, x._ptr, tok.ctypes.data, 1.0) == E.OK
+    assert backward(dx._ptr, g._ptr, g._ptr, x._ptr, tok.ctypes.data, four._ptr, None, 1.0) == E.OK
