@@ -173,7 +173,8 @@ struct LinShape {
     static constexpr int kOut = 32 * TN + 4;                             // the epilogue's rows of a wave
     static_assert(BM % (kRows * NW) == 0 && BN % (kRows * NW) == 0, "whole loads per wave");
     static constexpr int kLoadsA = BM / kRows / NW;
-    static constexpr bool kCut = TM * TN == 1;  // (of larger tiles the registers for it would spill)
+    // (of larger tiles the registers for it would spill; 256 x 256 as it is has 16 bytes of scratch a lane)
+    static constexpr bool kCut = TM * TN == 1;
 };
 
 // Tile of block `h` of nbm x nbn: the hardware deals blocks to the 8 XCDs in turn, each with its own
@@ -196,10 +197,12 @@ enum { LIN_WHOLE = 0, LIN_PART = 1, LIN_JOIN = 2 };
 
 // (A's rows are the second operand: a lane's results are of one row of A and, four at a time,
 // consecutive columns.)
-// What bounds it, at 8192 x 4096 -> 16384 on 256 x 256 tiles (541 us, 2.03 POP/s): 54 us of a tile's
-// 67 are its products, at the clock that the power leaves (2.5 POP/s); then all CUs store a tile at
-// once, 11 us at the memory's rate, with the scaling beside it.  gelu adds 6, in vector issue.  The
-// stores straight from the registers, 32 bytes of a row at a time, took 818 us in all.
+// What bounds it, at 8192 x 4096 -> 16384 on 256 x 256 tiles (541 us, 2.03 POP/s): of a tile's 124
+// thousand cycles (64 us) 101 are the main loop's, in which the matrix units are busy 65% of the time;
+// then all CUs store a tile at once, at the memory's rate, with the scaling beside it.  The cycles are
+// the same for codes of zeros, at 2.38 GHz and 456 us: with real ones the power leaves 1.95 GHz.  gelu
+// adds 6 us, in vector issue.  The stores straight from the registers, 32 bytes of a row at a time,
+// took 818 us in all.
 template <typename T, typename S, int MODE>
 __global__ __launch_bounds__(S::NT, S::PER_SIMD) void k_lin_mfma(LinArgs<T> g, int64_t nbm, int64_t nbn, int64_t b_base,
                                                                   i32x4 *parts, int splits)
@@ -604,8 +607,9 @@ static int launch_lin_shape(LinArgs<T> g)
     return check_launch();
 }
 
-// By the cost of each shape, in us for a depth of 4096 as measured here: the most tiles that fall to
-// one CU at what one costs it alone, or all tiles at what they cost when every CU works.  A small
+// By the cost of each shape, in us for a depth of 4096 as measured here (no other depth was; in a short
+// one the tiles' ends and stores weigh more): the most tiles that fall to one CU at what one costs it
+// alone, or all tiles at what they cost when every CU works.  A small
 // tile answers sooner where there are few of them, a large one reads less for each product:
 // 300 x 4096 -> 4096 15 us on 64 x 64 tiles, 25 on 128 x 128, 54 on 256 x 256; 1024 rows 33, 27,
 // 54; 2048 rows 58, 42, 55 and 40 on 128 x 256; 4096 rows 110, 93, 71 on 256 x 256.

@@ -204,7 +204,8 @@ struct RmsGradPlan {
 // lane's columns of dgamma summed over the rows.  The block's groups fold theirs through LDS
 // and the block leaves one row of partials, in the rows' type.  `block` of `blocks`.  Bound by HBM:
 // f32 [16384, 4096] 134 us (a copy of as many bytes 130), with dh 175 (175); [65536, 1000] 138 and
-// 193 (128, 172); [4096, 16384], gamma's sums by k_rms_cols, 150 and 211 (132, 177).
+// 193 (128, 172); [4096, 16384] 150 and 211 (132, 177).  f64 [8192, 4096] 139 and 181 (131, 175), [32768,
+// 1000] 146 and 195 (126, 170); [2048, 16384], gamma's sums by k_rms_cols, 228 and 313 (130, 175).
 template <typename T, int NT, int VPT, bool DH, bool SUMS, bool PAST>
 NH_DEV void rms_grad_rows(const RmsGradArgs<T> &a, int64_t block, int64_t blocks)
 {

@@ -50,7 +50,9 @@ struct RmsPlan {
 // Groups of NT lanes walk the rows, r = group, group + groups, ...: a row is read once, its
 // square sum and its largest |w| taken from the registers by one exchange.  Bound by HBM: f32
 // [16384, 4096] 85 us, with the residual 175, and to 8 bits 131 (a copy of as many bytes 83, 176,
-// 140); [65536, 1000] 92, 177, 132 (84, 171, 136); [4096, 16384] 94, 190, 152 (86, 176, 140).
+// 140); [65536, 1000] 92, 177, 132 (84, 171, 136); [4096, 16384] 94, 190, 152 (86, 176, 140).  f64
+// [8192, 4096] with the residual 175 (a copy 176), to 8 bits 138 (136), and to 8 bits alone 63 (47; the
+// vector units: codes of f64 rows are made in double).
 template <typename T, int NT, int VPT, bool ADD, int OUT, bool PAST>
 __global__ __launch_bounds__((RmsPlan<T, NT, VPT, ADD, OUT>::NB), (RmsPlan<T, NT, VPT, ADD, OUT>::kWaves)) void k_rms_rows(
     RmsArgs<T> a, int64_t r_base)

@@ -351,7 +351,8 @@ constexpr int lp_lanes(int nt, int mode) { return mode == LP_TOP_BESIDE ? 2 * nt
 // r_base: the launch's first row.  What bounds it where rows are many: the vector units, with HBM
 // close behind (f32: about 16 issue slots a value; [4096, 50257] 140 us, a copy's rate 137); with
 // alternatives the latency of ordering them (k = 1: 212 us, 20: 256, 64: 383; with four waves a
-// SIMD, for which nine registers were spilled, 231, 257 and 347).
+// SIMD, for which nine registers were spilled, 231, 257 and 347).  f64, an exponential in double a
+// value: [2048, 50257] 159 us (a copy's rate 133), k = 20 252.
 template <typename T, int NT, int VPT, int MODE>
 __global__ __launch_bounds__(lp_lanes(NT, MODE), (MODE == LP_SUMS ? 1 : 3)) void k_lp_parts(
     LpArgs<T> a, LpScratch<T> scratch, int parts, int64_t per, int64_t r_base)
@@ -753,6 +754,7 @@ NH_DEV void lp_far_row(const LpGradArgs<T> &q, LpGradRow<T> w, int64_t r, int la
 // whose rows start anywhere: 268 us, a copy of as many bytes 276; with all rows far 498, 267 from four
 // values; one far row of 131072 70 us and 4.1).  A block's 1024 vectors lie in two rows at most, mostly
 // in one: its numbers are the same for the block then, and nothing is read for a row that is not used.
+// f64 [2048, 50257] 268 us (a copy 272).
 constexpr int64_t kLpFlat = 4096;
 template <typename T>
 __global__ __launch_bounds__(256) void k_lp_grad_flat(LpGradArgs<T> a, int64_t head, int64_t b_base)
