@@ -266,3 +266,42 @@ def test_four_saved_values_refused(pn):
         assert not v.numpy().any()
     assert forward(None, None, four._ptr, None, None, 0, x._ptr, tok.ctypes.data, 1.0) == E.OK
     assert backward(dx._ptr, g._ptr, g._ptr, x._ptr, tok.ctypes.data, four._ptr, None, 1.0) == E.OK
+
+
+@pytest.mark.parametrize("four", [False, True])
+def test_graph_at_a_low_temperature(pn, rng, four):
+    """Forward and gradient captured, replayed over changed logits and tokens, eager calls in between."""
+    import torch
+    rows, V, temperature, lib, T = 14, 5003, 0.01, pn.core._lib, pn.Tensor
+    t = {"x": torch.zeros(rows, V, device="cuda"), "dx": torch.zeros(rows, V, device="cuda"),
+         "lse": torch.zeros(rows, 4 if four else 1, device="cuda"),
+         **{n: torch.zeros(rows, device="cuda") for n in ("entropy", "g", "e")}}
+    tok = torch.zeros(rows, dtype=torch.int64, device="cuda")
+    w = {n: T.from_torch(v) for n, v in t.items()}
+    P = lambda n: w[n]._ptr  # noqa: E731
+    stream = torch.cuda.Stream()
+    pn.set_stream(stream.cuda_stream)
+    try:
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            assert lib.neural_token_logprobs_forward(None, P("entropy"), P("lse"), None, None, 0, P("x"), tok.data_ptr(),
+                                                     temperature) == 0
+            assert lib.neural_token_logprobs_backward(P("dx"), P("g"), P("e"), P("x"), tok.data_ptr(), P("lse"),
+                                                      None if four else P("entropy"), temperature) == 0
+        for _ in range(3):
+            x, tokens = _rows(rng, V, np.float32, temperature)
+            x[::4] *= np.float32(0.01)
+            g, e = rng.normal(0, 1, rows).astype(np.float32), rng.normal(0, 1, rows).astype(np.float32)
+            for n, v in (("x", x), ("g", g), ("e", e)):
+                t[n].copy_(torch.from_numpy(v))
+            tok.copy_(torch.from_numpy(tokens))
+            torch.cuda.synchronize()
+            graph.replay()
+            torch.cuda.synchronize()
+            saved = _four(pn, x, tokens, temperature)
+            want = _backward(pn, x, tokens, g, e, saved if four else saved[:, 0].copy(),
+                             None if four else saved[:, 3].copy(), temperature)
+            same_bits(t["dx"].cpu().numpy(), want)
+    finally:
+        pn.set_stream(None)
