@@ -487,10 +487,11 @@ int neural_linear_q8(NeuralTensor *out, const int8_t *codes, int64_t stride, con
  * per row.  z = logits / temperature, lse = log sum_v exp z_v, p = exp(z - lse).
  *
  * Forward, every output one value per row in the logits' dtype, any of them NULL, not all:
- * logprob = z[token] - lse, entropy = -sum p log p (a term of p = 0 is 0), lse (for the
- * backward call; a tensor of four values per row takes what that call needs of it: lse, m = max
- * logit, log sum_v exp((logit_v - m) / temperature), entropy), and the k (0 to 64) largest logits, equal ones by index: top_ids [rows, k]
- * int64 (host or device memory) and top_logprobs [rows, k] (either may be NULL).
+ * logprob = z[token] - lse, entropy = -sum p log p (a term of p = 0 is 0), lse (for the backward
+ * call; a tensor of four values per row takes all that that call needs of it: lse, m = the largest
+ * logit, 0 where all are masked, log sum_v exp((logit_v - m) / temperature), entropy), and the k (0
+ * to 64) largest logits, equal ones by index: top_ids [rows, k] int64 (host or device memory) and
+ * top_logprobs [rows, k] (either may be NULL).
  * A logit of -inf is a masked one: it is no alternative, and where fewer than k are left the
  * rest is id -1, log probability -inf.  A row with all logits masked has lse and logprob
  * -inf and entropy 0.  A row with NaN or +inf has NaN, ids -1.
@@ -511,8 +512,8 @@ int neural_linear_q8(NeuralTensor *out, const int8_t *codes, int64_t stride, con
  * partial results, as neural_layer_norm_backward does.
  * Errors: NULL_POINTER, DTYPE_MISMATCH, DIM_MISMATCH (a 0-d tensor), SHAPE_MISMATCH,
  * TENSOR_TOO_LARGE, INVALID_ARGUMENT (non-contiguous tensors, k outside [0, 64], a temperature
- * outside [1e-10, 1e10], tokens or top_ids in host memory in a captured call, outputs that overlap an input, other than as allowed, or each
- * other). */
+ * outside [1e-10, 1e10], tokens or top_ids in host memory in a captured call, outputs that overlap an
+ * input, other than as allowed, or each other). */
 int neural_token_logprobs_forward(NeuralTensor *logprob, NeuralTensor *entropy, NeuralTensor *lse,
                                   int64_t *top_ids, NeuralTensor *top_logprobs, int64_t k,
                                   const NeuralTensor *logits, const int64_t *tokens, double temperature);
